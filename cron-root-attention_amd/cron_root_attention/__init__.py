@@ -17,6 +17,7 @@ from .core import (GPU_SM_MAP, CronRootAttentionV14, CronRootAttentionV14Functio
                    warmup_varlen_shapes)
 from .hybrid import CronRootAttentionHybrid, cron_root_attention_hybrid
 from .module import CronRootAttention, CronRootMultiheadAttention
+from .rotary import RotaryTable, qk_norm_rotary, rotary_embedding
 from . import _native
 
 
@@ -81,6 +82,9 @@ __all__ = [
     "CronRootMultiheadAttention",
     "cron_root_attention_hybrid",
     "CronRootAttentionHybrid",
+    "RotaryTable",
+    "rotary_embedding",
+    "qk_norm_rotary",
     "calibrate",
     "get_num_sms",
     "get_gpu_info",

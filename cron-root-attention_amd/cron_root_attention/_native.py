@@ -79,6 +79,14 @@ class Docs:
         return len(self.window)
 
 
+class CraTurn(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ("B", "H_q", "H_kv", "S", "D", "rot", "interleaved",
+                                               "norm", "dtype", "weight_dtype", "positions_64")]
+                + [("eps", ctypes.c_float), ("table", ctypes.c_void_p),
+                   ("table_rows", ctypes.c_int64), ("positions", ctypes.c_void_p),
+                   ("psb", ctypes.c_int64), ("pss", ctypes.c_int64)])
+
+
 class CraDeviceInfo(ctypes.Structure):
     _fields_ = [("cu_count", ctypes.c_int32), ("lds_bytes_per_cu", ctypes.c_int32),
                 ("arch_major", ctypes.c_int32), ("arch_minor", ctypes.c_int32),
@@ -95,6 +103,7 @@ class CraTileConfig(ctypes.Structure):
 # Exported symbols and their signatures (mirrors include/cra.h).
 _P = ctypes.POINTER(CraProblem)
 _D = ctypes.POINTER(CraDocs)
+_R = ctypes.POINTER(CraTurn)
 _SIGNATURES = {
     "cra_supported_head_dim": (ctypes.c_int, [ctypes.c_int32]),
     "cra_global_rows": (ctypes.c_int64, [_P]),
@@ -137,6 +146,13 @@ _SIGNATURES = {
                                       ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                       CraTensor, CraTensor, CraTensor, ctypes.c_void_p,
                                       ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "cra_rotary": (ctypes.c_int, [_R, CraTensor, CraTensor, ctypes.c_void_p, ctypes.c_void_p,
+                                  CraTensor, CraTensor, ctypes.c_int32, ctypes.c_void_p]),
+    "cra_rotary_bwd_workspace_bytes": (ctypes.c_size_t, [_R]),
+    "cra_norm_rotary_bwd": (ctypes.c_int, [_R, CraTensor, CraTensor, ctypes.c_void_p,
+                                           ctypes.c_void_p, CraTensor, CraTensor, CraTensor,
+                                           CraTensor, ctypes.c_void_p, ctypes.c_void_p,
+                                           ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "cra_device_info": (ctypes.c_int, [ctypes.c_int32, ctypes.POINTER(CraDeviceInfo)]),
     "cra_tile_config": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int32,
                                        ctypes.POINTER(CraTileConfig)]),
@@ -481,6 +497,77 @@ def forward_cpu(p: CraProblem, q, k, v, threads: int):
     _check(lib.cra_fwd_cpu(ctypes.byref(p), tensor_arg(q), tensor_arg(k), tensor_arg(v),
                            tensor_arg(o), max(1, int(threads))), "cra_fwd_cpu")
     return o
+
+
+# ---- rotary positions and head norms -------------------------------------
+
+class _OnDevice:
+    """Makes the device of a tensor current for the launches inside (a stream
+    belongs to its device); nothing where it is already."""
+
+    __slots__ = ("index", "prev")
+
+    def __init__(self, t: torch.Tensor):
+        self.index = t.device.index
+
+    def __enter__(self):
+        self.prev = torch.cuda.current_device()
+        if self.prev != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.prev != self.index:
+            torch.cuda.set_device(self.prev)
+
+
+def on_device(t: torch.Tensor) -> _OnDevice:
+    return _OnDevice(t)
+
+
+_NO_TENSOR = CraTensor(None, 0, 0, 0)
+
+
+def row_arg(t: Optional[torch.Tensor]) -> CraTensor:
+    """A [B, H, S, D] tensor with D contiguous; the stride of a dimension of one
+    element, which is never taken, is given as 0."""
+    if t is None:
+        return _NO_TENSOR
+    (B, H, S, _), (sb, sh, ss, _) = t.shape, t.stride()
+    return CraTensor(t.data_ptr(), sb if B > 1 else 0, sh if H > 1 else 0, ss if S > 1 else 0)
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def rotary(p: CraTurn, q, k, wq, wk, transpose: bool = False):
+    """cra_rotary into fresh tensors laid out as q and k."""
+    yq = torch.empty_like(q)
+    yk = None if k is None else torch.empty_like(k)
+    with on_device(q):
+        _check(load_library().cra_rotary(ctypes.byref(p), row_arg(q), row_arg(k), _ptr(wq), _ptr(wk),
+                                         row_arg(yq), row_arg(yk), int(transpose), _stream(q)),
+               "cra_rotary")
+    return yq, yk
+
+
+def norm_rotary_backward(p: CraTurn, q, k, wq, wk, dyq, dyk, want_wq: bool, want_wk: bool):
+    lib = load_library()
+    dq = torch.empty_like(q)
+    dk = None if k is None else torch.empty_like(k)
+    dwq = torch.empty_like(wq) if want_wq else None
+    dwk = torch.empty_like(wk) if want_wk else None
+    ws = None
+    if want_wq or want_wk:
+        ws = torch.empty(lib.cra_rotary_bwd_workspace_bytes(ctypes.byref(p)), dtype=torch.uint8,
+                         device=q.device)
+    with on_device(q):
+        _check(lib.cra_norm_rotary_bwd(ctypes.byref(p), row_arg(q), row_arg(k), _ptr(wq), _ptr(wk),
+                                       row_arg(dyq), row_arg(dyk), row_arg(dq), row_arg(dk),
+                                       _ptr(dwq), _ptr(dwk), _ptr(ws),
+                                       0 if ws is None else ws.numel(), _stream(q)),
+               "cra_norm_rotary_bwd")
+    return dq, dk, dwq, dwk
 
 
 def tile_config(dtype: torch.dtype, D: int) -> dict:

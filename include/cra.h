@@ -275,6 +275,47 @@ typedef struct {
 } cra_tile_config_t;
 int cra_tile_config(int32_t dtype, int32_t D, cra_tile_config_t* out);
 
+/* ---- rotary positions and norms of the heads of q and k -------------------
+ * One call turns q [B, H_q, S, D] and k [B, H_kv, S, D] (H_kv = 0: q alone):
+ * pair i of the first `rot` elements of a head, (i, i + rot/2) or with
+ * `interleaved` (2i, 2i + 1), by the angle of row p of the table; the rest of
+ * the head passes. With `norm` each head row is first divided by its root mean
+ * square, sqrt(mean(x^2) + eps), and multiplied by the D weights (NULL: ones).
+ * fp32 arithmetic, one rounding. D up to 256, any strides with D contiguous, no
+ * alignment beyond the element's (16-byte aligned rows are the fast ones).
+ * Inputs and outputs may not overlap, except that an output may be its input
+ * (same strides). The reference has no counterpart (positions and norms are
+ * its callers'). */
+typedef struct {
+  int32_t B, H_q, H_kv, S, D;
+  int32_t rot;          /* leading elements turned: even, 0..D (0: no rotation) */
+  int32_t interleaved;
+  int32_t norm;
+  int32_t dtype;        /* of q, k and the outputs */
+  int32_t weight_dtype; /* of the norm weights: dtype, or CRA_F32 */
+  int32_t positions_64; /* positions are int64 (else int32) */
+  float eps;
+  const float* table;   /* [table_rows, rot]: rot/2 cosines, then rot/2 sines */
+  int64_t table_rows;
+  const void* positions; /* of token (b, s): positions[b * psb + s * pss]; NULL: s.
+                            A position outside the table gives NaN where it turns. */
+  int64_t psb, pss;
+} cra_turn;
+
+/* transpose: turn by the negative angles (the backward of the rotation alone). */
+int cra_rotary(const cra_turn* p, cra_tensor q, cra_tensor k, const void* wq, const void* wk,
+               cra_tensor yq, cra_tensor yk, int32_t transpose, void* stream);
+
+/* Backward of norm and rotation: dq, dk from the forward's inputs q, k and the
+ * gradients dyq, dyk of its outputs. dwq, dwk (weight_dtype, D each) receive the
+ * weights' gradients, or are NULL; their sums run in a fixed order over partial
+ * sums in the workspace (not needed when both are NULL). */
+size_t cra_rotary_bwd_workspace_bytes(const cra_turn* p);
+int cra_norm_rotary_bwd(const cra_turn* p, cra_tensor q, cra_tensor k, const void* wq,
+                        const void* wk, cra_tensor dyq, cra_tensor dyk, cra_tensor dq,
+                        cra_tensor dk, void* dwq, void* dwk, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
 const char* cra_strerror(int32_t code);
 const char* cra_last_error(void);
 int32_t cra_abi_version(void);
