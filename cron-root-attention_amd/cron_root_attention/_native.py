@@ -87,6 +87,19 @@ class CraTurn(ctypes.Structure):
                    ("psb", ctypes.c_int64), ("pss", ctypes.c_int64)])
 
 
+class CraCache(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("k", "v", "k_norm", "k_scale", "v_scale")]
+                + [(n, ctypes.c_int32) for n in ("num_pages", "H_kv", "page_size", "D", "dtype",
+                                                 "store")])
+
+
+class CraBatch(ctypes.Structure):
+    _fields_ = [("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+                ("seq_lens", ctypes.c_void_p), ("cu_seqlens", ctypes.c_void_p),
+                ("n_seqs", ctypes.c_int32), ("pages_per_seq", ctypes.c_int32),
+                ("tokens", ctypes.c_int32), ("query_len", ctypes.c_int32)]
+
+
 class CraDeviceInfo(ctypes.Structure):
     _fields_ = [("cu_count", ctypes.c_int32), ("lds_bytes_per_cu", ctypes.c_int32),
                 ("arch_major", ctypes.c_int32), ("arch_minor", ctypes.c_int32),
@@ -104,6 +117,8 @@ class CraTileConfig(ctypes.Structure):
 _P = ctypes.POINTER(CraProblem)
 _D = ctypes.POINTER(CraDocs)
 _R = ctypes.POINTER(CraTurn)
+_C = ctypes.POINTER(CraCache)
+_B = ctypes.POINTER(CraBatch)
 _SIGNATURES = {
     "cra_supported_head_dim": (ctypes.c_int, [ctypes.c_int32]),
     "cra_global_rows": (ctypes.c_int64, [_P]),
@@ -153,6 +168,10 @@ _SIGNATURES = {
                                            ctypes.c_void_p, CraTensor, CraTensor, CraTensor,
                                            CraTensor, ctypes.c_void_p, ctypes.c_void_p,
                                            ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "cra_cache_write": (ctypes.c_int, [_C, _B, CraTensor, CraTensor, ctypes.c_int32,
+                                       ctypes.c_void_p]),
+    "cra_cache_read": (ctypes.c_int, [_C, _B, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,
+                                      ctypes.c_void_p, ctypes.c_void_p]),
     "cra_device_info": (ctypes.c_int, [ctypes.c_int32, ctypes.POINTER(CraDeviceInfo)]),
     "cra_tile_config": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int32,
                                        ctypes.POINTER(CraTileConfig)]),
@@ -568,6 +587,26 @@ def norm_rotary_backward(p: CraTurn, q, k, wq, wk, dyq, dyk, want_wq: bool, want
                                        0 if ws is None else ws.numel(), _stream(q)),
                "cra_norm_rotary_bwd")
     return dq, dk, dwq, dwk
+
+
+# ---- paged cache -----------------------------------------------------------
+
+STORE_SAME, STORE_E4M3, STORE_INT8 = 0, 1, 2
+
+
+def cache_write(c: CraCache, b: CraBatch, k, v):
+    with on_device(k):
+        _check(load_library().cra_cache_write(ctypes.byref(c), ctypes.byref(b), row_arg(k),
+                                              row_arg(v), k.shape[3], _stream(k)),
+               "cra_cache_write")
+
+
+def cache_read(c: CraCache, b: CraBatch, length: int, k, v):
+    """Into the contiguous k, v [n_seqs, H_kv, length, D]."""
+    with on_device(k):
+        _check(load_library().cra_cache_read(ctypes.byref(c), ctypes.byref(b), length, k.shape[3],
+                                             k.data_ptr(), v.data_ptr(), _stream(k)),
+               "cra_cache_read")
 
 
 def tile_config(dtype: torch.dtype, D: int) -> dict:

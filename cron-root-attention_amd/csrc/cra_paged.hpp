@@ -1,0 +1,112 @@
+// The paged key/value cache as the kernels see it, and the geometry of a
+// sequence's present length. Host-compilable: the index arithmetic is tested
+// on the CPU.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/cra.h"
+
+namespace cra {
+
+// Row (page, head, offset) of a cache whose pages are [H_kv, page_size] rows:
+// the index of the row in k, v, and of its norm and scales. 32 bits hold it
+// (the ABI refuses caches of 2^31 rows); byte offsets take 64.
+__host__ __device__ inline uint32_t cache_row(int page, int H_kv, int log_page, int h, int off) {
+  return (((uint32_t)page * (uint32_t)H_kv + (uint32_t)h) << log_page) + (uint32_t)off;
+}
+
+constexpr uint32_t kNoRow = 0xffffffffu;  // of a page outside the cache
+
+struct PagedView {
+  const char* k;
+  const char* v;
+  const float* k_norm;
+  const float* k_scale;
+  const float* v_scale;
+  const int32_t* table;  // [n_seqs, pages_per_seq], rows table_stride apart
+  const int32_t* lens;   // [n_seqs]
+  const int32_t* cu;     // [n_seqs + 1] first token of each sequence, or null
+  int64_t table_stride;
+  int num_pages, H_kv, log_page, n_seqs, pages_per_seq;
+  int tokens, query_len;  // cu: rows of the packed tensors; else tokens per sequence
+};
+
+// Length of a sequence, within what its row of the table can hold (lengths
+// live on the device and are not known when the launch is checked).
+__host__ __device__ inline int seq_length(int len, int pages_per_seq, int log_page) {
+  const int64_t most = (int64_t)pages_per_seq << log_page;
+  const int cap = most < 0x7fffffff ? (int)most : 0x7fffffff;
+  return len < 0 ? 0 : len < cap ? len : cap;
+}
+
+// Tokens [first, last) of sequence b in the packed tensors; within them
+// whatever cu holds.
+struct TokenRange {
+  int first, last;
+};
+__host__ __device__ inline TokenRange token_range(const int32_t* cu, int b, int tokens) {
+  const int a = cu[b] < 0 ? 0 : cu[b] < tokens ? cu[b] : tokens;
+  const int e = cu[b + 1] < a ? a : cu[b + 1] < tokens ? cu[b + 1] : tokens;
+  return TokenRange{a, e};
+}
+
+// Sequence of packed token t: the last b with cu[b] <= t, or -1 for a token
+// before the first or behind the last sequence.
+__host__ __device__ inline int seq_of_token(const int32_t* cu, int n_seqs, int t) {
+  if (t < cu[0] || t >= cu[n_seqs]) return -1;
+  int lo = 0, hi = n_seqs - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (cu[mid] <= t) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+// ceil(sqrt(n)), n >= 0.
+__host__ __device__ inline int ceil_sqrt(int n) {
+  if (n <= 0) return 0;
+  int64_t r = (int64_t)sqrtf((float)n);  // within one of it
+  while (r * r < n) ++r;
+  while (r > 1 && (r - 1) * (r - 1) >= n) --r;
+  return (int)r;
+}
+
+// The plan of a sequence of n tokens: window W (the rule, or the caller's,
+// within the length), rows per block of the global rows.
+struct SeqPlan {
+  int n, W, rpb;
+};
+__host__ __device__ inline SeqPlan seq_plan(int n, int window, int relay, int top_k) {
+  SeqPlan p;
+  p.n = n;
+  p.W = window > 0 ? (window < n ? window : n) : ceil_sqrt(n);
+  if (p.W < 1) p.W = 1;
+  p.rpb = (relay < 0 ? n > 2048 : relay != 0) ? 1 + top_k : 1;
+  return p;
+}
+
+// Global rows that the query at position i sees: a prefix of this length.
+__host__ __device__ inline int seq_prefix(int i, const SeqPlan& p) {
+  const int ls = i - p.W + 1 > 0 ? i - p.W + 1 : 0;
+  const int f = ls / p.W;
+  return p.rpb * f + (ls != f * p.W ? 1 : 0);
+}
+
+// Cache row of logical row `row` of a sequence whose table row is `pages`, or
+// kNoRow if its page lies outside the cache.
+__host__ __device__ inline uint32_t seq_row(const int32_t* pages, int row, int num_pages, int H_kv,
+                                            int log_page, int h) {
+  const int page = pages[row >> log_page];
+  if ((uint32_t)page >= (uint32_t)num_pages) return kNoRow;
+  return cache_row(page, H_kv, log_page, h, row & ((1 << log_page) - 1));
+}
+
+// Checks of the C ABI shared by its calls over a cache (CRA_OK or an error with
+// its text set), and the view the kernels take.
+int check_cache(const cra_cache* c);
+int check_batch(const cra_cache* c, const cra_batch* b);
+PagedView paged_view(const cra_cache* c, const cra_batch* b);
+
+}  // namespace cra

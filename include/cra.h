@@ -316,6 +316,63 @@ int cra_norm_rotary_bwd(const cra_turn* p, cra_tensor q, cra_tensor k, const voi
                         cra_tensor dk, void* dwq, void* dwk, void* workspace,
                         size_t workspace_bytes, void* stream);
 
+/* ---- paged key/value cache ------------------------------------------------
+ * No counterpart in the reference, which attends whole sequences only. */
+
+/* How a cache holds its elements: in its dtype, or in 8 bits with an fp32 scale
+ * for each row and head (the value of code c is c * scale). */
+enum { CRA_STORE_SAME = 0, CRA_STORE_E4M3 = 1, CRA_STORE_INT8 = 2 };
+
+/* Pages of page_size rows of every kv head. k, v: contiguous
+ * [num_pages, H_kv, page_size, D] of dtype or 8-bit codes; k_norm (the sum of
+ * squares of the key as it was written), k_scale, v_scale (8-bit stores only):
+ * contiguous fp32 [num_pages, H_kv, page_size]. page_size: a power of two from 16
+ * to 1024. D: a multiple of 16 up to 256 (narrower heads are padded with zeros).
+ * Fewer than 2^31 rows (page_size * H_kv * num_pages). */
+typedef struct {
+  void* k;
+  void* v;
+  float* k_norm;
+  float* k_scale;
+  float* v_scale;
+  int32_t num_pages, H_kv, page_size, D;
+  int32_t dtype;  /* of the values: CRA_F16, CRA_BF16, CRA_F32 */
+  int32_t store;  /* CRA_STORE_* */
+} cra_cache;
+
+/* Sequences of one call; page_table, seq_lens and cu_seqlens are device memory,
+ * read by the kernels (a captured graph sees what they hold at its replay).
+ * Row r of sequence b lies in page page_table[b * table_stride + r / page_size].
+ * seq_lens[b] is its length with its new tokens, which are its last ones:
+ * query_len of them each, token (b, t) of [n_seqs, H, query_len, D] tensors; or,
+ * with cu_seqlens (n_seqs + 1 entries, not falling), tokens cu_seqlens[b] ..
+ * cu_seqlens[b + 1] - 1 of [1, H, tokens, D] tensors. Tokens outside every
+ * sequence (a padded batch) are passed over. Lengths are held within what a row
+ * of the table can hold; nothing is read or written through a page id outside
+ * 0 .. num_pages - 1. */
+typedef struct {
+  const int32_t* page_table;
+  int64_t table_stride;
+  const int32_t* seq_lens;
+  const int32_t* cu_seqlens;  /* or NULL */
+  int32_t n_seqs, pages_per_seq;
+  int32_t tokens;             /* with cu_seqlens: rows of the packed tensors */
+  int32_t query_len;          /* without */
+} cra_batch;
+
+/* Stores the rows of the new tokens: k, v [n_seqs, H_kv, query_len, D] (or packed)
+ * of the cache's dtype, D a multiple of 8 up to the cache's row width (columns
+ * behind it are set to zero), rows 16-byte aligned. The caller sees to it that
+ * no page is written for two sequences. */
+int cra_cache_write(const cra_cache* c, const cra_batch* b, cra_tensor k, cra_tensor v, int32_t D,
+                    void* stream);
+
+/* Reads rows 0 .. length - 1 of every sequence into contiguous k, v
+ * [n_seqs, H_kv, length, D] of the cache's dtype (rounded once); rows behind a
+ * sequence are zeros, rows of a page outside the cache NaN. */
+int cra_cache_read(const cra_cache* c, const cra_batch* b, int32_t length, int32_t D, void* k,
+                   void* v, void* stream);
+
 const char* cra_strerror(int32_t code);
 const char* cra_last_error(void);
 int32_t cra_abi_version(void);
