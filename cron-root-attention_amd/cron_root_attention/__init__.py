@@ -17,6 +17,7 @@ from .core import (GPU_SM_MAP, CronRootAttentionV14, CronRootAttentionV14Functio
                    warmup_varlen_shapes)
 from .hybrid import CronRootAttentionHybrid, cron_root_attention_hybrid
 from .module import CronRootAttention, CronRootMultiheadAttention
+from .paged import PagedBatch, PagedKVCache, cron_root_attention_paged
 from .rotary import RotaryTable, qk_norm_rotary, rotary_embedding
 from . import _native
 
@@ -73,6 +74,9 @@ def get_gpu_info() -> dict:
 
 cron_root_attention = cron_root_attention_v14
 
+# The reference's own list (a star import gives what the reference's gives); what
+# this package adds is reached by name: RotaryTable, rotary_embedding,
+# qk_norm_rotary, PagedKVCache, PagedBatch, cron_root_attention_paged.
 __all__ = [
     "cron_root_attention",
     "cron_root_attention_v14",
@@ -82,9 +86,6 @@ __all__ = [
     "CronRootMultiheadAttention",
     "cron_root_attention_hybrid",
     "CronRootAttentionHybrid",
-    "RotaryTable",
-    "rotary_embedding",
-    "qk_norm_rotary",
     "calibrate",
     "get_num_sms",
     "get_gpu_info",

@@ -100,6 +100,12 @@ class CraBatch(ctypes.Structure):
                 ("tokens", ctypes.c_int32), ("query_len", ctypes.c_int32)]
 
 
+class CraPagedPlan(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ("H_q", "D", "window", "relay", "top_k",
+                                               "max_query_len", "max_seqlen")]
+                + [("scale", ctypes.c_float)])
+
+
 class CraDeviceInfo(ctypes.Structure):
     _fields_ = [("cu_count", ctypes.c_int32), ("lds_bytes_per_cu", ctypes.c_int32),
                 ("arch_major", ctypes.c_int32), ("arch_minor", ctypes.c_int32),
@@ -119,6 +125,7 @@ _D = ctypes.POINTER(CraDocs)
 _R = ctypes.POINTER(CraTurn)
 _C = ctypes.POINTER(CraCache)
 _B = ctypes.POINTER(CraBatch)
+_G = ctypes.POINTER(CraPagedPlan)
 _SIGNATURES = {
     "cra_supported_head_dim": (ctypes.c_int, [ctypes.c_int32]),
     "cra_global_rows": (ctypes.c_int64, [_P]),
@@ -172,6 +179,9 @@ _SIGNATURES = {
                                        ctypes.c_void_p]),
     "cra_cache_read": (ctypes.c_int, [_C, _B, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,
                                       ctypes.c_void_p, ctypes.c_void_p]),
+    "cra_fwd_paged_workspace_bytes": (ctypes.c_size_t, [_C, _B, _G]),
+    "cra_fwd_paged": (ctypes.c_int, [_C, _B, _G, CraTensor, CraTensor, ctypes.c_void_p,
+                                     ctypes.c_size_t, ctypes.c_void_p]),
     "cra_device_info": (ctypes.c_int, [ctypes.c_int32, ctypes.POINTER(CraDeviceInfo)]),
     "cra_tile_config": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int32,
                                        ctypes.POINTER(CraTileConfig)]),
@@ -607,6 +617,17 @@ def cache_read(c: CraCache, b: CraBatch, length: int, k, v):
         _check(load_library().cra_cache_read(ctypes.byref(c), ctypes.byref(b), length, k.shape[3],
                                              k.data_ptr(), v.data_ptr(), _stream(k)),
                "cra_cache_read")
+
+
+def forward_paged(c: CraCache, b: CraBatch, p: CraPagedPlan, q, o):
+    """cra_fwd_paged into o."""
+    lib = load_library()
+    cp, bp, pp = ctypes.byref(c), ctypes.byref(b), ctypes.byref(p)
+    nbytes = lib.cra_fwd_paged_workspace_bytes(cp, bp, pp)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    with on_device(q):
+        _check(lib.cra_fwd_paged(cp, bp, pp, row_arg(q), row_arg(o), _ptr(ws), nbytes, _stream(q)),
+               "cra_fwd_paged")
 
 
 def tile_config(dtype: torch.dtype, D: int) -> dict:

@@ -4,8 +4,8 @@
 // A key row is stored with the sum of its squares, which the relay rows are
 // ranked by: 4 bytes a row instead of a pass over all keys whenever blocks are
 // formed for another length. The sum is that of the packed-row kernel of whole
-// sequences, bit for bit (8 elements left to right without fused multiply-adds,
-// then a butterfly over the D/8 lanes), so both choose the same rows.
+// sequences, bit for bit (8 elements left to right by fused multiply-adds, then a
+// butterfly over the D/8 lanes), so both choose the same rows.
 //
 // 8 bits: row x with m = max |x| is held as codes c and a scale s.
 //   e4m3: s = the smallest power of two with m <= 448 s, c = RNE(x / s). x / s
@@ -100,9 +100,9 @@ __device__ __forceinline__ void store_row(const float (&x)[8], const Row8<T>& ra
 #pragma unroll
     for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
     const float s = row_scale<STORE>(lanes_max(m, log_l));
-    if (lane * 8 < Ds)
+    if (lane * 8 < Ds)  // codes themselves are finite: the scale says what is not
       *reinterpret_cast<uint2*>(static_cast<char*>(base) + at) =
-          make_uint2(codes4<STORE>(x, s), codes4<STORE>(x + 4, s));
+          s == s ? make_uint2(codes4<STORE>(x, s), codes4<STORE>(x + 4, s)) : make_uint2(0, 0);
     if (lane == 0) scale[row] = s;
   }
 }
@@ -154,9 +154,9 @@ __global__ __launch_bounds__(kThreads) void cache_write_kernel(WriteArgs a) {
     kx[i] = to_f32(reinterpret_cast<const T*>(kr.w)[i]);
     vx[i] = to_f32(reinterpret_cast<const T*>(vr.w)[i]);
   }
-  float norm = 0.f;
+  float norm = kx[0] * kx[0];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) norm = __fadd_rn(norm, __fmul_rn(kx[i], kx[i]));
+  for (int i = 1; i < 8; ++i) norm = __builtin_fmaf(kx[i], kx[i], norm);
   for (int o = 1 << a.log_l >> 1; o > 0; o >>= 1) norm = __fadd_rn(norm, __shfl_xor(norm, o));
   if (lane == 0) a.k_norm[dst] = norm;
   store_row<T, STORE>(kx, kr, const_cast<char*>(a.c.k), a.k_scale, dst, a.Ds, lane, a.log_l);

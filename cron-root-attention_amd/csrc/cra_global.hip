@@ -13,7 +13,8 @@
 //
 // The squared norm of a row is summed in one fixed order so a CPU check can
 // reproduce it bit for bit: each lane sums the squares of its 8 consecutive
-// elements left to right (no fused multiply-add), then the D/8 lane partials
+// elements left to right (fp32: by fused multiply-adds, as the compiler contracts
+// them; products of 16-bit elements are exact either way), then the D/8 lane partials
 // are combined by a butterfly p += p[lane ^ off], off = D/16 .. 1.
 #include <type_traits>
 

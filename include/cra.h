@@ -373,6 +373,33 @@ int cra_cache_write(const cra_cache* c, const cra_batch* b, cra_tensor k, cra_te
 int cra_cache_read(const cra_cache* c, const cra_batch* b, int32_t length, int32_t D, void* k,
                    void* v, void* stream);
 
+/* Attention of the new tokens of every sequence over the cache (which holds
+ * them already: cra_cache_write first). Query i of a sequence of n tokens sees
+ * the rows it sees in the attention of the whole sequence (top of this file);
+ * the window is ceil(sqrt(n)) of the present length, or `window` within it
+ * (window >= n: plain causal attention); relay as in cra_problem, -1: n > 2048.
+ * With one window and relay switch for all of a sequence's calls, its rows are
+ * those of one call over the whole sequence. */
+typedef struct {
+  int32_t H_q, D;         /* columns of q and o: a multiple of 8 up to the cache's row width */
+  int32_t window;         /* 0: the rule */
+  int32_t relay;          /* -1: the rule, 0, 1 */
+  int32_t top_k;          /* 1..4 (ignored when relay == 0) */
+  int32_t max_query_len;  /* with cu_seqlens: bound on a sequence's new tokens */
+  int32_t max_seqlen;     /* bound on seq_lens; a sequence beyond a bound gives NaN */
+  float scale;            /* logit scale */
+} cra_paged_plan;
+
+/* q, o: [n_seqs, H_q, query_len, D] or packed [1, H_q, tokens, D] of the cache's
+ * dtype, rows 16-byte aligned; query head h reads kv head h / (H_q / H_kv). Rows
+ * outside every sequence are not written; a query that sees no row (its sequence
+ * holds fewer rows than new tokens) gives zeros; one that meets a page outside
+ * the cache gives NaN. The workspace may be any memory not used by another
+ * call at the same time; nothing in it needs clearing. */
+size_t cra_fwd_paged_workspace_bytes(const cra_cache* c, const cra_batch* b, const cra_paged_plan* p);
+int cra_fwd_paged(const cra_cache* c, const cra_batch* b, const cra_paged_plan* p, cra_tensor q,
+                  cra_tensor o, void* workspace, size_t workspace_bytes, void* stream);
+
 const char* cra_strerror(int32_t code);
 const char* cra_last_error(void);
 int32_t cra_abi_version(void);
