@@ -102,7 +102,7 @@ class CraBatch(ctypes.Structure):
 
 class CraPagedPlan(ctypes.Structure):
     _fields_ = ([(n, ctypes.c_int32) for n in ("H_q", "D", "window", "relay", "top_k",
-                                               "max_query_len", "max_seqlen")]
+                                               "max_query_len", "max_seqlen", "zero_outside")]
                 + [("scale", ctypes.c_float)])
 
 

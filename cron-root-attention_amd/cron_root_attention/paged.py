@@ -294,8 +294,8 @@ def cron_root_attention_paged(q: torch.Tensor, cache: PagedKVCache, page_table: 
         if x is not None and x < 1:
             raise ValueError(f"{name} must be >= 1, got {x}")
     if out is None:
-        # a fresh output's rows outside every sequence: zeros
-        o = torch.empty_like(q) if cu_seqlens is None and batch is not None else torch.zeros_like(q)
+        # rows outside every sequence are zeros in a fresh output
+        o = torch.zeros_like(q) if batch is None else torch.empty_like(q)
     else:
         if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
             raise ValueError("out must have the shape, dtype and device of q")
@@ -306,7 +306,7 @@ def cron_root_attention_paged(q: torch.Tensor, cache: PagedKVCache, page_table: 
         Hq, D + -D % 8, 0 if window is None else min(int(window), 2**31 - 1),
         -1 if relay is None else int(bool(relay)), int(relay_top_k),
         min(q.shape[2], max_query_len or q.shape[2]), min(held, max_seqlen or held, 2**31 - 1),
-        1.0 / math.sqrt(D))
+        int(out is None), 1.0 / math.sqrt(D))
     qr = _ready(q)
     if D % 8 == 0 and _aligned(o):
         _native.forward_paged(cache._struct, batch, plan, qr, o)

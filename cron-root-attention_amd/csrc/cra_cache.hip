@@ -285,7 +285,7 @@ int check_cache(const cra_cache* c) {
   if (!c->k || !c->v || !c->k_norm) return err(CRA_E_INVALID, "cache: NULL pointer");
   if (c->store != CRA_STORE_SAME && (!c->k_scale || !c->v_scale))
     return err(CRA_E_INVALID, "an 8-bit cache needs scales");
-  if (misaligned(c->k, 16) || misaligned(c->v, 16) || misaligned(c->k_norm, 4) ||
+  if (misaligned(c->k, 16) || misaligned(c->v, 16) || misaligned(c->k_norm, 16) ||
       misaligned(c->k_scale, 4) || misaligned(c->v_scale, 4))
     return err(CRA_E_LAYOUT, "cache: misaligned pointer");
   return CRA_OK;

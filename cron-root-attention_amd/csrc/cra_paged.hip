@@ -12,7 +12,7 @@
 // Launches: select_kernel ranks the stored norms and lists the cache rows of
 // the global rows (sequences with relay only); few_kernel takes the sequences
 // whose rows (new tokens x query heads of a kv head) fit one 16-row MFMA block,
-// its waves and workgroups splitting the keys, joined by combine_kernel;
+// their keys cut into pieces of equal length, joined by combine_kernel;
 // chunk_kernel takes the others in tiles of 128 rows, the rows of a kv head's
 // query heads side by side so that a K/V tile serves them all. fp32 runs
 // f32_kernel for both.
@@ -49,13 +49,15 @@ struct PagedArgs {
   int Hq, grp, D, Ds;  // query heads, per kv head; columns of q and o; of a cache row
   int window, relay, top_k, max_len;
   float scale;
-  FastDiv d_grp, d_hkv, d_splits;
+  FastDiv d_grp, d_hkv, d_steps;
   uint32_t* list;  // [n_seqs, H_kv, list_cap] cache rows of the global rows (relay)
   int list_cap;
-  float* part;     // few_kernel, splits > 1: [n_seqs, H_kv, splits, part_rows, Dp], then (m, l)
+  float* part;     // few rows: O of shared sequences' pieces, [piece, part_rows, Dp], and (m, l)
   float* part_ml;
-  int splits, part_rows;
+  int32_t* pieces;  // [n_seqs + 1] first piece of each sequence (a kv head), for combine_kernel
+  int part_rows, few_grid;
   int few_only;    // no chunk_kernel follows: longer sequences are refused (NaN)
+  int zero_outside;  // rows of tokens outside every sequence are set to zero
   int tiles;       // chunk tiles of a sequence (batches without cu)
   FastDiv d_tiles;
 };
@@ -104,86 +106,253 @@ __device__ __forceinline__ T* o_row(const PagedArgs& a, const Seq& s, int hk, in
 }
 
 // ---------------------------------------------------------------------------
-// The global rows of sequences with relay, as cache rows. One wave a W-block:
-// its strided row, and behind it (blocks that end before the last query's
-// window) the top_k rows of largest norm, of equals the earlier; a slot without
-// a row left is the block's first row, as in the packed rows of whole
-// sequences. NaN norms are never chosen.
+// The global rows of sequences with relay, as cache rows: of each W-block its
+// first row, and behind it (blocks that end before the last query's window) the
+// top_k rows of largest norm, of equals the earlier; a slot without a row left
+// is the block's first row, as in the packed rows of whole sequences. NaN norms
+// are never chosen.
+//
+// A wave takes whole blocks. Bound by the VALU work a block (and below a few
+// thousand blocks by the latency of page table and norm loads, the next block's
+// of which are on their way): in select_kernel a lane loads the norms of eight
+// rows with one page lookup, keeps the KEEP largest values by maximum and median
+// of three, and a picked value's row is found by comparing the lane's eight with
+// it. Against carrying rows along with the values, 64 rows at a time
+// (select_wide_kernel), 16 sequences of 700-131072 tokens, 8 heads: 23 -> WIDE us.
+// A block must fit one load of the wave; wider ones (windows above 505) go to
+// select_wide_kernel.
 // ---------------------------------------------------------------------------
-constexpr int kSelWaves = 4;
+constexpr int kSelWaves = 4, kSelLoads = 8;
+constexpr int kSelMost = 64 * 8 - 7;   // rows of a block in select_kernel, at any alignment
 
-__device__ __forceinline__ uint64_t wave_max(uint64_t x) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    const uint32_t lo = __shfl_xor((uint32_t)x, o), hi = __shfl_xor((uint32_t)(x >> 32), o);
-    const uint64_t y = (uint64_t)hi << 32 | lo;
-    x = y > x ? y : x;
-  }
+// Maximum over the wave, and sums up to each lane, by row shifts and broadcasts in
+// the VALU (lanes without a source take 0).
+#define CRA_DPP(x, ctrl, rows) (uint32_t) __builtin_amdgcn_update_dpp(0, (int)(x), ctrl, rows, 0xf, false)
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+  x = max(x, CRA_DPP(x, 0x111, 0xf));  // row_shr:1, 2, 4, 8: the row's last lane has its maximum
+  x = max(x, CRA_DPP(x, 0x112, 0xf));
+  x = max(x, CRA_DPP(x, 0x114, 0xf));
+  x = max(x, CRA_DPP(x, 0x118, 0xf));
+  x = max(x, CRA_DPP(x, 0x142, 0xf));  // row_bcast:15, row_bcast:31
+  x = max(x, CRA_DPP(x, 0x143, 0xf));
+  return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+}
+__device__ __forceinline__ uint32_t wave_upto(uint32_t x) {
+  x += CRA_DPP(x, 0x111, 0xf);
+  x += CRA_DPP(x, 0x112, 0xf);
+  x += CRA_DPP(x, 0x114, 0xf);
+  x += CRA_DPP(x, 0x118, 0xf);
+  x += CRA_DPP(x, 0x142, 0xa);  // the row before, into rows 1 and 3
+  x += CRA_DPP(x, 0x143, 0xc);  // the half before, into rows 2 and 3
   return x;
 }
 
+// The blocks of a wave: [first, end) of sequence b's, head h.
+struct SelWork {
+  SeqPlan p;
+  int b, h, full, first, end;
+  uint32_t* out;
+};
+__device__ __forceinline__ SelWork sel_work(const PagedArgs& a, int steps) {
+  SelWork k{};
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t bh = div_by(blockIdx.x, a.d_steps);  // workgroups a (sequence, head)
+  const int nw = steps * kSelWaves, w = (int)(blockIdx.x - bh * steps) * kSelWaves + wave;
+  k.b = (int)div_by(bh, a.d_hkv);
+  k.h = (int)(bh - (uint32_t)k.b * a.c.H_kv);
+  const Seq s = get_seq(a, k.b);
+  k.p = get_plan(a, s.n);
+  if (k.p.rpb == 1 || s.m < 1) return k;
+  const int ls = s.n - k.p.W > 0 ? s.n - k.p.W : 0;  // window start of the last query
+  k.full = ls / k.p.W;
+  const int blocks = k.full + (ls != k.full * k.p.W ? 1 : 0), per = (blocks + nw - 1) / nw;
+  k.first = w * per;
+  k.end = min(blocks, (w + 1) * per);
+  k.out = a.list + (int64_t)bh * a.list_cap;
+  return k;
+}
+
+__device__ __forceinline__ int wave_max_signed(int x) {  // at least -1
+  return (int)wave_max((uint32_t)(x + 1)) - 1;
+}
+
+template <int KEEP>
 __global__ __launch_bounds__(64 * kSelWaves) void select_kernel(PagedArgs a, int steps) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint32_t bh = div_by(blockIdx.x, a.d_splits);  // d_splits: blocks a (sequence, head)
-  const int first = (int)(blockIdx.x - bh * steps) * kSelWaves + wave;
-  const int b = (int)div_by(bh, a.d_hkv), h = (int)(bh - (uint32_t)b * a.c.H_kv);
-  const Seq s = get_seq(a, b);
-  const SeqPlan p = get_plan(a, s.n);
-  if (p.rpb == 1 || s.m < 1) return;
-  const int ls = s.n - p.W > 0 ? s.n - p.W : 0;  // window start of the last query
-  const int full = ls / p.W, blocks = full + (ls != full * p.W ? 1 : 0);
-  const int32_t* pages = a.c.table + b * a.c.table_stride;
-  uint32_t* out = a.list + (int64_t)bh * a.list_cap;
-  auto row_at = [&](int row) {
-    return seq_row(pages, row, a.c.num_pages, a.c.H_kv, a.c.log_page, h);
+  const int lane = threadIdx.x & 63;
+  const SelWork w = sel_work(a, steps);
+  if (w.first >= w.end) return;
+  const int W = w.p.W;
+  const int32_t* pages = a.c.table + w.b * a.c.table_stride;
+  // cache row of logical row 8 (first row / 8 + lane): eight rows of one page;
+  // lanes behind the last eight (of the block, or of the sequence) repeat it
+  auto load_row = [&](int blk) -> uint32_t {
+    const int last = min(blk * W + W - 1, w.p.n - 1);
+    if (blk >= w.end) return 0u;
+    return seq_row(pages, min((blk * W & ~7) + 8 * lane, last & ~7), a.c.num_pages, a.c.H_kv,
+                   a.c.log_page, w.h);
   };
-  for (int r = first; r < blocks; r += steps * kSelWaves) {
-    const int row0 = r * p.W;
-    uint32_t mine = kNoRow;  // lane j: list entry j of the block
-    if (lane == 0) mine = row_at(row0);
-    if (r < full) {
-      // each lane keeps the top four of its rows (which rise)
-      uint64_t key[4] = {0, 0, 0, 0};
-      bool bad = false;
-      constexpr int kU = 4;
-      for (int base = 0; base < p.W; base += 64 * kU) {
-        uint32_t at[kU];
-        float x[kU];
+  struct Eight {
+    float4 lo, hi;
+  };
+  auto load_norms = [&](int blk, uint32_t at) -> Eight {
+    if (blk >= w.end) return Eight{};
+    const float4* p = reinterpret_cast<const float4*>(a.c.k_norm + (at == kNoRow ? 0u : at));
+    return Eight{p[0], p[1]};
+  };
+  uint32_t at = load_row(w.first), at1 = load_row(w.first + 1);
+  Eight x = load_norms(w.first, at);
+  for (int blk = w.first; blk < w.end; ++blk) {
+    const Eight x1 = load_norms(blk + 1, at1);
+    const uint32_t at2 = load_row(blk + 2);
+    const int lead = blk * W & 7;
+    // cache row of the block's row i, from the lane that looked it up
+    auto slot_of = [&](int i) -> uint32_t {
+      const uint32_t q = (uint32_t)__builtin_amdgcn_readlane((int)at, (i + lead) >> 3);
+      return q == kNoRow ? kNoRow : q + ((i + lead) & 7);
+    };
+    uint32_t mine = slot_of(0);  // lane e: entry e of the block
+    if (blk < w.full) {
+      // a norm's bits, which order as the norms do; negative: not a row of the
+      // block, or NaN
+      int key[8], top[KEEP];
+      const float f[8] = {x.lo.x, x.lo.y, x.lo.z, x.lo.w, x.hi.x, x.hi.y, x.hi.z, x.hi.w};
 #pragma unroll
-        for (int u = 0; u < kU; ++u)
-          at[u] = row_at(row0 + min(base + 64 * u + lane, p.W - 1));
+      for (int j = 0; j < KEEP; ++j) top[j] = -1;
 #pragma unroll
-        for (int u = 0; u < kU; ++u) {
-          bad |= at[u] == kNoRow;
-          x[u] = at[u] == kNoRow ? 0.f : a.c.k_norm[at[u]];
-        }
+      for (int j = 0; j < 8; ++j) {
+        const bool in = (uint32_t)(8 * lane + j - lead) < (uint32_t)W;
+        key[j] = in ? __float_as_int(fmaxf(f[j], -1.f)) : -1;
 #pragma unroll
-        for (int u = 0; u < kU; ++u) {
-          const int i = base + 64 * u + lane;
-          if (i >= p.W || !(x[u] >= 0.f)) continue;
-          uint64_t k = (uint64_t)(__float_as_uint(x[u]) | 0x80000000u) << 32 | (uint32_t)~(uint32_t)i;
+        for (int t = KEEP - 1; t >= 1; --t)  // median of three
+          top[t] = max(min(top[t - 1], key[j]), min(max(top[t - 1], key[j]), top[t]));
+        top[0] = max(top[0], key[j]);
+      }
+      const bool bad = __any(at == kNoRow);
+      for (int j = 0; j < a.top_k; ++j) {
+        const int m = wave_max_signed(max(top[0], -1));
+        int pick = 0;
+        if (m >= 0) {
+          const int l = __builtin_ctzll(__ballot(top[0] == m));  // lanes rise with their rows
+          int e = 7;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint64_t old = key[j];
-            key[j] = k > old ? k : old;
-            k = k > old ? old : k;
+          for (int i = 6; i >= 0; --i) e = key[i] == m ? i : e;
+          e = __builtin_amdgcn_readlane(e, l);
+          pick = 8 * l + e - lead;
+          if (lane == l) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) key[i] = i == e ? -1 : key[i];
+#pragma unroll
+            for (int i = 0; i + 1 < KEEP; ++i) top[i] = top[i + 1];
+            top[KEEP - 1] = -1;
           }
         }
-      }
-      const bool any_bad = __any(bad);
-      for (int j = 0; j < a.top_k; ++j) {
-        const uint64_t m = wave_max(key[0]);
-        const int i = m ? (int)~(uint32_t)m : 0;
-        if (m && key[0] == m) {  // keys differ in their rows: one lane has it
-          key[0] = key[1];
-          key[1] = key[2];
-          key[2] = key[3];
-          key[3] = 0;
-        }
-        if (lane == 1 + j) mine = any_bad ? kNoRow : row_at(row0 + i);
+        const uint32_t slot = bad ? kNoRow : slot_of(pick);
+        mine = lane == 1 + j ? slot : mine;
       }
     }
-    if (lane < (r < full ? p.rpb : 1)) out[(int64_t)p.rpb * r + lane] = mine;
+    if (lane < (blk < w.full ? w.p.rpb : 1)) w.out[(int64_t)w.p.rpb * blk + lane] = mine;
+    at = at1, at1 = at2, x = x1;
+  }
+}
+
+template <int KEEP>
+__global__ __launch_bounds__(64 * kSelWaves) void select_wide_kernel(PagedArgs a, int steps) {
+  const int lane = threadIdx.x & 63;
+  const SelWork w = sel_work(a, steps);
+  if (w.first >= w.end) return;
+  const SeqPlan p = w.p;
+  const int full = w.full, first = w.first, end = w.end;
+  const int32_t* pages = a.c.table + w.b * a.c.table_stride;
+  auto row_at = [&](int row) {
+    return seq_row(pages, row, a.c.num_pages, a.c.H_kv, a.c.log_page, w.h);
+  };
+  constexpr int kPiece = 64 * kSelLoads;
+  auto load_rows = [&](int blk, int base, uint32_t (&at)[kSelLoads]) {
+#pragma unroll
+    for (int u = 0; u < kSelLoads; ++u)
+      at[u] = blk < min(end, full) && base + 64 * u < p.W  // whole wave
+                  ? row_at(blk * p.W + min(base + 64 * u + lane, p.W - 1))
+                  : 0u;
+  };
+  auto load_norms = [&](int blk, int base, const uint32_t (&at)[kSelLoads], float (&x)[kSelLoads]) {
+#pragma unroll
+    for (int u = 0; u < kSelLoads; ++u)
+      x[u] = blk < min(end, full) && base + 64 * u < p.W && at[u] != kNoRow ? a.c.k_norm[at[u]] : -1.f;
+  };
+  auto advance = [&](int& blk, int& base) {
+    base += kPiece;
+    if (base >= p.W) ++blk, base = 0;
+  };
+  uint32_t at[kSelLoads], at2[kSelLoads];
+  float x[kSelLoads];
+  int blk = first, base = 0, blk1 = first, base1 = 0;
+  load_rows(blk, base, at);
+  load_norms(blk, base, at, x);
+  advance(blk1, base1);
+  load_rows(blk1, base1, at2);
+  uint32_t key[KEEP];  // norm's bits + 1, falling; 0: none
+  int row[KEEP];
+  bool bad = false;
+#pragma unroll
+  for (int j = 0; j < KEEP; ++j) key[j] = 0, row[j] = 0;
+  while (blk < end) {
+    float xn[kSelLoads];
+    uint32_t atn[kSelLoads];
+    int blk2 = blk1, base2 = base1;
+    load_norms(blk1, base1, at2, xn);
+    advance(blk2, base2);
+    load_rows(blk2, base2, atn);
+#pragma unroll
+    for (int u = 0; u < kSelLoads; ++u) {
+      if (base + 64 * u >= p.W) break;  // whole wave
+      const int i = base + 64 * u + lane;
+      bad |= at[u] == kNoRow;
+      uint32_t k = i < p.W && x[u] >= 0.f ? __float_as_uint(x[u]) + 1 : 0u;
+      int ri = i;
+#pragma unroll
+      for (int j = 0; j < KEEP; ++j) {  // rows rise: of equals the earlier stays
+        const bool up = k > key[j];
+        const uint32_t ok = key[j];
+        const int orow = row[j];
+        key[j] = up ? k : ok;
+        row[j] = up ? ri : orow;
+        k = up ? ok : k;
+        ri = up ? orow : ri;
+      }
+    }
+    if (base + kPiece >= p.W || blk >= full) {  // the block is complete
+      const bool any_bad = __any(bad);
+      int mine = 0;  // lane e: entry e of the block
+      for (int j = 0; j < a.top_k; ++j) {
+        const uint32_t m = wave_max(key[0]);
+        int pick = 0;
+        if (m) {
+          uint64_t eq = __ballot(key[0] == m);
+          int l = __builtin_ctzll(eq);
+          pick = __builtin_amdgcn_readlane(row[0], l);
+          for (eq &= eq - 1; eq; eq &= eq - 1) {  // equal norms: the earliest row
+            const int l2 = __builtin_ctzll(eq);
+            const int other = __builtin_amdgcn_readlane(row[0], l2);
+            if (other < pick) pick = other, l = l2;
+          }
+          if (lane == l) {
+#pragma unroll
+            for (int i = 0; i + 1 < KEEP; ++i) key[i] = key[i + 1], row[i] = row[i + 1];
+            key[KEEP - 1] = 0;
+          }
+        }
+        if (lane == 1 + j) mine = any_bad ? -1 : pick;
+      }
+      if (lane < (blk < full ? p.rpb : 1))
+        w.out[(int64_t)p.rpb * blk + lane] = mine < 0 ? kNoRow : row_at(blk * p.W + mine);
+      bad = false;
+#pragma unroll
+      for (int j = 0; j < KEEP; ++j) key[j] = 0, row[j] = 0;
+    }
+#pragma unroll
+    for (int u = 0; u < kSelLoads; ++u) at[u] = at2[u], at2[u] = atn[u], x[u] = xn[u];
+    blk = blk1, base = base1;
+    blk1 = blk2, base1 = base2;
   }
 }
 
@@ -299,13 +468,114 @@ __device__ __forceinline__ void pv_not_finite(V v, const Frag<T> (&pf)[QB], f32x
 }
 
 // ---------------------------------------------------------------------------
-// Few rows: at most 16 rows a (sequence, kv head). Each wave takes whole 32-key
-// tiles of its own, filled with per-lane addresses straight into its part of
-// LDS (a row of a page is contiguous, rows lie anywhere), two stages deep, with
-// no barrier until the end; the 16-column operand Q^T holds the rows. Bound by
-// memory: the rows seen, once per kv head. The waves' results, and those of the
-// `splits` workgroups that share a sequence's keys, are joined by their maxima.
+// Few rows: at most 16 rows a (sequence, kv head). The keys of all sequences are
+// cut into pieces of equal length, as many as keep the resident workgroups busy
+// about twice over; each workgroup takes pieces from the grid's stride, each
+// wave of it whole 32-key tiles, filled with per-lane addresses straight into
+// its part of LDS (a row of a page is contiguous, rows lie anywhere), with no
+// barrier until the piece's end; the 16-column operand Q^T holds the rows.
+// Bound by memory latency and bandwidth: the rows seen, once per kv head. The
+// waves' results, and those of a sequence's pieces, are joined by their maxima.
 // ---------------------------------------------------------------------------
+constexpr int kFewWaves = 4;
+
+// 32-key tiles of a sequence that few rows attend (0: it has no new tokens, or
+// more rows than the kernel takes), found out from the device's lengths.
+struct FewTiles {
+  int tiles;
+  bool mine;  // takes at least one piece
+};
+__device__ __forceinline__ FewTiles few_tiles(const PagedArgs& a, int b) {
+  const Seq s = get_seq(a, b);
+  const int64_t rows = (int64_t)s.m * a.grp;
+  // more rows than the caller's bound: one piece, which answers NaN
+  if (rows == 0 || (rows > a.part_rows && !a.few_only)) return FewTiles{0, false};
+  if (rows > a.part_rows) return FewTiles{0, true};
+  const SeqPlan p = get_plan(a, s.n);
+  const int G = s.n > 0 ? seq_prefix(s.n - 1, p) : 0;
+  const int lo = max(0, max(s.n - s.m, 0) - p.W + 1);
+  return FewTiles{((G + 31) >> 5) + ((s.n - lo + 31) >> 5), true};
+}
+// The pieces of the call: tiles a piece, and pieces a kv head. Every wave adds
+// the sequences up, 64 at a time; the first 64 stay in registers (lane b).
+struct FewPieces {
+  int per, total;
+  int n, upto;  // of sequence `lane`: pieces, and pieces up to its last
+};
+__device__ __forceinline__ int few_count(const FewTiles& t, int per) {
+  return t.mine ? max(1, (t.tiles + per - 1) / per) : 0;
+}
+__device__ __forceinline__ FewPieces few_pieces(const PagedArgs& a) {
+  const int lane = threadIdx.x & 63;
+  FewTiles t0{0, false};
+  int64_t tiles = 0;
+  for (int base = 0; base < a.c.n_seqs; base += 64) {
+    FewTiles t{0, false};
+    if (base + lane < a.c.n_seqs) t = few_tiles(a, base + lane);
+    if (base == 0) t0 = t;
+    tiles += (uint32_t)__builtin_amdgcn_readlane((int)wave_upto(t.tiles), 63);
+  }
+  // at most 2 few_grid pieces of whole length, and one short one a sequence
+  const int64_t per = (tiles * a.c.H_kv + 2 * a.few_grid - 1) / (2 * a.few_grid);
+  FewPieces f{};
+  f.per = (int)min(max(per, (int64_t)1) + kFewWaves - 1, (int64_t)1 << 28) / kFewWaves * kFewWaves;
+  for (int base = 0; base < a.c.n_seqs; base += 64) {
+    FewTiles t = t0;
+    if (base > 0) {
+      t = FewTiles{0, false};
+      if (base + lane < a.c.n_seqs) t = few_tiles(a, base + lane);
+    }
+    const int n = few_count(t, f.per), upto = f.total + (int)wave_upto(n);
+    if (base == 0) f.n = n, f.upto = upto;
+    if (blockIdx.x == 0 && threadIdx.x < 64 && base + lane < a.c.n_seqs) a.pieces[base + lane] = upto - n;
+    f.total = __builtin_amdgcn_readlane(upto, 63);
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.pieces[a.c.n_seqs] = f.total;
+  return f;
+}
+// Sequence of piece `idx` of a kv head, which of its pieces it is, and whether
+// it is its only one.
+struct FewPiece {
+  int b, piece;
+  bool only;
+};
+__device__ __forceinline__ FewPiece few_piece(const PagedArgs& a, const FewPieces& f, int idx) {
+  const int lane = threadIdx.x & 63;
+  int n = f.n, upto = f.upto;
+  for (int base = 0;;) {
+    const uint64_t hit = __ballot(upto > idx);
+    if (hit) {
+      const int l = __builtin_ctzll(hit), mine = __builtin_amdgcn_readlane(n, l);
+      return FewPiece{base + l, idx - (__builtin_amdgcn_readlane(upto, l) - mine), mine == 1};
+    }
+    base += 64;
+    if (base >= a.c.n_seqs) return FewPiece{-1, 0, false};
+    const int before = __builtin_amdgcn_readlane(upto, 63);
+    FewTiles t{0, false};
+    if (base + lane < a.c.n_seqs) t = few_tiles(a, base + lane);
+    n = few_count(t, f.per);
+    upto = before + (int)wave_upto(n);
+  }
+}
+
+// Rows of tokens before the first and behind the last sequence: zeros, shared by
+// the grid's workgroups (a fresh output; the caller's own is left as it is).
+template <typename T>
+__device__ __forceinline__ void zero_outside(const PagedArgs& a, int threads) {
+  if (!a.zero_outside || !a.c.cu) return;
+  const int first = token_range(a.c.cu, 0, a.c.tokens).first;
+  const int last = token_range(a.c.cu, a.c.n_seqs - 1, a.c.tokens).last;
+  const int64_t outside = (int64_t)first + a.c.tokens - last, quads = a.D / 4;
+  const int64_t all = outside * a.Hq * quads;
+  for (int64_t i = (int64_t)blockIdx.x * threads + threadIdx.x; i < all; i += (int64_t)gridDim.x * threads) {
+    const int64_t row = i / quads;
+    const int64_t tok = row / a.Hq, t = tok < first ? tok : last + (tok - first);
+    T* p = static_cast<T*>(a.o) + (row - tok * a.Hq) * a.osh + t * a.oss + (i - row * quads) * 4;
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<t4*>(p) = t4{(T)0.f, (T)0.f, (T)0.f, (T)0.f};
+  }
+}
+
 // ROWS rows of RB bytes, 16-byte chunks XOR-swizzled as in SwzTile.
 template <int RB, int ROWS>
 struct ByteTile {
@@ -320,50 +590,52 @@ struct ByteTile {
   }
 };
 
-constexpr int kFewWaves = 4;
-template <int D, int STORE>
-constexpr int kFewStages = D * (STORE == kSame ? 2 : 1) > 256 ? 1 : 2;
-
 // All of the wave's loads have landed (in LDS too) and its LDS reads are done; no
 // memory access moves across.
 __device__ __forceinline__ void wait_all() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
 
 template <typename T, int STORE, int D>
-__global__ __launch_bounds__(64 * kFewWaves) void few_kernel(PagedArgs a) {
-  constexpr int NW = kFewWaves, NS = kFewStages<D, STORE>;
+__global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(D > 128 ? 1 : 2)))
+void few_kernel(PagedArgs a) {
+  constexpr int NW = kFewWaves;
   constexpr int ES = STORE == kSame ? 2 : 1;
   using Tile = ByteTile<D * ES, 32>;
-  // the stages as objects of their own, so that reads of one do not wait for the fill of the other
-  __shared__ __attribute__((aligned(1024))) char stage0[NW][2][Tile::kBytes];
-  __shared__ __attribute__((aligned(1024))) char stage1[NS == 2 ? NW : 1][2][NS == 2 ? Tile::kBytes : 16];
+  __shared__ __attribute__((aligned(1024))) char stage[NW][2][Tile::kBytes];
   __shared__ float scales[NW][64];
   __shared__ float join_ml[NW][kFewRows][2];
 
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t bh = div_by(blockIdx.x, a.d_splits);
-  const int split = (int)(blockIdx.x - bh * a.splits);
-  const int b = (int)div_by(bh, a.d_hkv), hk = (int)(bh - (uint32_t)b * a.c.H_kv);
+  const int row_bytes = a.Ds * ES;
+  zero_outside<T>(a, 64 * NW);
+  const FewPieces fp = few_pieces(a);
+  for (int64_t item = blockIdx.x; item < (int64_t)fp.total * a.c.H_kv; item += gridDim.x) {
+  const uint32_t idx = div_by((uint32_t)item, a.d_hkv);
+  const int hk = (int)((uint32_t)item - idx * a.c.H_kv);
+  const FewPiece fi = few_piece(a, fp, (int)idx);
+  const int b = fi.b;
+  if (b < 0) break;
   const Seq s = get_seq(a, b);
   const int64_t rows64 = (int64_t)s.m * a.grp;
-  if (rows64 == 0) return;
-  if (rows64 > a.part_rows) {  // kFewRows, or fewer by the caller's bound
-    if (a.few_only && split == 0)  // more new tokens than the caller's bound
-      for (int64_t i = tid; i < rows64 * a.D; i += 64 * NW) {
-        const int r = (int)(i / a.D);
-        o_row<T>(a, s, hk, r)[i - (int64_t)r * a.D] = from_f32<T>(__builtin_nanf(""));
-      }
-    return;
+  if (rows64 > a.part_rows) {  // more new tokens than the caller's bound
+    for (int64_t i = tid; i < rows64 * a.D; i += 64 * NW) {
+      const int r = (int)(i / a.D);
+      o_row<T>(a, s, hk, r)[i - (int64_t)r * a.D] = from_f32<T>(__builtin_nanf(""));
+    }
+    continue;
   }
   const int rows = (int)rows64;
   const SeqPlan p = get_plan(a, s.n);
   const int pos0 = s.n - s.m;  // of the first new token
   const int G = s.n > 0 ? seq_prefix(s.n - 1, p) : 0;
   const int lo = max(0, max(pos0, 0) - p.W + 1);
-  const int nG = (G + 31) >> 5, nT = nG + ((s.n - lo + 31) >> 5);
+  const int nG = (G + 31) >> 5, nAll = nG + ((s.n - lo + 31) >> 5);
+  const int nT = min(nAll, (fi.piece + 1) * fp.per);  // the piece's tiles end here
   const int32_t* pages = a.c.table + b * a.c.table_stride;
-  const uint32_t* list = a.list + (int64_t)bh * a.list_cap;
+  const uint32_t* list = a.list + ((int64_t)b * a.c.H_kv + hk) * a.list_cap;
   bool bad = s.over;
+  const int step = NW;
+  int it = fi.piece * fp.per + wave;
 
   // cache row of the tile's row lane % 32
   auto slot_of = [&](int it) -> uint32_t {
@@ -376,7 +648,6 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(PagedArgs a) {
     const int i = min(lo + (it - nG) * 32 + ko, s.n - 1);
     return seq_row(pages, i, a.c.num_pages, a.c.H_kv, a.c.log_page, hk);
   };
-  const int row_bytes = a.Ds * ES;
   auto fill = [&](char (&dst)[2][Tile::kBytes], uint32_t slot) {
 #pragma unroll
     for (int i = 0; i < Tile::kInstr; ++i) {
@@ -401,20 +672,16 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(PagedArgs a) {
     return slot == kNoRow ? 0u : slot;
   };
 
-  const int step = a.splits * NW;
-  int it = split * NW + wave;
   if (D * ES > row_bytes) {  // columns that no load fills
-    for (int i = lane; i < 2 * Tile::kBytes / 16; i += 64) {
-      reinterpret_cast<uint4*>(stage0[wave])[i] = make_uint4(0, 0, 0, 0);
-      if constexpr (NS == 2) reinterpret_cast<uint4*>(stage1[wave])[i] = make_uint4(0, 0, 0, 0);
-    }
+    for (int i = lane; i < 2 * Tile::kBytes / 16; i += 64)
+      reinterpret_cast<uint4*>(stage[wave])[i] = make_uint4(0, 0, 0, 0);
     wait_all();  // before loads to the same memory
   }
   float sc = 0.f;
   uint32_t next = 0;
   if (it < nT) {
     const uint32_t first = checked(slot_of(it));
-    fill(stage0[wave], first);
+    fill(stage[wave], first);
     sc = load_scale(first);
     if (it + step < nT) next = slot_of(it + step);
   }
@@ -547,35 +814,16 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(PagedArgs a) {
         acc[db][0] = mma(acc[db][0], v_frag(db), pf[0]);
     }
   };
-  auto turn = [&](auto second) __attribute__((always_inline)) {
-    constexpr bool kSecond = decltype(second)::value && NS == 2;
+  for (; it < nT; it += step) {
     wait_all();
-    const float sc_now = sc;
-    const bool more = it + step < nT;
-    auto refill = [&](char (&dst)[2][Tile::kBytes]) {
+    attend(stage[wave], it, sc);
+    wait_all();  // LDS reads are done before the loads that overwrite
+    if (it + step < nT) {
       const uint32_t slot = checked(next);
-      fill(dst, slot);
+      fill(stage[wave], slot);
       sc = load_scale(slot);
       if (it + 2 * step < nT) next = slot_of(it + 2 * step);
-    };
-    if constexpr (NS == 2) {
-      if constexpr (kSecond) {
-        if (more) refill(stage0[wave]);
-        attend(stage1[wave], it, sc_now);
-      } else {
-        if (more) refill(stage1[wave]);
-        attend(stage0[wave], it, sc_now);
-      }
-    } else {
-      attend(stage0[wave], it, sc_now);
-      wait_all();
-      if (more) refill(stage0[wave]);
     }
-    it += step;
-  };
-  while (it < nT) {
-    turn(std::false_type{});
-    if (it < nT) turn(std::true_type{});
   }
 
   // join the waves
@@ -583,8 +831,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(PagedArgs a) {
   if (__any(bad)) l_run = __builtin_nanf("");
   __syncthreads();
   // the tiles' memory holds the waves' O now: [wave][row][D], quads swizzled by row
-  static_assert(sizeof(float) * NW * kFewRows * D <= sizeof(stage0), "join area");
-  f32x4* join_o = reinterpret_cast<f32x4*>(&stage0[0][0][0]);
+  static_assert(sizeof(float) * NW * kFewRows * D <= sizeof(stage), "join area");
+  f32x4* join_o = reinterpret_cast<f32x4*>(&stage[0][0][0]);
   auto join_at = [](int w, int r, int quad) {
     return (w * kFewRows + r) * (D / 4) + (quad ^ (r & (D / 4 - 1)));
   };
@@ -609,7 +857,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(PagedArgs a) {
       L += e * join_ml[w][r][1];
       o += join_o[join_at(w, r, c / 4)] * e;
     }
-    if (a.splits == 1) {
+    if (fi.only) {
       if (c >= a.D) continue;
       const float inv = L == 0.f ? 0.f : 1.f / L;
       T e[4];
@@ -617,7 +865,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(PagedArgs a) {
       for (int j = 0; j < 4; ++j) e[j] = from_f32<T>(o[j] * inv);
       *reinterpret_cast<uint2*>(o_row<T>(a, s, hk, r) + c) = *reinterpret_cast<const uint2*>(e);
     } else {
-      const int64_t at = ((int64_t)bh * a.splits + split) * a.part_rows + r;
+      const int64_t at = item * a.part_rows + r;
       *reinterpret_cast<f32x4*>(a.part + at * D + c) = o;
       if (c == 0) {
         a.part_ml[2 * at] = M;
@@ -625,9 +873,12 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(PagedArgs a) {
       }
     }
   }
+  __syncthreads();  // the join area is the next piece's tiles
+  }
 }
 
-// Joins the splits of few rows: one workgroup a (sequence, kv head, row).
+// Joins the pieces of sequences that have more than one: one workgroup a
+// (sequence, kv head, row), its threads 4 columns each of some of the pieces.
 template <typename T>
 __global__ __launch_bounds__(256) void combine_kernel(PagedArgs a, int Dp) {
   __shared__ float red[256][4];
@@ -636,22 +887,24 @@ __global__ __launch_bounds__(256) void combine_kernel(PagedArgs a, int Dp) {
   const int r = blockIdx.x % a.part_rows;
   const uint32_t bh = blockIdx.x / a.part_rows;
   const int b = (int)div_by(bh, a.d_hkv), hk = (int)(bh - (uint32_t)b * a.c.H_kv);
+  const int first = a.pieces[b], n = a.pieces[b + 1] - first;
+  if (n < 2) return;
   const Seq s = get_seq(a, b);
-  const int64_t rows = (int64_t)s.m * a.grp;
-  if (rows > a.part_rows || r >= rows) return;
-  const int quads = Dp / 4, lanes = 256 / quads;  // split groups
+  if (r >= (int64_t)s.m * a.grp) return;
+  const int quads = Dp / 4, lanes = 256 / quads;  // groups of pieces
   const int quad = tid % quads, sg = tid / quads;
-  const float* ml = a.part_ml + 2 * ((int64_t)bh * a.splits * a.part_rows + r);
-  const float* po = a.part + ((int64_t)bh * a.splits * a.part_rows + r) * Dp + quad * 4;
+  auto at = [&](int i) { return ((int64_t)(first + i) * a.c.H_kv + hk) * a.part_rows + r; };
   float M = -kInf;
-  for (int i = 0; i < a.splits; ++i) M = fmaxf(M, ml[(int64_t)2 * i * a.part_rows]);
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) M = fmaxf(M, a.part_ml[2 * at(i)]);
   float L = 0.f;
   f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int i = sg; i < a.splits; i += lanes) {
-    const float mi = ml[(int64_t)2 * i * a.part_rows];
+#pragma unroll 2
+  for (int i = sg; i < n; i += lanes) {
+    const float mi = a.part_ml[2 * at(i)];
     const float e = mi == -kInf ? 0.f : __builtin_amdgcn_exp2f(mi - M);
-    L += e * ml[(int64_t)2 * i * a.part_rows + 1];
-    o += *reinterpret_cast<const f32x4*>(po + (int64_t)i * a.part_rows * Dp) * e;
+    L += e * a.part_ml[2 * at(i) + 1];
+    o += *reinterpret_cast<const f32x4*>(a.part + at(i) * Dp + quad * 4) * e;
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) red[tid][j] = o[j];
@@ -693,21 +946,15 @@ __device__ __forceinline__ void find_tile(const PagedArgs& a, int item, int& b, 
       const int64_t rows = (int64_t)(t.last - t.first) * a.grp;
       count = rows > kFewRows ? (int)((rows + BM - 1) / BM) : 0;
     }
-    int upto = count;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int x = __shfl_up(upto, o);
-      if (lane >= o) upto += x;
-    }
-    const uint64_t hit = __ballot(before + upto > item);
+    const int upto = before + (int)wave_upto(count);
+    const uint64_t hit = __ballot(upto > item);
     if (hit) {
       const int l = __builtin_ctzll(hit);
-      const int end = before + __shfl(upto, l);
       b = base + l;
-      tile = end - 1 - item;
+      tile = __builtin_amdgcn_readlane(upto, l) - 1 - item;
       return;
     }
-    before += __shfl(upto, 63);
+    before = __builtin_amdgcn_readlane(upto, 63);
   }
 }
 
@@ -1003,40 +1250,18 @@ __device__ __forceinline__ f32x4 mma4(f32x4 c, float x, float y) {
 
 constexpr int kF32Rows = 64, kF32Keys = 32;
 
-template <int STORE, int D, bool FEW>
-__global__ __launch_bounds__(256) void f32_kernel(PagedArgs a) {
+// One work item: rows r0.. of a (sequence, kv head) over its key tiles from
+// t_first up to t_end; the result goes to o, or (part_at >= 0) to the partial rows.
+template <int STORE, int D>
+__device__ void f32_item(const PagedArgs& a, const Seq& s, int b, int hk, int r0, int t_first, int t_end,
+                         int64_t part_at) {
   constexpr int BN = kF32Keys, kStride = D + 4;
   __shared__ __attribute__((aligned(16))) float tK[BN][kStride];
   __shared__ __attribute__((aligned(16))) float tV[BN][kStride];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, g = lane >> 4;
-  int b, tile = 0, hk, split = 0, nsplit = 1;
-  if constexpr (FEW) {
-    const uint32_t bh = div_by(blockIdx.x, a.d_splits);
-    split = (int)(blockIdx.x - bh * a.splits);
-    nsplit = a.splits;
-    b = (int)div_by(bh, a.d_hkv);
-    hk = (int)(bh - (uint32_t)b * a.c.H_kv);
-  } else {
-    const uint32_t item = div_by(blockIdx.x, a.d_hkv);
-    hk = (int)(blockIdx.x - item * a.c.H_kv);
-    find_tile<kF32Rows>(a, (int)item, b, tile);
-    if (b < 0) return;
-  }
-  const Seq s = get_seq(a, b);
-  const int64_t rows64 = (int64_t)s.m * a.grp;
-  if (rows64 == 0) return;
-  if (FEW && rows64 > a.part_rows) {
-    if (a.few_only && split == 0)
-      for (int64_t i = tid; i < rows64 * a.D; i += 256) {
-        const int r = (int)(i / a.D);
-        o_row<float>(a, s, hk, r)[i - (int64_t)r * a.D] = __builtin_nanf("");
-      }
-    return;
-  }
-  const int rows = (int)rows64;
-  if (!FEW && (rows <= kFewRows || tile * kF32Rows >= rows)) return;
+  const int rows = s.m * a.grp, q0 = r0 + 16 * wave;
   const SeqPlan p = get_plan(a, s.n);
-  const int pos0 = s.n - s.m, r0 = tile * kF32Rows, q0 = r0 + 16 * wave;
+  const int pos0 = s.n - s.m;
   auto pos_of = [&](int r) { return pos0 + row_token(a, r); };
   const int wg_first = pos_of(r0), wg_last = pos_of(min(r0 + kF32Rows, rows) - 1);
   const int lo_k = max(0, wg_first - p.W + 1), hi = max(0, wg_last + 1);
@@ -1090,7 +1315,8 @@ __global__ __launch_bounds__(256) void f32_kernel(PagedArgs a) {
       *reinterpret_cast<f32x4*>(&tV[frow][fcol + 32 * j]) = rv[j];
     }
   };
-  if (split < ntot) load(split);
+  const int t_last = min(t_end, ntot);
+  if (t_first < t_last) load(t_first);
 
   const int r = q0 + l16;
   const bool have = r < rows, active = q0 < rows;
@@ -1112,11 +1338,11 @@ __global__ __launch_bounds__(256) void f32_kernel(PagedArgs a) {
 #pragma unroll
   for (int db = 0; db < D / 16; ++db) acc[db] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  for (int it = split; it < ntot; it += nsplit) {
+  for (int it = t_first; it < t_last; ++it) {
     __syncthreads();  // every wave is done with the previous tile
     store();
     __syncthreads();
-    if (it + nsplit < ntot) load(it + nsplit);
+    if (it + 1 < t_last) load(it + 1);
     const bool loc = it >= nglob;
     const int ts = loc ? lo_k + (it - nglob) * BN : it * BN;
     if (!(active && (loc ? ts <= last && ts + BN - 1 >= w_lo : ts < g_any))) continue;
@@ -1189,14 +1415,14 @@ __global__ __launch_bounds__(256) void f32_kernel(PagedArgs a) {
   l_run = group_sum(l_run);
   if (bad) l_run = __builtin_nanf("");
   if (!have) return;
-  if (!FEW || nsplit == 1) {
+  if (part_at < 0) {
     const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
     float* op = o_row<float>(a, s, hk, r);
 #pragma unroll
     for (int db = 0; db < D / 16; ++db)
       if (16 * db + 4 * g < a.D) *reinterpret_cast<f32x4*>(op + 16 * db + 4 * g) = acc[db] * inv;
   } else {
-    const int64_t at = (((int64_t)b * a.c.H_kv + hk) * a.splits + split) * a.part_rows + r;
+    const int64_t at = part_at + r;
 #pragma unroll
     for (int db = 0; db < D / 16; ++db)
       *reinterpret_cast<f32x4*>(a.part + at * D + 16 * db + 4 * g) = acc[db];
@@ -1204,6 +1430,41 @@ __global__ __launch_bounds__(256) void f32_kernel(PagedArgs a) {
       a.part_ml[2 * at] = m_run;
       a.part_ml[2 * at + 1] = l_run;
     }
+  }
+}
+
+template <int STORE, int D, bool FEW>
+__global__ __launch_bounds__(256) void f32_kernel(PagedArgs a) {
+  if constexpr (FEW) {
+    zero_outside<float>(a, 256);
+    const FewPieces fp = few_pieces(a);
+    for (int64_t item = blockIdx.x; item < (int64_t)fp.total * a.c.H_kv; item += gridDim.x) {
+      const uint32_t idx = div_by((uint32_t)item, a.d_hkv);
+      const int hk = (int)((uint32_t)item - idx * a.c.H_kv);
+      const FewPiece fi = few_piece(a, fp, (int)idx);
+      if (fi.b < 0) break;
+      const Seq s = get_seq(a, fi.b);
+      const int64_t rows = (int64_t)s.m * a.grp;
+      if (rows > a.part_rows) {  // more new tokens than the caller's bound
+        for (int64_t i = threadIdx.x; i < rows * a.D; i += 256) {
+          const int r = (int)(i / a.D);
+          o_row<float>(a, s, hk, r)[i - (int64_t)r * a.D] = __builtin_nanf("");
+        }
+        continue;
+      }
+      f32_item<STORE, D>(a, s, fi.b, hk, 0, fi.piece * fp.per, (fi.piece + 1) * fp.per,
+                         fi.only ? -1 : item * a.part_rows);
+    }
+  } else {
+    const uint32_t item = div_by(blockIdx.x, a.d_hkv);
+    const int hk = (int)(blockIdx.x - item * a.c.H_kv);
+    int b, tile;
+    find_tile<kF32Rows>(a, (int)item, b, tile);
+    if (b < 0) return;
+    const Seq s = get_seq(a, b);
+    const int64_t rows = (int64_t)s.m * a.grp;
+    if (rows <= kFewRows || (int64_t)tile * kF32Rows >= rows) return;
+    f32_item<STORE, D>(a, s, b, hk, tile * kF32Rows, 0, 0x7fffffff, -1);
   }
 }
 
@@ -1224,13 +1485,15 @@ int hip_err(hipError_t e, const char* where) {
 struct Launch {
   int grp, max_len, Dp;
   bool few, chunk;
-  bool list;
+  bool list, wide;        // relay rows are listed; blocks too wide for select_kernel
   int64_t list_cap;
   int sel_steps;          // select workgroups a (sequence, head)
-  int splits, part_rows;
+  int part_rows, few_grid;
+  bool join;              // a sequence's keys may be cut into pieces
   int64_t tiles;          // chunk workgroups a kv head
   int tiles_seq;          // of a sequence (batches without cu)
-  size_t list_bytes, part_bytes, ml_bytes;
+  size_t list_bytes, part_bytes, ml_bytes, piece_bytes;
+  size_t bytes() const { return list_bytes + part_bytes + ml_bytes + piece_bytes; }
 };
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
@@ -1271,19 +1534,28 @@ Launch plan_launch(const cra_cache* c, const cra_batch* b, const cra_paged_plan*
   const int64_t cap = p->window > 0 ? blocks : ceil_sqrt(l.max_len);
   l.list = sp.rpb > 1 && cap > 0;
   l.list_cap = l.list ? cap * sp.rpb : 0;
-  l.sel_steps = (int)std::min<int64_t>((cap + kSelWaves - 1) / kSelWaves, 4096);
+  l.wide = sp.W > kSelMost;  // no shorter sequence has wider blocks
   const int64_t bh = (int64_t)b->n_seqs * c->H_kv;
+  // a wave a block while that is at most 4096 workgroups: sixteen a CU hide the
+  // loads' latency, more of them cost their launch
+  l.sel_steps = (int)std::max<int64_t>(1, std::min<int64_t>((cap + kSelWaves - 1) / kSelWaves, 4096 / bh));
   l.list_bytes = up256(bh * l.list_cap * 4);
-  // few rows: about two workgroups a CU, each wave with at least one tile
-  const int64_t keys = blocks * sp.rpb + std::min<int64_t>((int64_t)sp.W + kFewRows, l.max_len);
-  const int64_t tiles = (keys + 31) / 32 + 1;
-  const int64_t share = f32 ? tiles : (tiles + 3) / 4;
-  l.splits = (int)std::max<int64_t>(1, std::min<int64_t>((2 * 256 + bh - 1) / bh, share));
-  if (!l.few) l.splits = 1;
   l.part_rows = (int)std::min<int64_t>(kFewRows, most_rows);
-  if (l.splits > 1) {
-    l.part_bytes = up256(bh * l.splits * l.part_rows * (int64_t)l.Dp * 4);
-    l.ml_bytes = up256(bh * l.splits * l.part_rows * 2 * 4);
+  if (l.few) {
+    // the workgroups that are resident at once (LDS and registers allow two to
+    // four a CU), but no more than there can be pieces of four tiles
+    const int64_t keys = blocks * sp.rpb + std::min<int64_t>((int64_t)sp.W + kFewRows, l.max_len);
+    const int64_t pieces = (keys / 32 + 2 + kFewWaves - 1) / kFewWaves;
+    const int lds = kFewWaves * 64 * l.Dp * (f32 ? 2 : c->store == CRA_STORE_SAME ? 2 : 1);
+    const int per_cu = lds > 80 * 1024 ? 1 : l.Dp >= 128 ? 2 : 4;
+    l.few_grid = (int)std::min<int64_t>(256 * per_cu, bh * pieces);
+    l.join = pieces > 1;
+    const int64_t most_pieces = bh + 2 * (int64_t)l.few_grid;  // few_pieces()
+    if (l.join) {
+      l.part_bytes = up256(most_pieces * l.part_rows * (int64_t)l.Dp * 4);
+      l.ml_bytes = up256(most_pieces * l.part_rows * 2 * 4);
+    }
+    l.piece_bytes = up256(((int64_t)b->n_seqs + 1) * 4);
   }
   const int BM = f32 ? kF32Rows : l.Dp > 128 ? 64 : 128;
   if (b->cu_seqlens) {
@@ -1315,11 +1587,11 @@ template <typename T, int STORE, int D>
 hipError_t launch_rows(const PagedArgs& a, const Launch& l, int64_t bh, hipStream_t st) {
   if (l.few) {
     if constexpr (std::is_same<T, float>::value)
-      f32_kernel<STORE, D, true><<<(uint32_t)(bh * l.splits), 256, 0, st>>>(a);
+      f32_kernel<STORE, D, true><<<(uint32_t)l.few_grid, 256, 0, st>>>(a);
     else
-      few_kernel<T, STORE, D><<<(uint32_t)(bh * l.splits), 64 * kFewWaves, 0, st>>>(a);
+      few_kernel<T, STORE, D><<<(uint32_t)l.few_grid, 64 * kFewWaves, 0, st>>>(a);
     if (hipError_t e = hipGetLastError()) return e;
-    if (l.splits > 1) {
+    if (l.join) {
       combine_kernel<T><<<(uint32_t)(bh * l.part_rows), 256, 0, st>>>(a, D);
       if (hipError_t e = hipGetLastError()) return e;
     }
@@ -1344,8 +1616,7 @@ extern "C" {
 
 size_t cra_fwd_paged_workspace_bytes(const cra_cache* c, const cra_batch* b, const cra_paged_plan* p) {
   if (check_paged(c, b, p)) return 0;
-  const Launch l = plan_launch(c, b, p);
-  return l.list_bytes + l.part_bytes + l.ml_bytes;
+  return plan_launch(c, b, p).bytes();
 }
 
 int cra_fwd_paged(const cra_cache* c, const cra_batch* b, const cra_paged_plan* p, cra_tensor q,
@@ -1358,7 +1629,7 @@ int cra_fwd_paged(const cra_cache* c, const cra_batch* b, const cra_paged_plan* 
       return err(CRA_E_LAYOUT, "rows of q and o must be 16-byte aligned");
   }
   const Launch l = plan_launch(c, b, p);
-  const size_t need = l.list_bytes + l.part_bytes + l.ml_bytes;
+  const size_t need = l.bytes();
   if (need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16))
     return err(CRA_E_INVALID, "workspace: NULL or misaligned pointer");
   if (workspace_bytes < need) {
@@ -1367,7 +1638,7 @@ int cra_fwd_paged(const cra_cache* c, const cra_batch* b, const cra_paged_plan* 
     return err(CRA_E_WORKSPACE, msg);
   }
   const int64_t bh = (int64_t)b->n_seqs * c->H_kv;
-  const int64_t most = std::max({bh * l.sel_steps, bh * l.splits, bh * l.part_rows, l.tiles * c->H_kv});
+  const int64_t most = std::max({bh * l.sel_steps, bh * l.part_rows, l.tiles * c->H_kv});
   if (most >= (int64_t)1 << 24) return err(CRA_E_INVALID, "too many sequences or rows for one launch");
   PagedArgs a{};
   a.c = paged_view(c, b);
@@ -1383,18 +1654,22 @@ int cra_fwd_paged(const cra_cache* c, const cra_batch* b, const cra_paged_plan* 
   a.list = reinterpret_cast<uint32_t*>(ws);
   a.part = reinterpret_cast<float*>(ws + l.list_bytes);
   a.part_ml = reinterpret_cast<float*>(ws + l.list_bytes + l.part_bytes);
-  a.splits = l.splits;
+  a.pieces = reinterpret_cast<int32_t*>(ws + l.list_bytes + l.part_bytes + l.ml_bytes);
   a.part_rows = l.part_rows;
+  a.few_grid = std::max(1, l.few_grid);
+  a.zero_outside = p->zero_outside != 0;
   a.few_only = !l.chunk;
   a.tiles = l.tiles_seq;
   a.d_tiles = fast_div(std::max(1, l.tiles_seq));
   hipStream_t st = (hipStream_t)stream;
   if (l.list) {
-    a.d_splits = fast_div(l.sel_steps);
-    select_kernel<<<(uint32_t)(bh * l.sel_steps), 64 * kSelWaves, 0, st>>>(a, l.sel_steps);
+    a.d_steps = fast_div(l.sel_steps);
+    const uint32_t grid = (uint32_t)(bh * l.sel_steps);
+    auto kernel = l.wide ? (p->top_k <= 2 ? select_wide_kernel<2> : select_wide_kernel<4>)
+                         : (p->top_k <= 2 ? select_kernel<2> : select_kernel<4>);
+    kernel<<<grid, 64 * kSelWaves, 0, st>>>(a, l.sel_steps);
     if (int e = hip_err(hipGetLastError(), "cra_fwd_paged (relay rows)")) return e;
   }
-  a.d_splits = fast_div(l.splits);
   return hip_err(with_dim(l.Dp, [&](auto d) {
     return with_store(c->store, [&](auto s) {
       constexpr int D = decltype(d)::value, S = decltype(s)::value;

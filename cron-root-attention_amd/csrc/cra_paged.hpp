@@ -64,12 +64,14 @@ __host__ __device__ inline int seq_of_token(const int32_t* cu, int n_seqs, int t
   return lo;
 }
 
-// ceil(sqrt(n)), n >= 0.
+// ceil(sqrt(n)), n >= 0: the float root is within one of it, squares of up to
+// 46342 fit 32 bits.
 __host__ __device__ inline int ceil_sqrt(int n) {
   if (n <= 0) return 0;
-  int64_t r = (int64_t)sqrtf((float)n);  // within one of it
-  while (r * r < n) ++r;
-  while (r > 1 && (r - 1) * (r - 1) >= n) --r;
+  uint32_t r = (uint32_t)sqrtf((float)n);
+  r = r > 0 ? r - 1 : 0;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) r += r * r < (uint32_t)n ? 1 : 0;
   return (int)r;
 }
 

@@ -404,24 +404,27 @@ __global__ __launch_bounds__(kThreads) void turn_bwd_kernel(TurnArgs g) {
   }
 }
 
-// dw = sum of the partial rows, in row order within each of 16 interleaved
-// sequences, those in order. One workgroup: 16 columns of one tensor.
+// dw = sum of the partial rows: 64 interleaved sequences of them, each in row
+// order, then the sequences in order. One workgroup: 16 columns of one tensor.
+constexpr int kDwSeqs = 64;
 template <typename W>
-__global__ __launch_bounds__(256) void turn_dw_kernel(const float* pq, int nq, W* dwq,
-                                                      const float* pk, int nk, W* dwk, int D) {
-  __shared__ float red[16][17];
+__global__ __launch_bounds__(16 * kDwSeqs) void turn_dw_kernel(const float* pq, int nq, W* dwq,
+                                                               const float* pk, int nk, W* dwk, int D) {
+  __shared__ float red[kDwSeqs][17];
   const float* p = blockIdx.y ? pk : pq;
   W* dw = blockIdx.y ? dwk : dwq;
   const int n = blockIdx.y ? nk : nq;
   if (!dw) return;
   const int col = threadIdx.x & 15, seq = threadIdx.x >> 4, e = blockIdx.x * 16 + col;
   float sum = 0.f;
-  if (e < D)
-    for (int r = seq; r < n; r += 16) sum += p[(int64_t)r * D + e];
+  if (e < D) {
+#pragma unroll 8
+    for (int r = seq; r < n; r += kDwSeqs) sum += p[(int64_t)r * D + e];
+  }
   red[seq][col] = sum;
   __syncthreads();
   if (seq == 0 && e < D) {
-    for (int i = 1; i < 16; ++i) sum += red[i][col];
+    for (int i = 1; i < kDwSeqs; ++i) sum += red[i][col];
     dw[e] = from_f32<W>(sum);
   }
 }
@@ -662,7 +665,7 @@ int cra_norm_rotary_bwd(const cra_turn* p, cra_tensor q, cra_tensor k, const voi
   const dim3 grid((p->D + 15) / 16, 2);
   return hip_err(with_type(p->weight_dtype, [&](auto z) {
     using W = decltype(z);
-    turn_dw_kernel<W><<<grid, 256, 0, st>>>(g.t[0].partial, g.t[0].blocks, static_cast<W*>(dwq),
+    turn_dw_kernel<W><<<grid, 16 * kDwSeqs, 0, st>>>(g.t[0].partial, g.t[0].blocks, static_cast<W*>(dwq),
                                             g.t[1].partial, g.t[1].blocks, static_cast<W*>(dwk), p->D);
     return hipGetLastError();
   }), "cra_norm_rotary_bwd (weights)");

@@ -92,7 +92,7 @@ CACHE = dict(k=P, v=P, k_norm=P, k_scale=None, v_scale=None, num_pages=10, H_kv=
              dtype=0, store=0)
 BATCH = dict(page_table=P, table_stride=5, seq_lens=P, cu_seqlens=None, n_seqs=3, pages_per_seq=5, tokens=0,
              query_len=4)
-PLAN = dict(H_q=8, D=128, window=0, relay=-1, top_k=2, max_query_len=4, max_seqlen=320, scale=0.1)
+PLAN = dict(H_q=8, D=128, window=0, relay=-1, top_k=2, max_query_len=4, max_seqlen=320, zero_outside=0, scale=0.1)
 T = N.CraTensor(P, 1 << 16, 128, 1024)
 
 

@@ -225,6 +225,9 @@ CASES = [
     ([0, 10, 0, 50], [0, 3, 0, 20], 2, 1, 64, 16, {}),                      # empty sequences
     ([4, 7], [6, 40], 2, 1, 64, 16, {}),                                    # more new tokens than rows
     ([64, 128, 192], [32, 64, 128], 2, 1, 64, 16, dict(window=64)),         # everything on tile borders
+    ([2300, 1700], [1, 30], 2, 2, 64, 32, dict(window=600, relay=True, relay_top_k=3)),  # wide blocks
+    ([1100, 2040], [20, 1], 2, 2, 64, 16, dict(window=506, relay=True)),
+    ([1100, 2040], [1, 20], 2, 2, 64, 16, dict(window=505, relay=True, relay_top_k=4)),
 ]
 
 
@@ -380,12 +383,17 @@ def test_repeated_pages():
     check(run(s, q, [1, 1], window=64), *s.expect(q, [1, 1], window=64), BF16)
 
 
-def test_equal_norms_take_the_earlier_row():
+@pytest.mark.parametrize("window,top_k", [(None, 2), (46, 4), (600, 2), (600, 4)])
+def test_equal_norms_take_the_earlier_row(window, top_k):
     s = Setup([2100], 1, 64, F16)
-    s.k[:] = s.k.sign() * 0.5  # every row has the same norm
+    s.k[:] = s.k.sign() * 0.5  # every row has the same norm, but for a few pairs
+    s.k[50:52] *= 2
+    s.k[700:703] *= 2
+    s.k[1300], s.k[1350] = s.k[1300] * 4, s.k[1350] * 4
     s.write(s.k, s.v, [2100], [0, 2100])
     q = (8 * torch.randn(1, 1, 64, generator=s.g)).half()
-    check(run(s, q, [1]), *s.expect(q, [1]), F16)
+    check(run(s, q, [1], window=window, relay=True, relay_top_k=top_k),
+          *s.expect(q, [1], window=window, relay=True, top_k=top_k), F16)
 
 
 def test_nan_norms_are_not_chosen():
