@@ -28,82 +28,13 @@
 
 #include "cra_common.hpp"
 #include "cra_internal.hpp"
-#include "cra_paged.hpp"
-#include "cra_tile.hpp"
+#include "cra_paged_dev.hpp"
 
 namespace cra {
 
 int set_error(int code, const char* msg);
 
 namespace {
-
-constexpr float kInf = __builtin_huge_valf();
-constexpr int kFewRows = 16;  // rows of few_kernel's MFMA block
-enum { kSame = CRA_STORE_SAME, kE4M3 = CRA_STORE_E4M3, kInt8 = CRA_STORE_INT8 };
-
-struct PagedArgs {
-  PagedView c;
-  const void* q;
-  void* o;
-  int64_t qsb, qsh, qss, osb, osh, oss;
-  int Hq, grp, D, Ds;  // query heads, per kv head; columns of q and o; of a cache row
-  int window, relay, top_k, max_len;
-  float scale;
-  FastDiv d_grp, d_hkv, d_steps;
-  uint32_t* list;  // [n_seqs, H_kv, list_cap] cache rows of the global rows (relay)
-  int list_cap;
-  float* part;     // few rows: O of shared sequences' pieces, [piece, part_rows, Dp], and (m, l)
-  float* part_ml;
-  int32_t* pieces;  // [n_seqs + 1] first piece of each sequence (a kv head), for combine_kernel
-  int part_rows, few_grid;
-  int few_only;    // no chunk_kernel follows: longer sequences are refused (NaN)
-  int zero_outside;  // rows of tokens outside every sequence are set to zero
-  int tiles;       // chunk tiles of a sequence (batches without cu)
-  FastDiv d_tiles;
-};
-
-// A sequence of the call: length, new tokens, and where they lie in q and o.
-struct Seq {
-  int n, m, qb, q0;
-  bool over;  // longer than the caller's bound, or than its table: nothing is read
-};
-__device__ __forceinline__ Seq get_seq(const PagedArgs& a, int b) {
-  Seq s;
-  const int len = a.c.lens[b];
-  s.over = len > a.max_len;
-  s.n = s.over || len < 0 ? 0 : len;
-  if (a.c.cu) {
-    const TokenRange t = token_range(a.c.cu, b, a.c.tokens);
-    s.m = t.last - t.first;
-    s.qb = 0;
-    s.q0 = t.first;
-  } else {
-    s.m = a.c.query_len;
-    s.qb = b;
-    s.q0 = 0;
-  }
-  return s;
-}
-
-__device__ __forceinline__ SeqPlan get_plan(const PagedArgs& a, int n) {
-  return seq_plan(n, a.window, a.relay, a.top_k);
-}
-
-// Row r of a kv head's rows is query head r % grp of the kv head, new token r / grp.
-__device__ __forceinline__ int row_token(const PagedArgs& a, int r) { return (int)div_by(r, a.d_grp); }
-
-template <typename T>
-__device__ __forceinline__ const T* q_row(const PagedArgs& a, const Seq& s, int hk, int r) {
-  const int t = row_token(a, r);
-  return static_cast<const T*>(a.q) + s.qb * a.qsb + (int64_t)(hk * a.grp + r - t * a.grp) * a.qsh +
-         (int64_t)(s.q0 + t) * a.qss;
-}
-template <typename T>
-__device__ __forceinline__ T* o_row(const PagedArgs& a, const Seq& s, int hk, int r) {
-  const int t = row_token(a, r);
-  return static_cast<T*>(a.o) + s.qb * a.osb + (int64_t)(hk * a.grp + r - t * a.grp) * a.osh +
-         (int64_t)(s.q0 + t) * a.oss;
-}
 
 // ---------------------------------------------------------------------------
 // The global rows of sequences with relay, as cache rows: of each W-block its
@@ -125,28 +56,6 @@ __device__ __forceinline__ T* o_row(const PagedArgs& a, const Seq& s, int hk, in
 constexpr int kSelWaves = 4, kSelLoads = 8;
 constexpr int kSelMost = 64 * 8 - 7;   // rows of a block in select_kernel, at any alignment
 
-// Maximum over the wave, and sums up to each lane, by row shifts and broadcasts in
-// the VALU (lanes without a source take 0).
-#define CRA_DPP(x, ctrl, rows) (uint32_t) __builtin_amdgcn_update_dpp(0, (int)(x), ctrl, rows, 0xf, false)
-__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
-  x = max(x, CRA_DPP(x, 0x111, 0xf));  // row_shr:1, 2, 4, 8: the row's last lane has its maximum
-  x = max(x, CRA_DPP(x, 0x112, 0xf));
-  x = max(x, CRA_DPP(x, 0x114, 0xf));
-  x = max(x, CRA_DPP(x, 0x118, 0xf));
-  x = max(x, CRA_DPP(x, 0x142, 0xf));  // row_bcast:15, row_bcast:31
-  x = max(x, CRA_DPP(x, 0x143, 0xf));
-  return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
-}
-__device__ __forceinline__ uint32_t wave_upto(uint32_t x) {
-  x += CRA_DPP(x, 0x111, 0xf);
-  x += CRA_DPP(x, 0x112, 0xf);
-  x += CRA_DPP(x, 0x114, 0xf);
-  x += CRA_DPP(x, 0x118, 0xf);
-  x += CRA_DPP(x, 0x142, 0xa);  // the row before, into rows 1 and 3
-  x += CRA_DPP(x, 0x143, 0xc);  // the half before, into rows 2 and 3
-  return x;
-}
-
 // The blocks of a wave: [first, end) of sequence b's, head h.
 struct SelWork {
   SeqPlan p;
@@ -160,7 +69,7 @@ __device__ __forceinline__ SelWork sel_work(const PagedArgs& a, int steps) {
   const int nw = steps * kSelWaves, w = (int)(blockIdx.x - bh * steps) * kSelWaves + wave;
   k.b = (int)div_by(bh, a.d_hkv);
   k.h = (int)(bh - (uint32_t)k.b * a.c.H_kv);
-  const Seq s = get_seq(a, k.b);
+  const Seq s = wave_seq(a, k.b);
   k.p = get_plan(a, s.n);
   if (k.p.rpb == 1 || s.m < 1) return k;
   const int ls = s.n - k.p.W > 0 ? s.n - k.p.W : 0;  // window start of the last query
@@ -357,117 +266,6 @@ __global__ __launch_bounds__(64 * kSelWaves) void select_wide_kernel(PagedArgs a
 }
 
 // ---------------------------------------------------------------------------
-// 8-bit codes to operands of a 2-byte type (exact for both stores).
-// ---------------------------------------------------------------------------
-template <typename T, int STORE>
-__device__ __forceinline__ uint2 widen4(uint32_t w) {  // four codes -> four elements
-  uint2 r;
-  if constexpr (STORE == kE4M3) {
-    if constexpr (std::is_same<T, bf16>::value) {
-      r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.f, false));
-      r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.f, true));
-    } else {
-      r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.f, false));
-      r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.f, true));
-    }
-  } else {
-    typedef T t2 __attribute__((ext_vector_type(2)));
-    const uint32_t u = w ^ 0x80808080u;
-    float f[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = (float)(u >> (8 * i) & 0xffu) - 128.f;
-    r.x = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{f[0], f[1]}, t2));
-    r.y = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{f[2], f[3]}, t2));
-  }
-  return r;
-}
-template <int STORE>
-__device__ __forceinline__ float code_value(uint32_t w, int i) {  // code i of four, i constant
-  if constexpr (STORE == kE4M3) {
-    switch (i) {
-      case 0: return __builtin_amdgcn_cvt_f32_fp8((int)w, 0);
-      case 1: return __builtin_amdgcn_cvt_f32_fp8((int)w, 1);
-      case 2: return __builtin_amdgcn_cvt_f32_fp8((int)w, 2);
-      default: return __builtin_amdgcn_cvt_f32_fp8((int)w, 3);
-    }
-  } else {
-    return (float)(int8_t)(w >> (8 * i) & 0xffu);
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ Frag<T> zero_frag() {
-  Frag<T> f;
-  f.w[0] = make_uint4(0, 0, 0, 0);
-  return f;
-}
-
-// Whether a lane of the wave holds an operand element that is not finite (or
-// elements whose sum leaves fp32), from their sum over the tile's rows and columns.
-__device__ __forceinline__ bool any_not_finite(f32x4 sum) {
-  const float z = (sum[0] - sum[0]) + (sum[1] - sum[1]) + (sum[2] - sum[2]) + (sum[3] - sum[3]);
-  return __any(!(z == 0.f));
-}
-
-// O^T += scale V^T . P^T where rows that not every query sees hold elements that
-// are not finite (0 times them would be NaN). The product takes V with those
-// elements set to zero; which queries see one is counted by products of
-// indicators (of +inf, -inf and NaN in V, and of the rows that a query sees),
-// and their sums become what such a row makes of them. v(db): the V operand of
-// 16-column block db; row of slot s of lane group g: k0 + 4g + s (s < 4),
-// k0 + 16 + 4g + s - 4.
-template <typename T, int NDB, int QB, typename V>
-__device__ __forceinline__ void pv_not_finite(V v, const Frag<T> (&pf)[QB], f32x4 (&acc)[NDB][QB],
-                                              const TileMask<QB>& mk, int k0, int g, float scale) {
-  constexpr uint32_t kExp = std::is_same<T, bf16>::value ? 0x7f80u : 0x7c00u;
-  constexpr uint32_t kOne = std::is_same<T, bf16>::value ? 0x3f80u : 0x3c00u;
-  const f32x4 zero = f32x4{0.f, 0.f, 0.f, 0.f};
-  Frag<T> sees[QB];
-#pragma unroll
-  for (int qb = 0; qb < QB; ++qb)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = k0 + (i < 2 ? 0 : 16) + 4 * g + 2 * (i & 1);
-      reinterpret_cast<uint32_t*>(sees[qb].w)[i] = (mk.ok(row, qb) ? kOne : 0u) |
-                                                   (mk.ok(row + 1, qb) ? kOne << 16 : 0u);
-    }
-#pragma unroll
-  for (int db = 0; db < NDB; ++db) {
-    Frag<T> f[4];  // V without them; +inf, -inf, NaN
-    f[0] = v(db);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t w = reinterpret_cast<const uint32_t*>(f[0].w)[i];
-      uint32_t o[4] = {0, 0, 0, 0};
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t x = w >> (16 * h) & 0xffffu, mag = x & 0x7fffu;
-        o[0] |= (mag < kExp ? x : 0u) << (16 * h);
-        o[1] |= (x == kExp ? kOne : 0u) << (16 * h);
-        o[2] |= (x == (kExp | 0x8000u) ? kOne : 0u) << (16 * h);
-        o[3] |= (mag > kExp ? kOne : 0u) << (16 * h);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) reinterpret_cast<uint32_t*>(f[j].w)[i] = o[j];
-    }
-#pragma unroll
-    for (int qb = 0; qb < QB; ++qb) {
-      const f32x4 o = mma(zero, f[0], pf[qb]) * scale;
-      const f32x4 pos = mma(zero, f[1], sees[qb]), neg = mma(zero, f[2], sees[qb]);
-      const f32x4 nan = mma(zero, f[3], sees[qb]);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float x = o[r];
-        if (pos[r] > 0.f) x += kInf;
-        if (neg[r] > 0.f) x -= kInf;
-        if (nan[r] > 0.f) x = __builtin_nanf("");
-        acc[db][qb][r] += x;
-      }
-    }
-  }
-}
-
-// ---------------------------------------------------------------------------
 // Few rows: at most 16 rows a (sequence, kv head). The keys of all sequences are
 // cut into pieces of equal length, as many as keep the resident workgroups busy
 // about twice over; each workgroup takes pieces from the grid's stride, each
@@ -590,10 +388,6 @@ struct ByteTile {
   }
 };
 
-// All of the wave's loads have landed (in LDS too) and its LDS reads are done; no
-// memory access moves across.
-__device__ __forceinline__ void wait_all() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
-
 template <typename T, int STORE, int D>
 __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(D > 128 ? 1 : 2)))
 void few_kernel(PagedArgs a) {
@@ -615,7 +409,7 @@ void few_kernel(PagedArgs a) {
   const FewPiece fi = few_piece(a, fp, (int)idx);
   const int b = fi.b;
   if (b < 0) break;
-  const Seq s = get_seq(a, b);
+  const Seq s = wave_seq(a, b);
   const int64_t rows64 = (int64_t)s.m * a.grp;
   if (rows64 > a.part_rows) {  // more new tokens than the caller's bound
     for (int64_t i = tid; i < rows64 * a.D; i += 64 * NW) {
@@ -889,7 +683,7 @@ __global__ __launch_bounds__(256) void combine_kernel(PagedArgs a, int Dp) {
   const int b = (int)div_by(bh, a.d_hkv), hk = (int)(bh - (uint32_t)b * a.c.H_kv);
   const int first = a.pieces[b], n = a.pieces[b + 1] - first;
   if (n < 2) return;
-  const Seq s = get_seq(a, b);
+  const Seq s = wave_seq(a, b);
   if (r >= (int64_t)s.m * a.grp) return;
   const int quads = Dp / 4, lanes = 256 / quads;  // groups of pieces
   const int quad = tid % quads, sg = tid / quads;
@@ -920,322 +714,6 @@ __global__ __launch_bounds__(256) void combine_kernel(PagedArgs a, int Dp) {
     float x = 0.f;
     for (int i = 0; i < lanes; ++i) x += red[i * quads + quad][j];
     op[j] = from_f32<T>(x * inv);
-  }
-}
-
-// ---------------------------------------------------------------------------
-// Chunks: tiles of 128 (D = 256: 64) rows of a (sequence, kv head), four waves.
-// ---------------------------------------------------------------------------
-// The work item of a workgroup: sequence and tile, tiles of a sequence's last
-// tokens (the longest ranges) first; -1: none. With cu every wave adds up the
-// sequences' tiles, 64 at a time.
-template <int BM>
-__device__ __forceinline__ void find_tile(const PagedArgs& a, int item, int& b, int& tile) {
-  if (!a.c.cu) {
-    b = (int)div_by(item, a.d_tiles);
-    tile = a.tiles - 1 - (item - b * a.tiles);
-    return;
-  }
-  const int lane = threadIdx.x & 63;
-  int before = 0;
-  b = -1;
-  for (int base = 0; base < a.c.n_seqs; base += 64) {
-    int count = 0;
-    if (base + lane < a.c.n_seqs) {
-      const TokenRange t = token_range(a.c.cu, base + lane, a.c.tokens);
-      const int64_t rows = (int64_t)(t.last - t.first) * a.grp;
-      count = rows > kFewRows ? (int)((rows + BM - 1) / BM) : 0;
-    }
-    const int upto = before + (int)wave_upto(count);
-    const uint64_t hit = __ballot(upto > item);
-    if (hit) {
-      const int l = __builtin_ctzll(hit);
-      b = base + l;
-      tile = __builtin_amdgcn_readlane(upto, l) - 1 - item;
-      return;
-    }
-    before = __builtin_amdgcn_readlane(upto, 63);
-  }
-}
-
-// P.V of a 32-row half that not all of the wave's queries see.
-template <typename T, int D, int BN, int QB>
-__device__ __forceinline__ void pv_half_masked(const char* tV, int kh, const LaneOffs<D>& lo,
-                                               const Frag<T> (&pf)[QB], f32x4 (&acc)[D / 16][QB],
-                                               const TileMask<QB>& mk, const Frag<T>& one, int g) {
-  using Tile = SwzTile<D, BN>;
-  auto v_frag = [&](int db) __attribute__((always_inline)) {
-    const char* pa = tV + 2 * kh * Tile::kBlk16 + lo.tr_at(db);
-    return Tile::template tr_frag_at<T>(pa, pa + Tile::kBlk16);
-  };
-  f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int db = 0; db < D / 16; ++db) sum = mma(sum, v_frag(db), one);
-  if (any_not_finite(sum))
-    pv_not_finite<T, D / 16, QB>(v_frag, pf, acc, mk, 32 * kh, g, 1.f);
-  else
-    pv_half<T, D, BN, QB>(tV, kh, lo, pf, acc);
-}
-
-// Scores of 8-bit keys: the rows' scales (LDS) come in here, exactly as fp32.
-template <int QB>
-__device__ __forceinline__ void scale_scores(f32x4 (&s)[2][QB], const float* ks, int kc, int g) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const f32x4 k = *reinterpret_cast<const f32x4*>(ks + 32 * kc + 16 * h + 4 * g);
-#pragma unroll
-    for (int qb = 0; qb < QB; ++qb) s[h][qb] *= k;
-  }
-}
-
-template <typename T, int STORE, int D, int BN, int QB, bool MASK>
-__device__ __forceinline__ void attend_chunk(const char* tK, const char* tV, const float* ks,
-                                             const LaneOffs<D>& lo, const Frag<T> (&qf)[QB][D / 32],
-                                             f32x4 (&acc)[D / 16][QB], float (&m_run)[QB],
-                                             float (&l_run)[QB], float c2, int g,
-                                             const TileMask<QB>& mk, const Frag<T>& one,
-                                             int kc0, int kc1) {
-#pragma unroll
-  for (int kc = 0; kc < BN / 32; ++kc) {
-    if (MASK && (kc < kc0 || kc > kc1)) continue;  // no row of this half is seen
-    f32x4 s[2][QB];
-    tile_scores<T, D, BN, QB>(tK, lo, qf, kc, s);
-    if constexpr (STORE != kSame) scale_scores<QB>(s, ks, kc, g);
-    Frag<T> pf[QB];
-    float ps[QB];
-    bool high = false;
-#pragma unroll
-    for (int qb = 0; qb < QB; ++qb) {
-      half_exp<T, MASK, QB>(s, kc, qb, c2, m_run[qb], g, mk, one, pf[qb], ps[qb]);
-      high |= !(ps[qb] <= kSumMax);
-    }
-    if (__any(high)) {
-#pragma unroll
-      for (int qb = 0; qb < QB; ++qb)
-        if (__any(!(ps[qb] <= kSumMax)))
-          half_rescale<T, D, QB>(s, qb, c2, acc, m_run, l_run, one, pf[qb], ps[qb]);
-    }
-#pragma unroll
-    for (int qb = 0; qb < QB; ++qb) l_run[qb] += ps[qb];
-    if constexpr (MASK)
-      pv_half_masked<T, D, BN, QB>(tV, kc, lo, pf, acc, mk, one, g);
-    else
-      pv_half<T, D, BN, QB>(tV, kc, lo, pf, acc);
-  }
-}
-
-template <int D>
-constexpr int kChunkQB = D > 128 ? 1 : 2;
-template <int D>
-constexpr int kChunkBN = D > 128 ? 32 : 64;
-constexpr int kChunkWaves = 4;
-
-template <typename T, int STORE, int D>
-__global__ __launch_bounds__(64 * kChunkWaves) __attribute__((amdgpu_waves_per_eu(2)))
-void chunk_kernel(PagedArgs a) {
-  constexpr int NW = kChunkWaves, QB = kChunkQB<D>, BN = kChunkBN<D>, kQW = 16 * QB, BM = NW * kQW;
-  using Tile = SwzTile<D, BN>;
-  __shared__ __attribute__((aligned(1024))) char stage0[2][Tile::kBytes];
-  __shared__ __attribute__((aligned(1024))) char stage1[2][Tile::kBytes];
-  __shared__ __attribute__((aligned(16))) float kscale[2][BN];
-
-  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) & (NW - 1);
-  const uint32_t item = div_by(blockIdx.x, a.d_hkv);
-  const int hk = (int)(blockIdx.x - item * a.c.H_kv);  // neighbouring workgroups: another head, another XCD
-  int b, tile;
-  find_tile<BM>(a, (int)item, b, tile);
-  if (b < 0) return;
-  const Seq s = get_seq(a, b);
-  const int rows = s.m * a.grp;
-  if (rows <= kFewRows || tile * BM >= rows) return;
-  const SeqPlan p = get_plan(a, s.n);
-  const int pos0 = s.n - s.m;
-  const int r0 = tile * BM, q0 = r0 + wave * kQW;
-  auto pos_of = [&](int r) { return pos0 + row_token(a, r); };
-  const int wg_first = pos_of(r0), wg_last = pos_of(min(r0 + BM, rows) - 1);
-  const int lo_k = max(0, wg_first - p.W + 1), hi = max(0, wg_last + 1);
-  const int gmax = seq_prefix(wg_last, p);
-  const int nglob = (gmax + BN - 1) / BN, nloc = (hi - lo_k + BN - 1) / BN;
-  const int ntot = nglob + (hi > lo_k ? nloc : 0);
-  const int32_t* pages = a.c.table + b * a.c.table_stride;
-  const uint32_t* list = a.list + ((int64_t)b * a.c.H_kv + hk) * a.list_cap;
-  bool bad = s.over;
-
-  // global tiles first, then the window from its highest tile down
-  auto tile_start = [&](int it) {
-    return it >= nglob ? lo_k + (nloc - 1 - (it - nglob)) * BN : it * BN;
-  };
-  auto slot_of = [&](int it, int row) -> uint32_t {
-    const int ts = tile_start(it);
-    if (it < nglob) {
-      const int i = min(ts + row, gmax - 1);
-      if (p.rpb > 1) return list[i];
-      return seq_row(pages, i * p.W, a.c.num_pages, a.c.H_kv, a.c.log_page, hk);
-    }
-    return seq_row(pages, min(ts + row, hi - 1), a.c.num_pages, a.c.H_kv, a.c.log_page, hk);
-  };
-
-  // Rows of a tile that this thread fills. 16-bit: the wave's instruction t
-  // moves 1 KB, each lane one 16-byte chunk from its own address straight into
-  // LDS. 8-bit: pieces of 16 codes through registers, widened on the way (V
-  // times its scale: one more rounding; K's scales go to the scores).
-  constexpr int kPiecesRow = STORE == kSame ? Tile::kCPR : D / 16;
-  constexpr int kAll = BN * kPiecesRow, kPer = (kAll + 64 * NW - 1) / (64 * NW);
-  const int row_bytes = a.Ds * (STORE == kSame ? 2 : 1);
-  auto piece_of = [&](int i) { return STORE == kSame ? (i * NW + wave) * 64 + lane : i * 64 * NW + tid; };
-  uint32_t slot[kPer];
-  auto load_slots = [&](int it) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) slot[i] = slot_of(it, min(piece_of(i), kAll - 1) / kPiecesRow);
-  };
-  uint4 rk[STORE == kSame ? 1 : kPer], rv[STORE == kSame ? 1 : kPer];
-  float rks[STORE == kSame ? 1 : kPer], rvs[STORE == kSame ? 1 : kPer];
-  auto issue = [&](char (&dst)[2][Tile::kBytes]) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int piece = piece_of(i), row = piece / kPiecesRow;
-      if (kAll % (64 * NW) != 0 && piece >= kAll) break;
-      bad |= slot[i] == kNoRow;
-      const uint32_t sl = slot[i] == kNoRow ? 0u : slot[i];
-      const int col = piece % kPiecesRow;
-      if constexpr (STORE == kSame) {
-        const int chunk = col ^ Tile::swz(row);
-        const int64_t at = (int64_t)sl * row_bytes + chunk * 16;
-        if (D * 2 == row_bytes || chunk * 16 < row_bytes) {
-          const int lds = (i * NW + wave) * 1024;
-          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(a.c.k + at),
-                                           CRA_LDS(dst[0] + lds), 16, 0, 0);
-          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(a.c.v + at),
-                                           CRA_LDS(dst[1] + lds), 16, 0, 0);
-        }
-      } else {
-        const int64_t at = (int64_t)sl * row_bytes + col * 16;
-        const bool in = col * 16 < row_bytes;
-        rk[i] = in ? *reinterpret_cast<const uint4*>(a.c.k + at) : make_uint4(0, 0, 0, 0);
-        rv[i] = in ? *reinterpret_cast<const uint4*>(a.c.v + at) : make_uint4(0, 0, 0, 0);
-        rks[i] = a.c.k_scale[sl];
-        rvs[i] = a.c.v_scale[sl];
-      }
-    }
-  };
-  auto store = [&](char (&dst)[2][Tile::kBytes], float (&ks)[BN]) {
-    if constexpr (STORE != kSame) {
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int piece = piece_of(i), row = piece / kPiecesRow, col = piece % kPiecesRow;
-        if (kAll % (64 * NW) != 0 && piece >= kAll) break;
-        const uint32_t* wk = reinterpret_cast<const uint32_t*>(&rk[i]);
-        const uint32_t* wv = reinterpret_cast<const uint32_t*>(&rv[i]);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint2 x = widen4<T, STORE>(wk[2 * h]), y = widen4<T, STORE>(wk[2 * h + 1]);
-          *reinterpret_cast<uint4*>(dst[0] + Tile::off(row, 2 * col + h)) = make_uint4(x.x, x.y, y.x, y.y);
-          float f[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) f[j] = code_value<STORE>(wv[2 * h + j / 4], j % 4) * rvs[i];
-          *reinterpret_cast<uint4*>(dst[1] + Tile::off(row, 2 * col + h)) = pack8<T>(f).w[0];
-        }
-        if (col == 0) ks[row] = rks[i];
-      }
-    }
-  };
-  if (STORE == kSame && D * 2 > row_bytes) {  // columns that no load fills
-    for (int i = tid; i < 2 * Tile::kBytes / 16; i += 64 * NW) {
-      reinterpret_cast<uint4*>(stage0)[i] = make_uint4(0, 0, 0, 0);
-      reinterpret_cast<uint4*>(stage1)[i] = make_uint4(0, 0, 0, 0);
-    }
-    __syncthreads();
-  }
-  if (ntot > 0) {
-    load_slots(0);
-    issue(stage0);
-    store(stage0, kscale[0]);
-    if (ntot > 1) load_slots(1);
-  }
-
-  LaneOffs<D> lo;
-  lo.init(lane);
-  Frag<T> qf[QB][D / 32];
-  int pos[QB], glen[QB];
-  bool counts[QB];
-  float m_run[QB], l_run[QB];
-  f32x4 acc[D / 16][QB];
-#pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
-    const int r = q0 + 16 * qb + l16;
-    counts[qb] = r < rows;
-    pos[qb] = counts[qb] ? pos_of(r) : -1;
-    glen[qb] = pos[qb] >= 0 ? seq_prefix(pos[qb], p) : 0;
-    const T* qp = q_row<T>(a, s, hk, counts[qb] ? r : 0);
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c)
-      qf[qb][c] = counts[qb] && 32 * c + 8 * g < a.D ? lds_frag_row<T>(qp + 32 * c + 8 * g) : zero_frag<T>();
-    m_run[qb] = -kInf;
-    l_run[qb] = 0.f;
-#pragma unroll
-    for (int db = 0; db < D / 16; ++db) acc[db][qb] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  const float c2 = a.scale * kLog2e;
-  const bool active = q0 < rows;
-  const int first = active ? pos_of(q0) : 0;  // positions of the wave's rows: [first, last]
-  const int last = active ? pos_of(min(q0 + kQW, rows) - 1) : -1;
-  const int w_lo = max(0, first - p.W + 1);
-  const int g_all = active ? seq_prefix(first, p) : 0, g_any = active ? seq_prefix(last, p) : 0;
-  const Frag<T> one = ones_frag<T>();
-
-  auto turn = [&](auto second, int it) __attribute__((always_inline)) {
-    constexpr int kS = decltype(second)::value;
-    char(&cur)[2][Tile::kBytes] = kS ? stage1 : stage0;
-    char(&nxt)[2][Tile::kBytes] = kS ? stage0 : stage1;
-    if (STORE == kSame) wait_vmem();
-    __syncthreads();
-    if (it + 1 < ntot) {
-      issue(nxt);
-      if (it + 2 < ntot) load_slots(it + 2);
-    }
-    const bool loc = it >= nglob;
-    const int ts = tile_start(it);
-    const bool work = active && (loc ? ts <= last && ts + BN - 1 >= w_lo : ts < g_any);
-    if (work) {
-      const bool full = loc ? ts >= last - p.W + 1 && ts + BN - 1 <= first : ts + BN <= g_all;
-      TileMask<QB> mk;
-#pragma unroll
-      for (int qb = 0; qb < QB; ++qb) {
-        mk.hi[qb] = loc ? pos[qb] - ts : glen[qb] - 1 - ts;
-        mk.span[qb] = loc ? (unsigned)(p.W - 1) : 0x7fffffffu;
-      }
-      if (full) {
-        attend_chunk<T, STORE, D, BN, QB, false>(cur[0], cur[1], kscale[kS], lo, qf, acc, m_run, l_run,
-                                                 c2, g, mk, one, 0, 0);
-      } else {
-        const int vis_lo = loc ? max(0, w_lo - ts) : 0, vis_hi = loc ? last - ts : g_any - 1 - ts;
-        attend_chunk<T, STORE, D, BN, QB, true>(cur[0], cur[1], kscale[kS], lo, qf, acc, m_run, l_run,
-                                                c2, g, mk, one, vis_lo >> 5, vis_hi >> 5);
-      }
-    }
-    if (it + 1 < ntot) store(nxt, kscale[1 - kS]);
-  };
-  for (int it = 0; it < ntot; it += 2) {
-    turn(std::integral_constant<int, 0>{}, it);
-    if (it + 1 < ntot) turn(std::integral_constant<int, 1>{}, it + 1);
-  }
-
-  bad = __syncthreads_or(bad);
-#pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
-    if (!counts[qb]) continue;
-    const float l = l_run[qb];
-    const float inv = bad ? __builtin_nanf("") : l == 0.f ? 0.f : 1.f / l;
-    T* op = o_row<T>(a, s, hk, q0 + 16 * qb + l16);
-#pragma unroll
-    for (int db = 0; db < D / 16; ++db) {
-      if (16 * db + 4 * g >= a.D) continue;
-      T e[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) e[r] = from_f32<T>(acc[db][qb][r] * inv);
-      *reinterpret_cast<uint2*>(op + 16 * db + 4 * g) = *reinterpret_cast<const uint2*>(e);
-    }
   }
 }
 
@@ -1422,7 +900,7 @@ __device__ void f32_item(const PagedArgs& a, const Seq& s, int b, int hk, int r0
     for (int db = 0; db < D / 16; ++db)
       if (16 * db + 4 * g < a.D) *reinterpret_cast<f32x4*>(op + 16 * db + 4 * g) = acc[db] * inv;
   } else {
-    const int64_t at = part_at + r;
+    const int64_t at = part_at + (r - r0);
 #pragma unroll
     for (int db = 0; db < D / 16; ++db)
       *reinterpret_cast<f32x4*>(a.part + at * D + 16 * db + 4 * g) = acc[db];
@@ -1443,7 +921,7 @@ __global__ __launch_bounds__(256) void f32_kernel(PagedArgs a) {
       const int hk = (int)((uint32_t)item - idx * a.c.H_kv);
       const FewPiece fi = few_piece(a, fp, (int)idx);
       if (fi.b < 0) break;
-      const Seq s = get_seq(a, fi.b);
+      const Seq s = wave_seq(a, fi.b);
       const int64_t rows = (int64_t)s.m * a.grp;
       if (rows > a.part_rows) {  // more new tokens than the caller's bound
         for (int64_t i = threadIdx.x; i < rows * a.D; i += 256) {
@@ -1456,16 +934,15 @@ __global__ __launch_bounds__(256) void f32_kernel(PagedArgs a) {
                          fi.only ? -1 : item * a.part_rows);
     }
   } else {
-    const uint32_t item = div_by(blockIdx.x, a.d_hkv);
-    const int hk = (int)(blockIdx.x - item * a.c.H_kv);
-    int b, tile;
-    find_tile<kF32Rows>(a, (int)item, b, tile);
-    if (b < 0) return;
-    const Seq s = get_seq(a, b);
-    const int64_t rows = (int64_t)s.m * a.grp;
-    if (rows <= kFewRows || (int64_t)tile * kF32Rows >= rows) return;
-    f32_item<STORE, D>(a, s, b, hk, tile * kF32Rows, 0, 0x7fffffff, -1);
+    const ChunkWork w = chunk_work<kF32Rows, kF32Keys>(a);
+    if (w.b < 0) return;
+    f32_item<STORE, D>(a, wave_seq(a, w.b), w.b, w.hk, w.tile * kF32Rows, w.t_first, w.t_end, w.part);
   }
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void f32_join_kernel(PagedArgs a) {
+  join_chunk<float, kF32Rows, kF32Keys, D>(a);
 }
 
 // ---------------------------------------------------------------------------
@@ -1490,8 +967,7 @@ struct Launch {
   int sel_steps;          // select workgroups a (sequence, head)
   int part_rows, few_grid;
   bool join;              // a sequence's keys may be cut into pieces
-  int64_t tiles;          // chunk workgroups a kv head
-  int tiles_seq;          // of a sequence (batches without cu)
+  int64_t items, joins;   // chunk pieces and row tiles of cut sequences, over all kv heads, at most
   size_t list_bytes, part_bytes, ml_bytes, piece_bytes;
   size_t bytes() const { return list_bytes + part_bytes + ml_bytes + piece_bytes; }
 };
@@ -1557,12 +1033,22 @@ Launch plan_launch(const cra_cache* c, const cra_batch* b, const cra_paged_plan*
     }
     l.piece_bytes = up256(((int64_t)b->n_seqs + 1) * 4);
   }
-  const int BM = f32 ? kF32Rows : l.Dp > 128 ? 64 : 128;
-  if (b->cu_seqlens) {
-    l.tiles = (int64_t)b->tokens * l.grp / BM + b->n_seqs;
-  } else {
-    l.tiles_seq = (int)((most_rows + BM - 1) / BM);
-    l.tiles = (int64_t)l.tiles_seq * b->n_seqs;
+  if (l.chunk) {
+    const int BM = f32 ? kF32Rows : l.Dp > 128 ? 64 : 128, BN = f32 || l.Dp > 128 ? 32 : 64;
+    const int64_t tiles = b->cu_seqlens ? (int64_t)b->tokens * l.grp / BM + b->n_seqs
+                                        : (most_rows + BM - 1) / BM * b->n_seqs;
+    // a sequence is cut only from 16 key tiles on, and the pieces of cut ones are
+    // at most kChunkItems (chunk_find)
+    const int64_t local = std::min<int64_t>((int64_t)sp.W + BM / l.grp + 2, l.max_len);
+    const int64_t nk = (blocks * sp.rpb + BN - 1) / BN + (local + BN - 1) / BN + 1;
+    const bool cut = nk >= 16;
+    l.items = tiles * c->H_kv + (cut ? kChunkItems : 0);
+    l.joins = cut ? std::min<int64_t>(tiles * c->H_kv, kChunkItems / 2) : 0;
+    if (cut) {
+      const int64_t parts = std::min<int64_t>(kChunkItems, tiles * c->H_kv * (nk / 8)) * BM;
+      l.part_bytes = std::max(l.part_bytes, up256(parts * (int64_t)l.Dp * 4));
+      l.ml_bytes = std::max(l.ml_bytes, up256(parts * 2 * 4));
+    }
   }
   return l;
 }
@@ -1597,12 +1083,15 @@ hipError_t launch_rows(const PagedArgs& a, const Launch& l, int64_t bh, hipStrea
     }
   }
   if (l.chunk) {
-    const uint32_t grid = (uint32_t)(l.tiles * a.c.H_kv);
-    if constexpr (std::is_same<T, float>::value)
-      f32_kernel<STORE, D, false><<<grid, 256, 0, st>>>(a);
-    else
-      chunk_kernel<T, STORE, D><<<grid, 64 * kChunkWaves, 0, st>>>(a);
-    return hipGetLastError();
+    if constexpr (std::is_same<T, float>::value) {
+      f32_kernel<STORE, D, false><<<(uint32_t)l.items, 256, 0, st>>>(a);
+      if (hipError_t e = hipGetLastError()) return e;
+      if (l.joins) f32_join_kernel<D><<<(uint32_t)l.joins * (kF32Rows / kJoinRows), 256, 0, st>>>(a);
+      return hipGetLastError();
+    } else {
+      return launch_chunk(std::is_same<T, f16>::value ? CRA_F16 : CRA_BF16, STORE, D, a,
+                          (uint32_t)l.items, (uint32_t)l.joins, st);
+    }
   }
   return hipSuccess;
 }
@@ -1638,7 +1127,7 @@ int cra_fwd_paged(const cra_cache* c, const cra_batch* b, const cra_paged_plan* 
     return err(CRA_E_WORKSPACE, msg);
   }
   const int64_t bh = (int64_t)b->n_seqs * c->H_kv;
-  const int64_t most = std::max({bh * l.sel_steps, bh * l.part_rows, l.tiles * c->H_kv});
+  const int64_t most = std::max({bh * l.sel_steps, bh * l.part_rows, l.items});
   if (most >= (int64_t)1 << 24) return err(CRA_E_INVALID, "too many sequences or rows for one launch");
   PagedArgs a{};
   a.c = paged_view(c, b);
@@ -1659,8 +1148,6 @@ int cra_fwd_paged(const cra_cache* c, const cra_batch* b, const cra_paged_plan* 
   a.few_grid = std::max(1, l.few_grid);
   a.zero_outside = p->zero_outside != 0;
   a.few_only = !l.chunk;
-  a.tiles = l.tiles_seq;
-  a.d_tiles = fast_div(std::max(1, l.tiles_seq));
   hipStream_t st = (hipStream_t)stream;
   if (l.list) {
     a.d_steps = fast_div(l.sel_steps);

@@ -17,13 +17,13 @@ namespace cra {
 #define CRA_FWD_PF 3
 #endif
 
-template <typename T, int D, int BN, int QB>
+template <typename T, int D, int BN, int QB, int AHEAD = CRA_FWD_PF>
 __device__ __forceinline__ void tile_scores(const char* tK, const LaneOffs<D>& lo,
                                             const Frag<T> (&qf)[QB][D / 32], int kc,
                                             f32x4 (&s)[2][QB]) {
   using Tile = SwzTile<D, BN>;
   constexpr int NC = D / 32, NK = 2 * NC;
-  // K fragments are read CRA_FWD_PF steps ahead of the MFMAs that use them; fences
+  // K fragments are read AHEAD steps ahead of the MFMAs that use them; fences
   // keep the compiler from moving the reads next to their uses. Step t takes
   // key block t % 2 and D-chunk t / 2, so the four accumulators alternate and
   // each MFMA's accumulator was last written four MFMAs earlier (key block
@@ -31,7 +31,7 @@ __device__ __forceinline__ void tile_scores(const char* tK, const LaneOffs<D>& l
   auto k_frag = [&](int t) {
     return Tile::template row_frag_at<T>(tK + (2 * kc + t % 2) * Tile::kBlk16 + lo.row_at(t / 2));
   };
-  constexpr int PF = CRA_FWD_PF < NK ? CRA_FWD_PF : NK;
+  constexpr int PF = AHEAD < NK ? AHEAD : NK;
   Frag<T> kf[PF + 1];
 #pragma unroll
   for (int t = 0; t < PF; ++t) kf[t] = k_frag(t);
@@ -50,8 +50,8 @@ __device__ __forceinline__ void tile_scores(const char* tK, const LaneOffs<D>& l
 }
 
 // O^T += V^T . P^T for 32-key half kh: transposed V fragments read
-// CRA_FWD_PF steps ahead of the MFMAs that use them.
-template <typename T, int D, int BN, int QB>
+// AHEAD steps ahead of the MFMAs that use them.
+template <typename T, int D, int BN, int QB, int AHEAD = CRA_FWD_PF>
 __device__ __forceinline__ void pv_half(const char* tV, int kh, const LaneOffs<D>& lo,
                                         const Frag<T> (&pf)[QB], f32x4 (&acc)[D / 16][QB]) {
   using Tile = SwzTile<D, BN>;
@@ -60,7 +60,7 @@ __device__ __forceinline__ void pv_half(const char* tV, int kh, const LaneOffs<D
     const char* pa = tV + (2 * kh) * Tile::kBlk16 + lo.tr_at(db);
     return Tile::template tr_frag_at<T>(pa, pa + Tile::kBlk16);
   };
-  constexpr int PF = CRA_FWD_PF < NDB ? CRA_FWD_PF : NDB;
+  constexpr int PF = AHEAD < NDB ? AHEAD : NDB;
   Frag<T> vt[PF + 1];
 #pragma unroll
   for (int db = 0; db < PF; ++db) vt[db] = tr_v(db);
