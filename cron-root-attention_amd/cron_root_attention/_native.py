@@ -259,6 +259,18 @@ def attention_op():
     return _op_state["op"]
 
 
+_fast_state = {}
+
+
+def fast_op(name: str):
+    """``torch.ops.cra.<name>`` (rotary, cache_write, paged_attention), or None
+    without libcra_torch.so: the ctypes path then serves every call."""
+    if name not in _fast_state:
+        _fast_state[name] = (getattr(torch.ops.cra, name).default
+                             if attention_op() is not None else None)
+    return _fast_state[name]
+
+
 def _raise(code: int, func: str):
     lib = load_library()
     msg = (lib.cra_last_error() or b"").decode() or lib.cra_strerror(code).decode()

@@ -155,6 +155,12 @@ class PagedKVCache:
         """
         if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
             raise NotImplementedError("the cache has no backward; write under torch.no_grad()")
+        op = _native.fast_op("cache_write")
+        if op is not None and k.dtype == self.dtype and op(
+                k, v, self.k, self.v, self.k_norm, self.k_scale, self.v_scale, page_table, seq_lens,
+                cu_seqlens, self.head_dim):
+            return
+        # what the operator does not take (or nobody does: the checks say why)
         batch = _batch(self, k, self.n_kv_heads, page_table, seq_lens, cu_seqlens, "k")
         if v.shape != k.shape:
             raise ValueError(f"v shape {tuple(v.shape)} does not match k {tuple(k.shape)}")
@@ -281,6 +287,14 @@ def cron_root_attention_paged(q: torch.Tensor, cache: PagedKVCache, page_table: 
     if torch.is_grad_enabled() and q.requires_grad:
         raise NotImplementedError("cron_root_attention_paged has no backward; call it under "
                                   "torch.no_grad() (training: cron_root_attention)")
+    op = _native.fast_op("paged_attention")
+    if (op is not None and out is None and q.dtype == cache.dtype and window != 0
+            and max_query_len != 0 and max_seqlen != 0):
+        y = op(q, cache.k, cache.v, cache.k_norm, cache.k_scale, cache.v_scale, page_table, seq_lens,
+               cu_seqlens, cache.head_dim, max_query_len or 0, max_seqlen or 0, window or 0,
+               -1 if relay is None else int(bool(relay)), relay_top_k)
+        if y:
+            return y[0]
     batch = _batch(cache, q, None, page_table, seq_lens, cu_seqlens, "q")
     Hq, D = q.shape[1], q.shape[3]
     if Hq < 1 or Hq % cache.n_kv_heads:

@@ -253,6 +253,12 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], table: RotaryTa
 
     Returns: (q, k) turned, in their dtype and layout; without k only q.
     """
+    op = _native.fast_op("rotary") if type(table) is RotaryTable else None
+    if op is not None:
+        y = op(q, k, None, None, table.table, positions, table.interleaved, False, 0.0)
+        if y:
+            return y[0] if k is None else (y[0], y[1])
+    # what the operator does not take (or nobody does: the checks say why)
     _check_rows(q, k)
     if table is None:
         raise TypeError("table must be a RotaryTable")
@@ -279,6 +285,12 @@ def qk_norm_rotary(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: Optiona
 
     Returns: (q, k) in their dtype and layout; without k only q.
     """
+    op = _native.fast_op("rotary") if table is None or type(table) is RotaryTable else None
+    if op is not None:
+        y = op(q, k, q_weight, k_weight, None if table is None else table.table, positions,
+               table is not None and table.interleaved, True, eps)
+        if y:
+            return y[0] if k is None else (y[0], y[1])
     _check_rows(q, k)
     positions = _check_positions(q, table, positions)
     D = q.shape[3]
