@@ -1,9 +1,12 @@
 """nn.Module wrappers (reference module.py:1-247).
 
 ``CronRootAttention`` keeps the reference's constructor and forward
-(module.py:20-126) and adds two keyword arguments: ``hybrid`` (dispatch to
+(module.py:20-126) and adds keyword arguments: ``hybrid`` (dispatch to
 SDPA below the gfx950 crossover, as ``CronRootAttentionHybrid`` does) and
-``threshold``.  Grouped kv heads go to the kernel natively
+``threshold``; ``rotary`` (a :class:`RotaryTable`) and ``qk_norm`` (a norm of each
+head of q and k, with weights of its own), which stand between the projections
+and the attention; and ``cache`` and ``batch`` of forward, which serve new tokens
+over a :class:`PagedKVCache`.  Grouped kv heads go to the kernel natively
 (``kv_groups``) instead of being expanded with ``repeat_interleave``
 (module.py:111-113); query head h reads kv head h // kv_groups either way, so
 the result is the same.
@@ -18,6 +21,8 @@ import torch.nn.functional as F
 
 from .core import _layer_op
 from .hybrid import dispatch_backend
+from .paged import PagedBatch, PagedKVCache, cron_root_attention_paged
+from .rotary import RotaryTable, qk_norm_rotary, rotary_embedding
 
 
 class CronRootAttention(nn.Module):
@@ -25,7 +30,8 @@ class CronRootAttention(nn.Module):
 
     def __init__(self, d_model: int, n_heads: int, n_kv_heads: Optional[int] = None,
                  dropout: float = 0.0, bias: bool = False, hybrid: bool = False,
-                 threshold: Optional[int] = None):
+                 threshold: Optional[int] = None, rotary: Optional[RotaryTable] = None,
+                 qk_norm: bool = False, norm_eps: float = 1e-6):
         super().__init__()
         self.d_model = d_model
         self.n_heads = n_heads
@@ -42,6 +48,10 @@ class CronRootAttention(nn.Module):
         self.k_proj = nn.Linear(d_model, self.n_kv_heads * self.head_dim, bias=bias)
         self.v_proj = nn.Linear(d_model, self.n_kv_heads * self.head_dim, bias=bias)
         self.o_proj = nn.Linear(d_model, d_model, bias=bias)
+        self.rotary = rotary
+        self.norm_eps = norm_eps
+        self.q_norm = nn.Parameter(torch.ones(self.head_dim)) if qk_norm else None
+        self.k_norm = nn.Parameter(torch.ones(self.head_dim)) if qk_norm else None
         self._reset_parameters()
 
     def _reset_parameters(self):
@@ -60,13 +70,43 @@ class CronRootAttention(nn.Module):
                                 self.training and torch.is_grad_enabled(),
                                 x.shape[0] * self.n_heads, self.threshold)
 
-    def forward(self, x: torch.Tensor, kv: Optional[torch.Tensor] = None) -> torch.Tensor:
+    def _turned(self, q, k, positions):
+        """q and k normed and turned, as the layer was made to."""
+        if self.rotary is not None and self.rotary.device != q.device:
+            self.rotary = self.rotary.to(q.device)
+        if self.q_norm is not None:
+            return qk_norm_rotary(q, k, self.q_norm, self.k_norm, self.rotary, positions,
+                                  self.norm_eps)
+        if self.rotary is not None:
+            return rotary_embedding(q, k, self.rotary, positions)
+        return q, k
+
+    def forward(self, x: torch.Tensor, kv: Optional[torch.Tensor] = None,
+                positions: Optional[torch.Tensor] = None, cache: Optional[PagedKVCache] = None,
+                batch: Optional[PagedBatch] = None) -> torch.Tensor:
+        """x [B, S, d_model] -> [B, S, d_model].
+
+        ``positions`` (with ``rotary``): of the tokens, [S] or [B, S]; default 0 ..
+        S - 1, or with a cache the tokens' places in their sequences. With ``cache``
+        and ``batch`` x holds the new tokens of the batch's sequences, [N, S, d_model]
+        or (``cu_seqlens``) packed [1, T, d_model]: their keys and values are stored and
+        they attend to their sequences (no gradients)."""
         B, S, _ = x.shape
+        if (cache is None) != (batch is None):
+            raise ValueError("cache and batch belong together")
         kv = kv if kv is not None else x
         q = self.q_proj(x).view(B, S, self.n_heads, self.head_dim).transpose(1, 2)
         k = self.k_proj(kv).view(B, S, self.n_kv_heads, self.head_dim).transpose(1, 2)
         v = self.v_proj(kv).view(B, S, self.n_kv_heads, self.head_dim).transpose(1, 2)
-        if self.backend_for(x) == "sdpa":
+        if cache is not None and self.rotary is not None and positions is None:
+            positions = batch.positions(S)
+        q, k = self._turned(q, k, positions)
+        if cache is not None:
+            cache.write(k, v, batch.page_table, batch.seq_lens, batch.cu_seqlens)
+            out = cron_root_attention_paged(q, cache, batch.page_table, batch.seq_lens,
+                                            batch.cu_seqlens, batch.max_query_len, batch.max_seqlen,
+                                            batch.window, batch.relay)
+        elif self.backend_for(x) == "sdpa":
             out = F.scaled_dot_product_attention(q, k, v, is_causal=True,
                                                  enable_gqa=self.kv_groups > 1)
         else:
