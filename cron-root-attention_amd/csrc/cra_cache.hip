@@ -76,12 +76,26 @@ __device__ __forceinline__ uint32_t codes4(const float* x, float s) {
     c = __builtin_amdgcn_cvt_pk_fp8_f32(x[2] * inv, x[3] * inv, c, true);
     return (uint32_t)c;
   }
-  uint32_t r = 0;
+  // RNE(x / s) by a multiplication: x times the rounded 1 / s is within 2^-16 of
+  // x / s (at most 127), so the integers agree unless that is nearer than 2^-14
+  // to halfway between two; a wave that meets such an element divides.
+  const float inv = __fdiv_rn(1.f, s);
+  float q[4];
+  bool near = false;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float q = __builtin_rintf(__fdiv_rn(x[i], s));
-    r |= ((uint32_t)(int)fminf(fmaxf(q, -127.f), 127.f) & 0xffu) << (8 * i);
+    const float y = x[i] * inv;
+    q[i] = __builtin_rintf(y);
+    near |= !(fabsf(y - q[i]) < 0.5f - 0x1p-14f);
   }
+  if (__any(near)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = __builtin_rintf(__fdiv_rn(x[i], s));
+  }
+  uint32_t r = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    r |= ((uint32_t)(int)fminf(fmaxf(q[i], -127.f), 127.f) & 0xffu) << (8 * i);
   return r;
 }
 
@@ -120,25 +134,9 @@ __global__ __launch_bounds__(kThreads) void cache_write_kernel(WriteArgs a) {
     h = (int)div_by(r, a.dT);
     t = (int)(r - (uint32_t)h * a.c.tokens);
   }
-  int b, first, count, tb, ts;  // sequence, its first token and tokens; where the token lies in k and v
-  if (a.c.cu) {
-    b = seq_of_token(a.c.cu, a.c.n_seqs, t);
-    if (b < 0) return;
-    const TokenRange tr = token_range(a.c.cu, b, a.c.tokens);
-    first = tr.first, count = tr.last - tr.first;
-    tb = 0, ts = t;
-  } else {
-    b = (int)div_by(t, a.dM);
-    first = b * a.c.query_len, count = a.c.query_len;
-    tb = b, ts = t - first;
-  }
-  const int n = seq_length(a.c.lens[b], a.c.pages_per_seq, a.c.log_page);
-  const int row = n - count + (t - first);
-  const bool inside = row >= 0 && row < n;
-  const uint32_t dst = inside ? seq_row(a.c.table + b * a.c.table_stride, row, a.c.num_pages,
-                                        a.c.H_kv, a.c.log_page, h)
-                              : kNoRow;
-  if (dst == kNoRow) return;  // nothing of the row is written
+  // the rows are loaded before the place they go to is known: finding it takes four
+  // loads in turn (offsets, length, page id)
+  const int tb = a.c.cu ? 0 : (int)div_by(t, a.dM), ts = a.c.cu ? t : t - tb * a.c.query_len;
   Row8<T> kr, vr;
   float kx[8], vx[8];
   const bool have = lane * 8 < a.Din;
@@ -149,6 +147,20 @@ __global__ __launch_bounds__(kThreads) void cache_write_kernel(WriteArgs a) {
     kr.w[i] = have ? reinterpret_cast<const uint4*>(kp)[i] : make_uint4(0, 0, 0, 0);
     vr.w[i] = have ? reinterpret_cast<const uint4*>(vp)[i] : make_uint4(0, 0, 0, 0);
   }
+  int b = tb, first = tb * a.c.query_len, count = a.c.query_len;  // sequence, its first token and tokens
+  if (a.c.cu) {
+    b = seq_of_token(a.c.cu, a.c.n_seqs, t);
+    if (b < 0) return;
+    const TokenRange tr = token_range(a.c.cu, b, a.c.tokens);
+    first = tr.first, count = tr.last - tr.first;
+  }
+  const int n = seq_length(a.c.lens[b], a.c.pages_per_seq, a.c.log_page);
+  const int row = n - count + (t - first);
+  const bool inside = row >= 0 && row < n;
+  const uint32_t dst = inside ? seq_row(a.c.table + b * a.c.table_stride, row, a.c.num_pages,
+                                        a.c.H_kv, a.c.log_page, h)
+                              : kNoRow;
+  if (dst == kNoRow) return;  // nothing of the row is written
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     kx[i] = to_f32(reinterpret_cast<const T*>(kr.w)[i]);

@@ -14,10 +14,12 @@
 // Bound by memory: x in, y out (backward: x and dy in, dx out). A row belongs
 // to L lanes of a wave, each with the two V-element chunks of a pair of 16-byte
 // (or 8-, 4-byte) loads, so the rotation needs no exchange between lanes and
-// the norm's sum is log2(L) shuffles. A thread takes the same chunks of K heads
-// of one token: table row and weights are loaded once for them, and K rows of
-// loads are in flight. Threads of a wave go to neighbouring heads or tokens,
-// whichever lie closer in memory.
+// the norm's sum is log2(L) shuffles. Neighbouring rows of a wave are heads or
+// tokens, whichever lie closer in memory; the table row of a token is read again
+// for each head, from the caches. One row a thread: with several (table row and
+// weights loaded once for them) the registers cost more waves than the loads
+// save (S=32768 H=16/4 D=128 bf16, a training step with 1, 2, 4 heads a thread in
+// the backward: 218, 240, 270 us; in the forward 219, 217, 218).
 #include <stdio.h>
 
 #include <algorithm>
@@ -42,11 +44,11 @@ struct TurnTensor {
   const void* w;   // norm weights, or null
   float* partial;  // backward: [blocks, D] sums of dw, or null
   int64_t xsb, xsh, xss, dsb, dsh, dss, ysb, ysh, yss;
-  int H, HG;       // heads; groups of K heads
+  int H;           // heads
   int blocks;      // workgroups of this tensor
-  uint32_t items;  // B * S * HG
-  FastDiv dHG, dSHG;
-  int head_fast;   // neighbouring items are head groups of a token (else tokens)
+  uint32_t items;  // rows: B * S * H
+  FastDiv dH, dSH;
+  int head_fast;   // neighbouring rows are heads of a token (else tokens)
 };
 
 struct TurnArgs {
@@ -173,21 +175,20 @@ __device__ __forceinline__ float lanes_sum(float x, int log_l) {
 }
 
 struct Item {
-  int b, s, h0;
+  int b, s, h;
 };
-__device__ __forceinline__ Item item_at(const TurnArgs& g, const TurnTensor& t, uint32_t it, int K) {
+__device__ __forceinline__ Item item_at(const TurnArgs& g, const TurnTensor& t, uint32_t it) {
   Item r;
   if (t.head_fast) {
-    const uint32_t tok = div_by(it, t.dHG);
-    r.h0 = (int)(it - tok * t.HG) * K;
+    const uint32_t tok = div_by(it, t.dH);
+    r.h = (int)(it - tok * t.H);
     r.b = (int)div_by(tok, g.dS);
     r.s = (int)(tok - (uint32_t)r.b * g.S);
   } else {
-    r.b = (int)div_by(it, t.dSHG);
-    const uint32_t rest = it - (uint32_t)r.b * g.S * t.HG;
-    const uint32_t hg = div_by(rest, g.dS);
-    r.h0 = (int)hg * K;
-    r.s = (int)(rest - hg * g.S);
+    r.b = (int)div_by(it, t.dSH);
+    const uint32_t rest = it - (uint32_t)r.b * g.S * t.H;
+    r.h = (int)div_by(rest, g.dS);
+    r.s = (int)(rest - (uint32_t)r.h * g.S);
   }
   return r;
 }
@@ -255,8 +256,8 @@ __device__ __forceinline__ void load_pair(const T* p, const Unit& u, bool on, fl
   if (on && u.b) load_vec<T, V>(p + u.eb, b);
 }
 
-// V elements a chunk, U units a lane (more than one only for V = 1), K heads a thread.
-template <typename T, int V, int U, int K, bool NORM>
+// V elements a chunk, U units a lane (more than one only for V = 1).
+template <typename T, int V, int U, bool NORM>
 __global__ __launch_bounds__(kThreads) void turn_fwd_kernel(TurnArgs g) {
   const bool second = (int)blockIdx.x >= g.t[0].blocks;
   const TurnTensor& t = g.t[second];
@@ -264,55 +265,47 @@ __global__ __launch_bounds__(kThreads) void turn_fwd_kernel(TurnArgs g) {
   const int lane = threadIdx.x & ((1 << g.log_l) - 1), slot = threadIdx.x >> g.log_l;
   const uint32_t it = block * (kThreads >> g.log_l) + slot;
   const bool on = it < t.items;
-  const Item im = item_at(g, t, on ? it : t.items - 1, K);
+  const Item im = item_at(g, t, on ? it : t.items - 1);
   Unit un[U];
 #pragma unroll
   for (int j = 0; j < U; ++j) un[j] = unit_at<V>(g, lane + 64 * j);
 
-  const T* x = static_cast<const T*>(t.x) + im.b * t.xsb + im.s * t.xss;
-  float a[K][U][V], b[K][U][V];
+  const T* x = static_cast<const T*>(t.x) + im.b * t.xsb + im.s * t.xss + im.h * t.xsh;
+  float a[U][V], b[U][V];
 #pragma unroll
-  for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int j = 0; j < U; ++j)
-      load_pair<T, V>(x + (int64_t)(im.h0 + k) * t.xsh, un[j], on && im.h0 + k < t.H, a[k][j], b[k][j]);
+  for (int j = 0; j < U; ++j) load_pair<T, V>(x, un[j], on, a[j], b[j]);
   float c[U][V], s[U][V], wa[U][V], wb[U][V];
   load_turns<V, U>(g, table_row(g, im), lane, un, c, s);
-  if (NORM) load_weights<T, V, U>(g, t, un, wa, wb);
-
-  T* y = static_cast<T*>(t.y) + im.b * t.ysb + im.s * t.yss;
+  if (NORM) {
+    load_weights<T, V, U>(g, t, un, wa, wb);
+    float ss = 0.f;
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    if (NORM) {
-      float ss = 0.f;
+    for (int j = 0; j < U; ++j)
 #pragma unroll
-      for (int j = 0; j < U; ++j)
+      for (int i = 0; i < V; ++i) ss += a[j][i] * a[j][i] + b[j][i] * b[j][i];
+    const float r = rsqrtf(lanes_sum(ss, g.log_l) * g.inv_d + g.eps);
 #pragma unroll
-        for (int i = 0; i < V; ++i) ss += a[k][j][i] * a[k][j][i] + b[k][j][i] * b[k][j][i];
-      const float r = rsqrtf(lanes_sum(ss, g.log_l) * g.inv_d + g.eps);
+    for (int j = 0; j < U; ++j)
 #pragma unroll
-      for (int j = 0; j < U; ++j)
+      for (int i = 0; i < V; ++i) {
+        a[j][i] *= r * wa[j][i];
+        b[j][i] *= r * wb[j][i];
+      }
+  }
+  if (!on) return;
+  T* y = static_cast<T*>(t.y) + im.b * t.ysb + im.s * t.yss + im.h * t.ysh;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          a[k][j][i] *= r * wa[j][i];
-          b[k][j][i] *= r * wb[j][i];
-        }
-    }
-    if (!on || im.h0 + k >= t.H) continue;
-    T* row = y + (int64_t)(im.h0 + k) * t.ysh;
-#pragma unroll
-    for (int j = 0; j < U; ++j) {
-      if (un[j].turn) turn<V>(a[k][j], b[k][j], c[j], s[j], g.interleaved);
-      if (un[j].a) store_vec<T, V>(row + un[j].ea, a[k][j]);
-      if (un[j].b) store_vec<T, V>(row + un[j].eb, b[k][j]);
-    }
+  for (int j = 0; j < U; ++j) {
+    if (un[j].turn) turn<V>(a[j], b[j], c[j], s[j], g.interleaved);
+    if (un[j].a) store_vec<T, V>(y + un[j].ea, a[j]);
+    if (un[j].b) store_vec<T, V>(y + un[j].eb, b[j]);
   }
 }
 
 // Backward of norm + rotation. The workgroups of a tensor stride over its
-// items; each thread keeps the sums of dw of its chunks, added over the
+// rows; each thread keeps the sums of dw of its chunks, added over the
 // workgroup's rows in a fixed order and stored as one partial row.
-template <typename T, int V, int U, int K>
+template <typename T, int V, int U>
 __global__ __launch_bounds__(kThreads) void turn_bwd_kernel(TurnArgs g) {
   __shared__ float red[kThreads * 2 * V * U];
   const bool second = (int)blockIdx.x >= g.t[0].blocks;
@@ -335,57 +328,49 @@ __global__ __launch_bounds__(kThreads) void turn_bwd_kernel(TurnArgs g) {
   for (uint32_t base = block * slots; base < t.items; base += t.blocks * slots) {
     const uint32_t it = base + slot;
     const bool on = it < t.items;
-    const Item im = item_at(g, t, on ? it : t.items - 1, K);
-    const T* x = static_cast<const T*>(t.x) + im.b * t.xsb + im.s * t.xss;
-    const T* dy = static_cast<const T*>(t.dy) + im.b * t.dsb + im.s * t.dss;
-    float xa[K][U][V], xb[K][U][V], ga[K][U][V], gb[K][U][V], c[U][V], s[U][V];
+    const Item im = item_at(g, t, on ? it : t.items - 1);
+    const T* x = static_cast<const T*>(t.x) + im.b * t.xsb + im.s * t.xss + im.h * t.xsh;
+    const T* dy = static_cast<const T*>(t.dy) + im.b * t.dsb + im.s * t.dss + im.h * t.dsh;
+    float xa[U][V], xb[U][V], ga[U][V], gb[U][V], c[U][V], s[U][V];
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const bool row_on = on && im.h0 + k < t.H;
-        load_pair<T, V>(x + (int64_t)(im.h0 + k) * t.xsh, un[j], row_on, xa[k][j], xb[k][j]);
-        load_pair<T, V>(dy + (int64_t)(im.h0 + k) * t.dsh, un[j], row_on, ga[k][j], gb[k][j]);
-      }
+    for (int j = 0; j < U; ++j) {
+      load_pair<T, V>(x, un[j], on, xa[j], xb[j]);
+      load_pair<T, V>(dy, un[j], on, ga[j], gb[j]);
+    }
     load_turns<V, U>(g, table_row(g, im), lane, un, c, s);
-    T* y = static_cast<T*>(t.y) + im.b * t.ysb + im.s * t.yss;
+    float ss = 0.f;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const bool row_on = on && im.h0 + k < t.H;
-      float ss = 0.f;
+    for (int j = 0; j < U; ++j)
 #pragma unroll
-      for (int j = 0; j < U; ++j)
+      for (int i = 0; i < V; ++i) ss += xa[j][i] * xa[j][i] + xb[j][i] * xb[j][i];
+    const float r = rsqrtf(lanes_sum(ss, g.log_l) * g.inv_d + g.eps);
+    float dot = 0.f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) ss += xa[k][j][i] * xa[k][j][i] + xb[k][j][i] * xb[k][j][i];
-      const float r = rsqrtf(lanes_sum(ss, g.log_l) * g.inv_d + g.eps);
-      float dot = 0.f;
+    for (int j = 0; j < U; ++j) {
+      if (un[j].turn && on) turn<V>(ga[j], gb[j], c[j], s[j], g.interleaved);
 #pragma unroll
-      for (int j = 0; j < U; ++j) {
-        if (un[j].turn && row_on) turn<V>(ga[k][j], gb[k][j], c[j], s[j], g.interleaved);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          xa[k][j][i] *= r;
-          xb[k][j][i] *= r;
-          da[j][i] += ga[k][j][i] * xa[k][j][i];
-          db[j][i] += gb[k][j][i] * xb[k][j][i];
-          ga[k][j][i] *= wa[j][i];
-          gb[k][j][i] *= wb[j][i];
-          dot += ga[k][j][i] * xa[k][j][i] + gb[k][j][i] * xb[k][j][i];
-        }
+      for (int i = 0; i < V; ++i) {
+        xa[j][i] *= r;
+        xb[j][i] *= r;
+        da[j][i] += ga[j][i] * xa[j][i];
+        db[j][i] += gb[j][i] * xb[j][i];
+        ga[j][i] *= wa[j][i];
+        gb[j][i] *= wb[j][i];
+        dot += ga[j][i] * xa[j][i] + gb[j][i] * xb[j][i];
       }
-      dot = lanes_sum(dot, g.log_l) * g.inv_d;
-      if (!row_on) continue;
-      T* row = y + (int64_t)(im.h0 + k) * t.ysh;
+    }
+    dot = lanes_sum(dot, g.log_l) * g.inv_d;
+    if (!on) continue;
+    T* y = static_cast<T*>(t.y) + im.b * t.ysb + im.s * t.yss + im.h * t.ysh;
 #pragma unroll
-      for (int j = 0; j < U; ++j) {
+    for (int j = 0; j < U; ++j) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          ga[k][j][i] = r * (ga[k][j][i] - xa[k][j][i] * dot);
-          gb[k][j][i] = r * (gb[k][j][i] - xb[k][j][i] * dot);
-        }
-        if (un[j].a) store_vec<T, V>(row + un[j].ea, ga[k][j]);
-        if (un[j].b) store_vec<T, V>(row + un[j].eb, gb[k][j]);
+      for (int i = 0; i < V; ++i) {
+        ga[j][i] = r * (ga[j][i] - xa[j][i] * dot);
+        gb[j][i] = r * (gb[j][i] - xb[j][i] * dot);
       }
+      if (un[j].a) store_vec<T, V>(y + un[j].ea, ga[j]);
+      if (un[j].b) store_vec<T, V>(y + un[j].eb, gb[j]);
     }
   }
   if (!t.partial) return;
@@ -456,7 +441,7 @@ bool ptr_ok(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % 
 bool strides_ok(const cra_tensor& t, int v) { return t.sb % v == 0 && t.sh % v == 0 && t.ss % v == 0; }
 
 struct Shape {
-  int V, U, K, log_l, units;
+  int V, U, log_l, units;
 };
 
 // Elements a chunk: the widest load of at most 16 bytes that divides the
@@ -480,10 +465,6 @@ Shape shape_of(const cra_turn* p, const cra_tensor* const* ts, int n, const void
   while (s.log_l < 6 && (1 << s.log_l) < s.units) ++s.log_l;
   if (V == 1) s.log_l = 6;  // two units a lane
   s.U = V == 1 ? 2 : 1;
-  // four heads a thread where the chip is full all the same (256 CUs x 1024
-  // threads); one where it is not, for the latency of few rows
-  const int64_t threads = (int64_t)p->B * p->S * (p->H_q + p->H_kv) << s.log_l;
-  s.K = threads >= (int64_t)4 * 256 * 1024 ? 4 : 1;
   return s;
 }
 
@@ -508,7 +489,7 @@ void fill_args(TurnArgs& g, const cra_turn* p, const Shape& sh) {
   g.pss = p->pss;
 }
 
-void fill_tensor(TurnTensor& t, const cra_turn* p, const Shape& sh, int H, int K, const cra_tensor& x,
+void fill_tensor(TurnTensor& t, const cra_turn* p, const Shape& sh, int H, const cra_tensor& x,
                  const cra_tensor* dy, const cra_tensor& y, const void* w) {
   t.x = x.ptr;
   t.xsb = x.sb, t.xsh = x.sh, t.xss = x.ss;
@@ -517,10 +498,9 @@ void fill_tensor(TurnTensor& t, const cra_turn* p, const Shape& sh, int H, int K
   t.ysb = y.sb, t.ysh = y.sh, t.yss = y.ss;
   t.w = w;
   t.H = H;
-  t.HG = (H + K - 1) / K;
-  t.items = (uint32_t)p->B * p->S * t.HG;
-  t.dHG = fast_div(t.HG);
-  t.dSHG = fast_div((uint32_t)p->S * t.HG);
+  t.items = (uint32_t)p->B * p->S * H;
+  t.dH = fast_div(H);
+  t.dSH = fast_div((uint32_t)p->S * H);
   t.head_fast = y.sh < y.ss;
   const int slots = kThreads >> sh.log_l;
   t.blocks = (int)((t.items + slots - 1) / slots);
@@ -536,18 +516,18 @@ bool grid_fits(const TurnArgs& g) {
   return ((int64_t)g.t[0].blocks + g.t[1].blocks) * kThreads < (int64_t)1 << 32;
 }
 
-template <typename T, int V, int U, int K>
+template <typename T, int V, int U>
 hipError_t run_fwd(const TurnArgs& g, bool norm, hipStream_t st) {
   const int grid = g.t[0].blocks + g.t[1].blocks;
   if (norm)
-    turn_fwd_kernel<T, V, U, K, true><<<grid, kThreads, 0, st>>>(g);
+    turn_fwd_kernel<T, V, U, true><<<grid, kThreads, 0, st>>>(g);
   else
-    turn_fwd_kernel<T, V, U, K, false><<<grid, kThreads, 0, st>>>(g);
+    turn_fwd_kernel<T, V, U, false><<<grid, kThreads, 0, st>>>(g);
   return hipGetLastError();
 }
-template <typename T, int V, int U, int K>
+template <typename T, int V, int U>
 hipError_t run_bwd(const TurnArgs& g, hipStream_t st) {
-  turn_bwd_kernel<T, V, U, K><<<g.t[0].blocks + g.t[1].blocks, kThreads, 0, st>>>(g);
+  turn_bwd_kernel<T, V, U><<<g.t[0].blocks + g.t[1].blocks, kThreads, 0, st>>>(g);
   return hipGetLastError();
 }
 
@@ -558,9 +538,9 @@ hipError_t launch(int dtype, const Shape& s, const TurnArgs& g, bool norm, hipSt
     auto go = [&](auto v, auto u) {
       constexpr int V = decltype(v)::value, U = decltype(u)::value;
       if constexpr (BWD)
-        return s.K == 1 ? run_bwd<T, V, U, 1>(g, st) : run_bwd<T, V, U, 2>(g, st);
+        return run_bwd<T, V, U>(g, st);
       else
-        return s.K == 1 ? run_fwd<T, V, U, 1>(g, norm, st) : run_fwd<T, V, U, 4>(g, norm, st);
+        return run_fwd<T, V, U>(g, norm, st);
     };
     using I1 = std::integral_constant<int, 1>;
     if constexpr (sizeof(T) == 2)
@@ -616,8 +596,8 @@ int cra_rotary(const cra_turn* p, cra_tensor q, cra_tensor k, const void* wq, co
   TurnArgs g;
   fill_args(g, p, sh);
   g.neg = transpose != 0;
-  fill_tensor(g.t[0], p, sh, p->H_q, sh.K, q, nullptr, yq, ws[0]);
-  if (p->H_kv) fill_tensor(g.t[1], p, sh, p->H_kv, sh.K, k, nullptr, yk, ws[1]);
+  fill_tensor(g.t[0], p, sh, p->H_q, q, nullptr, yq, ws[0]);
+  if (p->H_kv) fill_tensor(g.t[1], p, sh, p->H_kv, k, nullptr, yk, ws[1]);
   if (!grid_fits(g)) return err(CRA_E_INVALID, "too many rows for one launch");
   return hip_err(launch<false>(p->dtype, sh, g, p->norm, (hipStream_t)stream), "cra_rotary");
 }
@@ -652,9 +632,8 @@ int cra_norm_rotary_bwd(const cra_turn* p, cra_tensor q, cra_tensor k, const voi
   TurnArgs g;
   fill_args(g, p, sh);
   g.neg = 1;
-  const int K = sh.K == 1 ? 1 : 2;
-  fill_tensor(g.t[0], p, sh, p->H_q, K, q, &dyq, dq, wq);
-  if (p->H_kv) fill_tensor(g.t[1], p, sh, p->H_kv, K, k, &dyk, dk, wk);
+  fill_tensor(g.t[0], p, sh, p->H_q, q, &dyq, dq, wq);
+  if (p->H_kv) fill_tensor(g.t[1], p, sh, p->H_kv, k, &dyk, dk, wk);
   share_blocks(g);
   float* part = static_cast<float*>(workspace);
   if (dwq) g.t[0].partial = part;
