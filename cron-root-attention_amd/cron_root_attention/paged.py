@@ -269,10 +269,11 @@ def cron_root_attention_paged(q: torch.Tensor, cache: PagedKVCache, page_table: 
             heads (query head h reads kv head h // (H_q / heads)).
         page_table, seq_lens, cu_seqlens: as in :meth:`PagedKVCache.write`.
         max_query_len: bound on a sequence's new tokens (with ``cu_seqlens``;
-            default T). At most 16 query rows a kv head run one kernel less.
+            default T). At most 16 query rows a kv head run one kernel less; a
+            sequence with more new tokens may give NaN.
         max_seqlen: bound on ``seq_lens`` (default: what a row of the table holds).
             A tighter bound makes for fewer, smaller pieces of work. A sequence
-            beyond a bound gives NaN.
+            longer than it gives NaN.
         window: None: ceil(sqrt(length)) of each sequence; else the window (and block
             size) of all, within their lengths.
         relay: None: relay rows for sequences of more than 2048 tokens; else on or off.

@@ -49,7 +49,8 @@ namespace {
 // rows with one page lookup, keeps the KEEP largest values by maximum and median
 // of three, and a picked value's row is found by comparing the lane's eight with
 // it. Against carrying rows along with the values, 64 rows at a time
-// (select_wide_kernel), 16 sequences of 700-131072 tokens, 8 heads: 23 -> WIDE us.
+// (select_wide_kernel): 16 sequences of 700-131072 tokens, 8 heads, 23.4 -> 16.6 us;
+// 64 of up to 32768 tokens 15.5 -> 11.4 us.
 // A block must fit one load of the wave; wider ones (windows above 505) go to
 // select_wide_kernel.
 // ---------------------------------------------------------------------------
@@ -289,10 +290,7 @@ __device__ __forceinline__ FewTiles few_tiles(const PagedArgs& a, int b) {
   // more rows than the caller's bound: one piece, which answers NaN
   if (rows == 0 || (rows > a.part_rows && !a.few_only)) return FewTiles{0, false};
   if (rows > a.part_rows) return FewTiles{0, true};
-  const SeqPlan p = get_plan(a, s.n);
-  const int G = s.n > 0 ? seq_prefix(s.n - 1, p) : 0;
-  const int lo = max(0, max(s.n - s.m, 0) - p.W + 1);
-  return FewTiles{((G + 31) >> 5) + ((s.n - lo + 31) >> 5), true};
+  return FewTiles{few_tile_count(s.n, s.m, get_plan(a, s.n)), true};
 }
 // The pieces of the call: tiles a piece, and pieces a kv head. Every wave adds
 // the sequences up, 64 at a time; the first 64 stay in registers (lane b).
@@ -968,6 +966,7 @@ struct Launch {
   int part_rows, few_grid;
   bool join;              // a sequence's keys may be cut into pieces
   int64_t items, joins;   // chunk pieces and row tiles of cut sequences, over all kv heads, at most
+  int64_t parts;          // pieces of cut sequences that the workspace holds
   size_t list_bytes, part_bytes, ml_bytes, piece_bytes;
   size_t bytes() const { return list_bytes + part_bytes + ml_bytes + piece_bytes; }
 };
@@ -990,6 +989,12 @@ int check_paged(const cra_cache* c, const cra_batch* b, const cra_paged_plan* p)
   const int64_t tokens = b->cu_seqlens ? b->tokens : (int64_t)b->n_seqs * b->query_len;
   if (tokens * (p->H_q / c->H_kv) >= (int64_t)1 << 30)
     return err(CRA_E_INVALID, "2^30 query rows of a kv head or more");
+  // sums of 64 sequences' tiles take 32 bits
+  const int64_t held = (int64_t)b->pages_per_seq * c->page_size;
+  const int most = (int)std::min<int64_t>(p->max_seqlen, std::min<int64_t>(held, 0x7fffffff));
+  const PlanMost pm = plan_most(most, p->window, p->relay, p->top_k);
+  if (pm.globals + pm.W >= (int64_t)1 << 30)
+    return err(CRA_E_INVALID, "2^30 keys of a query or more");
   return CRA_OK;
 }
 
@@ -1003,14 +1008,11 @@ Launch plan_launch(const cra_cache* c, const cra_batch* b, const cra_paged_plan*
   const int64_t most_rows = (int64_t)(b->cu_seqlens ? p->max_query_len : b->query_len) * l.grp;
   l.chunk = most_rows > kFewRows;
   l.few = b->cu_seqlens || !l.chunk;
-  const SeqPlan sp = seq_plan(l.max_len, p->window, p->relay, p->top_k);
-  const int64_t blocks = (std::max(0, l.max_len - sp.W) + (int64_t)sp.W - 1) / sp.W;
-  // shorter sequences have no more blocks under a fixed window, and at most
-  // ceil(sqrt(max_len)) under the rule
-  const int64_t cap = p->window > 0 ? blocks : ceil_sqrt(l.max_len);
-  l.list = sp.rpb > 1 && cap > 0;
-  l.list_cap = l.list ? cap * sp.rpb : 0;
-  l.wide = sp.W > kSelMost;  // no shorter sequence has wider blocks
+  const PlanMost pm = plan_most(l.max_len, p->window, p->relay, p->top_k);
+  const int64_t cap = pm.globals / pm.rpb;  // blocks
+  l.list = pm.rpb > 1 && cap > 0;
+  l.list_cap = l.list ? pm.globals : 0;
+  l.wide = pm.W > kSelMost;  // no shorter sequence has wider blocks
   const int64_t bh = (int64_t)b->n_seqs * c->H_kv;
   // a wave a block while that is at most 4096 workgroups: sixteen a CU hide the
   // loads' latency, more of them cost their launch
@@ -1020,8 +1022,7 @@ Launch plan_launch(const cra_cache* c, const cra_batch* b, const cra_paged_plan*
   if (l.few) {
     // the workgroups that are resident at once (LDS and registers allow two to
     // four a CU), but no more than there can be pieces of four tiles
-    const int64_t keys = blocks * sp.rpb + std::min<int64_t>((int64_t)sp.W + kFewRows, l.max_len);
-    const int64_t pieces = (keys / 32 + 2 + kFewWaves - 1) / kFewWaves;
+    const int64_t pieces = (few_tile_most(pm, kFewRows) + kFewWaves - 1) / kFewWaves;
     const int lds = kFewWaves * 64 * l.Dp * (f32 ? 2 : c->store == CRA_STORE_SAME ? 2 : 1);
     const int per_cu = lds > 80 * 1024 ? 1 : l.Dp >= 128 ? 2 : 4;
     l.few_grid = (int)std::min<int64_t>(256 * per_cu, bh * pieces);
@@ -1039,15 +1040,14 @@ Launch plan_launch(const cra_cache* c, const cra_batch* b, const cra_paged_plan*
                                         : (most_rows + BM - 1) / BM * b->n_seqs;
     // a sequence is cut only from 16 key tiles on, and the pieces of cut ones are
     // at most kChunkItems (chunk_find)
-    const int64_t local = std::min<int64_t>((int64_t)sp.W + BM / l.grp + 2, l.max_len);
-    const int64_t nk = (blocks * sp.rpb + BN - 1) / BN + (local + BN - 1) / BN + 1;
+    const int64_t nk = chunk_tile_most(pm, BM / l.grp + 2, BN);
     const bool cut = nk >= 16;
     l.items = tiles * c->H_kv + (cut ? kChunkItems : 0);
     l.joins = cut ? std::min<int64_t>(tiles * c->H_kv, kChunkItems / 2) : 0;
     if (cut) {
-      const int64_t parts = std::min<int64_t>(kChunkItems, tiles * c->H_kv * (nk / 8)) * BM;
-      l.part_bytes = std::max(l.part_bytes, up256(parts * (int64_t)l.Dp * 4));
-      l.ml_bytes = std::max(l.ml_bytes, up256(parts * 2 * 4));
+      l.parts = std::min<int64_t>(kChunkItems, tiles * c->H_kv * (nk / 8));
+      l.part_bytes = std::max(l.part_bytes, up256(l.parts * BM * (int64_t)l.Dp * 4));
+      l.ml_bytes = std::max(l.ml_bytes, up256(l.parts * BM * 2 * 4));
     }
   }
   return l;
@@ -1145,6 +1145,7 @@ int cra_fwd_paged(const cra_cache* c, const cra_batch* b, const cra_paged_plan* 
   a.part_ml = reinterpret_cast<float*>(ws + l.list_bytes + l.part_bytes);
   a.pieces = reinterpret_cast<int32_t*>(ws + l.list_bytes + l.part_bytes + l.ml_bytes);
   a.part_rows = l.part_rows;
+  a.parts = (int)l.parts;
   a.few_grid = std::max(1, l.few_grid);
   a.zero_outside = p->zero_outside != 0;
   a.few_only = !l.chunk;

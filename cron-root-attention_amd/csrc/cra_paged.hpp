@@ -96,6 +96,38 @@ __host__ __device__ inline int seq_prefix(int i, const SeqPlan& p) {
   return p.rpb * f + (ls != f * p.W ? 1 : 0);
 }
 
+// 32-key tiles of a sequence of n tokens, the last m of them new, that a row of
+// few_kernel meets; key tiles of BN rows that a row tile of the chunk kernels,
+// `span` new tokens wide, meets at most.
+__host__ __device__ inline int few_tile_count(int n, int m, const SeqPlan& p) {
+  const int pos0 = n - m > 0 ? n - m : 0, lo = pos0 - p.W + 1 > 0 ? pos0 - p.W + 1 : 0;
+  return ((n > 0 ? seq_prefix(n - 1, p) : 0) + 31) / 32 + (n - lo + 31) / 32;
+}
+__host__ __device__ inline int chunk_tile_count(int n, int span, int BN, const SeqPlan& p) {
+  const int64_t local = (int64_t)p.W + span;
+  return ((n > 0 ? seq_prefix(n - 1, p) : 0) + BN - 1) / BN + (int)(((local < n ? local : n) + BN - 1) / BN) + 1;
+}
+
+// The most of these over all lengths up to max_len: windows and the numbers of
+// blocks grow with the length.
+struct PlanMost {
+  int64_t globals;  // global rows
+  int W, max_len, rpb;
+};
+inline PlanMost plan_most(int max_len, int window, int relay, int top_k) {
+  const SeqPlan p = seq_plan(max_len, window, relay, top_k);
+  const int64_t below = max_len > p.W ? max_len - p.W : 0;
+  return PlanMost{(below + p.W - 1) / p.W * p.rpb, p.W, max_len, p.rpb};
+}
+inline int64_t few_tile_most(const PlanMost& m, int max_m) {
+  const int64_t local = (int64_t)m.W + max_m - 1;
+  return (m.globals + 31) / 32 + ((local < m.max_len ? local : m.max_len) + 31) / 32;
+}
+inline int64_t chunk_tile_most(const PlanMost& m, int span, int BN) {
+  const int64_t local = (int64_t)m.W + span;
+  return (m.globals + BN - 1) / BN + ((local < m.max_len ? local : m.max_len) + BN - 1) / BN + 1;
+}
+
 // Cache row of logical row `row` of a sequence whose table row is `pages`, or
 // kNoRow if its page lies outside the cache.
 __host__ __device__ inline uint32_t seq_row(const int32_t* pages, int row, int num_pages, int H_kv,

@@ -32,6 +32,7 @@ struct PagedArgs {
   float* part_ml;
   int32_t* pieces;  // [n_seqs + 1] first piece of each sequence (a kv head), for combine_kernel
   int part_rows, few_grid;
+  int parts;       // pieces of cut sequences (all kv heads) that the workspace holds
   int few_only;    // no chunk_kernel follows: longer sequences are refused (NaN)
   int zero_outside;  // rows of tokens outside every sequence are set to zero
 };
@@ -244,11 +245,7 @@ __device__ __forceinline__ ChunkSeq chunk_seq(const PagedArgs& a, int b) {
   const Seq s = get_seq(a, b);
   const int64_t rows = (int64_t)s.m * a.grp;
   if (rows <= kFewRows) return ChunkSeq{0, 0};
-  const SeqPlan p = get_plan(a, s.n);
-  const int G = s.n > 0 ? seq_prefix(s.n - 1, p) : 0;
-  const int64_t local = (int64_t)p.W + BM / a.grp + 2;
-  return ChunkSeq{(int)((rows + BM - 1) / BM),
-                  (G + BN - 1) / BN + (int)(((local < s.n ? local : s.n) + BN - 1) / BN) + 1};
+  return ChunkSeq{(int)((rows + BM - 1) / BM), chunk_tile_count(s.n, BM / a.grp + 2, BN, get_plan(a, s.n))};
 }
 
 struct ChunkFind {
@@ -267,9 +264,9 @@ __device__ __forceinline__ ChunkFind chunk_find(const PagedArgs& a, int idx) {
   uint64_t total = 0;
   for (int base = 0; base < a.c.n_seqs; base += 64) {
     const ChunkSeq c = base == 0 ? c0 : load(base);
-    const uint64_t all = (uint64_t)c.tiles * c.nk;  // far beyond any cut where it does not fit
-    total += (uint32_t)__builtin_amdgcn_readlane(
-        (int)wave_upto((uint32_t)(all < (1u << 25) ? all : 1u << 25)), 63);
+    const uint64_t all = (uint64_t)c.tiles * c.nk;  // below 2^50: summed in halves of 25 bits
+    total += (uint32_t)__builtin_amdgcn_readlane((int)wave_upto((uint32_t)(all & 0x1ffffffu)), 63);
+    total += (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)wave_upto((uint32_t)(all >> 25)), 63) << 25;
   }
   const uint64_t share = (total * a.c.H_kv + kChunkItems - 1) / kChunkItems;
   const int per = (int)(share < 8 ? 8 : share < (1u << 30) ? share : 1u << 30);
@@ -313,6 +310,9 @@ __device__ __forceinline__ ChunkWork chunk_work(const PagedArgs& a) {
   const ChunkFind f = chunk_find<BM, BN, false>(a, (int)item);
   w.b = f.b;
   if (f.b < 0) return w;
+  // offsets of tokens that run backwards may give more pieces than the call's
+  // tokens can have
+  if (f.pieces > 1 && (int64_t)(f.split0 + f.j + 1) * a.c.H_kv > a.parts) w.b = -1;
   const int t = f.j / f.pieces, piece = f.j - t * f.pieces;
   w.tile = f.tiles - 1 - t;
   w.t_first = f.pieces > 1 ? piece * f.len : 0;
@@ -331,7 +331,7 @@ __device__ void join_chunk(const PagedArgs& a) {
   const uint32_t item = div_by(block, a.d_hkv);
   const int hk = (int)(block - item * a.c.H_kv);
   const ChunkFind f = chunk_find<BM, BN, true>(a, (int)item);
-  if (f.b < 0) return;
+  if (f.b < 0 || (int64_t)(f.split0 + (f.j + 1) * f.pieces) * a.c.H_kv > a.parts) return;
   const Seq s = wave_seq(a, f.b);
   const int tile = f.tiles - 1 - f.j, rows = s.m * a.grp;
   const int64_t first = ((int64_t)(f.split0 + f.j * f.pieces) * a.c.H_kv + hk) * BM;

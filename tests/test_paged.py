@@ -57,6 +57,22 @@ int main() {
     bad += t.first < 0 || t.first > t.last || t.last > 10;
     ++cases;
   }
+  // the tiles of any sequence stay within what the launch reserves for the longest
+  for (int most : {1, 5, 16, 100, 676, 677, 2047, 2100, 2500, 5000})
+    for (int window : {0, 1, 3, 64, 700, 100000})
+      for (int relay : {-1, 0, 1}) {
+        const PlanMost pm = plan_most(most, window, relay, 3);
+        for (int n = 0; n <= most; ++n) {
+          const SeqPlan p = seq_plan(n, window, relay, 3);
+          bad += n > 0 && seq_prefix(n - 1, p) > pm.globals;
+          bad += p.W > pm.W;
+          for (int m : {1, 2, 16}) {
+            ++cases;
+            bad += few_tile_count(n, m, p) > few_tile_most(pm, 16);
+          }
+          for (int bn : {32, 64}) bad += chunk_tile_count(n, 10, bn, p) > chunk_tile_most(pm, 10, bn);
+        }
+      }
   // the sequence of a token, empty sequences among them
   const std::vector<int32_t> cu = {2, 2, 5, 5, 5, 9, 9};
   const int want[] = {-1, -1, 1, 1, 1, 4, 4, 4, 4, -1, -1};
@@ -159,6 +175,7 @@ def test_read_rejects(kw, code, msg):
     (dict(relay=1, top_k=9), "top_k"), (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"),
     (dict(max_seqlen=0), "max_seqlen"), (dict(cu_seqlens=P, tokens=5, max_query_len=0), "max_query_len"),
     (dict(n_seqs=1 << 14, query_len=1 << 15), "2^30"),
+    (dict(window=1 << 30, max_seqlen=1 << 30, pages_per_seq=1 << 24, table_stride=1 << 24), "2^30 keys"),
 ])
 def test_attention_rejects_plans(kw, msg):
     lib = N.load_library()

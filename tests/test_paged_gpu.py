@@ -371,6 +371,65 @@ def test_bad_pages_and_bounds_give_nan(dtype, store):
     assert got.isnan().all()
 
 
+@pytest.mark.parametrize("dtype,store", [(BF16, "same"), (F32, "same"), (F16, "int8")])
+def test_many_sequences(dtype, store):
+    """More sequences than a wave's lanes: single tokens, chunks, and both with empty sequences between them."""
+    g = random.Random(3)
+    lens = [g.choice([0, 1, 5, 33, 130, 300]) for _ in range(150)]
+    lens[77] = lens[130] = 2400
+    for kind in ("single", "mixed"):
+        new = [min(n, 1 if kind == "single" or b % 7 else g.randint(0, 30)) for b, n in enumerate(lens)]
+        s = Setup(lens, 2, 32, dtype, store, seed=5)
+        q = torch.randn(sum(new), 4, 32, generator=s.g).to(dtype)
+        check(run(s, q, new, max_query_len=max(new)), *s.expect(q, new), dtype)
+
+
+@pytest.mark.parametrize("dtype,store", [(F16, "same"), (BF16, "same"), (F32, "same"), (BF16, "e4m3"), (F16, "int8"),
+                                         (F32, "int8")])
+@pytest.mark.parametrize("D", [64, 256])
+def test_chunks_behind_long_wide_contexts(dtype, store, D):
+    """Few row tiles over thousands of keys each: their key ranges are cut into pieces and joined."""
+    s = Setup([3000, 70, 2000], 2, D, dtype, store, seed=D)
+    new = [40, 1, 90]
+    q = (1.5 * torch.randn(sum(new), 4, D, generator=s.g)).to(dtype)
+    for kw in (dict(window=1 << 30), dict(window=1900, relay=True), dict(window=3, relay=True, relay_top_k=4)):
+        okw = dict(window=kw["window"], relay=kw.get("relay"), top_k=kw.get("relay_top_k", 2))
+        good = run(s, q, new, max_seqlen=3000, **kw)
+        check(good, *s.expect(q, new, **okw), dtype)
+        assert torch.equal(run(s, q, new, max_seqlen=3000, **kw), good)
+    # a page outside the cache among the first piece's keys
+    s.dtable[0, 3] = -1
+    got = run(s, q, new, window=1 << 30)
+    assert got[:40].isnan().all() and not got[40:].isnan().any()
+
+
+@pytest.mark.parametrize("dtype,store", [(F16, "same"), (BF16, "e4m3"), (F32, "same")])
+@pytest.mark.parametrize("poison", [math.nan, math.inf])
+def test_unseen_rows_of_cut_chunks(dtype, store, poison):
+    """As above, with values that are not finite in rows that leave the window inside the chunk, and in the chunk."""
+    n, m, W = 3000, 40, 2000
+    s = Setup([n], 1, 64, dtype, store, seed=2)
+    q = torch.randn(m, 2, 64, generator=s.g).to(dtype)
+    o, mag = s.expect(q, [m], window=W, relay=False)
+    first, last = n - m - W + 1, n - 10  # seen by the first query alone; by the last ten
+    s.v[first, 0, 7] = s.v[last, 0, 7] = poison
+    s.k[last, 0, 9] = poison
+    s.write(s.k, s.v, [n], [0, n])
+    got = run(s, q, [m], window=W, relay=False)
+    mine = slice(1, m - 10)
+    check(got[mine], o[mine], mag[mine], dtype)
+    assert not got[0, :, 7].isfinite().any() and not got[m - 10:, :, 7].isfinite().any()
+
+
+@pytest.mark.parametrize("dtype,store", [(BF16, "same"), (F32, "e4m3")])
+def test_single_tokens_behind_long_wide_contexts(dtype, store):
+    s = Setup([5000, 3, 2500], 2, 64, dtype, store, seed=8)
+    q = torch.randn(3, 8, 64, generator=s.g).to(dtype)
+    for kw in (dict(window=1 << 30), dict(window=2, relay=True, relay_top_k=1)):
+        okw = dict(window=kw["window"], relay=kw.get("relay"), top_k=kw.get("relay_top_k", 2))
+        check(run(s, q, [1] * 3, max_query_len=1, **kw), *s.expect(q, [1] * 3, **okw), dtype)
+
+
 def test_repeated_pages():
     """Sequences that share their first pages, and a table that names one page twice."""
     s = Setup([64, 64], 1, 64, BF16)
