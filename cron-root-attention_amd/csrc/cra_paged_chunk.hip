@@ -9,7 +9,12 @@
 // straight into LDS (8-bit codes go through registers and are widened on the way).
 // The rows' cache rows are looked up a tile ahead of their loads.
 //
-// Bound by the matrix core and the VALU beside it. The fast loop takes no care of
+// Bound by the matrix core, the VALU beside it and the waits between them (two waves
+// a SIMD): 8192 new tokens of 131072, 16 heads, D = 128 fp16: 156 us, 606 TFLOP/s
+// (a large matrix product: 1118); two dense chunks of 1000 and 513 tokens among 14
+// single tokens, 16/4 heads, int8 store: 300 us, about 520 TFLOP/s, widening
+// included (codes widened on their way from a second stage of them while the next
+// loads ran, two turns unrolled: 310 us, eight registers spilled). The fast loop takes no care of
 // elements that are not finite in rows that some queries do not see: 0 times them
 // leaves NaN in the result, which is looked for once at the end; a wave that finds
 // it computes its rows again one by one, over the keys that each sees (careful_row).
@@ -253,12 +258,12 @@ void chunk_kernel(PagedArgs a) {
   constexpr int NW = kChunkWaves, QB = kChunkQB<D>, BN = kChunkBN<D>, kQW = 16 * QB, BM = NW * kQW;
   using Tile = SwzTile<D, BN>;
   constexpr bool k8 = STORE != kSame;
-  // 16-bit: two stages of K and V tiles. 8-bit: one, and two of the codes as they
-  // are loaded, which make the same 64 KB at D = 128 (two workgroups a CU)
+  // 16-bit: two stages of K and V tiles, one filled while the other is read. 8-bit:
+  // one, and one of the codes as they are loaded: widening empties it before the
+  // next tile's loads
   __shared__ __attribute__((aligned(1024))) char stage0[2][Tile::kBytes];
   __shared__ __attribute__((aligned(1024))) char stage1[2][k8 ? 16 : Tile::kBytes];
-  __shared__ __attribute__((aligned(1024))) char raw0[2][k8 ? BN * D : 16];
-  __shared__ __attribute__((aligned(1024))) char raw1[2][k8 ? BN * D : 16];
+  __shared__ __attribute__((aligned(1024))) char raw[2][k8 ? BN * D : 16];
   __shared__ __attribute__((aligned(16))) float kscale[2][BN], vscale[2][BN];
   __shared__ uint32_t slots[2][BN];
   __shared__ int2 reach[BM];  // of each row: position, global rows seen (masked tiles read it)
@@ -331,7 +336,7 @@ void chunk_kernel(PagedArgs a) {
       }
     }
   };
-  auto widen = [&](const auto& raw, const float (&vs)[BN]) {
+  auto widen = [&](const float (&vs)[BN]) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int piece = i * 64 * NW + tid, row = piece / kPiecesRow, col = piece % kPiecesRow;
@@ -368,8 +373,7 @@ void chunk_kernel(PagedArgs a) {
         reinterpret_cast<uint4*>(&x[0][0])[i] = make_uint4(0, 0, 0, 0);
     };
     if constexpr (k8) {
-      clear(raw0);
-      clear(raw1);
+      clear(raw);
     } else {
       clear(stage0);
       clear(stage1);
@@ -416,7 +420,7 @@ void chunk_kernel(PagedArgs a) {
     if (w.t_first + 1 < ntot) keep(w.t_first + 1, look_up(w.t_first + 1));
     __syncthreads();
     if constexpr (k8)
-      issue(w.t_first, raw0);
+      issue(w.t_first, raw);
     else
       issue(w.t_first, stage0);
     load_scales(w.t_first);
@@ -433,19 +437,13 @@ void chunk_kernel(PagedArgs a) {
       if (it + 2 < ntot) ahead = look_up(it + 2);
     };
     if constexpr (k8) {
-      if constexpr (kS) {
-        refill(raw0);
-        widen(raw1, vscale[it & 1]);
-      } else {
-        refill(raw1);
-        widen(raw0, vscale[it & 1]);
-      }
+      widen(vscale[it & 1]);
       __syncthreads();
+      refill(raw);
+    } else if constexpr (kS) {
+      refill(stage0);
     } else {
-      if constexpr (kS)
-        refill(stage0);
-      else
-        refill(stage1);
+      refill(stage1);
     }
     const char *tK = stage0[0], *tV = stage0[1];
     if constexpr (!k8 && kS) tK = stage1[0], tV = stage1[1];
@@ -478,9 +476,13 @@ void chunk_kernel(PagedArgs a) {
     if (it + 1 < ntot) keep_scales(it + 1);
     if (it + 2 < ntot) keep(it + 2, ahead);
   };
-  for (int it = w.t_first; it < ntot; it += 2) {
-    turn(std::false_type{}, it);
-    if (it + 1 < ntot) turn(std::true_type{}, it + 1);
+  if constexpr (k8) {
+    for (int it = w.t_first; it < ntot; ++it) turn(std::false_type{}, it);
+  } else {
+    for (int it = w.t_first; it < ntot; it += 2) {
+      turn(std::false_type{}, it);
+      if (it + 1 < ntot) turn(std::true_type{}, it + 1);
+    }
   }
   bool odd = false;
 #pragma unroll

@@ -130,10 +130,9 @@ __device__ __forceinline__ uint2 widen4(uint32_t w) {  // four codes -> four ele
     }
   } else {
     typedef T t2 __attribute__((ext_vector_type(2)));
-    const uint32_t u = w ^ 0x80808080u;
     float f[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = (float)(u >> (8 * i) & 0xffu) - 128.f;
+    for (int i = 0; i < 4; ++i) f[i] = (float)(int8_t)(w >> (8 * i) & 0xffu);
     r.x = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{f[0], f[1]}, t2));
     r.y = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{f[2], f[3]}, t2));
   }
