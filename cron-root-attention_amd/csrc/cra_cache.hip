@@ -13,8 +13,13 @@
 //   int8: s = m / 127, c = RNE(x / s).
 // s is at least 2^-126. A row that holds an infinity or NaN gets s = NaN.
 //
-// Bound by memory; a row belongs to D/8 lanes (a power of two), 16 bytes of k
-// and of v each.
+// Bound by memory, an int8 write nearly as much by the VALU; a row belongs to D/8
+// lanes (a power of two), 16 bytes of k and of v each. Measured, D = 128 16-bit:
+// writes of 32768 tokens of 16 heads as int8 101 us (407 MB, 4.0 TB/s; dividing each
+// element and exchanging by LDS shuffles 146 us), of 26000 ragged tokens of 4
+// heads as e4m3 30 us; reads 160 us (814 MB, 5.1 TB/s) and 46 us (16 sequences of
+// up to 9001 rows, padded: 322 MB). Two or four rows a thread gave nothing (146, 159
+// against 146 us), nor did neighbouring tokens in place of heads (152-160 us).
 #include <stdio.h>
 
 #include <algorithm>
@@ -42,7 +47,6 @@ struct WriteArgs {
   int head_fast;
 };
 
-// Row of 8 elements a lane into 8-bit codes. Returns the scale.
 enum { kSame = CRA_STORE_SAME, kE4M3 = CRA_STORE_E4M3, kInt8 = CRA_STORE_INT8 };
 
 template <typename T>
@@ -50,9 +54,36 @@ struct Row8 {
   uint4 w[sizeof(T) / 2];
 };
 
-__device__ __forceinline__ uint32_t lanes_max(uint32_t x, int log_l) {
-  for (int o = 1 << log_l >> 1; o > 0; o >>= 1) x = max(x, (uint32_t)__shfl_xor((int)x, o));
+// The value of the lane whose number differs in bit O, within groups of 2 O lanes and
+// more: row shifts in the VALU.
+template <int O>
+__device__ __forceinline__ uint32_t from_lane_xor(uint32_t x) {
+  const int v = (int)x;
+  if constexpr (O == 1) return (uint32_t)__builtin_amdgcn_update_dpp(v, v, 0xb1, 0xf, 0xf, false);  // quad 1 0 3 2
+  if constexpr (O == 2) return (uint32_t)__builtin_amdgcn_update_dpp(v, v, 0x4e, 0xf, 0xf, false);  // quad 2 3 0 1
+  if constexpr (O == 4) {  // banks of four lanes: even ones from above, odd ones from below
+    const int up = __builtin_amdgcn_update_dpp(v, v, 0x104, 0xf, 0x5, false);  // row_shl:4
+    return (uint32_t)__builtin_amdgcn_update_dpp(up, v, 0x114, 0xf, 0xa, false);  // row_shr:4
+  }
+  if constexpr (O == 8) return (uint32_t)__builtin_amdgcn_update_dpp(v, v, 0x128, 0xf, 0xf, false);  // row_ror:8
+  return (uint32_t)__shfl_xor(v, O);
+}
+template <typename F>
+__device__ __forceinline__ uint32_t lanes_fold(uint32_t x, int log_l, F f) {
+  if (log_l > 4) x = f(x, from_lane_xor<16>(x));
+  if (log_l > 3) x = f(x, from_lane_xor<8>(x));
+  if (log_l > 2) x = f(x, from_lane_xor<4>(x));
+  if (log_l > 1) x = f(x, from_lane_xor<2>(x));
+  if (log_l > 0) x = f(x, from_lane_xor<1>(x));
   return x;
+}
+__device__ __forceinline__ uint32_t lanes_max(uint32_t x, int log_l) {
+  return lanes_fold(x, log_l, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
+__device__ __forceinline__ float lanes_sum(float x, int log_l) {
+  return __uint_as_float(lanes_fold(__float_as_uint(x), log_l, [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__fadd_rn(__uint_as_float(a), __uint_as_float(b)));
+  }));
 }
 
 // Scale of a row from the bits of max |x| (which order as the values do, NaN
@@ -76,27 +107,26 @@ __device__ __forceinline__ uint32_t codes4(const float* x, float s) {
     c = __builtin_amdgcn_cvt_pk_fp8_f32(x[2] * inv, x[3] * inv, c, true);
     return (uint32_t)c;
   }
-  // RNE(x / s) by a multiplication: x times the rounded 1 / s is within 2^-16 of
-  // x / s (at most 127), so the integers agree unless that is nearer than 2^-14
-  // to halfway between two; a wave that meets such an element divides.
-  const float inv = __fdiv_rn(1.f, s);
-  float q[4];
-  bool near = false;
+  // RNE(x / s) by a multiplication: x times the reciprocal (one ulp off) is within
+  // 2^-14 of x / s (at most 127), so the integers agree unless that is nearer than
+  // 2^-12 to halfway between two; a wave that meets such an element divides. Adding
+  // 1.5 * 2^23 rounds to the integer and leaves it in the low byte.
+  constexpr float kMagic = 12582912.f;
+  const float inv = __builtin_amdgcn_rcpf(s);
+  float q[4], off = 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float y = x[i] * inv;
-    q[i] = __builtin_rintf(y);
-    near |= !(fabsf(y - q[i]) < 0.5f - 0x1p-14f);
+    q[i] = y + kMagic;
+    off = fmaxf(off, fabsf(y - (q[i] - kMagic)));
   }
-  if (__any(near)) {
+  if (__any(off > 0.5f - 0x1p-12f)) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) q[i] = __builtin_rintf(__fdiv_rn(x[i], s));
+    for (int i = 0; i < 4; ++i) q[i] = __fadd_rn(__fdiv_rn(x[i], s), kMagic);
   }
-  uint32_t r = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    r |= ((uint32_t)(int)fminf(fmaxf(q[i], -127.f), 127.f) & 0xffu) << (8 * i);
-  return r;
+  const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(q[1]), __float_as_uint(q[0]), 0x0c0c0400);
+  const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(q[3]), __float_as_uint(q[2]), 0x04000c0c);
+  return lo | hi;
 }
 
 template <typename T, int STORE>
@@ -149,7 +179,12 @@ __global__ __launch_bounds__(kThreads) void cache_write_kernel(WriteArgs a) {
   }
   int b = tb, first = tb * a.c.query_len, count = a.c.query_len;  // sequence, its first token and tokens
   if (a.c.cu) {
-    b = seq_of_token(a.c.cu, a.c.n_seqs, t);
+    const int at = threadIdx.x & 63 & ~lane;  // the row's lanes within the wave
+    b = seq_of_token(a.c.cu, a.c.n_seqs, t, 1 << a.log_l, [&](int first, int step, int n) {
+      const int64_t i = (int64_t)lane * step;
+      const uint64_t m = __ballot(i < n && a.c.cu[first + (i < n ? i : 0)] <= t) >> at;
+      return __popcll(m & ((1ull << (1 << a.log_l)) - 1));
+    });
     if (b < 0) return;
     const TokenRange tr = token_range(a.c.cu, b, a.c.tokens);
     first = tr.first, count = tr.last - tr.first;
@@ -169,7 +204,7 @@ __global__ __launch_bounds__(kThreads) void cache_write_kernel(WriteArgs a) {
   float norm = kx[0] * kx[0];
 #pragma unroll
   for (int i = 1; i < 8; ++i) norm = __builtin_fmaf(kx[i], kx[i], norm);
-  for (int o = 1 << a.log_l >> 1; o > 0; o >>= 1) norm = __fadd_rn(norm, __shfl_xor(norm, o));
+  norm = lanes_sum(norm, a.log_l);
   if (lane == 0) a.k_norm[dst] = norm;
   store_row<T, STORE>(kx, kr, const_cast<char*>(a.c.k), a.k_scale, dst, a.Ds, lane, a.log_l);
   store_row<T, STORE>(vx, vr, const_cast<char*>(a.c.v), a.v_scale, dst, a.Ds, lane, a.log_l);

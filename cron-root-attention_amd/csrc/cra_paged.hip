@@ -275,6 +275,9 @@ __global__ __launch_bounds__(64 * kSelWaves) void select_wide_kernel(PagedArgs a
 // barrier until the piece's end; the 16-column operand Q^T holds the rows.
 // Bound by memory latency and bandwidth: the rows seen, once per kv head. The
 // waves' results, and those of a sequence's pieces, are joined by their maxima.
+// Measured (D = 128, with combine_kernel's 4-5 us behind it): one token of 131072, 16
+// heads fp16 8 us; 64 of 1-32768, 32/8 heads bf16 15 us; 16 of 700-131072 over an
+// e4m3 store 15.5 us; 14 sequences of 1-20000, dense, 16/4 heads, int8 22 us + 12 us.
 // ---------------------------------------------------------------------------
 constexpr int kFewWaves = 4;
 

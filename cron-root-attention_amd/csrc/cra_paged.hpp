@@ -53,15 +53,18 @@ __host__ __device__ inline TokenRange token_range(const int32_t* cu, int b, int 
 }
 
 // Sequence of packed token t: the last b with cu[b] <= t, or -1 for a token
-// before the first or behind the last sequence.
-__host__ __device__ inline int seq_of_token(const int32_t* cu, int n_seqs, int t) {
-  if (t < cu[0] || t >= cu[n_seqs]) return -1;
-  int lo = 0, hi = n_seqs - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (cu[mid] <= t) lo = mid; else hi = mid - 1;
+// before the first or behind the last sequence. `lanes` offsets are looked at at
+// a time: upto(first, step, n) counts those of cu[first + i step] <= t, i < lanes,
+// i step < n (at least the first, whatever it answers).
+template <typename F>
+__host__ __device__ inline int seq_of_token(const int32_t* cu, int n_seqs, int t, int lanes, F upto) {
+  int lo = 0, n = n_seqs;
+  while (n > 1) {
+    const int step = (n + lanes - 1) / lanes, c = upto(lo, step, n), skip = (c > 1 ? c - 1 : 0) * step;
+    lo += skip;
+    n = step < n - skip ? step : n - skip;
   }
-  return lo;
+  return t < cu[0] || t >= cu[n_seqs] ? -1 : lo;
 }
 
 // ceil(sqrt(n)), n >= 0: the float root is within one of it, squares of up to

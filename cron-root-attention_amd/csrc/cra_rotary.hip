@@ -11,7 +11,8 @@
 //   dw = sum over rows of dz * xhat,  xhat = x r,
 //   dx = r (g - xhat mean(g xhat)),  g = dz * w.
 //
-// Bound by memory: x in, y out (backward: x and dy in, dx out). A row belongs
+// Bound by memory: x in, y out (backward: x and dy in, dx out): S=32768 H=16/4 D=128
+// bf16 with the norm 73 us (4.8 TB/s) and 122 us + 6 us for dw (4.3 TB/s). A row belongs
 // to L lanes of a wave, each with the two V-element chunks of a pair of 16-byte
 // (or 8-, 4-byte) loads, so the rotation needs no exchange between lanes and
 // the norm's sum is log2(L) shuffles. Neighbouring rows of a wave are heads or

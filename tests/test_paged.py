@@ -76,7 +76,35 @@ int main() {
   // the sequence of a token, empty sequences among them
   const std::vector<int32_t> cu = {2, 2, 5, 5, 5, 9, 9};
   const int want[] = {-1, -1, 1, 1, 1, 4, 4, 4, 4, -1, -1};
-  for (int t = 0; t < 11; ++t) bad += seq_of_token(cu.data(), 6, t) != want[t];
+  auto find = [](const std::vector<int32_t>& cu, int t, int lanes) {
+    const int n_seqs = (int)cu.size() - 1;
+    return seq_of_token(cu.data(), n_seqs, t, lanes, [&](int first, int step, int n) {
+      int c = 0;
+      for (int i = 0; i < lanes && (int64_t)i * step < n; ++i) c += cu[first + i * step] <= t;
+      return c;
+    });
+  };
+  for (int lanes : {2, 4, 32})
+    for (int t = 0; t < 11; ++t) bad += find(cu, t, lanes) != want[t];
+  for (int n_seqs : {1, 2, 3, 15, 16, 17, 64, 65, 300, 1025}) {
+    std::vector<int32_t> many(1, 3);
+    std::vector<int> owner(3, -1);
+    for (int b = 0; b < n_seqs; ++b) {
+      const int m = b * 7 % 5;
+      owner.insert(owner.end(), m, b);
+      many.push_back(many.back() + m);
+    }
+    owner.insert(owner.end(), 2, -1);
+    for (int lanes : {2, 4, 8, 16, 32})
+      for (int t = 0; t < (int)owner.size(); ++t, ++cases) bad += find(many, t, lanes) != owner[t];
+  }
+  // offsets that run backwards: some sequence of the batch
+  const std::vector<int32_t> back = {0, 90, 5, 70, -4, 2147483647, 3, 60, 20, 100};
+  for (int lanes : {2, 4, 8})
+    for (int t = 0; t < 100; ++t) {
+      const int b = find(back, t, lanes);
+      bad += b < 0 || b > 8;
+    }
   // rows of pages: in the page's place, and none of a page outside the cache
   const int32_t pages[] = {7, -1, 12, 11, 2147483647, -2147483647 - 1};
   bad += seq_row(pages, 5, 12, 3, 4, 2) != (7u * 3 + 2) * 16 + 5;
