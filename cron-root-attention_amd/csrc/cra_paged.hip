@@ -277,7 +277,7 @@ __global__ __launch_bounds__(64 * kSelWaves) void select_wide_kernel(PagedArgs a
 // waves' results, and those of a sequence's pieces, are joined by their maxima.
 // Measured (D = 128, with combine_kernel's 4-5 us behind it): one token of 131072, 16
 // heads fp16 8 us; 64 of 1-32768, 32/8 heads bf16 15 us; 16 of 700-131072 over an
-// e4m3 store 15.5 us; 14 sequences of 1-20000, dense, 16/4 heads, int8 22 us + 12 us.
+// e4m3 store 15.5 us; 14 sequences of 1-20000, dense, 16/4 heads, int8 23 us + 6 us.
 // ---------------------------------------------------------------------------
 constexpr int kFewWaves = 4;
 
@@ -689,12 +689,13 @@ __global__ __launch_bounds__(256) void combine_kernel(PagedArgs a, int Dp) {
   const int quads = Dp / 4, lanes = 256 / quads;  // groups of pieces
   const int quad = tid % quads, sg = tid / quads;
   auto at = [&](int i) { return ((int64_t)(first + i) * a.c.H_kv + hk) * a.part_rows + r; };
-  float M = -kInf;
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) M = fmaxf(M, a.part_ml[2 * at(i)]);
+  float M = -kInf;  // a lane a piece, each wave for itself
+  for (int i = tid & 63; i < n; i += 64) M = fmaxf(M, a.part_ml[2 * at(i)]);
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor(M, d));
   float L = 0.f;
   f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
+#pragma unroll 4
   for (int i = sg; i < n; i += lanes) {
     const float mi = a.part_ml[2 * at(i)];
     const float e = mi == -kInf ? 0.f : __builtin_amdgcn_exp2f(mi - M);
