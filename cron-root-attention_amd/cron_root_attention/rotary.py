@@ -182,7 +182,8 @@ class RotaryFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, table, positions):
-        ctx.table, ctx.positions = table, positions
+        ctx.table = table
+        ctx.save_for_backward(table.table, positions)  # a change before the backward raises
         ctx.set_materialize_grads(False)
         q, k = _rows(q), _rows(k)
         ctx.dtype = q.dtype
@@ -195,8 +196,9 @@ class RotaryFunction(torch.autograd.Function):
         if not one:
             return None, None, None, None
         one = [_rows(x.to(ctx.dtype)) for x in one]
+        _, positions = ctx.saved_tensors
         y = _native.rotary(_problem(one[0], one[1] if len(one) > 1 else None, ctx.table,
-                                    ctx.positions, False, ctx.dtype, 0.0),
+                                    positions, False, ctx.dtype, 0.0),
                            one[0], one[1] if len(one) > 1 else None, None, None, transpose=True)
         if len(one) == 2:
             return y[0], y[1], None, None
@@ -209,17 +211,17 @@ class NormRotaryFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, wq, wk, table, positions, eps):
         q, k = _rows(q), _rows(k)
-        ctx.args = table, positions, eps
+        ctx.args = table, eps
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(q, k, wq, wk)
+        ctx.save_for_backward(q, k, wq, wk, None if table is None else table.table, positions)
         return _native.rotary(_problem(q, k, table, positions, True, _weight_dtype(q, wq, wk), eps),
                               q, k, wq, wk)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dyq, dyk):
-        q, k, wq, wk = ctx.saved_tensors
-        table, positions, eps = ctx.args
+        q, k, wq, wk, _, positions = ctx.saved_tensors
+        table, eps = ctx.args
         if dyq is None and dyk is None:
             return (None,) * 7
         q, k = _rows(q), _rows(k)  # layouts that a saved-tensor hook changed

@@ -131,8 +131,8 @@ def test_norm_rotary_forward_and_backward(B, Hq, Hkv, S, D, rot, dtype, wdtype, 
         close(gw, ref, (nrow + D / 2 + 16) * U * (dmag * hat.abs()).sum((0, 1, 2)), "dw" + n)
 
 
-def test_many_rows_take_several_heads_a_thread():
-    """Row counts from which a thread takes four (backward: two) heads, with a head count that leaves a rest."""
+def test_many_rows():
+    """More rows than the backward has workgroups: each strides over several; the weights' gradients over all of them."""
     g = torch.Generator(device=DEV).manual_seed(3)
     B, Hq, Hkv, S, D = 2, 7, 5, 6000, 128
     q, k = (torch.randn(B, H, S, D, generator=g, device=DEV).bfloat16() for H in (Hq, Hkv))
@@ -142,7 +142,7 @@ def test_many_rows_take_several_heads_a_thread():
     leaves = [x.requires_grad_(True) for x in (q, k, wq, wk)]
     y = cra.qk_norm_rotary(q, k, wq, wk, table)
     got = torch.autograd.grad(y, leaves, (dq, dk))
-    # the same rows in small calls, one head a thread
+    # the same rows in small calls
     for h in (0, 3, 6):
         sl = q.detach()[:1, h:h + 1, 5000:5100]
         one = cra.qk_norm_rotary(sl, None, wq.detach(), None, table, torch.arange(5000, 5100, device=DEV))
@@ -272,3 +272,27 @@ def test_captured_step_replays():
         got = [x.detach().clone() for x in out]
         want = [x.detach() for x in step()]
         assert all(torch.equal(a, b) for a, b in zip(got, want)), i
+
+
+@pytest.mark.parametrize("path", ["op", "function"])
+@pytest.mark.parametrize("norm", [False, True])
+def test_positions_and_table_changed_before_the_backward(norm, path, monkeypatch):
+    """A buffer of positions (or the table) that is overwritten between forward and backward raises, as any saved tensor."""
+    if path == "function":
+        monkeypatch.setattr(cra.rotary._native, "fast_op", lambda name: None)
+    for change in ("none", "positions", "table"):
+        table = cra.RotaryTable(32, 50, device="cuda")
+        pos = torch.arange(8, device="cuda")
+        q = torch.randn(1, 2, 8, 32, device="cuda", requires_grad=True)
+        w = torch.randn(32, device="cuda", requires_grad=True)
+        y = cra.qk_norm_rotary(q, None, w, None, table, pos) if norm else cra.rotary_embedding(q, None, table, pos)
+        if change == "positions":
+            pos.add_(1)
+        elif change == "table":
+            table.table.mul_(2)
+        if change == "none":
+            y.sum().backward()
+            assert q.grad is not None
+        else:
+            with pytest.raises(RuntimeError, match="inplace operation"):
+                y.sum().backward()
