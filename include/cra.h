@@ -385,16 +385,17 @@ typedef struct {
   int32_t window;         /* 0: the rule */
   int32_t relay;          /* -1: the rule, 0, 1 */
   int32_t top_k;          /* 1..4 (ignored when relay == 0) */
-  int32_t max_query_len;  /* with cu_seqlens: bound on a sequence's new tokens */
-  int32_t max_seqlen;     /* bound on seq_lens; a sequence beyond a bound gives NaN */
+  int32_t max_query_len;  /* with cu_seqlens: bound on a sequence's new tokens; more may give NaN */
+  int32_t max_seqlen;     /* bound on seq_lens; a longer sequence gives NaN */
   int32_t zero_outside;   /* rows of o outside every sequence: 1: zeros, 0: left as they are */
   float scale;            /* logit scale */
 } cra_paged_plan;
 
 /* q, o: [n_seqs, H_q, query_len, D] or packed [1, H_q, tokens, D] of the cache's
- * dtype, rows 16-byte aligned; query head h reads kv head h / (H_q / H_kv). A query that sees no row (its sequence
- * holds fewer rows than new tokens) gives zeros; one that meets a page outside
- * the cache gives NaN. The workspace may be any memory not used by another
+ * dtype, rows 16-byte aligned; query head h reads kv head h / (H_q / H_kv). A
+ * query that sees no row (its sequence holds fewer rows than new tokens) gives
+ * zeros; one that meets a page outside the cache gives NaN. A query may have
+ * fewer than 2^30 keys (CRA_E_INVALID from the bounds). The workspace may be any memory not used by another
  * call at the same time; nothing in it needs clearing. */
 size_t cra_fwd_paged_workspace_bytes(const cra_cache* c, const cra_batch* b, const cra_paged_plan* p);
 int cra_fwd_paged(const cra_cache* c, const cra_batch* b, const cra_paged_plan* p, cra_tensor q,
