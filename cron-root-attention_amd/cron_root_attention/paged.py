@@ -220,6 +220,8 @@ def _batch(cache, x, heads, page_table, seq_lens, cu_seqlens, name):
         raise ValueError(f"{name} has {H} heads, the cache {heads}")
     if D != cache.head_dim:
         raise ValueError(f"{name} has head dim {D}, the cache {cache.head_dim}")
+    if max(*x.shape, *page_table.shape) > 2**31 - 1:
+        raise ValueError("a dimension of 2^31 or more")
     cu = None
     if cu_seqlens is not None:
         if not isinstance(cu_seqlens, torch.Tensor) or cu_seqlens.dtype != torch.int32:

@@ -10,6 +10,7 @@ order.
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional, Tuple
 
@@ -116,6 +117,8 @@ def _check_rows(q, k):
             raise TypeError(f"unsupported dtype {t.dtype}; use float16, bfloat16 or float32")
         if min(t.shape) < 1:
             raise ValueError(f"{name} has an empty dimension: {tuple(t.shape)}")
+        if max(t.shape) > 2**31 - 1:
+            raise ValueError(f"{name} has a dimension of 2^31 or more: {tuple(t.shape)}")
     if k is not None:
         if (q.shape[0], q.shape[2], q.shape[3]) != (k.shape[0], k.shape[2], k.shape[3]):
             raise ValueError(f"k shape {tuple(k.shape)} does not match q {tuple(q.shape)}")
@@ -177,6 +180,21 @@ def _grads(dys, like):
             for d, x in zip(dys, like)]
 
 
+def _once(backward):
+    """Gradients that are not differentiated again: under create_graph they carry a
+    node that raises when they are."""
+    @functools.wraps(backward)
+    def wrapped(ctx, *grads):
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return out
+        error = torch._C._functions.DelayedError(
+            f"{type(ctx).__name__} has no second derivative".encode(), len(out))
+        return error(*(t if t is None else t.detach().requires_grad_() for t in out))
+    return wrapped
+
+
 class RotaryFunction(torch.autograd.Function):
     """Rotation of q and k; the backward turns the gradients back."""
 
@@ -190,7 +208,7 @@ class RotaryFunction(torch.autograd.Function):
         return _native.rotary(_problem(q, k, table, positions, False, q.dtype, 0.0), q, k, None, None)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dyq, dyk):
         one = [x for x in (dyq, dyk) if x is not None]
         if not one:
@@ -218,7 +236,7 @@ class NormRotaryFunction(torch.autograd.Function):
                               q, k, wq, wk)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dyq, dyk):
         q, k, wq, wk, _, positions = ctx.saved_tensors
         table, eps = ctx.args

@@ -30,6 +30,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/autograd.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
 #include "cra.h"
@@ -325,6 +326,24 @@ at::Tensor rows_of(const at::Tensor& t) {
   return !t.defined() || t.stride(3) == 1 || t.size(3) == 1 ? t : t.contiguous();
 }
 
+// Whether the sizes fit the C ABI's 32-bit ones.
+bool sizes_fit(const at::Tensor& t) {
+  for (int64_t n : t.sizes())
+    if (n > INT32_MAX) return false;
+  return true;
+}
+
+// Gradients that are not differentiated again: under create_graph they carry a node
+// that raises when they are.
+torch::autograd::variable_list once(torch::autograd::variable_list out, const char* name) {
+  if (!at::GradMode::is_enabled()) return out;
+  auto node = std::make_shared<torch::autograd::DelayedError>(
+      std::string(name) + " has no second derivative", (int64_t)out.size());
+  for (at::Tensor& t : out)
+    if (t.defined()) t = t.detach().set_requires_grad(true);
+  return (*node)(std::move(out));
+}
+
 struct Turn {
   bool norm, interleaved;
   double eps;
@@ -418,7 +437,7 @@ class CraRotary : public torch::autograd::Function<CraRotary> {
       } else {
         out[1] = y[0];
       }
-      return out;
+      return once(std::move(out), "rotary_embedding");
     }
     const at::Tensor q = rows_of(s[0]), k = rows_of(s[1]);  // layouts that a saved-tensor hook changed
     const at::Tensor &wq = s[2], &wk = s[3];
@@ -443,7 +462,7 @@ class CraRotary : public torch::autograd::Function<CraRotary> {
     out[1] = dk;
     out[2] = dwq;
     out[3] = dwk;
-    return out;
+    return once(std::move(out), "qk_norm_rotary");
   }
 };
 
@@ -451,8 +470,8 @@ bool rotary_takes(const at::Tensor& q, const at::Tensor& k, const at::Tensor& wq
                   const at::Tensor& table, const at::Tensor& pos, bool norm, double eps) {
   if (q.dim() != 4 || !q.is_cuda() || !float_type(q.scalar_type()) || q.numel() == 0) return false;
   const int64_t B = q.size(0), S = q.size(2), D = q.size(3);
-  if (D > 256) return false;
-  if (k.defined() && (k.dim() != 4 || k.size(0) != B || k.size(2) != S || k.size(3) != D ||
+  if (D > 256 || !sizes_fit(q)) return false;
+  if (k.defined() && (!sizes_fit(k) || k.dim() != 4 || k.size(0) != B || k.size(2) != S || k.size(3) != D ||
                       k.size(1) < 1 || k.scalar_type() != q.scalar_type() || k.device() != q.device()))
     return false;
   if (!table.defined() && (pos.defined() || !norm)) return false;
@@ -503,7 +522,7 @@ bool paged_call(const at::Tensor& x, const at::Tensor& kc, const at::Tensor& vc,
                 const OptTensor& ks, const OptTensor& vs, const at::Tensor& table, const at::Tensor& lens,
                 const OptTensor& cu, int64_t head_dim, cra_cache& c, cra_batch& b) {
   if (x.dim() != 4 || x.device() != kc.device() || !float_type(x.scalar_type()) || x.numel() == 0 ||
-      x.size(3) != head_dim || head_dim % 8 || !paged_rows(x))
+      x.size(3) != head_dim || head_dim % 8 || !paged_rows(x) || !sizes_fit(x) || !sizes_fit(table))
     return false;
   if (table.scalar_type() != at::kInt || lens.scalar_type() != at::kInt || table.dim() != 2 ||
       lens.dim() != 1 || table.device() != kc.device() || lens.device() != kc.device() ||

@@ -296,3 +296,25 @@ def test_positions_and_table_changed_before_the_backward(norm, path, monkeypatch
         else:
             with pytest.raises(RuntimeError, match="inplace operation"):
                 y.sum().backward()
+
+
+@pytest.mark.parametrize("path", ["op", "function"])
+@pytest.mark.parametrize("norm", [False, True])
+def test_second_derivatives_raise(norm, path, monkeypatch):
+    """Gradients formed under create_graph are right; differentiating them again raises instead of leaving terms out."""
+    if path == "function":
+        monkeypatch.setattr(cra.rotary._native, "fast_op", lambda name: None)
+    table = cra.RotaryTable(32, 8, device=DEV)
+    q, k = (torch.randn(1, H, 8, 32, device=DEV, requires_grad=True) for H in (4, 2))
+
+    def y():
+        return cra.qk_norm_rotary(q, k, None, None, table) if norm else cra.rotary_embedding(q, k, table)
+
+    def loss():
+        return sum((t * t * t).sum() for t in y())
+
+    plain = torch.autograd.grad(loss(), (q, k))
+    for a, b in zip(plain, torch.autograd.grad(loss(), (q, k), create_graph=True)):
+        assert torch.equal(a, b)
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            b.sum().backward(retain_graph=True)
