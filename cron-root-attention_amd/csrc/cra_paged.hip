@@ -996,6 +996,8 @@ int check_paged(const cra_cache* c, const cra_batch* b, const cra_paged_plan* p)
   // sums of 64 sequences' tiles take 32 bits
   const int64_t held = (int64_t)b->pages_per_seq * c->page_size;
   const int most = (int)std::min<int64_t>(p->max_seqlen, std::min<int64_t>(held, 0x7fffffff));
+  if (most > 0x7fff0000)  // row numbers behind the last tile stay within 32 bits
+    return err(CRA_E_INVALID, "sequences of 2^31 - 2^16 tokens or more");
   const PlanMost pm = plan_most(most, p->window, p->relay, p->top_k);
   if (pm.globals + pm.W >= (int64_t)1 << 30)
     return err(CRA_E_INVALID, "2^30 keys of a query or more");

@@ -204,6 +204,7 @@ def test_read_rejects(kw, code, msg):
     (dict(max_seqlen=0), "max_seqlen"), (dict(cu_seqlens=P, tokens=5, max_query_len=0), "max_query_len"),
     (dict(n_seqs=1 << 14, query_len=1 << 15), "2^30"),
     (dict(window=1 << 30, max_seqlen=1 << 30, pages_per_seq=1 << 24, table_stride=1 << 24), "2^30 keys"),
+    (dict(max_seqlen=(1 << 31) - 1, pages_per_seq=1 << 25, table_stride=1 << 25), "2^31"),
 ])
 def test_attention_rejects_plans(kw, msg):
     lib = N.load_library()

@@ -225,6 +225,9 @@ CASES = [
     ([0, 10, 0, 50], [0, 3, 0, 20], 2, 1, 64, 16, {}),                      # empty sequences
     ([4, 7], [6, 40], 2, 1, 64, 16, {}),                                    # more new tokens than rows
     ([64, 128, 192], [32, 64, 128], 2, 1, 64, 16, dict(window=64)),         # everything on tile borders
+    ([0, 0, 5, 40], [1, 20, 9, 2], 2, 1, 64, 16, {}),                       # new tokens of empty sequences
+    ([2500, 40, 3000], [1, 3, 1], 40, 1, 64, 16, {}),                       # one kv head for many query heads
+    ([2500, 40, 3001], [1, 3, 1], 160, 1, 32, 16, dict(window=1 << 30)),
     ([2300, 1700], [1, 30], 2, 2, 64, 32, dict(window=600, relay=True, relay_top_k=3)),  # wide blocks
     ([1100, 2040], [20, 1], 2, 2, 64, 16, dict(window=506, relay=True)),
     ([1100, 2040], [1, 20], 2, 2, 64, 16, dict(window=505, relay=True, relay_top_k=4)),
