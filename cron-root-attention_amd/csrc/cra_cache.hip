@@ -10,7 +10,7 @@
 // 8 bits: row x with m = max |x| is held as codes c and a scale s.
 //   e4m3: s = the smallest power of two with m <= 448 s, c = RNE(x / s). x / s
 //         and c s are exact, codes keep their 3 bits whatever the row's scale.
-//   int8: s = m / 127, c = RNE(x / s).
+//   int8: s = m times the fp32 1/127 (so |x| / s stays below 127.5), c = RNE(x / s).
 // s is at least 2^-126. A row that holds an infinity or NaN gets s = NaN.
 //
 // Bound by memory, an int8 write nearly as much by the VALU; a row belongs to D/8
@@ -95,7 +95,7 @@ __device__ __forceinline__ float row_scale(uint32_t m) {
     const int e = (int)(m >> 23) - 127 - 8 + ((m & 0x7fffffu) > 0x600000u ? 1 : 0);
     return __uint_as_float((uint32_t)(max(e, -126) + 127) << 23);
   }
-  return fmaxf(__fdiv_rn(__uint_as_float(m), 127.f), 0x1p-126f);
+  return fmaxf(__uint_as_float(m) * (1.f / 127.f), 0x1p-126f);
 }
 
 // Four codes of x / s.

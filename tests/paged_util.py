@@ -16,7 +16,7 @@ def quantise(x, storage):
         part, power = torch.frexp(most.double() / 448.0)
         scale = torch.ldexp(torch.ones_like(part), (power - (part == 0.5).int()).clamp_min(-126)).float()
     else:
-        scale = most / 127.0
+        scale = most * torch.tensor(1 / 127, dtype=torch.float32)
     scale = torch.where(most > 0, scale, torch.zeros_like(scale)).clamp_min(torch.finfo(torch.float32).tiny)
     scale = torch.where(most.isfinite(), scale, torch.full_like(scale, math.nan))
     y = f / scale[..., None]
