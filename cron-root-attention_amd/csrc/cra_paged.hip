@@ -548,26 +548,28 @@ void few_kernel(PagedArgs a) {
       for (int db = 0; db < D / 16; ++db) acc[db][0] *= alpha;
       m_run = m_new;
     }
-    float vref = 1.f;
-    if constexpr (STORE != kSame && std::is_same<T, f16>::value) {
-      // p times a row's scale would leave fp16's range: it is taken relative to
-      // the tile's largest scale, which multiplies the product in fp32
-      float most = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) most = fmaxf(most, vs[i]);
-      vref = group_max(most);
-      vref = vref > 0.f ? vref : 1.f;
-    }
     float pv[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       pv[i] = __builtin_amdgcn_exp2f(x[i] - mu);
       l_run += pv[i];
     }
+    float vref = 1.f;
     if constexpr (STORE != kSame) {
-      const float inv = std::is_same<T, f16>::value ? 1.f / vref : 1.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) pv[i] = x[i] == -kInf ? 0.f : pv[i] * (vs[i] * inv);
+      for (int i = 0; i < 8; ++i) pv[i] = x[i] == -kInf ? 0.f : pv[i] * vs[i];
+      if constexpr (std::is_same<T, f16>::value) {
+        // p times a row's scale would leave fp16's range: it is taken relative to the
+        // query's largest in the tile, which multiplies the product in fp32
+        float most = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) most = fmaxf(most, pv[i]);
+        most = group_max(most);
+        vref = most > 0x1p-100f ? most : 1.f;
+        const float inv = 1.f / vref;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) pv[i] *= inv;
+      }
     }
     const Frag<T> pf[1] = {pack8<T>(pv)};
     auto v_frag = [&](int db) __attribute__((always_inline)) {

@@ -321,6 +321,22 @@ def test_rows_that_a_query_does_not_see_do_not_reach_it(dtype, store, poison):
         check(run(s, q, [new], window=1000)[:seen], o[:seen], mag[:seen], dtype)
 
 
+@pytest.mark.parametrize("store", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("new", [1, 5, 40])
+def test_rows_of_very_different_scales(dtype, store, new):
+    """A v row of the largest fp16 values among ordinary ones, not seen, seen, and seen with a small weight."""
+    for row, key in ((130, 0.0), (100, 0.0), (100, -9.0)):
+        s = Setup([200], 1, 64, dtype, store, seed=new)
+        q = torch.randn(new, 2, 64, generator=s.g).to(dtype)
+        s.k[row, 0] = key * q[0, 0] / 4
+        s.v[row, 0] = 60000 * torch.sign(s.v[row, 0].float()).to(dtype)
+        s.write(s.k, s.v, [200], [0, 200])
+        # below the window its multiples are seen: of 50 row 100 is one, of 64 row 130 is none
+        window = 64 if row == 130 else 50
+        check(run(s, q, [new], window=window), *s.expect(q, [new], window=window), dtype)
+
+
 def test_lowest_values_and_large_scores():
     """Keys whose scores are the type's largest: the softmax stays finite."""
     s = Setup([100], 1, 64, BF16)
