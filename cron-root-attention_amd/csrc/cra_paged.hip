@@ -945,8 +945,8 @@ __global__ __launch_bounds__(256) void f32_kernel(PagedArgs a) {
 }
 
 template <int D>
-__global__ __launch_bounds__(256) void f32_join_kernel(PagedArgs a) {
-  join_chunk<float, kF32Rows, kF32Keys, D>(a);
+__global__ __launch_bounds__(256) void f32_join_kernel(PagedArgs a, uint32_t items) {
+  join_chunk<float, kF32Rows, kF32Keys, D>(a, items);
 }
 
 // ---------------------------------------------------------------------------
@@ -1094,7 +1094,8 @@ hipError_t launch_rows(const PagedArgs& a, const Launch& l, int64_t bh, hipStrea
     if constexpr (std::is_same<T, float>::value) {
       f32_kernel<STORE, D, false><<<(uint32_t)l.items, 256, 0, st>>>(a);
       if (hipError_t e = hipGetLastError()) return e;
-      if (l.joins) f32_join_kernel<D><<<(uint32_t)l.joins * (kF32Rows / kJoinRows), 256, 0, st>>>(a);
+      const uint32_t items = (uint32_t)l.joins * (kF32Rows / join_rows<D>());
+      if (items) f32_join_kernel<D><<<std::min<uint32_t>(items, kJoinGrid), 256, 0, st>>>(a, items);
       return hipGetLastError();
     } else {
       return launch_chunk(std::is_same<T, f16>::value ? CRA_F16 : CRA_BF16, STORE, D, a,

@@ -532,37 +532,38 @@ void chunk_kernel(PagedArgs a) {
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(256) void join_kernel(PagedArgs a) {
-  join_chunk<T, 64 * kChunkQB<D>, kChunkBN<D>, D>(a);
+__global__ __launch_bounds__(256) void join_kernel(PagedArgs a, uint32_t items) {
+  join_chunk<T, 64 * kChunkQB<D>, kChunkBN<D>, D>(a, items);
 }
 
 template <typename T, int STORE, int D>
-hipError_t run(const PagedArgs& a, uint32_t grid, uint32_t join_grid, hipStream_t st) {
+hipError_t run(const PagedArgs& a, uint32_t grid, uint32_t join_tiles, hipStream_t st) {
   chunk_kernel<T, STORE, D><<<grid, 64 * kChunkWaves, 0, st>>>(a);
   if (hipError_t e = hipGetLastError()) return e;
-  if (join_grid) join_kernel<T, D><<<join_grid * (64 * kChunkQB<D> / kJoinRows), 256, 0, st>>>(a);
+  const uint32_t items = join_tiles * (64 * kChunkQB<D> / join_rows<D>());
+  if (items) join_kernel<T, D><<<items < kJoinGrid ? items : kJoinGrid, 256, 0, st>>>(a, items);
   return hipGetLastError();
 }
 template <typename T, int STORE>
-hipError_t run_dim(int Dp, const PagedArgs& a, uint32_t grid, uint32_t join_grid, hipStream_t st) {
+hipError_t run_dim(int Dp, const PagedArgs& a, uint32_t grid, uint32_t join_tiles, hipStream_t st) {
   switch (Dp) {
-    case 32: return run<T, STORE, 32>(a, grid, join_grid, st);
-    case 64: return run<T, STORE, 64>(a, grid, join_grid, st);
-    case 128: return run<T, STORE, 128>(a, grid, join_grid, st);
-    default: return run<T, STORE, 256>(a, grid, join_grid, st);
+    case 32: return run<T, STORE, 32>(a, grid, join_tiles, st);
+    case 64: return run<T, STORE, 64>(a, grid, join_tiles, st);
+    case 128: return run<T, STORE, 128>(a, grid, join_tiles, st);
+    default: return run<T, STORE, 256>(a, grid, join_tiles, st);
   }
 }
 
 }  // namespace
 
 hipError_t launch_chunk(int dtype, int store, int Dp, const PagedArgs& a, uint32_t grid,
-                        uint32_t join_grid, hipStream_t st) {
+                        uint32_t join_tiles, hipStream_t st) {
   const bool h = dtype == CRA_F16;
   if (store == CRA_STORE_SAME)
-    return h ? run_dim<f16, kSame>(Dp, a, grid, join_grid, st) : run_dim<bf16, kSame>(Dp, a, grid, join_grid, st);
+    return h ? run_dim<f16, kSame>(Dp, a, grid, join_tiles, st) : run_dim<bf16, kSame>(Dp, a, grid, join_tiles, st);
   if (store == CRA_STORE_E4M3)
-    return h ? run_dim<f16, kE4M3>(Dp, a, grid, join_grid, st) : run_dim<bf16, kE4M3>(Dp, a, grid, join_grid, st);
-  return h ? run_dim<f16, kInt8>(Dp, a, grid, join_grid, st) : run_dim<bf16, kInt8>(Dp, a, grid, join_grid, st);
+    return h ? run_dim<f16, kE4M3>(Dp, a, grid, join_tiles, st) : run_dim<bf16, kE4M3>(Dp, a, grid, join_tiles, st);
+  return h ? run_dim<f16, kInt8>(Dp, a, grid, join_tiles, st) : run_dim<bf16, kInt8>(Dp, a, grid, join_tiles, st);
 }
 
 }  // namespace cra

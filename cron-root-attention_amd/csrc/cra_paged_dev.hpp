@@ -320,47 +320,59 @@ __device__ __forceinline__ ChunkWork chunk_work(const PagedArgs& a) {
   return w;
 }
 
-// Adds the pieces of a cut sequence's row tile up: a workgroup of 256 threads takes
-// kJoinRows rows, a thread four columns of a row at a time.
-constexpr int kJoinRows = 32;
+// Adds the pieces of cut sequences' row tiles up: `items` of join_rows(D) rows each
+// over the grid's stride, a thread four columns of a row. One pass over the pieces
+// with a running maximum, eight pieces' loads on their way: a chunk of 32 rows behind
+// 26000 dense keys has 51 pieces 20 us (32 rows a workgroup, the maximum first:
+// 83); where nothing was cut the launch costs 4.7 us.
+constexpr int kJoinGrid = 1024;  // workgroups at most: calls without cut sequences pass through quickly
+template <int D>
+__host__ __device__ constexpr int join_rows() { return 1024 / D; }
 template <typename T, int BM, int BN, int D>
-__device__ void join_chunk(const PagedArgs& a) {
-  const int part = blockIdx.x % (BM / kJoinRows);
-  const uint32_t block = blockIdx.x / (BM / kJoinRows);
-  const uint32_t item = div_by(block, a.d_hkv);
-  const int hk = (int)(block - item * a.c.H_kv);
-  const ChunkFind f = chunk_find<BM, BN, true>(a, (int)item);
-  if (f.b < 0 || (int64_t)(f.split0 + (f.j + 1) * f.pieces) * a.c.H_kv > a.parts) return;
-  const Seq s = wave_seq(a, f.b);
-  const int tile = f.tiles - 1 - f.j, rows = s.m * a.grp;
-  const int64_t first = ((int64_t)(f.split0 + f.j * f.pieces) * a.c.H_kv + hk) * BM;
-  const int64_t step = (int64_t)a.c.H_kv * BM;  // partial rows from piece to piece
-  for (int i = threadIdx.x; i < kJoinRows * (D / 4); i += 256) {
-    const int r = part * kJoinRows + i / (D / 4), c = i % (D / 4) * 4;
-    if (tile * BM + r >= rows || c >= a.D) continue;
-    float M = -kInf;
-#pragma unroll 4
-    for (int k = 0; k < f.pieces; ++k) M = fmaxf(M, a.part_ml[2 * (first + k * step + r)]);
-    float L = 0.f;
+__device__ void join_chunk(const PagedArgs& a, uint32_t items) {
+  constexpr int R = join_rows<D>(), kParts = BM / R;
+  const int r0 = threadIdx.x / (D / 4), c = threadIdx.x % (D / 4) * 4;
+  for (uint32_t v = blockIdx.x; v < items; v += gridDim.x) {
+    const uint32_t block = v / kParts, item = div_by(block, a.d_hkv);
+    const int hk = (int)(block - item * a.c.H_kv);
+    const ChunkFind f = chunk_find<BM, BN, true>(a, (int)item);
+    if (f.b < 0 || (int64_t)(f.split0 + (f.j + 1) * f.pieces) * a.c.H_kv > a.parts) return;
+    const Seq s = wave_seq(a, f.b);
+    const int r = (int)(v % kParts) * R + r0, row = (f.tiles - 1 - f.j) * BM + r;
+    if (row >= s.m * a.grp || c >= a.D) continue;
+    const int64_t first = ((int64_t)(f.split0 + f.j * f.pieces) * a.c.H_kv + hk) * BM + r;
+    const int64_t step = (int64_t)a.c.H_kv * BM;  // partial rows from piece to piece
+    float M = -kInf, L = 0.f;
     f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int k = 0; k < f.pieces; ++k) {
-      const int64_t at = first + k * step + r;
-      const float m = a.part_ml[2 * at];
-      const float e = m == -kInf ? 0.f : __builtin_amdgcn_exp2f(m - M);
-      L += e * a.part_ml[2 * at + 1];
-      o += *reinterpret_cast<const f32x4*>(a.part + at * D + c) * e;
+    for (int k = 0; k < f.pieces; k += 8) {
+      float2 ml[8];
+      f32x4 x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int64_t at = first + min(k + i, f.pieces - 1) * step;
+        ml[i] = *reinterpret_cast<const float2*>(a.part_ml + 2 * at);
+        x[i] = *reinterpret_cast<const f32x4*>(a.part + at * D + c);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (k + i >= f.pieces) break;
+        const float m = fmaxf(M, ml[i].x), mu = m == -kInf ? 0.f : m;
+        const float e = __builtin_amdgcn_exp2f(M - mu), en = __builtin_amdgcn_exp2f(ml[i].x - mu);
+        L = L * e + ml[i].y * en;
+        o = o * e + x[i] * en;
+        M = m;
+      }
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
-    T* op = o_row<T>(a, s, hk, tile * BM + r) + c;
+    T* op = o_row<T>(a, s, hk, row) + c;
 #pragma unroll
     for (int j = 0; j < 4; ++j) op[j] = from_f32<T>(o[j] * inv);
   }
 }
 
 // chunk_kernel and the joining of its pieces (cra_paged_chunk.hip): grid
-// workgroups, at most join_grid (sequence, tile, kv head)s of several pieces.
+// workgroups, at most join_tiles (sequence, tile, kv head)s of several pieces.
 hipError_t launch_chunk(int dtype, int store, int Dp, const PagedArgs& a, uint32_t grid,
-                        uint32_t join_grid, hipStream_t st);
+                        uint32_t join_tiles, hipStream_t st);
 
 }  // namespace cra
