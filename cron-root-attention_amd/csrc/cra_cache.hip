@@ -54,20 +54,6 @@ struct Row8 {
   uint4 w[sizeof(T) / 2];
 };
 
-// The value of the lane whose number differs in bit O, within groups of 2 O lanes and
-// more: row shifts in the VALU.
-template <int O>
-__device__ __forceinline__ uint32_t from_lane_xor(uint32_t x) {
-  const int v = (int)x;
-  if constexpr (O == 1) return (uint32_t)__builtin_amdgcn_update_dpp(v, v, 0xb1, 0xf, 0xf, false);  // quad 1 0 3 2
-  if constexpr (O == 2) return (uint32_t)__builtin_amdgcn_update_dpp(v, v, 0x4e, 0xf, 0xf, false);  // quad 2 3 0 1
-  if constexpr (O == 4) {  // banks of four lanes: even ones from above, odd ones from below
-    const int up = __builtin_amdgcn_update_dpp(v, v, 0x104, 0xf, 0x5, false);  // row_shl:4
-    return (uint32_t)__builtin_amdgcn_update_dpp(up, v, 0x114, 0xf, 0xa, false);  // row_shr:4
-  }
-  if constexpr (O == 8) return (uint32_t)__builtin_amdgcn_update_dpp(v, v, 0x128, 0xf, 0xf, false);  // row_ror:8
-  return (uint32_t)__shfl_xor(v, O);
-}
 template <typename F>
 __device__ __forceinline__ uint32_t lanes_fold(uint32_t x, int log_l, F f) {
   if (log_l > 4) x = f(x, from_lane_xor<16>(x));

@@ -85,6 +85,20 @@ __device__ __forceinline__ Frag<T> lds_frag_row(const T* p) {
   return f;
 }
 
+// The value of the lane whose number differs in bit O, within groups of 2 O lanes and
+// more: row shifts in the VALU.
+template <int O>
+__device__ __forceinline__ uint32_t from_lane_xor(uint32_t x) {
+  const int v = (int)x;
+  if constexpr (O == 1) return (uint32_t)__builtin_amdgcn_update_dpp(v, v, 0xb1, 0xf, 0xf, false);  // quad 1 0 3 2
+  if constexpr (O == 2) return (uint32_t)__builtin_amdgcn_update_dpp(v, v, 0x4e, 0xf, 0xf, false);  // quad 2 3 0 1
+  if constexpr (O == 4) {  // banks of four lanes: even ones from above, odd ones from below
+    const int up = __builtin_amdgcn_update_dpp(v, v, 0x104, 0xf, 0x5, false);  // row_shl:4
+    return (uint32_t)__builtin_amdgcn_update_dpp(up, v, 0x114, 0xf, 0xa, false);  // row_shr:4
+  }
+  if constexpr (O == 8) return (uint32_t)__builtin_amdgcn_update_dpp(v, v, 0x128, 0xf, 0xf, false);  // row_ror:8
+  return (uint32_t)__shfl_xor(v, O);
+}
 // Cross-lane helpers on the 4 lane groups of a wave (lanes l, l^16, l^32, l^48).
 // The swaps exchange 16- or 32-lane halves of two registers in the VALU: both
 // holding x, they come back as x of the lane and of its partner in some order

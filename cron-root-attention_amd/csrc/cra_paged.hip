@@ -43,16 +43,16 @@ namespace {
 // is the block's first row, as in the packed rows of whole sequences. NaN norms
 // are never chosen.
 //
-// A wave takes whole blocks. Bound by the VALU work a block (and below a few
-// thousand blocks by the latency of page table and norm loads, the next block's
-// of which are on their way): in select_kernel a lane loads the norms of eight
-// rows with one page lookup, keeps the KEEP largest values by maximum and median
-// of three, and a picked value's row is found by comparing the lane's eight with
-// it. Against carrying rows along with the values, 64 rows at a time
-// (select_wide_kernel): 16 sequences of 700-131072 tokens, 8 heads, 23.4 -> 16.6 us;
-// 64 of up to 32768 tokens 15.5 -> 11.4 us.
-// A block must fit one load of the wave; wider ones (windows above 505) go to
-// select_wide_kernel.
+// A lane loads the norms of eight rows with one page lookup; a block of up to 121,
+// 249 or 505 rows (at any alignment) takes 16, 32 or 64 lanes, so a wave picks in
+// four, two or one blocks at a time: the largest norm of a lane, then of its group, by
+// exchanges in the VALU; the lane that holds a pick stores its cache row. Bound by
+// that VALU work (and below a few thousand blocks by the latency of page table and
+// norm loads, the next blocks' of which are on their way). Wider blocks go to
+// select_wide_kernel, which carries rows along with norms, 64 rows at a time.
+// Measured, 8 heads: 16 sequences of 700-131072 tokens 14.5 us (select_wide_kernel
+// 23.4; a block a wave, picks found by the whole wave, 16.6), 64 of up to 32768 tokens
+// 7.1 us (15.5; 11.4); 34000 blocks of 31 rows 12.5 us (a block a wave 34).
 // ---------------------------------------------------------------------------
 constexpr int kSelWaves = 4, kSelLoads = 8;
 constexpr int kSelMost = 64 * 8 - 7;   // rows of a block in select_kernel, at any alignment
@@ -63,7 +63,9 @@ struct SelWork {
   int b, h, full, first, end;
   uint32_t* out;
 };
-__device__ __forceinline__ SelWork sel_work(const PagedArgs& a, int steps) {
+// A wave takes a multiple of `at_once(W)` blocks.
+template <typename F>
+__device__ __forceinline__ SelWork sel_work(const PagedArgs& a, int steps, F at_once) {
   SelWork k{};
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t bh = div_by(blockIdx.x, a.d_steps);  // workgroups a (sequence, head)
@@ -75,30 +77,48 @@ __device__ __forceinline__ SelWork sel_work(const PagedArgs& a, int steps) {
   if (k.p.rpb == 1 || s.m < 1) return k;
   const int ls = s.n - k.p.W > 0 ? s.n - k.p.W : 0;  // window start of the last query
   k.full = ls / k.p.W;
-  const int blocks = k.full + (ls != k.full * k.p.W ? 1 : 0), per = (blocks + nw - 1) / nw;
+  const int blocks = k.full + (ls != k.full * k.p.W ? 1 : 0), n = at_once(k.p.W);
+  const int per = ((blocks + nw - 1) / nw + n - 1) / n * n;
   k.first = w * per;
-  k.end = min(blocks, (w + 1) * per);
+  k.end = min(blocks, k.first + per);
   k.out = a.list + (int64_t)bh * a.list_cap;
   return k;
 }
 
-__device__ __forceinline__ int wave_max_signed(int x) {  // at least -1
-  return (int)wave_max((uint32_t)(x + 1)) - 1;
+// Maximum over the lane's group of G lanes, in all of them.
+template <int G>
+__device__ __forceinline__ int lanes_max(int x) {
+  auto with = [&](uint32_t o) { x = max(x, (int)o); };
+  if constexpr (G == 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap((uint32_t)x, (uint32_t)x, false, false);
+    x = max((int)r[0], (int)r[1]);
+  }
+  if constexpr (G >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap((uint32_t)x, (uint32_t)x, false, false);
+    x = max((int)r[0], (int)r[1]);
+  }
+  with(from_lane_xor<8>((uint32_t)x));
+  with(from_lane_xor<4>((uint32_t)x));
+  with(from_lane_xor<2>((uint32_t)x));
+  with(from_lane_xor<1>((uint32_t)x));
+  return x;
 }
 
-template <int KEEP>
-__global__ __launch_bounds__(64 * kSelWaves) void select_kernel(PagedArgs a, int steps) {
-  const int lane = threadIdx.x & 63;
-  const SelWork w = sel_work(a, steps);
-  if (w.first >= w.end) return;
+// The wave's blocks, 64 / G at a time.
+template <int G>
+__device__ __forceinline__ void select_blocks(const PagedArgs& a, const SelWork& w) {
+  constexpr int P = 64 / G;
+  const int lane = threadIdx.x & 63, l = lane & (G - 1), grp = lane / G;
+  const uint64_t mine = (G == 64 ? ~0ull : (1ull << (G & 63)) - 1) << (lane & ~(G - 1));  // the group's lanes
+  const uint64_t below = mine & ((1ull << lane) - 1);
   const int W = w.p.W;
   const int32_t* pages = a.c.table + w.b * a.c.table_stride;
-  // cache row of logical row 8 (first row / 8 + lane): eight rows of one page;
-  // lanes behind the last eight (of the block, or of the sequence) repeat it
+  // cache row of logical row 8 (first row / 8 + l): eight rows of one page; lanes
+  // behind the last eight (of the block, or of the sequence) repeat it
   auto load_row = [&](int blk) -> uint32_t {
-    const int last = min(blk * W + W - 1, w.p.n - 1);
     if (blk >= w.end) return 0u;
-    return seq_row(pages, min((blk * W & ~7) + 8 * lane, last & ~7), a.c.num_pages, a.c.H_kv,
+    const int last = min(blk * W + W - 1, w.p.n - 1);
+    return seq_row(pages, min((blk * W & ~7) + 8 * l, last & ~7), a.c.num_pages, a.c.H_kv,
                    a.c.log_page, w.h);
   };
   struct Eight {
@@ -109,66 +129,66 @@ __global__ __launch_bounds__(64 * kSelWaves) void select_kernel(PagedArgs a, int
     const float4* p = reinterpret_cast<const float4*>(a.c.k_norm + (at == kNoRow ? 0u : at));
     return Eight{p[0], p[1]};
   };
-  uint32_t at = load_row(w.first), at1 = load_row(w.first + 1);
-  Eight x = load_norms(w.first, at);
-  for (int blk = w.first; blk < w.end; ++blk) {
-    const Eight x1 = load_norms(blk + 1, at1);
-    const uint32_t at2 = load_row(blk + 2);
+  int blk = w.first + grp;
+  uint32_t at = load_row(blk), at1 = load_row(blk + P);
+  Eight x = load_norms(blk, at);
+  for (int base = w.first; base < w.end; base += P, blk += P) {
+    const Eight x1 = load_norms(blk + P, at1);
+    const uint32_t at2 = load_row(blk + 2 * P);
     const int lead = blk * W & 7;
-    // cache row of the block's row i, from the lane that looked it up
-    auto slot_of = [&](int i) -> uint32_t {
-      const uint32_t q = (uint32_t)__builtin_amdgcn_readlane((int)at, (i + lead) >> 3);
-      return q == kNoRow ? kNoRow : q + ((i + lead) & 7);
-    };
-    uint32_t mine = slot_of(0);  // lane e: entry e of the block
-    if (blk < w.full) {
-      // a norm's bits, which order as the norms do; negative: not a row of the
-      // block, or NaN
-      int key[8], top[KEEP];
-      const float f[8] = {x.lo.x, x.lo.y, x.lo.z, x.lo.w, x.hi.x, x.hi.y, x.hi.z, x.hi.w};
+    const bool full = blk < w.full;
+    uint32_t* out = w.out + (int64_t)w.p.rpb * blk;
+    const uint32_t head = at == kNoRow ? kNoRow : at + lead;  // lane 0 of the group: the block's first row
+    if (blk < w.end && l == 0) out[0] = head;
+    const bool bad = (__ballot(at == kNoRow) & mine) != 0;
+    // a norm's bits, which order as the norms do; negative: not a row of a whole
+    // block, or NaN
+    int key[8], top = -1;
+    const float f[8] = {x.lo.x, x.lo.y, x.lo.z, x.lo.w, x.hi.x, x.hi.y, x.hi.z, x.hi.w};
+    const uint32_t rows = full ? W : 0;
 #pragma unroll
-      for (int j = 0; j < KEEP; ++j) top[j] = -1;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const bool in = (uint32_t)(8 * lane + j - lead) < (uint32_t)W;
-        key[j] = in ? __float_as_int(fmaxf(f[j], -1.f)) : -1;
-#pragma unroll
-        for (int t = KEEP - 1; t >= 1; --t)  // median of three
-          top[t] = max(min(top[t - 1], key[j]), min(max(top[t - 1], key[j]), top[t]));
-        top[0] = max(top[0], key[j]);
-      }
-      const bool bad = __any(at == kNoRow);
-      for (int j = 0; j < a.top_k; ++j) {
-        const int m = wave_max_signed(max(top[0], -1));
-        int pick = 0;
-        if (m >= 0) {
-          const int l = __builtin_ctzll(__ballot(top[0] == m));  // lanes rise with their rows
-          int e = 7;
-#pragma unroll
-          for (int i = 6; i >= 0; --i) e = key[i] == m ? i : e;
-          e = __builtin_amdgcn_readlane(e, l);
-          pick = 8 * l + e - lead;
-          if (lane == l) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) key[i] = i == e ? -1 : key[i];
-#pragma unroll
-            for (int i = 0; i + 1 < KEEP; ++i) top[i] = top[i + 1];
-            top[KEEP - 1] = -1;
-          }
-        }
-        const uint32_t slot = bad ? kNoRow : slot_of(pick);
-        mine = lane == 1 + j ? slot : mine;
-      }
+    for (int j = 0; j < 8; ++j) {
+      const bool in = (uint32_t)(8 * l + j - lead) < rows;
+      key[j] = in ? __float_as_int(fmaxf(f[j], -1.f)) : -1;
+      top = max(top, key[j]);
     }
-    if (lane < (blk < w.full ? w.p.rpb : 1)) w.out[(int64_t)w.p.rpb * blk + lane] = mine;
+    for (int j = 0; j < a.top_k; ++j) {
+      const int m = lanes_max<G>(top);
+      const bool has = m >= 0 && top == m;
+      const bool pick = has && (__ballot(has) & below) == 0;  // lanes rise with their rows
+      if (pick) {
+        int e = 7;
+#pragma unroll
+        for (int i = 6; i >= 0; --i) e = key[i] == m ? i : e;
+        out[1 + j] = bad ? kNoRow : at + e;
+        top = -1;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          key[i] = i == e ? -1 : key[i];
+          top = max(top, key[i]);
+        }
+      }
+      if (full && m < 0 && l == 0) out[1 + j] = bad ? kNoRow : head;  // no row is left
+    }
     at = at1, at1 = at2, x = x1;
   }
+}
+
+__global__ __launch_bounds__(64 * kSelWaves) void select_kernel(PagedArgs a, int steps) {
+  const SelWork w = sel_work(a, steps, [](int W) { return W <= 121 ? 4 : W <= 249 ? 2 : 1; });
+  if (w.first >= w.end) return;
+  if (w.p.W <= 121)
+    select_blocks<16>(a, w);
+  else if (w.p.W <= 249)
+    select_blocks<32>(a, w);
+  else
+    select_blocks<64>(a, w);
 }
 
 template <int KEEP>
 __global__ __launch_bounds__(64 * kSelWaves) void select_wide_kernel(PagedArgs a, int steps) {
   const int lane = threadIdx.x & 63;
-  const SelWork w = sel_work(a, steps);
+  const SelWork w = sel_work(a, steps, [](int) { return 1; });
   if (w.first >= w.end) return;
   const SeqPlan p = w.p;
   const int full = w.full, first = w.first, end = w.end;
@@ -1023,7 +1043,8 @@ Launch plan_launch(const cra_cache* c, const cra_batch* b, const cra_paged_plan*
   l.wide = pm.W > kSelMost;  // no shorter sequence has wider blocks
   const int64_t bh = (int64_t)b->n_seqs * c->H_kv;
   // a wave a block while that is at most 4096 workgroups: sixteen a CU hide the
-  // loads' latency, more of them cost their launch
+  // loads' latency, more of them cost their launch (the 16 and the 64 sequences of
+  // select_kernel's figures with 2048, 4096, 8192: 13.2, 14.5, 19.1 and 12.9, 7.1, 9.6 us)
   l.sel_steps = (int)std::max<int64_t>(1, std::min<int64_t>((cap + kSelWaves - 1) / kSelWaves, 4096 / bh));
   l.list_bytes = up256(bh * l.list_cap * 4);
   l.part_rows = (int)std::min<int64_t>(kFewRows, most_rows);
@@ -1163,7 +1184,7 @@ int cra_fwd_paged(const cra_cache* c, const cra_batch* b, const cra_paged_plan* 
     a.d_steps = fast_div(l.sel_steps);
     const uint32_t grid = (uint32_t)(bh * l.sel_steps);
     auto kernel = l.wide ? (p->top_k <= 2 ? select_wide_kernel<2> : select_wide_kernel<4>)
-                         : (p->top_k <= 2 ? select_kernel<2> : select_kernel<4>);
+                         : select_kernel;
     kernel<<<grid, 64 * kSelWaves, 0, st>>>(a, l.sel_steps);
     if (int e = hip_err(hipGetLastError(), "cra_fwd_paged (relay rows)")) return e;
   }

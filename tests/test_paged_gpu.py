@@ -231,6 +231,10 @@ CASES = [
     ([2300, 1700], [1, 30], 2, 2, 64, 32, dict(window=600, relay=True, relay_top_k=3)),  # wide blocks
     ([1100, 2040], [20, 1], 2, 2, 64, 16, dict(window=506, relay=True)),
     ([1100, 2040], [1, 20], 2, 2, 64, 16, dict(window=505, relay=True, relay_top_k=4)),
+    ([1000, 777], [1, 3], 2, 2, 64, 16, dict(window=121, relay=True, relay_top_k=4)),  # blocks of 16, 32, 64 lanes
+    ([1000, 777], [1, 3], 2, 2, 64, 16, dict(window=122, relay=True, relay_top_k=4)),
+    ([1000, 1777], [1, 3], 2, 2, 64, 64, dict(window=249, relay=True, relay_top_k=3)),
+    ([1000, 1777], [1, 30], 2, 2, 64, 64, dict(window=250, relay=True)),
 ]
 
 
@@ -461,7 +465,7 @@ def test_repeated_pages():
     check(run(s, q, [1, 1], window=64), *s.expect(q, [1, 1], window=64), BF16)
 
 
-@pytest.mark.parametrize("window,top_k", [(None, 2), (46, 4), (600, 2), (600, 4)])
+@pytest.mark.parametrize("window,top_k", [(None, 2), (46, 4), (600, 2), (600, 4), (150, 3), (300, 4)])
 def test_equal_norms_take_the_earlier_row(window, top_k):
     s = Setup([2100], 1, 64, F16)
     s.k[:] = s.k.sign() * 0.5  # every row has the same norm, but for a few pairs
