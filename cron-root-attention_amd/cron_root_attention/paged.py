@@ -285,7 +285,7 @@ def cron_root_attention_paged(q: torch.Tensor, cache: PagedKVCache, page_table: 
 
     Returns: like q (laid out as q). Rows of tokens outside every sequence are zeros; so
     is a query that sees no row (more new tokens than the sequence's length). A
-    query that meets a page outside the cache gives NaN.
+    query that meets a page outside the cache gives NaN, and so may others of its sequence.
     """
     if torch.is_grad_enabled() and q.requires_grad:
         raise NotImplementedError("cron_root_attention_paged has no backward; call it under "

@@ -394,10 +394,10 @@ typedef struct {
 /* q, o: [n_seqs, H_q, query_len, D] or packed [1, H_q, tokens, D] of the cache's
  * dtype, rows 16-byte aligned; query head h reads kv head h / (H_q / H_kv). A
  * query that sees no row (its sequence holds fewer rows than new tokens) gives
- * zeros; one that meets a page outside the cache gives NaN. The bounds
- * may allow sequences of at most 2^31 - 2^16 tokens and queries of fewer than 2^30
- * keys (else CRA_E_INVALID). The workspace may be any memory not used by another
- * call at the same time; nothing in it needs clearing. */
+ * zeros; one that meets a page outside the cache gives NaN, and so may others of
+ * its sequence. The bounds may allow sequences of at most 2^31 - 2^16 tokens and
+ * queries of fewer than 2^30 keys (else CRA_E_INVALID). The workspace may be any
+ * memory not used by another call at the same time; nothing in it needs clearing. */
 size_t cra_fwd_paged_workspace_bytes(const cra_cache* c, const cra_batch* b, const cra_paged_plan* p);
 int cra_fwd_paged(const cra_cache* c, const cra_batch* b, const cra_paged_plan* p, cra_tensor q,
                   cra_tensor o, void* workspace, size_t workspace_bytes, void* stream);
