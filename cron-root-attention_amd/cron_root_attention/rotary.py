@@ -139,6 +139,9 @@ def _check_positions(q, table, positions):
         raise TypeError("table must be a RotaryTable")
     if table.device != q.device:
         raise ValueError(f"the table is on {table.device} but q is on {q.device}")
+    t = table.table
+    if t.dtype != torch.float32 or not t.is_contiguous() or t.shape[1:] != (table.rotary_dim,):
+        raise ValueError(f"the table's rows must be contiguous float32 [positions, {table.rotary_dim}]")
     if table.rotary_dim > D:
         raise ValueError(f"the table turns {table.rotary_dim} elements, the heads have {D}")
     if positions is None:

@@ -475,7 +475,9 @@ bool rotary_takes(const at::Tensor& q, const at::Tensor& k, const at::Tensor& wq
                       k.size(1) < 1 || k.scalar_type() != q.scalar_type() || k.device() != q.device()))
     return false;
   if (!table.defined() && (pos.defined() || !norm)) return false;
-  if (table.defined() && (table.device() != q.device() || table.size(1) > D)) return false;
+  if (table.defined() && (table.device() != q.device() || table.dim() != 2 || table.size(1) > D ||
+                          table.scalar_type() != at::kFloat || !table.is_contiguous()))
+    return false;
   if (pos.defined()) {
     if (pos.device() != q.device() || (pos.scalar_type() != at::kInt && pos.scalar_type() != at::kLong))
       return false;

@@ -318,3 +318,12 @@ def test_second_derivatives_raise(norm, path, monkeypatch):
         assert torch.equal(a, b)
         with pytest.raises(RuntimeError, match="no second derivative"):
             b.sum().backward(retain_graph=True)
+
+
+def test_tables_that_the_kernels_cannot_read():
+    q = torch.randn(1, 2, 8, 32, device=DEV)
+    for change in (lambda t: t.half(), lambda t: t.t().contiguous().t(), lambda t: t[:, :16], lambda t: t[:, ::2]):
+        table = cra.RotaryTable(32, 50, device=DEV)
+        table.table = change(table.table)
+        with pytest.raises(ValueError, match="contiguous float32"):
+            cra.rotary_embedding(q, None, table)
