@@ -446,8 +446,10 @@ class CraRotary : public torch::autograd::Function<CraRotary> {
     c10::DeviceGuard guard(q.device());
     at::Tensor dq = at::empty_like(q), dk, dwq, dwk, ws;
     if (k.defined()) dk = at::empty_like(k);
-    if (wq.defined() && ctx->needs_input_grad(2)) dwq = at::empty_like(wq);
-    if (wk.defined() && ctx->needs_input_grad(3)) dwk = at::empty_like(wk);
+    // needs_input_grad counts edges: an absent tensor before the weights has none
+    const size_t eq = 1 + k.defined(), ek = eq + wq.defined();
+    if (wq.defined() && ctx->needs_input_grad(eq)) dwq = at::empty_like(wq);
+    if (wk.defined() && ctx->needs_input_grad(ek)) dwk = at::empty_like(wk);
     const cra_turn p = make_turn(t, q, k, true, wq.defined() ? wq : wk);
     size_t nws = 0;
     if (dwq.defined() || dwk.defined()) {

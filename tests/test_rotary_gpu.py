@@ -327,3 +327,40 @@ def test_tables_that_the_kernels_cannot_read():
         table.table = change(table.table)
         with pytest.raises(ValueError, match="contiguous float32"):
             cra.rotary_embedding(q, None, table)
+
+
+@pytest.mark.parametrize("path", ["op", "function"])
+@pytest.mark.parametrize("turned", [False, True])
+@pytest.mark.parametrize("present", ["q wq", "q k wq", "q k wk", "q k wq wk", "q k"])
+def test_gradients_with_a_tensor_or_weight_absent(present, turned, path, monkeypatch):
+    """One tensor, one weight, no table: every input that is there gets its gradient, whatever stands before it."""
+    if path == "function":
+        monkeypatch.setattr(cra.rotary._native, "fast_op", lambda name: None)
+    g = torch.Generator().manual_seed(21)
+    B, S, D, eps = 2, 13, 64, 1e-6
+    have = present.split()
+    q, k = (torch.randn(B, H, S, D, generator=g).to(DEV) for H in (4, 2))
+    wq, wk = ((1 + 0.3 * torch.randn(D, generator=g)).to(DEV) for _ in range(2))
+    dys = [torch.randn(B, H, S, D, generator=g).to(DEV) for H in (4, 2)]
+    args = {n: x.requires_grad_(True) for n, x in dict(q=q, k=k, wq=wq, wk=wk).items() if n in have}
+    table = cra.RotaryTable(48, S, device=DEV) if turned else None
+    y = cra.qk_norm_rotary(q, args.get("k"), args.get("wq"), args.get("wk"), table, eps=eps)
+    y = (y,) if torch.is_tensor(y) else y
+    torch.autograd.backward(y, dys[:len(y)])
+    for x, w, dy, n in ((q, "wq", dys[0], "q"), (k, "wk", dys[1], "k")):
+        if n not in have:
+            continue
+        dz, dmag = dy.double().cpu(), dy.double().cpu().abs()
+        if turned:
+            dz, dmag = turn64(dz, torch.arange(S)[None], table, None, 10000.0, back=True)
+        x64 = x.detach().double().cpu()
+        w64 = args[w].detach().double().cpu() if w in have else torch.ones(D, dtype=torch.float64)
+        hat, r = norm64(x64, None, eps)
+        gg = dz * w64
+        dots = (dmag * w64.abs() * hat.abs()).mean(-1, keepdim=True)
+        close(x.grad, r * (gg - hat * (gg * hat).mean(-1, keepdim=True)),
+              (2 * D + 24) * U * r * (dmag * w64.abs() + hat.abs() * dots), "d" + n)
+        if w in have:
+            assert args[w].grad is not None, w
+            close(args[w].grad, (dz * hat).sum((0, 1, 2)),
+                  (B * x.shape[1] * S + D / 2 + 16) * U * (dmag * hat.abs()).sum((0, 1, 2)), "d" + w)
