@@ -344,7 +344,9 @@ __global__ __launch_bounds__(kThreads) void turn_bwd_kernel(TurnArgs g) {
     for (int j = 0; j < U; ++j)
 #pragma unroll
       for (int i = 0; i < V; ++i) ss += xa[j][i] * xa[j][i] + xb[j][i] * xb[j][i];
-    const float r = rsqrtf(lanes_sum(ss, g.log_l) * g.inv_d + g.eps);
+    // 0 behind the last row: its zeros times rsqrt(0 + eps) are NaN where eps is 0, and
+    // the sums of dw go on below
+    const float mean = lanes_sum(ss, g.log_l) * g.inv_d, r = on ? rsqrtf(mean + g.eps) : 0.f;
     float dot = 0.f;
 #pragma unroll
     for (int j = 0; j < U; ++j) {

@@ -364,3 +364,19 @@ def test_gradients_with_a_tensor_or_weight_absent(present, turned, path, monkeyp
             assert args[w].grad is not None, w
             close(args[w].grad, (dz * hat).sum((0, 1, 2)),
                   (B * x.shape[1] * S + D / 2 + 16) * U * (dmag * hat.abs()).sum((0, 1, 2)), "d" + w)
+
+
+@pytest.mark.parametrize("D,dtype", [(64, torch.float16), (64, torch.float32), (33, torch.float16), (256, torch.bfloat16)])
+def test_weight_gradients_with_eps_zero(D, dtype):
+    """Threads behind the last row add nothing to the weights' gradients, with eps = 0 too."""
+    g = torch.Generator().manual_seed(D)
+    for B, Hq, Hkv, S in ((1, 1, 1, 1), (2, 5, 3, 10), (1, 7, 1, 129)):
+        q, k = (torch.randn(B, H, S, D, generator=g).to(dtype).to(DEV).requires_grad_(True) for H in (Hq, Hkv))
+        wq, wk = ((1 + 0.3 * torch.randn(D, generator=g)).to(dtype).to(DEV).requires_grad_(True) for _ in range(2))
+        dys = [torch.randn(B, H, S, D, generator=g).to(dtype).to(DEV) for H in (Hq, Hkv)]
+        got = torch.autograd.grad(cra.qk_norm_rotary(q, k, wq, wk, eps=0.0), (q, k, wq, wk), dys)
+        assert all(bool(x.isfinite().all()) for x in got)
+        for x, dy, gw in ((q, dys[0], got[2]), (k, dys[1], got[3])):
+            hat, _ = norm64(x.detach().double().cpu(), None, 0.0)
+            dz = dy.double().cpu()
+            close(gw, (dz * hat).sum((0, 1, 2)), (B * x.shape[1] * S + D / 2 + 16) * U * (dz * hat).abs().sum((0, 1, 2)), "dw")
