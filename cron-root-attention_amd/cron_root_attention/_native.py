@@ -16,6 +16,7 @@ import threading
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 _LIB_NAME = "libcra_hip.so"
 _lock = threading.Lock()
@@ -541,6 +542,11 @@ def forward_cpu(p: CraProblem, q, k, v, threads: int):
 
 
 # ---- rotary positions and head norms -------------------------------------
+
+def has_tangent(*ts: Optional[torch.Tensor]) -> bool:
+    """Whether one of the tensors is a dual tensor (forward-mode derivatives)."""
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts)
+
 
 class _OnDevice:
     """Makes the device of a tensor current for the launches inside (a stream

@@ -161,6 +161,8 @@ class PagedKVCache:
                 cu_seqlens, self.head_dim):
             return
         # what the operator does not take (or nobody does: the checks say why)
+        if _native.has_tangent(k, v):
+            raise NotImplementedError("the cache has no forward-mode derivatives")
         batch = _batch(self, k, self.n_kv_heads, page_table, seq_lens, cu_seqlens, "k")
         if v.shape != k.shape:
             raise ValueError(f"v shape {tuple(v.shape)} does not match k {tuple(k.shape)}")
@@ -298,6 +300,8 @@ def cron_root_attention_paged(q: torch.Tensor, cache: PagedKVCache, page_table: 
                -1 if relay is None else int(bool(relay)), relay_top_k)
         if y:
             return y[0]
+    if _native.has_tangent(q):
+        raise NotImplementedError("cron_root_attention_paged has no forward-mode derivatives")
     batch = _batch(cache, q, None, page_table, seq_lens, cu_seqlens, "q")
     Hq, D = q.shape[1], q.shape[3]
     if Hq < 1 or Hq % cache.n_kv_heads:

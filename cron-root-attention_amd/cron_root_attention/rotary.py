@@ -260,7 +260,9 @@ def _weight_dtype(q, wq, wk):
 
 
 def _grad(*ts) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        return True
+    return _native.has_tangent(*ts)  # the Functions raise: forward mode is not built
 
 
 @torch.compiler.disable

@@ -503,8 +503,10 @@ std::vector<at::Tensor> rotary_autograd(const at::Tensor& q, const OptTensor& k,
                                         const OptTensor& pos, bool interleaved, bool norm, double eps) {
   const at::Tensor k_ = get(k), wq_ = get(wq), wk_ = get(wk), table_ = get(table), pos_ = get(pos);
   if (!rotary_takes(q, k_, wq_, wk_, table_, pos_, norm, eps)) return {};
-  auto wants = [](const at::Tensor& t) { return t.defined() && t.requires_grad(); };
-  if (at::GradMode::is_enabled() && (wants(q) || wants(k_) || wants(wq_) || wants(wk_)))
+  auto wants = [](const at::Tensor& t) {
+    return t.defined() && ((at::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined());
+  };
+  if (wants(q) || wants(k_) || wants(wq_) || wants(wk_))  // (a tangent raises in there)
     return CraRotary::apply(q, k, wq, wk, table, pos, interleaved, norm, eps);
   at::AutoDispatchBelowADInplaceOrView below;
   const at::Tensor qr = rows_of(q), kr = rows_of(k_);
@@ -526,7 +528,8 @@ bool paged_call(const at::Tensor& x, const at::Tensor& kc, const at::Tensor& vc,
                 const OptTensor& ks, const OptTensor& vs, const at::Tensor& table, const at::Tensor& lens,
                 const OptTensor& cu, int64_t head_dim, cra_cache& c, cra_batch& b) {
   if (x.dim() != 4 || x.device() != kc.device() || !float_type(x.scalar_type()) || x.numel() == 0 ||
-      x.size(3) != head_dim || head_dim % 8 || !paged_rows(x) || !sizes_fit(x) || !sizes_fit(table))
+      x.size(3) != head_dim || head_dim % 8 || !paged_rows(x) || !sizes_fit(x) || !sizes_fit(table) ||
+      x._fw_grad(0).defined())
     return false;
   if (table.scalar_type() != at::kInt || lens.scalar_type() != at::kInt || table.dim() != 2 ||
       lens.dim() != 1 || table.device() != kc.device() || lens.device() != kc.device() ||
@@ -562,7 +565,7 @@ bool cache_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& kc,
   cra_batch b;
   if (!paged_call(k, kc, vc, norm, ks, vs, table, lens, cu, head_dim, c, b) || v.sizes() != k.sizes() ||
       v.scalar_type() != k.scalar_type() || v.device() != k.device() || !paged_rows(v) ||
-      k.size(1) != kc.size(1))
+      v._fw_grad(0).defined() || k.size(1) != kc.size(1))
     return false;
   c10::DeviceGuard guard(k.device());
   check(api().cache_write(&c, &b, row_arg(k), row_arg(v), (int32_t)head_dim, stream_of(k)),

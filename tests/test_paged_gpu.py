@@ -645,3 +645,24 @@ def test_refusals_on_the_gpu():
         cra.PagedKVCache.from_tensors(half.transpose(0, 2).contiguous().transpose(0, 2), half, norm)
     with pytest.raises(RuntimeError):
         cra.PagedKVCache.from_tensors(half, half, norm.cpu())
+
+
+@pytest.mark.parametrize("path", ["op", "function"])
+def test_tangents_are_refused(path, monkeypatch):
+    """Nothing of the paged path has derivatives: dual tensors raise, as those that require a gradient do."""
+    from torch.autograd import forward_ad
+    if path == "function":
+        monkeypatch.setattr(cra.paged._native, "fast_op", lambda name: None)
+    s = Setup([20], 2, 64, F16)
+    q, k = (torch.randn(1, H, 1, 64, device=DEV).half() for H in (4, 2))
+    lens = s.ints(s.lens)
+    before = s.cache.k.clone()
+    with forward_ad.dual_level(), torch.no_grad():
+        dq, dk = (forward_ad.make_dual(x, torch.ones_like(x)) for x in (q, k))
+        with pytest.raises(NotImplementedError):
+            cra.cron_root_attention_paged(dq, s.cache, s.dtable, lens)
+        for kk, vv in ((dk, k), (k, dk)):
+            with pytest.raises(NotImplementedError):
+                s.cache.write(kk, vv, s.dtable, lens)
+        cra.cron_root_attention_paged(q, s.cache, s.dtable, lens)  # without a tangent
+    assert torch.equal(s.cache.k.nan_to_num(-9), before.nan_to_num(-9))

@@ -380,3 +380,25 @@ def test_weight_gradients_with_eps_zero(D, dtype):
             hat, _ = norm64(x.detach().double().cpu(), None, 0.0)
             dz = dy.double().cpu()
             close(gw, (dz * hat).sum((0, 1, 2)), (B * x.shape[1] * S + D / 2 + 16) * U * (dz * hat).abs().sum((0, 1, 2)), "dw")
+
+
+@pytest.mark.parametrize("path", ["op", "function"])
+def test_tangents_are_refused(path, monkeypatch):
+    """Forward-mode derivatives are not built: a dual tensor raises instead of losing its tangent."""
+    from torch.autograd import forward_ad
+    if path == "function":
+        monkeypatch.setattr(cra.rotary._native, "fast_op", lambda name: None)
+    table = cra.RotaryTable(32, 8, device=DEV)
+    q, k = (torch.randn(1, H, 8, 32, device=DEV) for H in (4, 2))
+    w = torch.rand(32, device=DEV)
+    with forward_ad.dual_level():
+        dq, dk, dw = (forward_ad.make_dual(x, torch.ones_like(x)) for x in (q, k, w))
+        calls = [lambda: cra.rotary_embedding(dq, k, table), lambda: cra.rotary_embedding(q, dk, table),
+                 lambda: cra.rotary_embedding(dq, None, table), lambda: cra.qk_norm_rotary(dq, k, w, w, table),
+                 lambda: cra.qk_norm_rotary(q, k, w, dw, table), lambda: cra.qk_norm_rotary(q, None, dw, None)]
+        for call in calls:
+            with pytest.raises(RuntimeError, match="jvp"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="jvp"):
+                call()
+        cra.qk_norm_rotary(q, k, w, w, table)  # without a tangent
