@@ -143,8 +143,8 @@ class PagedKVCache:
             k, v: [N, n_kv_heads, M, D], M new tokens of each of N sequences; or
                 with ``cu_seqlens`` packed [1, n_kv_heads, T, D].
             page_table: int32 [N, pages]: row r of sequence b lies in page
-                page_table[b, r // page_size]. A page id outside the cache is
-                never written.
+                page_table[b, r // page_size]. Nothing is written to a page id
+                outside the cache, nor behind the last page of a sequence's row.
             seq_lens: int32 [N], lengths with the new tokens.
             cu_seqlens: int32 [N + 1]: the new tokens of sequence b are
                 cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of T; tokens outside every

@@ -175,12 +175,10 @@ __global__ __launch_bounds__(kThreads) void cache_write_kernel(WriteArgs a) {
     const TokenRange tr = token_range(a.c.cu, b, a.c.tokens);
     first = tr.first, count = tr.last - tr.first;
   }
-  const int n = seq_length(a.c.lens[b], a.c.pages_per_seq, a.c.log_page);
-  const int row = n - count + (t - first);
-  const bool inside = row >= 0 && row < n;
-  const uint32_t dst = inside ? seq_row(a.c.table + b * a.c.table_stride, row, a.c.num_pages,
-                                        a.c.H_kv, a.c.log_page, h)
-                              : kNoRow;
+  const int row = write_row(a.c.lens[b], count, t - first, a.c.pages_per_seq, a.c.log_page);
+  const uint32_t dst = row >= 0 ? seq_row(a.c.table + b * a.c.table_stride, row, a.c.num_pages,
+                                          a.c.H_kv, a.c.log_page, h)
+                                : kNoRow;
   if (dst == kNoRow) return;  // nothing of the row is written
 #pragma unroll
   for (int i = 0; i < 8; ++i) {

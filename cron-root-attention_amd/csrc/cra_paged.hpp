@@ -41,6 +41,15 @@ __host__ __device__ inline int seq_length(int len, int pages_per_seq, int log_pa
   return len < 0 ? 0 : len < cap ? len : cap;
 }
 
+// Row that new token `t` of a sequence's `count` new ones is written to, or -1: before
+// the first row (more new tokens than the length), or behind what the table's row
+// holds. Counted back from the length as it is given: from one held within the table a
+// sequence that outgrew it would overwrite its last rows.
+__host__ __device__ inline int write_row(int len, int count, int t, int pages_per_seq, int log_page) {
+  const int64_t row = (int64_t)len - count + t;
+  return row >= 0 && row < seq_length(len, pages_per_seq, log_page) ? (int)row : -1;
+}
+
 // Tokens [first, last) of sequence b in the packed tensors; within them
 // whatever cu holds.
 struct TokenRange {

@@ -347,8 +347,9 @@ typedef struct {
  * query_len of them each, token (b, t) of [n_seqs, H, query_len, D] tensors; or,
  * with cu_seqlens (n_seqs + 1 entries, not falling), tokens cu_seqlens[b] ..
  * cu_seqlens[b + 1] - 1 of [1, H, tokens, D] tensors. Tokens outside every
- * sequence (a padded batch) are passed over. Lengths are held within what a row
- * of the table can hold; nothing is read or written through a page id outside
+ * sequence (a padded batch) are passed over. Of a sequence longer than a row of the
+ * table can hold a write passes over the rows behind it, a read stops there and
+ * attention gives NaN; nothing is read or written through a page id outside
  * 0 .. num_pages - 1. */
 typedef struct {
   const int32_t* page_table;

@@ -278,3 +278,41 @@ def test_python_refusals_without_a_gpu():
         cra.PagedKVCache.from_tensors(k, k[:3], n)
     with pytest.raises(ValueError, match="scales"):
         cra.PagedKVCache.from_tensors(k, k, n, n, n)
+
+
+WRITE_ROWS = r"""
+#include "cra_paged.hpp"
+#include <cstdio>
+using namespace cra;
+int main() {
+  long bad = 0;
+  for (int pages : {1, 2, 5})
+    for (int len = -3; len <= 100; ++len)
+      for (int count : {1, 2, 17, 200})
+        for (int t = 0; t < count; ++t) {
+          const int row = len - count + t, cap = pages * 16;
+          bad += write_row(len, count, t, pages, 4) != (len > 0 && row >= 0 && row < cap && row < len ? row : -1);
+        }
+  // the ends of the range
+  bad += write_row(0x7fffffff, 1, 0, 4, 4) != -1 || write_row(-0x7fffffff - 1, 0x7fffffff, 0, 4, 4) != -1;
+  bad += write_row(0x7fffffff, 5, 1, 0x7fffffff, 10) != 0x7ffffffb || write_row(64, 0x7fffffff, 0x7ffffffe, 4, 4) != 63;
+  // offsets that run backwards: a token outside its sequence's range stays inside the table
+  for (int t : {-0x7fffffff - 1, -70, 3, 70, 0x7fffffff})
+    for (int len : {1, 64, 0x7fffffff}) {
+      const int row = write_row(len, 2, t, 4, 4);
+      bad += row < -1 || row >= 64;
+    }
+  printf("%ld\n", bad);
+  return 0;
+}
+"""
+
+
+@pytest.mark.skipif(not os.path.exists(HIPCC), reason="hipcc not available")
+def test_rows_that_new_tokens_are_written_to(tmp_path):
+    src, exe = tmp_path / "rows.cpp", tmp_path / "rows"
+    src.write_text(WRITE_ROWS)
+    subprocess.run([HIPCC, "-std=c++17", "-O1", "-I", CSRC, str(src), "-o", str(exe)], check=True,
+                   capture_output=True, timeout=300)
+    out = subprocess.run([str(exe)], check=True, capture_output=True, text=True, timeout=120)
+    assert int(out.stdout) == 0

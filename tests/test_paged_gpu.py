@@ -666,3 +666,30 @@ def test_tangents_are_refused(path, monkeypatch):
                 s.cache.write(kk, vv, s.dtable, lens)
         cra.cron_root_attention_paged(q, s.cache, s.dtable, lens)  # without a tangent
     assert torch.equal(s.cache.k.nan_to_num(-9), before.nan_to_num(-9))
+
+
+@pytest.mark.parametrize("store", ["same", "e4m3", "int8"])
+def test_write_of_sequences_that_outgrew_their_table(store):
+    """Tokens behind what a row of the table holds are passed over; those before them go to their own rows."""
+    D, H, room = 64, 2, 64
+    s = Setup([room, room], H, D, F16, store, page=16)
+    tensors = [t for t in (s.cache.k, s.cache.v, s.cache.k_norm, s.cache.k_scale, s.cache.v_scale) if t is not None]
+    before = [t.clone() for t in tensors]
+    x = torch.randn(2, H, 6, D, device=DEV).half()
+    packed = x.transpose(0, 1).reshape(1, H, 12, D)
+
+    def same():
+        return all(torch.equal(a.float().nan_to_num(-9), b.float().nan_to_num(-9)) for a, b in zip(before, tensors))
+    # every new token behind the table's last row
+    for lens in ([room + 6, room + 1000], [2**31 - 1, room + 6]):
+        s.cache.write(x, x, s.dtable, s.ints(lens))
+        s.cache.write(packed, packed, s.dtable, s.ints(lens), cu_seqlens=s.ints([0, 6, 12]))
+        assert same(), lens
+    # rows 60 .. 63 are the first four of six new tokens; the other sequence's are its last six
+    twin = Setup([room, room], H, D, F16, store, page=16)
+    want = torch.zeros(1, H, 10, D, device=DEV).half()
+    want[0, :, :4], want[0, :, 4:] = x[0, :, :4], x[1]
+    twin.cache.write(want, want, twin.dtable, s.ints([room, room]), cu_seqlens=s.ints([0, 4, 10]))
+    s.cache.write(x, x, s.dtable, s.ints([room + 2, room]))
+    for a, b in zip(s.cache.read(s.dtable, s.ints([room, room])), twin.cache.read(twin.dtable, s.ints([room, room]))):
+        assert torch.equal(a, b)
