@@ -410,7 +410,7 @@ struct ByteTile {
 };
 
 template <typename T, int STORE, int D>
-__global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(D > 128 ? 1 : 2)))
+__global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(D > 128 ? 1 : D > 64 ? 2 : 3)))
 void few_kernel(PagedArgs a) {
   constexpr int NW = kFewWaves;
   constexpr int ES = STORE == kSame ? 2 : 1;
@@ -494,12 +494,14 @@ void few_kernel(PagedArgs a) {
   }
   float sc = 0.f;
   uint32_t next = 0;
-  if (it < nT) {
+  auto start = [&]() {
+    if (it >= nT) return;
     const uint32_t first = checked(slot_of(it));
     fill(stage[wave], first);
     sc = load_scale(first);
     if (it + step < nT) next = slot_of(it + step);
-  }
+  };
+  start();
 
   Frag<T> qf[D / 32];
   const bool have = l16 < rows;
@@ -515,6 +517,7 @@ void few_kernel(PagedArgs a) {
   f32x4 acc[D / 16][1];
 #pragma unroll
   for (int db = 0; db < D / 16; ++db) acc[db][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+  bool careful = false;  // look for elements of V that are not finite in every tile
 
   auto attend = [&](const char (&cur)[2][Tile::kBytes], int it, float sc_now) __attribute__((always_inline)) {
     const char *tK = cur[0], *tV = cur[1];
@@ -608,9 +611,10 @@ void few_kernel(PagedArgs a) {
       }
       return vt;
     };
-    // one new token: every row of the tile, a repeated last one too, is a row that its query sees
+    // one new token: every row of the tile, a repeated last one too, is a row that its
+    // query sees, and what is not finite in it shows in the result
     const bool full = s.m == 1 || (loc ? ts >= s.n - p.W && ts + 31 <= pos0 : ts + 32 <= glen0);
-    if (!full) {
+    if (!full || careful) {
       f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
       const Frag<T> one = ones_frag<T>();
 #pragma unroll
@@ -631,16 +635,35 @@ void few_kernel(PagedArgs a) {
         acc[db][0] = mma(acc[db][0], v_frag(db), pf[0]);
     }
   };
-  for (; it < nT; it += step) {
-    wait_all();
-    attend(stage[wave], it, sc);
-    wait_all();  // LDS reads are done before the loads that overwrite
-    if (it + step < nT) {
-      const uint32_t slot = checked(next);
-      fill(stage[wave], slot);
-      sc = load_scale(slot);
-      if (it + 2 * step < nT) next = slot_of(it + 2 * step);
+  for (;;) {
+    for (; it < nT; it += step) {
+      wait_all();
+      attend(stage[wave], it, sc);
+      wait_all();  // LDS reads are done before the loads that overwrite
+      if (it + step < nT) {
+        const uint32_t slot = checked(next);
+        fill(stage[wave], slot);
+        sc = load_scale(slot);
+        if (it + 2 * step < nT) next = slot_of(it + 2 * step);
+      }
     }
+    if (STORE != kSame || careful) break;  // (8-bit codes are finite: P holds a scale that is not)
+    // An infinity in V times a weight of 0 (of a repeated last row, or rounded to 0 in
+    // fp16) has made a NaN where the row's query gets the infinity: the wave's tiles
+    // once more.
+    float z = 0.f;
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) z += acc[db][0][r] - acc[db][0][r];
+    if (!__any(have && !(z == 0.f))) break;
+    careful = true;
+    m_run = -kInf;
+    l_run = 0.f;
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db) acc[db][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+    it = fi.piece * fp.per + wave;
+    start();
   }
 
   // join the waves

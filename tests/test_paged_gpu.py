@@ -693,3 +693,31 @@ def test_write_of_sequences_that_outgrew_their_table(store):
     s.cache.write(x, x, s.dtable, s.ints([room + 2, room]))
     for a, b in zip(s.cache.read(s.dtable, s.ints([room, room])), twin.cache.read(twin.dtable, s.ints([room, room]))):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype,store", [(F16, "same"), (BF16, "same"), (F32, "same"), (F16, "e4m3"), (BF16, "int8"),
+                                         (F32, "int8")])
+@pytest.mark.parametrize("poison,D", [(math.inf, 64), (-math.inf, 64), (math.nan, 64), (math.inf, 256), (math.inf, 40),
+                                      (math.nan, 128)])
+def test_values_that_are_not_finite_in_rows_that_are_seen(dtype, store, poison, D):
+    """What a seen row of v holds reaches the query, its weight however small: in the last row of a tile cut short
+    (n = 200: 200 keys, or 15 of the window and 13 strided ones), in whole tiles, for one new token and for more."""
+    for n, new, window, row, low in ((200, 1, 1000, 199, False), (200, 1, 1000, 40, True), (224, 1, 1000, 223, False),
+                                     (200, 1, None, 199, False), (200, 1, None, 180, False), (200, 4, 1000, 40, True),
+                                     (200, 40, 1000, 40, True), (3000, 1, 3000, 2999, False), (3000, 1, 3000, 500, True)):
+        s = Setup([n], 1, D, dtype, store, seed=n + new)
+        q = torch.randn(new, 1, D, generator=s.g).to(dtype)
+        q[:] = q[0]
+        if low:  # a weight of about exp(-30): nothing of it is left in fp16
+            s.k[row, 0] = (-30 * math.sqrt(D) * q[0, 0].double() / q[0, 0].double().square().sum()).to(dtype)
+        o, mag = s.expect(q, [new], window=window)
+        s.v[row, 0, 3] = poison
+        s.write(s.k, s.v, [n], [0, n])
+        got = run(s, q, [new], window=window)
+        if store == "same":
+            hit = got[..., 3].float()
+            assert (hit.isnan() if math.isnan(poison) else hit == poison).all(), (n, new, window, row)
+            keep = [c for c in range(D) if c != 3]
+            check(got[..., keep], o[..., keep], mag[..., keep], dtype)
+        else:
+            assert got.isnan().all()  # the row's scale is NaN
