@@ -254,7 +254,7 @@ def _ready(t: torch.Tensor) -> torch.Tensor:
     """Rows of a multiple of 8 elements, 16-byte aligned (a copy where they are not)."""
     if t.shape[3] % 8:
         t = F.pad(t, (0, -t.shape[3] % 8))
-    return t if _aligned(t) else t.contiguous()
+    return t if _aligned(t) else t.clone(memory_format=torch.contiguous_format)
 
 
 @torch.compiler.disable

@@ -721,3 +721,24 @@ def test_values_that_are_not_finite_in_rows_that_are_seen(dtype, store, poison, 
             check(got[..., keep], o[..., keep], mag[..., keep], dtype)
         else:
             assert got.isnan().all()  # the row's scale is NaN
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_contiguous_rows_at_odd_addresses(packed):
+    """q, k, v and out that are contiguous but start between 16-byte addresses are copied, not refused."""
+    def odd(x):
+        y = torch.zeros(x.numel() + 1, dtype=x.dtype, device=DEV)[1:].view(x.shape)
+        y.copy_(x)
+        assert y.is_contiguous() and y.data_ptr() % 16
+        return y
+    s = Setup([40], 2, 64, F16)
+    lens, cu = s.ints([40]), s.ints([0, 3]) if packed else None
+    q, k, v = (torch.randn(1, H, 3, 64, device=DEV).half() for H in (4, 2, 2))
+    s.cache.write(odd(k), odd(v), s.dtable, lens, cu_seqlens=cu)
+    for x, y in zip(s.cache.read(s.dtable, lens, 40), (k, v)):
+        assert torch.equal(x[:, :, 37:], y)
+    want = cra.cron_root_attention_paged(q, s.cache, s.dtable, lens, cu_seqlens=cu)
+    assert torch.equal(cra.cron_root_attention_paged(odd(q), s.cache, s.dtable, lens, cu_seqlens=cu), want)
+    out = odd(torch.zeros_like(q))
+    cra.cron_root_attention_paged(q, s.cache, s.dtable, lens, cu_seqlens=cu, out=out)
+    assert torch.equal(out, want)
