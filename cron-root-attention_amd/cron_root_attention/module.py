@@ -94,6 +94,8 @@ class CronRootAttention(nn.Module):
         B, S, _ = x.shape
         if (cache is None) != (batch is None):
             raise ValueError("cache and batch belong together")
+        if positions is not None and self.rotary is None:
+            raise ValueError("positions without rotary: the layer has nothing to turn by")
         kv = kv if kv is not None else x
         q = self.q_proj(x).view(B, S, self.n_heads, self.head_dim).transpose(1, 2)
         k = self.k_proj(kv).view(B, S, self.n_kv_heads, self.head_dim).transpose(1, 2)

@@ -28,3 +28,11 @@ def test_positions_of_a_batch():
     cu = torch.tensor([1, 3, 3, 6], dtype=torch.int32)  # one token before, two behind, an empty sequence
     pos = cra.PagedBatch(table, lens, cu).positions(8)
     assert pos.dtype == torch.int32 and pos.tolist() == [[0, 3, 4, 0, 1, 2, 0, 0]]
+
+
+def test_positions_need_rotary():
+    """Positions that nothing would turn by are refused, not passed over."""
+    x, pos = torch.zeros(1, 4, 64), torch.arange(4)
+    for qk_norm in (False, True):
+        with pytest.raises(ValueError, match="rotary"):
+            cra.CronRootAttention(64, 2, qk_norm=qk_norm)(x, positions=pos)
