@@ -237,10 +237,14 @@ def _batch(cache, x, heads, page_table, seq_lens, cu_seqlens, name):
         cu = cu_seqlens.data_ptr()
     elif B != N:
         raise ValueError(f"{name} has {B} sequences, the page table {N}")
-    if N == 0 or M == 0 or page_table.shape[1] == 0:
+    if N == 0 or M == 0:
         return None
-    return _native.CraBatch(page_table.data_ptr(), page_table.stride(0), seq_lens.data_ptr(), cu, N,
-                            page_table.shape[1], M if cu is not None else 0, 0 if cu is not None else M)
+    if page_table.shape[1] == 0:  # no pages: as a table of pages outside the cache
+        page_table = page_table.new_full((N, 1), -1)
+    batch = _native.CraBatch(page_table.data_ptr(), page_table.stride(0), seq_lens.data_ptr(), cu, N,
+                             page_table.shape[1], M if cu is not None else 0, 0 if cu is not None else M)
+    batch.table = page_table  # lives as long
+    return batch
 
 
 def _aligned(t: torch.Tensor) -> bool:
@@ -310,7 +314,7 @@ def cron_root_attention_paged(q: torch.Tensor, cache: PagedKVCache, page_table: 
         raise ValueError(f"window must be >= 1, got {window}")
     if relay is not False and not 1 <= relay_top_k <= 4:
         raise ValueError(f"relay_top_k={relay_top_k} outside [1, 4]")
-    held = page_table.shape[1] * cache.page_size
+    held = max(1, page_table.shape[1]) * cache.page_size
     for name, x in (("max_query_len", max_query_len), ("max_seqlen", max_seqlen)):
         if x is not None and x < 1:
             raise ValueError(f"{name} must be >= 1, got {x}")

@@ -742,3 +742,21 @@ def test_contiguous_rows_at_odd_addresses(packed):
     out = odd(torch.zeros_like(q))
     cra.cron_root_attention_paged(q, s.cache, s.dtable, lens, cu_seqlens=cu, out=out)
     assert torch.equal(out, want)
+
+
+def test_table_without_pages():
+    """Pages of no sequence: an empty one gives zeros, one with rows is longer than its table (NaN); rows of out outside
+    every sequence stay; nothing is written."""
+    cache = cra.PagedKVCache(4, 2, 64, 16, F16, device=DEV)
+    none = torch.zeros(2, 0, dtype=torch.int32, device=DEV)
+    lens = torch.tensor([0, 3], dtype=torch.int32, device=DEV)
+    q = torch.ones(2, 4, 2, 64, device=DEV).half()
+    o = cra.cron_root_attention_paged(q, cache, none, lens)
+    assert not o[0].any() and o[1].isnan().all()
+    out = torch.full((1, 4, 6, 64), 7.0, device=DEV).half()
+    cu = torch.tensor([1, 3, 5], dtype=torch.int32, device=DEV)
+    cra.cron_root_attention_paged(out.clone(), cache, none, lens, cu_seqlens=cu, out=out)
+    assert (out[:, :, [0, 5]] == 7).all() and not out[:, :, 1:3].any() and out[:, :, 3:5].isnan().all()
+    cache.write(q[:, :2], q[:, :2], none, lens)
+    assert not cache.k.any() and not cache.k_norm.any()
+    assert cache.read(none, lens)[0].shape == (2, 2, 0, 64) and not cache.read(none, lens, 5)[0].any()
