@@ -70,7 +70,8 @@ class PagedKVCache:
         """A cache over the caller's own contiguous tensors (shapes as above; ``dtype``
         of the values where k and v hold 8-bit codes)."""
         self = object.__new__(cls)
-        self._set(k, v, k_norm, k_scale, v_scale, dtype or k.dtype, head_dim or k.shape[-1])
+        self._set(k, v, k_norm, k_scale, v_scale, k.dtype if dtype is None else dtype,
+                  k.shape[-1] if head_dim is None else head_dim)
         return self
 
     def _set(self, k, v, k_norm, k_scale, v_scale, dtype, head_dim):

@@ -316,3 +316,9 @@ def test_rows_that_new_tokens_are_written_to(tmp_path):
                    capture_output=True, timeout=300)
     out = subprocess.run([str(exe)], check=True, capture_output=True, text=True, timeout=120)
     assert int(out.stdout) == 0
+
+
+def test_a_head_dim_of_zero_is_no_default():
+    k, n = torch.zeros(4, 2, 16, 64), torch.zeros(4, 2, 16)
+    with pytest.raises(NotImplementedError, match="head dim 0"):
+        cra.PagedKVCache.from_tensors(k, k, n, head_dim=0)
