@@ -766,8 +766,8 @@ __global__ __launch_bounds__(256) void combine_kernel(PagedArgs a, int Dp) {
 
 // ---------------------------------------------------------------------------
 // fp32: tiles of 64 rows, 32 keys at a time as fp32 in LDS (8-bit codes times
-// their scale), v_mfma_f32_16x16x4_f32. FEW: at most 16 rows and a share of
-// the key tiles (splits), else a chunk tile.
+// their scale), v_mfma_f32_16x16x4_f32. FEW: at most 16 rows (one of the four waves
+// has rows, all of them load) and a piece of the key tiles, else a chunk tile.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ f32x4 mma4(f32x4 c, float x, float y) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(x, y, c, 0, 0, 0);
@@ -796,8 +796,8 @@ __device__ void f32_item(const PagedArgs& a, const Seq& s, int b, int hk, int r0
   const uint32_t* list = a.list + ((int64_t)b * a.c.H_kv + hk) * a.list_cap;
   bool bad = s.over;
 
-  // 16 threads a row pair: thread's row tid / 8, D / 8 columns each
-  constexpr int kCols = D / 8;  // columns of a thread, 4 at a time
+  // eight threads a row, D / 8 columns each: quads of them, 32 columns apart
+  constexpr int kCols = D / 8;
   const int frow = tid >> 3, fcol = (tid & 7) * 4;
   f32x4 rk[kCols / 4], rv[kCols / 4];
   auto load = [&](int it) {

@@ -54,7 +54,7 @@ struct TurnTensor {
 
 struct TurnArgs {
   TurnTensor t[2];  // q, k
-  int S, D, rot, interleaved, nturn, units, log_l;
+  int S, D, rot, interleaved, nturn, log_l;
   FastDiv dS;
   float eps, inv_d;
   int w_f32;  // weights are fp32 (else the rows' type)
@@ -478,7 +478,6 @@ void fill_args(TurnArgs& g, const cra_turn* p, const Shape& sh) {
   g.rot = p->rot;
   g.interleaved = p->interleaved != 0;
   g.nturn = p->rot / (2 * sh.V);
-  g.units = sh.units;
   g.log_l = sh.log_l;
   g.dS = fast_div(p->S);
   g.eps = p->eps;
