@@ -142,6 +142,8 @@ def _check_positions(q, table, positions):
     t = table.table
     if t.dtype != torch.float32 or not t.is_contiguous() or t.shape[1:] != (table.rotary_dim,):
         raise ValueError(f"the table's rows must be contiguous float32 [positions, {table.rotary_dim}]")
+    if _grad(t):
+        raise NotImplementedError("a rotary table has no gradient")
     if table.rotary_dim > D:
         raise ValueError(f"the table turns {table.rotary_dim} elements, the heads have {D}")
     if positions is None:

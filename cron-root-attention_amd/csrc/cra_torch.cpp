@@ -478,7 +478,8 @@ bool rotary_takes(const at::Tensor& q, const at::Tensor& k, const at::Tensor& wq
     return false;
   if (!table.defined() && (pos.defined() || !norm)) return false;
   if (table.defined() && (table.device() != q.device() || table.dim() != 2 || table.size(1) > D ||
-                          table.scalar_type() != at::kFloat || !table.is_contiguous()))
+                          table.scalar_type() != at::kFloat || !table.is_contiguous() ||
+                          (at::GradMode::is_enabled() && table.requires_grad()) || table._fw_grad(0).defined()))
     return false;
   if (pos.defined()) {
     if (pos.device() != q.device() || (pos.scalar_type() != at::kInt && pos.scalar_type() != at::kLong))

@@ -402,3 +402,19 @@ def test_tangents_are_refused(path, monkeypatch):
             with torch.no_grad(), pytest.raises(RuntimeError, match="jvp"):
                 call()
         cra.qk_norm_rotary(q, k, w, w, table)  # without a tangent
+
+
+@pytest.mark.parametrize("path", ["op", "function"])
+def test_a_table_that_wants_a_gradient_is_refused(path, monkeypatch):
+    """The angles' gradient is not built: asked for, it raises instead of staying away."""
+    if path == "function":
+        monkeypatch.setattr(cra.rotary._native, "fast_op", lambda name: None)
+    table = cra.RotaryTable(32, 8, device=DEV)
+    table.table.requires_grad_(True)
+    q = torch.randn(1, 2, 8, 32, device=DEV)
+    for leaf in (q, q.clone().requires_grad_(True)):
+        for call in (lambda: cra.rotary_embedding(leaf, None, table), lambda: cra.qk_norm_rotary(leaf, None, None, None, table)):
+            with pytest.raises(NotImplementedError, match="no gradient"):
+                call()
+    with torch.no_grad():
+        assert cra.rotary_embedding(q, None, table).isfinite().all()
