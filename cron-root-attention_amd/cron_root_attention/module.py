@@ -5,8 +5,9 @@
 SDPA below the gfx950 crossover, as ``CronRootAttentionHybrid`` does) and
 ``threshold``; ``rotary`` (a :class:`RotaryTable`) and ``qk_norm`` (a norm of each
 head of q and k, with weights of its own), which stand between the projections
-and the attention; and ``cache`` and ``batch`` of forward, which serve new tokens
-over a :class:`PagedKVCache`.  Grouped kv heads go to the kernel natively
+and the attention (on the GPU: the plain layer's path for CPU tensors has neither);
+and ``cache`` and ``batch`` of forward, which serve new tokens over a
+:class:`PagedKVCache`.  Grouped kv heads go to the kernel natively
 (``kv_groups``) instead of being expanded with ``repeat_interleave``
 (module.py:111-113); query head h reads kv head h // kv_groups either way, so
 the result is the same.

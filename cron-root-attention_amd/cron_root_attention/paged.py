@@ -13,7 +13,8 @@ length through its window (ceil(sqrt(n))) and the relay switch (n > 2048): with
 the defaults a step's rows are the last rows of ``cron_root_attention`` over the
 sequence of the present length; a program that wants all its steps to agree with
 one pass over the whole sequence passes the same ``window`` and ``relay`` to all of
-them.  ``window`` at least the length is plain causal attention.
+them.  ``window`` at least the length is plain causal attention.  Relay rows count as
+they are (there is no ``relay_log_scale`` here).
 """
 from __future__ import annotations
 
@@ -278,8 +279,9 @@ def cron_root_attention_paged(q: torch.Tensor, cache: PagedKVCache, page_table: 
             heads (query head h reads kv head h // (H_q / heads)).
         page_table, seq_lens, cu_seqlens: as in :meth:`PagedKVCache.write`.
         max_query_len: bound on a sequence's new tokens (with ``cu_seqlens``;
-            default T). At most 16 query rows a kv head run one kernel less; a
-            sequence with more new tokens may give NaN.
+            default T). Where it times the query heads of a kv head is at most 16 the
+            kernels for chunks are not launched; a sequence with more new tokens may
+            give NaN.
         max_seqlen: bound on ``seq_lens`` (default: what a row of the table holds).
             A tighter bound makes for fewer, smaller pieces of work. A sequence
             longer than it gives NaN.
@@ -346,7 +348,10 @@ def cron_root_attention_paged(q: torch.Tensor, cache: PagedKVCache, page_table: 
 @dataclasses.dataclass
 class PagedBatch:
     """The sequences of one step of a layer over its cache: the arguments of
-    :func:`cron_root_attention_paged` that are not the layer's own."""
+    :func:`cron_root_attention_paged` that are not the layer's own (two relay rows a
+    block, as in its training path). A packed step should bound its new tokens
+    (``max_query_len``, 1 for decoding): without a bound the kernels for chunks are
+    launched too."""
 
     page_table: torch.Tensor
     seq_lens: torch.Tensor

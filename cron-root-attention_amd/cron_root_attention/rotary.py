@@ -5,8 +5,8 @@ pass over q and k between the projections and the attention
 (``csrc/cra_rotary.hip``): read once, written once, with the angles from a table
 and fp32 arithmetic.  Both operators take and give ``[B, H, S, D]`` tensors in
 any layout with D contiguous (a slice of a fused projection is read in place)
-and are differentiable; the gradients of the norm weights are summed in a fixed
-order.
+and are differentiable once, in reverse mode; the gradients of the norm weights are
+summed in a fixed order.
 """
 from __future__ import annotations
 

@@ -13,12 +13,14 @@
 //   int8: s = m times the fp32 1/127 (so |x| / s stays below 127.5), c = RNE(x / s).
 // s is at least 2^-126. A row that holds an infinity or NaN gets s = NaN.
 //
-// Bound by memory, an int8 write nearly as much by the VALU; a row belongs to D/8
+// Bound by memory, 8-bit writes nearly as much by the VALU; a row belongs to D/8
 // lanes (a power of two), 16 bytes of k and of v each. Measured, D = 128 16-bit:
-// writes of 32768 tokens of 16 heads as int8 101 us (407 MB, 4.0 TB/s; dividing each
-// element and exchanging by LDS shuffles 146 us), of 26000 ragged tokens of 4
-// heads as e4m3 30 us; reads 160 us (814 MB, 5.1 TB/s) and 46 us (16 sequences of
-// up to 9001 rows, padded: 322 MB). Two or four rows a thread gave nothing (146, 159
+// writes of 32768 tokens of 16 heads as they are 106 us (539 MB, 5.1 TB/s), as int8
+// 100 us (409 MB, 4.1 TB/s; dividing each element and exchanging by LDS shuffles
+// 146 us); of 26000 ragged tokens of 4 heads as they are 21 us (107 MB), as e4m3 31
+// us (81 MB; the VALU is busy for about 16 of them, and waves wait for two thirds of
+// their time, offsets, length and page id of a row in turn); reads 155 us (814 MB,
+// 5.2 TB/s) and 44 us (16 sequences of up to 9001 rows, padded: 322 MB). Two or four rows a thread gave nothing (146, 159
 // against 146 us), nor did neighbouring tokens in place of heads (152-160 us).
 #include <stdio.h>
 

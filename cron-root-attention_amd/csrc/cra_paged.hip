@@ -20,7 +20,9 @@
 // A row that a query does not see never reaches its result, whatever it holds
 // (NaN and infinity included): masked scores are replaced, and where a tile that
 // not every query sees holds such values P.V is formed apart from them
-// (pv_not_finite). A query that sees no row gives zeros.
+// (pv_not_finite). What a seen row of V holds reaches the query however small its
+// weight: an infinity times a weight that is 0 is found in the result, and the tiles
+// are gone through once more. A query that sees no row gives zeros.
 #include <stdio.h>
 
 #include <algorithm>
@@ -296,8 +298,10 @@ __global__ __launch_bounds__(64 * kSelWaves) void select_wide_kernel(PagedArgs a
 // Bound by memory latency and bandwidth: the rows seen, once per kv head. The
 // waves' results, and those of a sequence's pieces, are joined by their maxima.
 // Measured (D = 128, with combine_kernel's 4-5 us behind it): one token of 131072, 16
-// heads fp16 8 us; 64 of 1-32768, 32/8 heads bf16 15 us; 16 of 700-131072 over an
-// e4m3 store 15.5 us; 14 sequences of 1-20000, dense, 16/4 heads, int8 23 us + 6 us.
+// heads fp16 9 us; 64 of 1-32768, 32/8 heads bf16 17 us; 16 of 700-131072 over an
+// e4m3 store 16 us; 14 sequences of 1-20000, dense, 16/4 heads, int8 23 us + 6 us.
+// Up to D = 64 the registers are held to three waves a SIMD (D = 64: 168; left to
+// itself the compiler takes 170, and two waves).
 // ---------------------------------------------------------------------------
 constexpr int kFewWaves = 4;
 

@@ -10,9 +10,9 @@
 // The rows' cache rows are looked up a tile ahead of their loads.
 //
 // Bound by the matrix core, the VALU beside it and the waits between them (two waves
-// a SIMD): 8192 new tokens of 131072, 16 heads, D = 128 fp16: 156 us, 606 TFLOP/s
-// (a large matrix product: 1118); two dense chunks of 1000 and 513 tokens among 14
-// single tokens, 16/4 heads, int8 store: 300 us, about 520 TFLOP/s, widening
+// a SIMD): 8192 new tokens of 131072, 16 heads, D = 128 fp16: a call of 155 us, 608
+// TFLOP/s (a large matrix product: 1118); two dense chunks of 1000 and 513 tokens among
+// 14 single tokens, 16/4 heads, int8 store: 305 us, about 510 TFLOP/s, widening
 // included (codes widened on their way from a second stage of them while the next
 // loads ran, two turns unrolled: 310 us, eight registers spilled). The fast loop takes no care of
 // elements that are not finite in rows that some queries do not see: 0 times them
@@ -305,7 +305,11 @@ void chunk_kernel(PagedArgs a) {
   // Rows of a tile that this thread fills: the wave's instruction t moves 1 KB, each
   // lane one 16-byte chunk from its own address straight into LDS, at its
   // swizzled place (16-bit) or in order (8-bit codes, which are widened from
-  // there: V times its scale, one more rounding; K's scales go to the scores).
+  // there; K's scales go to the scores). V is widened times its scale, which rounds
+  // it once more: with the scales in P instead (as few_kernel has them) the normaliser,
+  // which sums the rounded P on the matrix core, would need a P of its own, and fp16 a
+  // reference for each query and tile. The cost: dense int8 chunks of 1000 tokens are
+  // off by 2.4e-3 of the result (relative norm) where one rounding of it leaves 1.6e-3.
   constexpr int kPiecesRow = k8 ? D / 16 : Tile::kCPR;
   constexpr int kAll = BN * kPiecesRow, kPer = (kAll + 64 * NW - 1) / (64 * NW);
   const int row_bytes = a.Ds * (k8 ? 1 : 2);
