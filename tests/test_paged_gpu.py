@@ -760,3 +760,42 @@ def test_table_without_pages():
     cache.write(q[:, :2], q[:, :2], none, lens)
     assert not cache.k.any() and not cache.k_norm.any()
     assert cache.read(none, lens)[0].shape == (2, 2, 0, 64) and not cache.read(none, lens, 5)[0].any()
+
+
+@pytest.mark.parametrize("dtype,store", [(F16, "same"), (BF16, "int8"), (F32, "same")])
+def test_captured_mixed_step_replays_over_other_batches(dtype, store):
+    """One captured packed step (write + attention): replays take chunks, single tokens, empty sequences and padding
+    from the offsets, lengths and tables that are there then."""
+    D, H, Hq, T, N_ = 64, 2, 4, 200, 4
+    caches = [cra.PagedKVCache(4 * 160, H, D, 16, dtype, STORES[store], device=DEV) for _ in range(2)]
+    table = torch.randperm(4 * 160, device=DEV).int().view(N_, 160)
+    lens, cu = torch.zeros(N_, dtype=torch.int32, device=DEV), torch.zeros(N_ + 1, dtype=torch.int32, device=DEV)
+    k, v, q = (torch.zeros(1, h, T, D, device=DEV, dtype=dtype) for h in (H, H, Hq))
+    g = torch.Generator(device=DEV).manual_seed(4)
+    for c in caches:  # the same old rows in both
+        x = torch.randn(N_, H, 2500, D, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)).to(dtype)
+        c.write(x, x.flip(1), table, lens + 2500)
+
+    def step(cache):
+        cache.write(k, v, table, lens, cu_seqlens=cu)
+        return cra.cron_root_attention_paged(q, cache, table, lens, cu_seqlens=cu)
+    warm = cra.PagedKVCache(4 * 160, H, D, 16, dtype, STORES[store], device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(warm)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = step(caches[0])
+    for offsets, lengths in (([0, 1, 2, 3, 4], [2500, 1, 2049, 17]), ([0, 100, 100, 190, 200], [2400, 0, 90, 2048]),
+                             ([5, 30, 31, 31, 150], [2501, 40, 7, 119]), ([200, 200, 200, 200, 200], [9, 9, 9, 9]),
+                             ([0, 0, 0, 0, 200], [1, 2, 3, 2300]), ([0, 1, 2, 3, 4], [2500, 1, 2049, 17])):
+        cu.copy_(torch.tensor(offsets)), lens.copy_(torch.tensor(lengths))
+        for x in (k, v, q):
+            x.copy_(torch.randn(x.shape, device=DEV, generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = o.clone()
+        want = step(caches[1])
+        assert want[:, :, offsets[0]:offsets[-1]].isfinite().all() and torch.equal(got, want), offsets

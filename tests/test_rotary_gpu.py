@@ -418,3 +418,26 @@ def test_a_table_that_wants_a_gradient_is_refused(path, monkeypatch):
                 call()
     with torch.no_grad():
         assert cra.rotary_embedding(q, None, table).isfinite().all()
+
+
+@pytest.mark.parametrize("path", ["op", "function"])
+def test_positions_and_weights_in_any_layout(path, monkeypatch):
+    """Strided, shared and one-row positions, weights that are a slice: as their contiguous copies."""
+    if path == "function":
+        monkeypatch.setattr(cra.rotary._native, "fast_op", lambda name: None)
+    B, S, D = 3, 20, 64
+    table = cra.RotaryTable(D, 200, device=DEV)
+    q, k = (torch.randn(B, H, S, D, device=DEV) for H in (4, 2))
+    wide = torch.randint(0, 200, (2 * B, 3 * S), device=DEV)
+    w = torch.randn(2 * D, device=DEV)[::2].requires_grad_(True)
+    for pos in (wide[::2, ::3], wide[:B, :S].int()[:, :], wide[:1, S:2 * S], wide[0, ::3], wide[:1, :S].expand(B, S),
+                wide[:B, :1].expand(B, S), wide[:S, :B].t() if 2 * B >= S else wide.t()[:S, :B].t()):
+        a = cra.qk_norm_rotary(q, k, w, None, table, pos)
+        b = cra.qk_norm_rotary(q, k, w.detach().contiguous(), None, table, pos.contiguous())
+        assert all(torch.equal(x, y) for x, y in zip(a, b)), (pos.shape, pos.stride())
+        full = pos.expand(B, S) if pos.dim() == 2 else pos[None].expand(B, S)
+        for i in range(B):  # each sequence by itself
+            c = cra.qk_norm_rotary(q[i:i + 1], k[i:i + 1], w, None, table, full[i].contiguous())
+            assert all(torch.equal(x, y[i:i + 1]) for x, y in zip(c, a))
+    gw, = torch.autograd.grad(a[0].sum(), w)
+    assert gw.shape == (D,) and gw.isfinite().all()
