@@ -178,6 +178,9 @@ _SIGNATURES = {
                                            ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "cra_cache_write": (ctypes.c_int, [_C, _B, CraTensor, CraTensor, ctypes.c_int32,
                                        ctypes.c_void_p]),
+    "cra_cache_append": (ctypes.c_int, [_C, _B, _R, CraTensor, CraTensor, CraTensor,
+                                        ctypes.c_void_p, ctypes.c_void_p, CraTensor,
+                                        ctypes.c_void_p]),
     "cra_cache_read": (ctypes.c_int, [_C, _B, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,
                                       ctypes.c_void_p, ctypes.c_void_p]),
     "cra_fwd_paged_workspace_bytes": (ctypes.c_size_t, [_C, _B, _G]),
@@ -264,7 +267,7 @@ _fast_state = {}
 
 
 def fast_op(name: str):
-    """``torch.ops.cra.<name>`` (rotary, cache_write, paged_attention), or None
+    """``torch.ops.cra.<name>`` (rotary, cache_write, cache_append, paged_attention), or None
     without libcra_torch.so: the ctypes path then serves every call."""
     if name not in _fast_state:
         _fast_state[name] = (getattr(torch.ops.cra, name).default

@@ -71,10 +71,24 @@ class CronRootAttention(nn.Module):
                                 self.training and torch.is_grad_enabled(),
                                 x.shape[0] * self.n_heads, self.threshold)
 
+    def _table(self, device):
+        if self.rotary is not None and self.rotary.device != device:
+            self.rotary = self.rotary.to(device)
+        return self.rotary
+
+    def _appended(self, q, k, v, positions, cache, batch):
+        """q normed and turned as the layer was made to; k, too, and stored with v."""
+        args = batch.page_table, batch.seq_lens, batch.cu_seqlens
+        if self.rotary is None and self.q_norm is None:
+            cache.write(k, v, *args)
+            return q
+        return cache.append(q, k, v, *args, table=self._table(q.device), positions=positions,
+                            norm=self.q_norm is not None, q_weight=self.q_norm, k_weight=self.k_norm,
+                            eps=self.norm_eps)
+
     def _turned(self, q, k, positions):
         """q and k normed and turned, as the layer was made to."""
-        if self.rotary is not None and self.rotary.device != q.device:
-            self.rotary = self.rotary.to(q.device)
+        self._table(q.device)
         if self.q_norm is not None:
             return qk_norm_rotary(q, k, self.q_norm, self.k_norm, self.rotary, positions,
                                   self.norm_eps)
@@ -101,18 +115,17 @@ class CronRootAttention(nn.Module):
         q = self.q_proj(x).view(B, S, self.n_heads, self.head_dim).transpose(1, 2)
         k = self.k_proj(kv).view(B, S, self.n_kv_heads, self.head_dim).transpose(1, 2)
         v = self.v_proj(kv).view(B, S, self.n_kv_heads, self.head_dim).transpose(1, 2)
-        if cache is not None and self.rotary is not None and positions is None:
-            positions = batch.positions(S)
-        q, k = self._turned(q, k, positions)
         if cache is not None:
-            cache.write(k, v, batch.page_table, batch.seq_lens, batch.cu_seqlens)
+            q = self._appended(q, k, v, positions, cache, batch)
             out = cron_root_attention_paged(q, cache, batch.page_table, batch.seq_lens,
                                             batch.cu_seqlens, batch.max_query_len, batch.max_seqlen,
                                             batch.window, batch.relay)
         elif self.backend_for(x) == "sdpa":
+            q, k = self._turned(q, k, positions)
             out = F.scaled_dot_product_attention(q, k, v, is_causal=True,
                                                  enable_gqa=self.kv_groups > 1)
         else:
+            q, k = self._turned(q, k, positions)
             out = _layer_op(self.o_proj)(q, k, v, kv_groups=self.kv_groups)
         out = out.permute(0, 2, 1, 3).reshape(B, S, self.d_model)
         return self.drop(self.o_proj(out))

@@ -26,6 +26,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _native
+from .rotary import RotaryTable, qk_norm_rotary, rotary_embedding
 
 _DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 _STORES = {torch.float8_e4m3fn: _native.STORE_E4M3, torch.int8: _native.STORE_INT8}
@@ -173,6 +174,68 @@ class PagedKVCache:
         if batch is None:
             return
         _native.cache_write(self._struct, batch, _ready(k), _ready(v))
+
+    @torch.compiler.disable
+    def append(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor,
+               seq_lens: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None, *,
+               table: Optional[RotaryTable] = None, positions: Optional[torch.Tensor] = None,
+               norm: bool = False, q_weight: Optional[torch.Tensor] = None,
+               k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6) -> torch.Tensor:
+        """Norm and turn q and k of new tokens and store k and v, in one pass:
+        :func:`qk_norm_rotary` (``norm``) or :func:`rotary_embedding` and then
+        :meth:`write` (elements that turn may differ from those calls' in the last bit of
+        fp32 before they are rounded). No gradients.
+
+        Args:
+            q: [N, H_q, M, D] or packed [1, H_q, T, D]; k, v, page_table, seq_lens,
+                cu_seqlens: as in :meth:`write`.
+            table: the angles (None: the norm alone).
+            positions: as in :func:`rotary_embedding`; None: each token's place in its
+                sequence (seq_lens[b] - new tokens + t).
+            norm, q_weight, k_weight, eps: as in :func:`qk_norm_rotary`.
+
+        Returns: q turned, in its dtype and layout; rows of tokens outside every
+        sequence are zeros.
+        """
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                           for t in (q, k, v, q_weight, k_weight)):
+            raise NotImplementedError("the cache has no backward; append under torch.no_grad()")
+        op = _native.fast_op("cache_append")
+        if (op is not None and k.dtype == self.dtype and (table is None or type(table) is RotaryTable)
+                and not (table is not None and table.table.requires_grad)):
+            y = op(q, k, v, self.k, self.v, self.k_norm, self.k_scale, self.v_scale, page_table, seq_lens,
+                   cu_seqlens, self.head_dim, q_weight, k_weight, None if table is None else table.table,
+                   positions, table is not None and table.interleaved, norm, eps)
+            if y:
+                return y[0]
+        # what the operator does not take (or nobody does: the checks say why)
+        if _native.has_tangent(q, k, v, q_weight, k_weight):
+            raise NotImplementedError("the cache has no forward-mode derivatives")
+        if table is None and not norm:
+            raise ValueError("neither a table nor the norm: nothing to do to q and k (write stores them)")
+        if not norm and (q_weight is not None or k_weight is not None):
+            raise ValueError("weights without the norm")
+        batch = _batch(self, k, self.n_kv_heads, page_table, seq_lens, cu_seqlens, "k")
+        if v.shape != k.shape:
+            raise ValueError(f"v shape {tuple(v.shape)} does not match k {tuple(k.shape)}")
+        if v.dtype != k.dtype or v.device != k.device:
+            raise TypeError("k and v must have one dtype and device")
+        if q.dim() != 4 or (q.shape[0], *q.shape[2:]) != (k.shape[0], *k.shape[2:]):
+            raise ValueError(f"q shape {tuple(q.shape)} does not match k {tuple(k.shape)}")
+        if batch is None:
+            return torch.zeros_like(q)
+        if positions is None and table is not None:
+            positions = PagedBatch(page_table, seq_lens, cu_seqlens).positions(q.shape[2])
+        if norm:
+            q, k = qk_norm_rotary(q, k, q_weight, k_weight, table, positions, eps)
+        else:
+            q, k = rotary_embedding(q, k, table, positions)
+        self.write(k, v, page_table, seq_lens, cu_seqlens)
+        if cu_seqlens is not None:
+            t = torch.arange(q.shape[2], device=q.device)
+            inside = (t >= cu_seqlens[0]) & (t < cu_seqlens[-1])
+            q.masked_fill_(~inside[:, None], 0.0)
+        return q
 
     @torch.compiler.disable
     def read(self, page_table: torch.Tensor, seq_lens: torch.Tensor,

@@ -10,6 +10,8 @@
 
 namespace cra {
 
+enum { kSame = CRA_STORE_SAME, kE4M3 = CRA_STORE_E4M3, kInt8 = CRA_STORE_INT8 };
+
 // Row (page, head, offset) of a cache whose pages are [H_kv, page_size] rows:
 // the index of the row in k, v, and of its norm and scales. 32 bits hold it
 // (the ABI refuses caches of 2^31 rows); byte offsets take 64.

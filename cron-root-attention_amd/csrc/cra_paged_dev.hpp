@@ -15,7 +15,6 @@ namespace cra {
 constexpr float kInf = __builtin_huge_valf();
 constexpr int kFewRows = 16;  // rows of few_kernel's MFMA block
 constexpr int kChunkItems = 1024;  // pieces that chunk_kernel aims at: two rounds of resident workgroups
-enum { kSame = CRA_STORE_SAME, kE4M3 = CRA_STORE_E4M3, kInt8 = CRA_STORE_INT8 };
 
 struct PagedArgs {
   PagedView c;

@@ -13,8 +13,8 @@
 // varlen, CPU tensors) stays on the Python path; both reach the same C ABI.
 //
 // Beside them: rotary (rotary positions and head norms of q and k, with their
-// autograd), cache_write and paged_attention (a paged cache and the attention of new
-// tokens over it), for the same reason: at a few rows a call's host time is what
+// autograd), cache_write, cache_append and paged_attention (a paged cache and the
+// attention of new tokens over it), for the same reason: at a few rows a call's host time is what
 // it costs.
 //
 // The library is bound at run time (cra::bind(path)) so that the op uses the
@@ -50,6 +50,7 @@ struct Api {
   decltype(&cra_rotary_bwd_workspace_bytes) rotary_ws = nullptr;
   decltype(&cra_norm_rotary_bwd) norm_rotary_bwd = nullptr;
   decltype(&cra_cache_write) cache_write = nullptr;
+  decltype(&cra_cache_append) cache_append = nullptr;
   decltype(&cra_fwd_paged_workspace_bytes) paged_ws = nullptr;
   decltype(&cra_fwd_paged) fwd_paged = nullptr;
   decltype(&cra_strerror) strerror_ = nullptr;
@@ -87,6 +88,7 @@ void bind(std::string path) {
   resolve(h, path, "cra_rotary_bwd_workspace_bytes", api.rotary_ws);
   resolve(h, path, "cra_norm_rotary_bwd", api.norm_rotary_bwd);
   resolve(h, path, "cra_cache_write", api.cache_write);
+  resolve(h, path, "cra_cache_append", api.cache_append);
   resolve(h, path, "cra_fwd_paged_workspace_bytes", api.paged_ws);
   resolve(h, path, "cra_fwd_paged", api.fwd_paged);
   resolve(h, path, "cra_strerror", api.strerror_);
@@ -468,6 +470,23 @@ class CraRotary : public torch::autograd::Function<CraRotary> {
   }
 };
 
+// Positions [S], [1, S] or [B, S] of rows q [B, H, S, D].
+bool positions_fit(const at::Tensor& pos, const at::Tensor& q) {
+  if (pos.device() != q.device() || (pos.scalar_type() != at::kInt && pos.scalar_type() != at::kLong))
+    return false;
+  const int64_t n = pos.dim();
+  return n >= 1 && n <= 2 && pos.size(n - 1) == q.size(2) &&
+         (n == 1 || pos.size(0) == 1 || pos.size(0) == q.size(0));
+}
+
+bool weights_fit(const at::Tensor& wq, const at::Tensor& wk, const at::Tensor& q) {
+  for (const at::Tensor& w : {wq, wk})
+    if (w.defined() && (w.dim() != 1 || w.size(0) != q.size(3) || w.device() != q.device() || !w.is_contiguous() ||
+                        (w.scalar_type() != q.scalar_type() && w.scalar_type() != at::kFloat)))
+      return false;
+  return !wq.defined() || !wk.defined() || wq.scalar_type() == wk.scalar_type();
+}
+
 bool rotary_takes(const at::Tensor& q, const at::Tensor& k, const at::Tensor& wq, const at::Tensor& wk,
                   const at::Tensor& table, const at::Tensor& pos, bool norm, double eps) {
   if (q.dim() != 4 || !q.is_cuda() || !float_type(q.scalar_type()) || q.numel() == 0) return false;
@@ -482,19 +501,11 @@ bool rotary_takes(const at::Tensor& q, const at::Tensor& k, const at::Tensor& wq
                           (at::GradMode::is_enabled() && table.requires_grad()) || table._fw_grad(0).defined()))
     return false;
   if (pos.defined()) {
-    if (pos.device() != q.device() || (pos.scalar_type() != at::kInt && pos.scalar_type() != at::kLong))
-      return false;
-    const int64_t n = pos.dim();
-    if (n < 1 || n > 2 || pos.size(n - 1) != S || (n == 2 && pos.size(0) != 1 && pos.size(0) != B))
-      return false;
+    if (!positions_fit(pos, q)) return false;
   } else if (table.defined() && S > table.size(0)) {
     return false;
   }
-  for (const at::Tensor& w : {wq, wk})
-    if (w.defined() && (w.dim() != 1 || w.size(0) != D || w.device() != q.device() || !w.is_contiguous() ||
-                        (w.scalar_type() != q.scalar_type() && w.scalar_type() != at::kFloat)))
-      return false;
-  if (wq.defined() && wk.defined() && wq.scalar_type() != wk.scalar_type()) return false;
+  if (!weights_fit(wq, wk, q)) return false;
   if (wk.defined() && !k.defined()) return false;
   return !norm || eps >= 0;
 }
@@ -574,6 +585,46 @@ bool cache_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& kc,
   return true;
 }
 
+// q normed and turned, with k and v stored; nothing where the plain path does not take
+// the call.
+std::vector<at::Tensor> cache_append(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                     const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& norm,
+                                     const OptTensor& ks, const OptTensor& vs, const at::Tensor& table,
+                                     const at::Tensor& lens, const OptTensor& cu, int64_t head_dim,
+                                     const OptTensor& wq_in, const OptTensor& wk_in,
+                                     const OptTensor& angles_in, const OptTensor& pos_in,
+                                     bool interleaved, bool normed, double eps) {
+  const at::Tensor wq = get(wq_in), wk = get(wk_in), angles = get(angles_in), pos = get(pos_in);
+  cra_cache c;
+  cra_batch b;
+  if (!paged_call(k, kc, vc, norm, ks, vs, table, lens, cu, head_dim, c, b) || v.sizes() != k.sizes() ||
+      v.scalar_type() != k.scalar_type() || v.device() != k.device() || !paged_rows(v) ||
+      v._fw_grad(0).defined() || k.size(1) != kc.size(1) || q.dim() != 4 || q.numel() == 0 ||
+      (!angles.defined() && !normed) || (angles.defined() && angles.size(0) < 1) ||
+      (pos.defined() && !angles.defined()))
+    return {};
+  if (q.size(0) != k.size(0) || q.size(2) != k.size(2) || q.size(3) != head_dim ||
+      q.scalar_type() != k.scalar_type() || q.device() != k.device() || !sizes_fit(q) || !paged_rows(q) ||
+      q._fw_grad(0).defined())
+    return {};
+  if (angles.defined() &&
+      (angles.device() != q.device() || angles.dim() != 2 || angles.size(1) > head_dim || angles.size(1) % 2 ||
+       angles.scalar_type() != at::kFloat || !angles.is_contiguous() || angles._fw_grad(0).defined()))
+    return {};
+  if (pos.defined() && !positions_fit(pos, q)) return {};
+  if (!weights_fit(wq, wk, q) || (normed && !(eps >= 0)) || (!normed && (wq.defined() || wk.defined())))
+    return {};
+  c10::DeviceGuard guard(q.device());
+  at::Tensor y = at::empty_like(q);
+  if (!paged_rows(y)) return {};
+  const cra_turn p = make_turn(Turn{normed, interleaved, eps, angles, pos}, q, k, normed, wq.defined() ? wq : wk);
+  const int code = api().cache_append(&c, &b, &p, row_arg(q), row_arg(k), row_arg(v), ptr_of(wq),
+                                      ptr_of(wk), row_arg(y), stream_of(q));
+  if (code == CRA_E_UNSUPPORTED) return {};
+  check(code, "cra_cache_append");
+  return {y};
+}
+
 std::vector<at::Tensor> paged_attention(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc,
                                         const at::Tensor& norm, const OptTensor& ks, const OptTensor& vs,
                                         const at::Tensor& table, const at::Tensor& lens,
@@ -619,6 +670,11 @@ TORCH_LIBRARY(cra, m) {
       " Tensor(d!)? k_scale, Tensor(e!)? v_scale, Tensor page_table, Tensor seq_lens,"
       " Tensor? cu_seqlens, int head_dim) -> bool");
   m.def(
+      "cache_append(Tensor q, Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages,"
+      " Tensor(c!) k_norm, Tensor(d!)? k_scale, Tensor(e!)? v_scale, Tensor page_table,"
+      " Tensor seq_lens, Tensor? cu_seqlens, int head_dim, Tensor? wq, Tensor? wk, Tensor? table,"
+      " Tensor? positions, bool interleaved, bool norm, float eps) -> Tensor[]");
+  m.def(
       "paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor k_norm, Tensor? k_scale,"
       " Tensor? v_scale, Tensor page_table, Tensor seq_lens, Tensor? cu_seqlens, int head_dim,"
       " int max_query_len, int max_seqlen, int window, int relay, int top_k) -> Tensor[]");
@@ -635,5 +691,6 @@ TORCH_LIBRARY_IMPL(cra, CUDA, m) {
   m.impl("layer_attention", &attention_forward<true>);
   m.impl("rotary", &rotary_autograd);
   m.impl("cache_write", &cache_write);
+  m.impl("cache_append", &cache_append);
   m.impl("paged_attention", &paged_attention);
 }

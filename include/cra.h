@@ -368,6 +368,18 @@ typedef struct {
 int cra_cache_write(const cra_cache* c, const cra_batch* b, cra_tensor k, cra_tensor v, int32_t D,
                     void* stream);
 
+/* The norm and rotation of q and k (as cra_rotary: p->D columns, p->H_q heads of q and
+ * the cache's of k, p->norm with weights wq, wk) with k and v stored behind them (as
+ * cra_cache_write), in one launch; elements that turn may differ from those calls' in the
+ * last bit of fp32 before they are rounded. p->B and p->S are the
+ * batch's (n_seqs and query_len, or 1 and tokens). Without p->positions a token's is
+ * its place in its sequence. yq: like q; rows of tokens outside every sequence are
+ * zeros. Rows 16-byte aligned. CRA_E_UNSUPPORTED for weights, or halves of the turned
+ * part, that lie between 4-byte (fp32: 8-byte) steps. */
+int cra_cache_append(const cra_cache* c, const cra_batch* b, const cra_turn* p, cra_tensor q,
+                     cra_tensor k, cra_tensor v, const void* wq, const void* wk, cra_tensor yq,
+                     void* stream);
+
 /* Reads rows 0 .. length - 1 of every sequence into contiguous k, v
  * [n_seqs, H_kv, length, D] of the cache's dtype (rounded once); rows behind a
  * sequence are zeros, rows of a page outside the cache NaN. */
