@@ -15,6 +15,7 @@ import torch as _torch
 from .core import (GPU_SM_MAP, CronRootAttentionV14, CronRootAttentionV14Function,
                    cron_root_attention_v14, cron_root_attention_varlen, get_num_sms,
                    warmup_varlen_shapes)
+from .e4m3 import E4M3Linear, E4M3Weight, linear_e4m3
 from .hybrid import CronRootAttentionHybrid, cron_root_attention_hybrid
 from .module import CronRootAttention, CronRootMultiheadAttention
 from .paged import PagedBatch, PagedKVCache, cron_root_attention_paged
@@ -76,7 +77,8 @@ cron_root_attention = cron_root_attention_v14
 
 # The reference's own list (a star import gives what the reference's gives); what
 # this package adds is reached by name: RotaryTable, rotary_embedding,
-# qk_norm_rotary, PagedKVCache, PagedBatch, cron_root_attention_paged.
+# qk_norm_rotary, PagedKVCache, PagedBatch, cron_root_attention_paged,
+# E4M3Weight, E4M3Linear, linear_e4m3.
 __all__ = [
     "cron_root_attention",
     "cron_root_attention_v14",

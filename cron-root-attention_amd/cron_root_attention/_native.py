@@ -107,6 +107,10 @@ class CraPagedPlan(ctypes.Structure):
                 + [("scale", ctypes.c_float)])
 
 
+class CraLinear(ctypes.Structure):
+    _fields_ = [("M", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in ("N", "K", "dtype")]
+
+
 class CraDeviceInfo(ctypes.Structure):
     _fields_ = [("cu_count", ctypes.c_int32), ("lds_bytes_per_cu", ctypes.c_int32),
                 ("arch_major", ctypes.c_int32), ("arch_minor", ctypes.c_int32),
@@ -127,6 +131,7 @@ _R = ctypes.POINTER(CraTurn)
 _C = ctypes.POINTER(CraCache)
 _B = ctypes.POINTER(CraBatch)
 _G = ctypes.POINTER(CraPagedPlan)
+_L = ctypes.POINTER(CraLinear)
 _SIGNATURES = {
     "cra_supported_head_dim": (ctypes.c_int, [ctypes.c_int32]),
     "cra_global_rows": (ctypes.c_int64, [_P]),
@@ -186,6 +191,17 @@ _SIGNATURES = {
     "cra_fwd_paged_workspace_bytes": (ctypes.c_size_t, [_C, _B, _G]),
     "cra_fwd_paged": (ctypes.c_int, [_C, _B, _G, CraTensor, CraTensor, ctypes.c_void_p,
                                      ctypes.c_size_t, ctypes.c_void_p]),
+    "cra_e4m3_rows": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
+                                     ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,
+                                     ctypes.c_void_p, ctypes.c_void_p]),
+    "cra_e4m3_weight": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32,
+                                       ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,
+                                       ctypes.c_void_p, ctypes.c_void_p]),
+    "cra_linear_e4m3_workspace_bytes": (ctypes.c_size_t, [_L]),
+    "cra_linear_e4m3": (ctypes.c_int, [_L, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
+                                       ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                       ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t,
+                                       ctypes.c_void_p]),
     "cra_device_info": (ctypes.c_int, [ctypes.c_int32, ctypes.POINTER(CraDeviceInfo)]),
     "cra_tile_config": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int32,
                                        ctypes.POINTER(CraTileConfig)]),
@@ -267,7 +283,7 @@ _fast_state = {}
 
 
 def fast_op(name: str):
-    """``torch.ops.cra.<name>`` (rotary, cache_write, cache_append, paged_attention), or None
+    """``torch.ops.cra.<name>`` (rotary, cache_write, cache_append, paged_attention, linear_e4m3), or None
     without libcra_torch.so: the ctypes path then serves every call."""
     if name not in _fast_state:
         _fast_state[name] = (getattr(torch.ops.cra, name).default
@@ -649,6 +665,30 @@ def forward_paged(c: CraCache, b: CraBatch, p: CraPagedPlan, q, o):
     with on_device(q):
         _check(lib.cra_fwd_paged(cp, bp, pp, row_arg(q), row_arg(o), _ptr(ws), nbytes, _stream(q)),
                "cra_fwd_paged")
+
+
+# ---- products in 8-bit floating point --------------------------------------
+
+def e4m3_weight(w, codes, exponents):
+    """cra_e4m3_weight of w [N, K], columns contiguous."""
+    N, K = w.shape
+    with on_device(w):
+        _check(load_library().cra_e4m3_weight(w.data_ptr(), w.stride(0) if N > 1 else K, N, K,
+                                              dtype_code(w.dtype), codes.data_ptr(),
+                                              exponents.data_ptr(), _stream(w)), "cra_e4m3_weight")
+
+
+def linear_e4m3(x, codes, exponents, bias, y):
+    """cra_linear_e4m3 of x [M, K] (columns contiguous) into the contiguous y [M, N]."""
+    lib = load_library()
+    (M, K), N = x.shape, y.shape[1]
+    p = CraLinear(M, N, K, dtype_code(x.dtype))
+    nbytes = lib.cra_linear_e4m3_workspace_bytes(ctypes.byref(p))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    with on_device(x):
+        _check(lib.cra_linear_e4m3(ctypes.byref(p), x.data_ptr(), x.stride(0) if M > 1 else K,
+                                   codes.data_ptr(), exponents.data_ptr(), _ptr(bias), y.data_ptr(), N,
+                                   _ptr(ws), nbytes, _stream(x)), "cra_linear_e4m3")
 
 
 def tile_config(dtype: torch.dtype, D: int) -> dict:

@@ -1,0 +1,635 @@
+// Products in 8-bit floating point: y = x w^T (+ bias), both operands e4m3 codes with a
+// power-of-two scale, x for each row and block of 128 columns, w for each block of
+// 128 x 128; and the bringing of rows and weights into that form. C ABI front end.
+//
+// Block b of a row with m = max |x| is held as codes c and a scale s:
+//   s = the smallest power of two with m <= 448 s, at least 2^-126;  c = RNE(x / s)
+// (x / s and c s are exact but for that rounding, whatever the block's magnitude), and
+//   y_ij = sum_b s_ib t_jb (sum_{k in b} c_ik d_jk) + bias_j.
+// The scale is its exponent byte, as the matrix instruction takes it: the 16x16x128 MFMA
+// multiplies by both operands' scales on the way, so a block of 128 is one instruction
+// and no scaling is left to the VALU. A block that holds an infinity or NaN gets NaN
+// codes: its row of y is NaN.
+//
+// Sums: the 8-bit MFMA cuts the products it adds at about 2^-16 of the largest (measured:
+// 1.4e-5 of the result's norm for random operands, whatever K; its accumulator is fp32).
+// That is below the rounding of 16-bit results (fp16: 2e-4). fp32 results take the codes
+// widened to bf16 with their scales (exact) through the bf16 MFMA instead, at half its
+// rate or less: 3e-7.
+#include <stdio.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "../../include/cra.h"
+#include "cra_cache_dev.hpp"
+#include "cra_common.hpp"
+#include "cra_internal.hpp"
+#include "cra_paged.hpp"
+
+namespace cra {
+
+int set_error(int code, const char* msg);
+
+namespace {
+
+constexpr int kBlock = 128;
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+__host__ __device__ inline int up(int64_t n, int m) { return (int)((n + m - 1) / m); }
+
+// ---------------------------------------------------------------------------
+// Into 8 bits.
+// ---------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int n, bool wide, float (&x)[8]) {
+  if (wide) {
+    const Row8<T> r = *reinterpret_cast<const Row8<T>*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_f32(reinterpret_cast<const T*>(r.w)[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = i < n ? to_f32(p[i]) : 0.f;
+  }
+}
+__device__ __forceinline__ uint32_t largest(const float (&x)[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+  return m;
+}
+// Codes of eight elements of a block whose largest magnitude has the bits m, and the
+// block's exponent byte.
+__device__ __forceinline__ uint2 codes8(const float (&x)[8], uint32_t m, uint8_t& e) {
+  const float s = row_scale<kE4M3>(m);
+  e = s == s ? (uint8_t)(__float_as_uint(s) >> 23) : 127;
+  return s == s ? make_uint2(codes4<kE4M3>(x, s), codes4<kE4M3>(x + 4, s))
+                : make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
+}
+
+struct RowsArgs {
+  const void* x;
+  int64_t ldx;
+  uint8_t* codes;   // [M, 128 Kb]
+  uint8_t* scales;  // [M, Ks]
+  uint32_t blocks;  // M * Kb
+  int K, Kb, Ks;
+  FastDiv dKb;
+  int wide;         // rows lie between 16-byte addresses
+};
+
+// 16 lanes a block of a row, eight elements each.
+template <typename T>
+__global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
+  const uint32_t i = blockIdx.x * 16u + (threadIdx.x >> 4);
+  if (i >= a.blocks) return;  // whole rows of lanes
+  const uint32_t row = div_by(i, a.dKb);
+  const int b = (int)(i - row * a.Kb), lane = threadIdx.x & 15, col = b * kBlock + lane * 8;
+  float x[8];
+  load8<T>(static_cast<const T*>(a.x) + row * a.ldx + col, a.K - col, a.wide && col + 8 <= a.K, x);
+  uint8_t e;
+  const uint2 c = codes8(x, lanes_max(largest(x), 4), e);
+  *reinterpret_cast<uint2*>(a.codes + (int64_t)row * a.Kb * kBlock + col) = c;
+  if (lane == 0) a.scales[(int64_t)row * a.Ks + b] = e;
+}
+
+// A workgroup a block of 128 x 128: two threads a row.
+template <typename T>
+__global__ __launch_bounds__(256) void weight_kernel(const T* w, int64_t ldw, int N, int K, int Kb, int Ks,
+                                                     int wide, uint8_t* codes, uint8_t* scales) {
+  __shared__ uint32_t most[4];
+  const int row = blockIdx.y * kBlock + (threadIdx.x >> 1);
+  const int col0 = blockIdx.x * kBlock + (threadIdx.x & 1) * 64;
+  float x[8][8];
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int col = col0 + 8 * j;
+    load8<T>(w + (int64_t)min(row, N - 1) * ldw + col, row < N ? K - col : 0, wide && row < N && col + 8 <= K, x[j]);
+    m = max(m, largest(x[j]));
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o));
+  if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = m;
+  __syncthreads();
+  m = max(max(most[0], most[1]), max(most[2], most[3]));
+  uint8_t e;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint2 c = codes8(x[j], m, e);
+    if (row < N) *reinterpret_cast<uint2*>(codes + (int64_t)row * Kb * kBlock + col0 + 8 * j) = c;
+  }
+  if (threadIdx.x == 0) scales[(int64_t)blockIdx.y * Ks + blockIdx.x] = e;
+}
+
+// ---------------------------------------------------------------------------
+// Products. A wave holds w as the MFMA's rows and x as its columns: a lane's four
+// results are neighbours of one row of y.
+// ---------------------------------------------------------------------------
+struct LinearArgs {
+  const void* x;       // rows as they are (few rows)
+  int64_t ldx;
+  const uint8_t *xc, *xs;  // codes [M, Kp] and exponents [M, Ks]
+  const uint8_t *wc, *ws;  // codes [N, Kp] and exponents [ceil(N / 128), Ks]
+  const void* bias;
+  void* y;
+  int64_t ldy;
+  int64_t M;
+  int N, K, Kb, Kp, Ks;  // blocks of a row; columns of codes; exponents of a row
+  int tiles_m, tiles_n;
+  int wide_x, wide_y;    // rows of x between 16-byte addresses; four results of y as one store
+};
+
+// 32 codes of a row of a block: the same columns for both operands, in any order.
+struct Frag8 {
+  uint4 lo, hi;
+};
+
+// One 16 x 16 x 128 step: rows of w, columns of x, exponents of both in byte 0.
+__device__ __forceinline__ f32x4 mma8(f32x4 c, const Frag8& w, const Frag8& x, uint32_t sw, uint32_t sx) {
+  i32x8 a, b;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    a[i] = reinterpret_cast<const int*>(&w.lo)[i];
+    a[4 + i] = reinterpret_cast<const int*>(&w.hi)[i];
+    b[i] = reinterpret_cast<const int*>(&x.lo)[i];
+    b[4 + i] = reinterpret_cast<const int*>(&x.hi)[i];
+  }
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, (int)sw, 0, (int)sx);
+}
+
+// The codes as bf16 numbers, scale included.
+struct Wide {
+  Frag<bf16> f[4];
+};
+__device__ __forceinline__ Wide widen(const Frag8& c, uint32_t e) {
+  const float s = __uint_as_float((e & 0xffu) << 23);
+  Wide r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t w = i < 4 ? reinterpret_cast<const uint32_t*>(&c.lo)[i] : reinterpret_cast<const uint32_t*>(&c.hi)[i - 4];
+    uint32_t* o = reinterpret_cast<uint32_t*>(r.f[i / 2].w) + 2 * (i & 1);
+    o[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, s, false));
+    o[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, s, true));
+  }
+  return r;
+}
+__device__ __forceinline__ f32x4 mma_wide(f32x4 c, const Wide& w, const Wide& x) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c = mma(c, w.f[i], x.f[i]);
+  return c;
+}
+
+// Four results of row m, columns n .. n + 3.
+template <typename T>
+__device__ __forceinline__ void store4(const LinearArgs& a, int64_t m, int n, f32x4 c) {
+  if (m >= a.M || n >= a.N) return;
+  const T* bias = static_cast<const T*>(a.bias);
+  T e[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) e[r] = from_f32<T>(bias ? c[r] + to_f32(bias[min(n + r, a.N - 1)]) : c[r]);
+  T* p = static_cast<T*>(a.y) + m * a.ldy + n;
+  if (a.wide_y) {
+    if constexpr (sizeof(T) == 2)
+      *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(e);
+    else
+      *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(e);
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (n + r < a.N) p[r] = e[r];
+  }
+}
+
+// ROWS x 128 codes in LDS, 16-byte chunks XOR-swizzled so that 16 lanes reading one chunk
+// of 16 rows hit every bank once. A wave's instruction brings eight rows.
+template <int ROWS, int NW>
+struct CodeTile {
+  static constexpr int kBytes = ROWS * kBlock;
+  static constexpr int kPer = kBytes / 1024 / NW;  // instructions of a wave
+  static_assert(kPer * NW * 1024 == kBytes && NW % 2 == 0, "the swizzle repeats every 16 rows");
+  __device__ __forceinline__ static int off(int row, int chunk) {
+    return row * kBlock + ((chunk ^ (row >> 1 & 7)) << 4);
+  }
+  __device__ __forceinline__ static int lane_off(int wave, int lane, int Kp) {
+    const int row = wave * 8 + (lane >> 3);
+    return row * Kp + (((lane & 7) ^ (row >> 1 & 7)) << 4);
+  }
+  // rows behind the resource's last one load as zeros
+  __device__ __forceinline__ static void load(char* lds, __amdgpu_buffer_rsrc_t rsrc, int off, int Kp, int wave) {
+    const int w = __builtin_amdgcn_readfirstlane(wave) & (NW - 1);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, CRA_LDS(lds + (i * NW + w) * 1024), 16, off + i * NW * 8 * Kp, 0, 0, 0);
+  }
+  // 32 codes of row 16 blk + lane % 16: chunks g and g + 4
+  __device__ __forceinline__ static Frag8 frag(const char* lds, int blk, int lane) {
+    const int row = lane & 15, g = lane >> 4;
+    const char* p = lds + blk * 16 * kBlock;
+    return Frag8{*reinterpret_cast<const uint4*>(p + off(row, g)), *reinterpret_cast<const uint4*>(p + off(row, g + 4))};
+  }
+};
+
+// Tile of a workgroup: the dispatcher sends workgroup i to XCD i % 8; each XCD takes a
+// contiguous eighth of the tiles, which go down eight row tiles before the next column
+// tile, so that its L2 holds what its workgroups share.
+__device__ __forceinline__ void tile_of(const LinearArgs& a, int& tm, int& tn) {
+  const int all = a.tiles_m * a.tiles_n, x = blockIdx.x & 7, base = all >> 3, extra = all & 7;
+  const int i = x * base + min(x, extra) + (blockIdx.x >> 3);
+  constexpr int kDown = 8;
+  const int group = i / (kDown * a.tiles_n), first = group * kDown, down = min(kDown, a.tiles_m - first);
+  const int j = i - group * kDown * a.tiles_n;
+  tn = j / down;
+  tm = first + j - tn * down;
+}
+
+// WM x WN waves of (16 FM) x (16 FN) results over LDS tiles of a block of 128 columns,
+// two stages: the next block's loads run while this one is multiplied.
+template <typename T, int WM, int WN, int FM, int FN>
+__global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)))
+void linear_kernel(LinearArgs a) {
+  constexpr bool kWide = std::is_same<T, float>::value;
+  constexpr int NW = WM * WN, BM = 16 * FM * WM, BN = 16 * FN * WN;
+  static_assert(16 * FN <= kBlock && kBlock % (16 * FN) == 0, "one exponent of w a wave");
+  using TX = CodeTile<BM, NW>;
+  using TW = CodeTile<BN, NW>;
+  __shared__ __attribute__((aligned(1024))) char x0[TX::kBytes], w0[TW::kBytes], x1[TX::kBytes], w1[TW::kBytes];
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
+  int tm, tn;
+  tile_of(a, tm, tn);
+  const int64_t m0 = (int64_t)tm * BM;
+  const int n0 = tn * BN;
+  const int mrows = (int)min((int64_t)BM, a.M - m0), nrows = min(BN, a.N - n0);
+  const __amdgpu_buffer_rsrc_t rx = make_rsrc(a.xc + m0 * a.Kp, (uint32_t)mrows * a.Kp);
+  const __amdgpu_buffer_rsrc_t rw = make_rsrc(a.wc + (int64_t)n0 * a.Kp, (uint32_t)nrows * a.Kp);
+  const int ox = TX::lane_off(wave, lane, a.Kp), ow = TW::lane_off(wave, lane, a.Kp);
+  // exponents: of four blocks at once; a lane's rows of x, the wave's block of w
+  const uint32_t* sx[FM];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+    sx[i] = reinterpret_cast<const uint32_t*>(a.xs + min(m0 + 16 * (wm * FM + i) + l16, a.M - 1) * a.Ks);
+  const int nb = min((n0 + 16 * FN * wn) / kBlock, (a.N - 1) / kBlock);
+  const uint32_t* sw = reinterpret_cast<const uint32_t*>(a.ws + (int64_t)nb * a.Ks);
+  uint32_t ex[FM], ew;
+  uint32_t ex1[FM], ew1;
+#pragma unroll
+  for (int i = 0; i < FM; ++i) ex1[i] = sx[i][0];
+  ew1 = sw[0];
+
+  f32x4 acc[FN][FM];
+#pragma unroll
+  for (int n = 0; n < FN; ++n)
+#pragma unroll
+    for (int m = 0; m < FM; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  TX::load(x0, rx, ox, a.Kp, wave);
+  TW::load(w0, rw, ow, a.Kp, wave);
+  auto step = [&](auto second, int kb) __attribute__((always_inline)) {
+    constexpr bool kS = decltype(second)::value;
+    wait_vmem();
+    __syncthreads();
+    if (kb + 1 < a.Kb) {
+      if constexpr (kS) {
+        TX::load(x0, rx, ox + (kb + 1) * kBlock, a.Kp, wave);
+        TW::load(w0, rw, ow + (kb + 1) * kBlock, a.Kp, wave);
+      } else {
+        TX::load(x1, rx, ox + (kb + 1) * kBlock, a.Kp, wave);
+        TW::load(w1, rw, ow + (kb + 1) * kBlock, a.Kp, wave);
+      }
+    }
+    if ((kb & 3) == 0) {
+#pragma unroll
+      for (int i = 0; i < FM; ++i) ex[i] = ex1[i];
+      ew = ew1;
+      const int next = min(kb / 4 + 1, a.Ks / 4 - 1);
+#pragma unroll
+      for (int i = 0; i < FM; ++i) ex1[i] = sx[i][next];
+      ew1 = sw[next];
+    } else {
+#pragma unroll
+      for (int i = 0; i < FM; ++i) ex[i] >>= 8;
+      ew >>= 8;
+    }
+    const char* tx = (kS ? x1 : x0) + wm * FM * 16 * kBlock;
+    const char* tw = (kS ? w1 : w0) + wn * FN * 16 * kBlock;
+    if constexpr (kWide) {
+      Wide xf[FM];
+#pragma unroll
+      for (int m = 0; m < FM; ++m) xf[m] = widen(TX::frag(tx, m, lane), ex[m]);
+#pragma unroll
+      for (int n = 0; n < FN; ++n) {
+        const Wide wf = widen(TW::frag(tw, n, lane), ew);
+#pragma unroll
+        for (int m = 0; m < FM; ++m) acc[n][m] = mma_wide(acc[n][m], wf, xf[m]);
+      }
+    } else {
+      Frag8 xf[FM], wf[2];
+      wf[0] = TW::frag(tw, 0, lane);
+#pragma unroll
+      for (int m = 0; m < FM; ++m) xf[m] = TX::frag(tx, m, lane);
+#pragma unroll
+      for (int n = 0; n < FN; ++n) {
+        if (n + 1 < FN) wf[(n + 1) & 1] = TW::frag(tw, n + 1, lane);
+#pragma unroll
+        for (int m = 0; m < FM; ++m) acc[n][m] = mma8(acc[n][m], wf[n & 1], xf[m], ew, ex[m]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  };
+  for (int kb = 0; kb < a.Kb; kb += 2) {
+    step(std::false_type{}, kb);
+    if (kb + 1 < a.Kb) step(std::true_type{}, kb + 1);
+  }
+#pragma unroll
+  for (int m = 0; m < FM; ++m)
+#pragma unroll
+    for (int n = 0; n < FN; ++n)
+      store4<T>(a, m0 + 16 * (wm * FM + m) + l16, n0 + 16 * (wn * FN + n) + 4 * g, acc[n][m]);
+}
+
+// Few rows of x: bound by the reading of w. A workgroup takes 16 columns of y and all
+// (16 FM) rows, its waves a share of the blocks each, straight from memory into registers,
+// the first ones' loads on their way before x is looked at; they add up through LDS in
+// their order. RAW: x comes as it is, and each wave brings its blocks of the at most
+// kRawRows rows into 8 bits for itself.
+constexpr int kFewWaves = 8, kAheadBlocks = 4, kRawRows = 4, kRawBlocks = 16;
+
+template <typename T, typename X, int FM, bool RAW>
+__global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(LinearArgs a) {
+  constexpr bool kWide = std::is_same<T, float>::value;
+  constexpr int NW = kFewWaves, R = 16 * FM;
+  constexpr int kRawBytes = RAW ? kRawBlocks * kRawRows * kBlock : 16;
+  __shared__ __attribute__((aligned(16))) char raw[NW][kRawBytes];
+  __shared__ uint8_t raw_e[NW][RAW ? kRawBlocks * kRawRows : 4];
+  __shared__ float sums[NW][R][17];
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n0 = blockIdx.x * 16, M = (int)a.M;
+  const int per = (a.Kb + NW - 1) / NW, k0 = wave * per, k1 = min(a.Kb, k0 + per);
+  const uint8_t* wp = a.wc + (int64_t)min(n0 + l16, a.N - 1) * a.Kp + 16 * g;
+  const uint8_t* sw = a.ws + (int64_t)(n0 / kBlock) * a.Ks;
+  auto load_w = [&](int kb) {
+    const uint4* p = reinterpret_cast<const uint4*>(wp + (int64_t)kb * kBlock);
+    return Frag8{p[0], p[4]};
+  };
+  Frag8 wf[kAheadBlocks];
+  uint32_t ew[kAheadBlocks];
+#pragma unroll
+  for (int i = 0; i < kAheadBlocks; ++i) {
+    const int kb = max(min(k0 + i, k1 - 1), 0);
+    wf[i] = load_w(kb);
+    ew[i] = sw[kb];
+  }
+  if constexpr (RAW) {
+    const int n = (k1 - k0) * M;  // (block, row) pairs, four at a time
+    for (int i = g; i < n; i += 4) {
+      const int b = i / M, row = i - b * M, col = (k0 + b) * kBlock + l16 * 8;
+      float x[8];
+      load8<X>(static_cast<const X*>(a.x) + row * a.ldx + col, a.K - col, a.wide_x && col + 8 <= a.K, x);
+      uint8_t e;
+      const uint2 c = codes8(x, lanes_max(largest(x), 4), e);
+      *reinterpret_cast<uint2*>(raw[wave] + i * kBlock + l16 * 8) = c;
+      if (l16 == 0) raw_e[wave][i] = e;
+    }
+    __builtin_amdgcn_wave_barrier();  // the wave's own LDS, in order
+  }
+  f32x4 acc[FM];
+#pragma unroll
+  for (int m = 0; m < FM; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int base = k0; base < k1; base += kAheadBlocks) {
+#pragma unroll
+    for (int i = 0; i < kAheadBlocks; ++i) {
+      const int kb = base + i;
+      if (kb >= k1) break;
+      Frag8 xf[FM];
+      uint32_t ex[FM];
+#pragma unroll
+      for (int m = 0; m < FM; ++m) {
+        const int row = 16 * m + l16;
+        if constexpr (RAW) {
+          const int at = (kb - k0) * M + min(row, M - 1);
+          const uint4* p = reinterpret_cast<const uint4*>(raw[wave] + at * kBlock + 16 * g);
+          xf[m] = Frag8{p[0], p[4]};
+          ex[m] = raw_e[wave][at];
+        } else {
+          const int64_t r = min(row, M - 1);
+          const uint4* p = reinterpret_cast<const uint4*>(a.xc + r * a.Kp + (int64_t)kb * kBlock + 16 * g);
+          xf[m] = Frag8{p[0], p[4]};
+          ex[m] = a.xs[r * a.Ks + kb];
+        }
+      }
+      const Frag8 w = wf[i];
+      const uint32_t e = ew[i];
+      if (kb + kAheadBlocks < k1) {
+        wf[i] = load_w(kb + kAheadBlocks);
+        ew[i] = sw[kb + kAheadBlocks];
+      }
+      if constexpr (kWide) {
+        const Wide ww = widen(w, e);
+#pragma unroll
+        for (int m = 0; m < FM; ++m) acc[m] = mma_wide(acc[m], ww, widen(xf[m], ex[m]));
+      } else {
+#pragma unroll
+        for (int m = 0; m < FM; ++m) acc[m] = mma8(acc[m], w, xf[m], e, ex[m]);
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < FM; ++m)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sums[wave][16 * m + l16][4 * g + r] = acc[m][r];
+  __syncthreads();
+  for (int i = tid; i < 4 * R; i += 64 * NW) {
+    const int row = i >> 2, c = (i & 3) * 4;
+    f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < NW; ++w)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[r] += sums[w][row][c + r];
+    store4<T>(a, row, n0 + c, s);
+  }
+}
+
+int err(int code, const char* msg) { return set_error(code, msg); }
+
+int hip_err(hipError_t e, const char* where) {
+  if (e == hipSuccess) return CRA_OK;
+  char msg[256];
+  snprintf(msg, sizeof(msg), "%s: %s", where, hipGetErrorString(e));
+  return err(CRA_E_HIP, msg);
+}
+
+bool aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+template <typename F>
+hipError_t with_type(int dtype, F f) {
+  return dtype == CRA_F16 ? f(f16()) : dtype == CRA_BF16 ? f(bf16()) : f(float());
+}
+
+int check_type(int dtype) {
+  return dtype == CRA_F16 || dtype == CRA_BF16 || dtype == CRA_F32 ? CRA_OK : err(CRA_E_DTYPE, "unknown dtype code");
+}
+
+int check_linear(const cra_linear* p) {
+  if (!p) return err(CRA_E_INVALID, "linear is NULL");
+  if (int e = check_type(p->dtype)) return e;
+  if (p->M < 1 || p->N < 1 || p->K < 1) return err(CRA_E_INVALID, "M, N and K must be >= 1");
+  if (p->K > 1 << 22) return err(CRA_E_INVALID, "K above 2^22 is not built");  // a tile's rows within 2^31 bytes
+  if (p->M * (int64_t)up(p->K, kBlock) >= (int64_t)1 << 32) return err(CRA_E_INVALID, "M * K / 128 exceeds 2^32");
+  return CRA_OK;
+}
+
+// What a call launches.
+struct Plan {
+  int Kb, Kp, Ks;
+  bool few, raw;
+  int tile;  // 64, 128, 256
+  int64_t tiles_m;
+  int tiles_n;
+  size_t code_bytes, scale_bytes;
+};
+Plan plan_of(const cra_linear* p) {
+  Plan l{};
+  l.Kb = up(p->K, kBlock);
+  l.Kp = l.Kb * kBlock;
+  l.Ks = up(l.Kb, 4) * 4;
+  l.few = p->M <= 64;
+  l.raw = p->M <= kRawRows && up(l.Kb, kFewWaves) <= kRawBlocks;
+  l.tile = 256;
+  auto tiles = [&](int t) { return (int64_t)up(p->M, t) * up(p->N, t); };
+  if (tiles(256) < 256) l.tile = 128;
+  if (tiles(128) < 256) l.tile = 64;
+  l.tiles_m = up(p->M, l.tile);
+  l.tiles_n = up(p->N, l.tile);
+  if (!l.raw) {
+    l.code_bytes = ((size_t)p->M * l.Kp + 255) / 256 * 256;
+    l.scale_bytes = ((size_t)p->M * l.Ks + 255) / 256 * 256;
+  }
+  return l;
+}
+
+template <typename T>
+hipError_t run_rows(const RowsArgs& r, hipStream_t st) {
+  rows_kernel<T><<<(r.blocks + 15) / 16, 256, 0, st>>>(r);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t run_linear(const LinearArgs& a, const Plan& l, hipStream_t st) {
+  if (l.few) {
+    const uint32_t grid = (uint32_t)up(a.N, 16);
+    if (l.raw)
+      few_rows_kernel<T, T, 1, true><<<grid, 64 * kFewWaves, 0, st>>>(a);
+    else if (a.M <= 16)
+      few_rows_kernel<T, T, 1, false><<<grid, 64 * kFewWaves, 0, st>>>(a);
+    else if (a.M <= 32)
+      few_rows_kernel<T, T, 2, false><<<grid, 64 * kFewWaves, 0, st>>>(a);
+    else
+      few_rows_kernel<T, T, 4, false><<<grid, 64 * kFewWaves, 0, st>>>(a);
+    return hipGetLastError();
+  }
+  const uint32_t grid = (uint32_t)(l.tiles_m * l.tiles_n);
+  if (l.tile == 256) {
+    if constexpr (std::is_same<T, float>::value)
+      linear_kernel<T, 4, 2, 4, 8><<<grid, 512, 0, st>>>(a);
+    else
+      linear_kernel<T, 4, 2, 4, 8><<<grid, 512, 0, st>>>(a);
+  } else if (l.tile == 128) {
+    linear_kernel<T, 2, 2, 4, 4><<<grid, 256, 0, st>>>(a);
+  } else {
+    linear_kernel<T, 2, 2, 2, 2><<<grid, 256, 0, st>>>(a);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace
+}  // namespace cra
+
+using namespace cra;
+
+extern "C" {
+
+int cra_e4m3_rows(const void* x, int64_t ldx, int64_t M, int32_t K, int32_t dtype, void* codes,
+                  void* scales, void* stream) {
+  const cra_linear p{M, 1, K, dtype};
+  if (int e = check_linear(&p)) return e;
+  if (!x || !codes || !scales) return err(CRA_E_INVALID, "x, codes or scales is NULL");
+  const int esz = dtype == CRA_F32 ? 4 : 2;
+  if (!aligned(x, esz) || !aligned(codes, 16) || !aligned(scales, 4))
+    return err(CRA_E_LAYOUT, "x, codes or scales: misaligned pointer");
+  RowsArgs r{};
+  r.x = x, r.ldx = ldx;
+  r.codes = static_cast<uint8_t*>(codes);
+  r.scales = static_cast<uint8_t*>(scales);
+  r.K = K, r.Kb = up(K, kBlock), r.Ks = up(r.Kb, 4) * 4;
+  r.blocks = (uint32_t)(M * r.Kb);
+  r.dKb = fast_div(r.Kb);
+  r.wide = aligned(x, 16) && ldx * esz % 16 == 0;
+  if ((uint64_t)r.blocks * 16 >= (uint64_t)1 << 32) return err(CRA_E_INVALID, "too many rows for one launch");
+  return hip_err(with_type(dtype, [&](auto z) { return run_rows<decltype(z)>(r, (hipStream_t)stream); }),
+                 "cra_e4m3_rows");
+}
+
+int cra_e4m3_weight(const void* w, int64_t ldw, int32_t N, int32_t K, int32_t dtype, void* codes,
+                    void* scales, void* stream) {
+  const cra_linear p{1, N, K, dtype};
+  if (int e = check_linear(&p)) return e;
+  if (!w || !codes || !scales) return err(CRA_E_INVALID, "w, codes or scales is NULL");
+  const int esz = dtype == CRA_F32 ? 4 : 2;
+  if (!aligned(w, esz) || !aligned(codes, 16) || !aligned(scales, 4))
+    return err(CRA_E_LAYOUT, "w, codes or scales: misaligned pointer");
+  const int Kb = up(K, kBlock), Ks = up(Kb, 4) * 4;
+  if (up(N, kBlock) > 65535) return err(CRA_E_INVALID, "N above 2^23 is not built");
+  const int wide = aligned(w, 16) && ldw * esz % 16 == 0;
+  const dim3 grid(Kb, up(N, kBlock));
+  return hip_err(with_type(dtype, [&](auto z) {
+    using T = decltype(z);
+    weight_kernel<T><<<grid, 256, 0, (hipStream_t)stream>>>(static_cast<const T*>(w), ldw, N, K, Kb, Ks, wide,
+                                                            static_cast<uint8_t*>(codes),
+                                                            static_cast<uint8_t*>(scales));
+    return hipGetLastError();
+  }), "cra_e4m3_weight");
+}
+
+size_t cra_linear_e4m3_workspace_bytes(const cra_linear* p) {
+  if (check_linear(p)) return 0;
+  const Plan l = plan_of(p);
+  return l.code_bytes + l.scale_bytes;
+}
+
+int cra_linear_e4m3(const cra_linear* p, const void* x, int64_t ldx, const void* w_codes,
+                    const void* w_scales, const void* bias, void* y, int64_t ldy, void* workspace,
+                    size_t workspace_bytes, void* stream) {
+  if (int e = check_linear(p)) return e;
+  if (!x || !w_codes || !w_scales || !y) return err(CRA_E_INVALID, "x, w or y is NULL");
+  const int esz = p->dtype == CRA_F32 ? 4 : 2;
+  if (!aligned(x, esz) || !aligned(y, esz) || !aligned(bias, esz) || !aligned(w_codes, 16) || !aligned(w_scales, 4))
+    return err(CRA_E_LAYOUT, "x, w, bias or y: misaligned pointer");
+  const Plan l = plan_of(p);
+  const size_t need = l.code_bytes + l.scale_bytes;
+  if (need && (!workspace || !aligned(workspace, 16)))
+    return err(CRA_E_INVALID, "workspace: NULL or misaligned pointer");
+  if (workspace_bytes < need) return err(CRA_E_WORKSPACE, "workspace too small (cra_linear_e4m3_workspace_bytes)");
+  if (l.tiles_m * l.tiles_n >= (int64_t)1 << 22) return err(CRA_E_INVALID, "too many tiles for one launch");
+  hipStream_t st = (hipStream_t)stream;
+  LinearArgs a{};
+  a.x = x, a.ldx = ldx;
+  a.wc = static_cast<const uint8_t*>(w_codes);
+  a.ws = static_cast<const uint8_t*>(w_scales);
+  a.bias = bias;
+  a.y = y, a.ldy = ldy;
+  a.M = p->M, a.N = p->N, a.K = p->K;
+  a.Kb = l.Kb, a.Kp = l.Kp, a.Ks = l.Ks;
+  a.tiles_m = (int)l.tiles_m, a.tiles_n = l.tiles_n;
+  a.wide_x = aligned(x, 16) && ldx * esz % 16 == 0;
+  a.wide_y = p->N % 4 == 0 && ldy % 4 == 0 && aligned(y, 4 * esz);
+  if (!l.raw) {
+    char* ws = static_cast<char*>(workspace);
+    if (int e = cra_e4m3_rows(x, ldx, p->M, p->K, p->dtype, ws, ws + l.code_bytes, stream)) return e;
+    a.xc = reinterpret_cast<const uint8_t*>(ws);
+    a.xs = reinterpret_cast<const uint8_t*>(ws + l.code_bytes);
+  }
+  return hip_err(with_type(p->dtype, [&](auto z) { return run_linear<decltype(z)>(a, l, st); }), "cra_linear_e4m3");
+}
+
+}  // extern "C"

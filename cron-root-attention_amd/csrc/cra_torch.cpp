@@ -53,6 +53,8 @@ struct Api {
   decltype(&cra_cache_append) cache_append = nullptr;
   decltype(&cra_fwd_paged_workspace_bytes) paged_ws = nullptr;
   decltype(&cra_fwd_paged) fwd_paged = nullptr;
+  decltype(&cra_linear_e4m3_workspace_bytes) linear_ws = nullptr;
+  decltype(&cra_linear_e4m3) linear_e4m3 = nullptr;
   decltype(&cra_strerror) strerror_ = nullptr;
   decltype(&cra_last_error) last_error = nullptr;
   decltype(&cra_abi_version) abi_version = nullptr;
@@ -91,6 +93,8 @@ void bind(std::string path) {
   resolve(h, path, "cra_cache_append", api.cache_append);
   resolve(h, path, "cra_fwd_paged_workspace_bytes", api.paged_ws);
   resolve(h, path, "cra_fwd_paged", api.fwd_paged);
+  resolve(h, path, "cra_linear_e4m3_workspace_bytes", api.linear_ws);
+  resolve(h, path, "cra_linear_e4m3", api.linear_e4m3);
   resolve(h, path, "cra_strerror", api.strerror_);
   resolve(h, path, "cra_last_error", api.last_error);
   resolve(h, path, "cra_abi_version", api.abi_version);
@@ -650,6 +654,39 @@ std::vector<at::Tensor> paged_attention(const at::Tensor& q, const at::Tensor& k
   return {o};
 }
 
+// x [.., K] times the transpose of an 8-bit weight; nothing where the plain path does not
+// take the call.
+std::vector<at::Tensor> linear_e4m3(const at::Tensor& x, const at::Tensor& codes, const at::Tensor& exps,
+                                    const OptTensor& bias_in, int64_t N, int64_t K) {
+  const at::Tensor bias = get(bias_in);
+  const int64_t d = x.dim();
+  if (d < 1 || x.size(d - 1) != K || !float_type(x.scalar_type()) || x.device() != codes.device() ||
+      x.numel() == 0 || (K > 1 && x.stride(d - 1) != 1) || x._fw_grad(0).defined())
+    return {};
+  int64_t M = 1, ld = K;
+  if (d == 2) {
+    M = x.size(0);
+    ld = M > 1 ? x.stride(0) : K;
+  } else {
+    if (!x.is_contiguous()) return {};
+    M = x.numel() / K;
+  }
+  if (bias.defined() && (bias.dim() != 1 || bias.size(0) != N || bias.scalar_type() != x.scalar_type() ||
+                         bias.device() != x.device() || !bias.is_contiguous() || bias._fw_grad(0).defined()))
+    return {};
+  c10::DeviceGuard guard(x.device());
+  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = N;
+  at::Tensor y = at::empty(shape, x.options()), ws;
+  const cra_linear p{M, (int32_t)N, (int32_t)K, dtype_code(x.scalar_type())};
+  const size_t n = api().linear_ws(&p);
+  if (n) ws = at::empty({(int64_t)n}, x.options().dtype(at::kByte));
+  check(api().linear_e4m3(&p, x.data_ptr(), ld, codes.data_ptr(), exps.data_ptr(), ptr_of(bias), y.data_ptr(),
+                          N, ptr_of(ws), n, stream_of(x)),
+        "cra_linear_e4m3");
+  return {y};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(cra, m) {
@@ -678,6 +715,9 @@ TORCH_LIBRARY(cra, m) {
       "paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor k_norm, Tensor? k_scale,"
       " Tensor? v_scale, Tensor page_table, Tensor seq_lens, Tensor? cu_seqlens, int head_dim,"
       " int max_query_len, int max_seqlen, int window, int relay, int top_k) -> Tensor[]");
+  m.def(
+      "linear_e4m3(Tensor x, Tensor codes, Tensor exponents, Tensor? bias, int out_features,"
+      " int in_features) -> Tensor[]");
 }
 
 TORCH_LIBRARY_IMPL(cra, Autograd, m) {
@@ -693,4 +733,5 @@ TORCH_LIBRARY_IMPL(cra, CUDA, m) {
   m.impl("cache_write", &cache_write);
   m.impl("cache_append", &cache_append);
   m.impl("paged_attention", &paged_attention);
+  m.impl("linear_e4m3", &linear_e4m3);
 }

@@ -415,6 +415,37 @@ size_t cra_fwd_paged_workspace_bytes(const cra_cache* c, const cra_batch* b, con
 int cra_fwd_paged(const cra_cache* c, const cra_batch* b, const cra_paged_plan* p, cra_tensor q,
                   cra_tensor o, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- products in 8-bit floating point --------------------------------------
+ * No counterpart in the reference. y = x w^T + bias with x [M, K], w [N, K] as e4m3
+ * codes (NaN: 0x7f) and power-of-two scales given as exponent bytes e (2^(e - 127)):
+ * x for each row and block of 128 columns, w for each block of 128 x 128. Codes have
+ * rows of Kp = 128 ceil(K / 128) bytes (behind K zeros), exponents rows of Ks =
+ * 4 ceil(ceil(K / 128) / 4) bytes (what lies behind the blocks is not read as such). A
+ * block's scale is the smallest power of two s with max |x| <= 448 s, at least 2^-126;
+ * a block that holds an infinity or NaN has NaN codes. */
+typedef struct {
+  int64_t M;      /* rows of x and y */
+  int32_t N, K;   /* K up to 2^22 */
+  int32_t dtype;  /* of x, y and bias */
+} cra_linear;
+
+/* Rows x (ldx elements apart, columns contiguous) into codes [M, Kp], exponents [M, Ks]. */
+int cra_e4m3_rows(const void* x, int64_t ldx, int64_t M, int32_t K, int32_t dtype, void* codes,
+                  void* scales, void* stream);
+
+/* Weights w [N, K] (any dtype) into codes [N, Kp], exponents [ceil(N / 128), Ks]. */
+int cra_e4m3_weight(const void* w, int64_t ldw, int32_t N, int32_t K, int32_t dtype, void* codes,
+                    void* scales, void* stream);
+
+/* x and y as they are (rows ldx, ldy elements apart); bias [N] or NULL. Sums are fp32;
+ * 16-bit results take the 8-bit matrix instruction, which cuts products off at about
+ * 2^-16 of the largest it adds. The workspace (16-byte aligned; it may be none) is not
+ * used by another call at the same time. */
+size_t cra_linear_e4m3_workspace_bytes(const cra_linear* p);
+int cra_linear_e4m3(const cra_linear* p, const void* x, int64_t ldx, const void* w_codes,
+                    const void* w_scales, const void* bias, void* y, int64_t ldy, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
 const char* cra_strerror(int32_t code);
 const char* cra_last_error(void);
 int32_t cra_abi_version(void);
