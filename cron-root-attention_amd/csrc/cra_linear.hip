@@ -137,7 +137,7 @@ struct LinearArgs {
   int64_t M;
   int N, K, Kb, Kp, Ks;  // blocks of a row; columns of codes; exponents of a row
   int tiles_m, tiles_n;
-  int wide_x, wide_y;    // rows of x between 16-byte addresses; four results of y as one store
+  int wide_x, wide_y, wide_y8;  // rows of x between 16-byte addresses; four and eight results of y as one store
 };
 
 // 32 codes of a row of a block: the same columns for both operands, in any order.
@@ -231,16 +231,17 @@ struct CodeTile {
 };
 
 // Tile of a workgroup: the dispatcher sends workgroup i to XCD i % 8; each XCD takes a
-// contiguous eighth of the tiles, which go down eight row tiles before the next column
-// tile, so that its L2 holds what its workgroups share.
+// contiguous eighth of the tiles, which go down four row tiles before the next column
+// tile, so that its L2 holds what its workgroups share (16384 x 6144 x 4096 with four,
+// eight, sixteen: 297, 316, 320 us).
 __device__ __forceinline__ void tile_of(const LinearArgs& a, int& tm, int& tn) {
   const int all = a.tiles_m * a.tiles_n, x = blockIdx.x & 7, base = all >> 3, extra = all & 7;
   const int i = x * base + min(x, extra) + (blockIdx.x >> 3);
-  constexpr int kDown = 8;
+  constexpr int kDown = 4;
   const int group = i / (kDown * a.tiles_n), first = group * kDown, down = min(kDown, a.tiles_m - first);
   const int j = i - group * kDown * a.tiles_n;
-  tn = j / down;
-  tm = first + j - tn * down;
+  tn = __builtin_amdgcn_readfirstlane(j / down);  // what follows from them stays scalar
+  tm = __builtin_amdgcn_readfirstlane(first + j - tn * down);
 }
 
 // WM x WN waves of (16 FM) x (16 FN) results over LDS tiles of a block of 128 columns,
@@ -339,6 +340,196 @@ void linear_kernel(LinearArgs a) {
   for (int kb = 0; kb < a.Kb; kb += 2) {
     step(std::false_type{}, kb);
     if (kb + 1 < a.Kb) step(std::true_type{}, kb + 1);
+  }
+#pragma unroll
+  for (int m = 0; m < FM; ++m)
+#pragma unroll
+    for (int n = 0; n < FN; ++n)
+      store4<T>(a, m0 + 16 * (wm * FM + m) + l16, n0 + 16 * (wn * FN + n) + 4 * g, acc[n][m]);
+}
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+// Buffer resource over `bytes` bytes at `base`, in scalar registers.
+__device__ __forceinline__ u32x4 words_of(const void* base, uint32_t bytes) {
+  const uint64_t p = reinterpret_cast<uint64_t>(base);
+  u32x4 r;
+  r[0] = __builtin_amdgcn_readfirstlane((uint32_t)p);
+  r[1] = __builtin_amdgcn_readfirstlane((uint32_t)(p >> 32) & 0xffffu);
+  r[2] = __builtin_amdgcn_readfirstlane(bytes);
+  r[3] = 0x00020000;
+  return r;
+}
+__device__ __forceinline__ uint32_t lds_at(const void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
+}
+// One load of every lane, 16 or 4 bytes each, from resource + off + soff to LDS, lane after
+// lane. A row behind the resource's last byte loads as zeros: soff stays below one row.
+template <int BYTES>
+__device__ __forceinline__ void to_lds(uint32_t lds, u32x4 rsrc, int off, int soff) {
+  static_assert(BYTES == 16 || BYTES == 4, "a lane's load");
+  if constexpr (BYTES == 16)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                 :: "s"(lds), "v"(off), "s"(rsrc), "s"(soff) : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"
+                 :: "s"(lds), "v"(off), "s"(rsrc), "s"(soff) : "memory", "m0");
+}
+// All but the newest eight loads have landed, and the wave's LDS reads are done.
+__device__ __forceinline__ void wait_barrier() {
+  asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// Large 16-bit products: 256 x 256 results a workgroup, eight waves of 64 x 128, two waves
+// a SIMD, one workgroup a CU (132 KB of LDS). A block of 128 columns is 64 MFMAs a SIMD
+// (2048 cycles) beside 24 LDS reads of 1 KB a wave and 64 KB of loads.
+//
+// What bounds it is the loads' latency: with each block's loads issued a block ahead and
+// waited for at one barrier the kernel stood at 1.7 PFLOP/s (2.7 without the loads). So the
+// two stages are refilled piece by piece, as soon as a piece has been read: a block is two
+// halves with a barrier each; x is read into registers during the half before it is used,
+// so its place is free for the block after the next at the first barrier, a half of w
+// (64 of each wave's 128 columns) half a block after its reading. Every piece is on its way
+// for one and a half blocks, and a barrier waits for all but the newest eight of a wave's
+// loads. The loads are written as instructions: the compiler would wait for all of
+// them before each read of LDS.
+//
+// Measured, 8192 x 8192 x 8192 bf16: 384 us, 2.86 PFLOP/s; 16384 x 6144 x 4096: 297 us, 2.78
+// (library products of one scale: 2.66 and 2.98).
+template <typename T>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2)))
+void large_kernel(LinearArgs a) {
+  constexpr int FM = 4, FN = 8, NW = 8, WN = 2, BM = 256, BN = 256;
+  using TX = CodeTile<BM, NW>;
+  using TW = CodeTile<BN, NW>;
+  __shared__ __attribute__((aligned(1024))) char x0[TX::kBytes], x1[TX::kBytes], w00[TW::kBytes / 2], w01[TW::kBytes / 2], w10[TW::kBytes / 2], w11[TW::kBytes / 2];
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
+  int tm, tn;
+  tile_of(a, tm, tn);
+  const int64_t m0 = (int64_t)tm * BM;
+  const int n0 = tn * BN;
+  const int mrows = (int)min((int64_t)BM, a.M - m0), nrows = min(BN, a.N - n0);
+  const u32x4 rx = words_of(a.xc + m0 * a.Kp, (uint32_t)mrows * a.Kp);
+  const u32x4 rw = words_of(a.wc + (int64_t)n0 * a.Kp, (uint32_t)nrows * a.Kp);
+  const u32x4 re = words_of(a.xs + m0 * a.Ks, (uint32_t)mrows * a.Ks);
+  __shared__ uint32_t exps[2][NW][64];
+  const int ox = TX::lane_off(wave, lane, a.Kp), ow = TW::lane_off(wave, lane, a.Kp);
+  const int nb = min((n0 + 16 * FN * wn) / kBlock, (a.N - 1) / kBlock);
+  const __attribute__((address_space(4))) uint32_t* sw = (const __attribute__((address_space(4))) uint32_t*)(a.ws + (int64_t)nb * a.Ks);
+  uint32_t ex[FM], ew;
+  const int oe = (wm * 64 + lane) * a.Ks;
+  f32x4 acc[FN][FM];
+#pragma unroll
+  for (int n = 0; n < FN; ++n)
+#pragma unroll
+    for (int m = 0; m < FM; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int row8 = NW * 8 * a.Kp;
+  auto fill_x = [&](char* dst, int kb) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) to_lds<16>(lds_at(dst) + (i * NW + wave) * 1024, rx, ox + i * row8, kb * kBlock);
+  };
+  // half h of the columns of each of the two column waves: 64 of every 128 rows of w
+  auto fill_w = [&](char* dst, int h, int kb) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) to_lds<16>(lds_at(dst) + (i * NW + wave) * 1024, rw, ow + (2 * i + h) * row8, kb * kBlock);
+  };
+  auto fill_e = [&](int s, int q) __attribute__((always_inline)) { to_lds<4>(lds_at(exps[s][wave]), re, oe, 4 * q); };
+  const int last = a.Kb - 1, lastq = a.Ks / 4 - 1;
+  fill_e(0, 0);
+  fill_x(x0, 0);
+  fill_w(w00, 0, 0);
+  fill_x(x1, min(1, last));
+  fill_w(w01, 1, 0);
+  fill_w(w10, 0, min(1, last));
+  int q = 0;
+  Frag8 xf[2][FM];
+  wait_barrier();  // x of the first block (ten loads are newer)
+#pragma unroll
+  for (int m = 0; m < FM; ++m) xf[0][m] = TX::frag(x0 + wm * FM * 16 * kBlock, m, lane);
+  auto step = [&](auto second, int kb) __attribute__((always_inline)) {
+    constexpr bool kS = decltype(second)::value;
+    const char* txn = (kS ? x0 : x1) + wm * FM * 16 * kBlock;
+    const char* tw0 = (kS ? w10 : w00) + wn * 64 * kBlock;
+    const char* tw1 = (kS ? w11 : w01) + wn * 64 * kBlock;
+    wait_barrier();  // the first half of w has landed; x and the other stage's second half have been read
+    Frag8 wf[2];
+#pragma unroll
+    for (int n = 0; n < 1; ++n) wf[n] = TW::frag(tw0, n, lane);
+    fill_x(kS ? x1 : x0, min(kb + 2, last));
+    fill_w(kS ? w01 : w11, 1, min(kb + 1, last));
+    if (!kS && (kb & 2) == 0) {
+#pragma unroll
+      for (int i = 0; i < FM; ++i) ex[i] = exps[q & 1][wave][16 * i + l16];
+      ew = sw[q];
+      q = min(q + 1, lastq);
+      fill_e(q & 1, q);
+    } else {
+#pragma unroll
+      for (int i = 0; i < FM; ++i) ex[i] >>= 8;
+      ew >>= 8;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      if (n + 1 < 4) wf[(n + 1) & 1] = TW::frag(tw0, n + 1, lane);
+#pragma unroll
+      for (int m = 0; m < FM; ++m) acc[n][m] = mma8(acc[n][m], wf[n & 1], xf[kS][m], ew, ex[m]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    wait_barrier();  // the second half of w and the next x have landed; the first half has been read
+#pragma unroll
+    for (int n = 0; n < 1; ++n) wf[n] = TW::frag(tw1, n, lane);
+    fill_w(kS ? w10 : w00, 0, min(kb + 2, last));
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      if (n + 1 < 4) wf[(n + 1) & 1] = TW::frag(tw1, n + 1, lane);
+      xf[!kS][n] = TX::frag(txn, n, lane);
+#pragma unroll
+      for (int m = 0; m < FM; ++m) acc[4 + n][m] = mma8(acc[4 + n][m], wf[n & 1], xf[kS][m], ew, ex[m]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  for (int kb = 0; kb < a.Kb; kb += 2) {
+    step(std::false_type{}, kb);
+    if (kb + 1 < a.Kb) step(std::true_type{}, kb + 1);
+  }
+  wait_vmem();  // loads past the last block, too: LDS is used again
+  if (a.wide_y8) {
+    // rows of y leave as whole 256-byte pieces: through LDS, 64 rows of 128 columns a
+    // wave, chunks of 16 bytes swizzled by row
+    __syncthreads();
+    char* mine = wave < 2   ? x0 + wave * 16384
+                 : wave < 4 ? x1 + (wave - 2) * 16384
+                 : wave < 6 ? (wave == 4 ? w00 : w01)
+                            : (wave == 6 ? w10 : w11);
+#pragma unroll
+    for (int n = 0; n < FN; ++n) {
+      const int col = n0 + 16 * (wn * FN + n) + 4 * g;
+      f32x4 bias = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (a.bias && col < a.N) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) bias[r] = to_f32(static_cast<const T*>(a.bias)[col + r]);
+      }
+#pragma unroll
+      for (int m = 0; m < FM; ++m) {
+        const int row = 16 * m + l16, chunk = 2 * n + (g >> 1);
+        T e[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) e[r] = from_f32<T>(acc[n][m][r] + bias[r]);
+        *reinterpret_cast<uint2*>(mine + row * 256 + ((chunk ^ l16) << 4) + (g & 1) * 8) =
+            *reinterpret_cast<const uint2*>(e);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int row = 4 * i + g;
+      const uint4 v = *reinterpret_cast<const uint4*>(mine + row * 256 + ((l16 ^ (row & 15)) << 4));
+      const int64_t m = m0 + wm * 64 + row;
+      const int n = n0 + wn * 128 + l16 * 8;
+      if (m < a.M && n < a.N) *reinterpret_cast<uint4*>(static_cast<T*>(a.y) + m * a.ldy + n) = v;
+    }
+    return;
   }
 #pragma unroll
   for (int m = 0; m < FM; ++m)
@@ -533,7 +724,7 @@ hipError_t run_linear(const LinearArgs& a, const Plan& l, hipStream_t st) {
     if constexpr (std::is_same<T, float>::value)
       linear_kernel<T, 4, 2, 4, 8><<<grid, 512, 0, st>>>(a);
     else
-      linear_kernel<T, 4, 2, 4, 8><<<grid, 512, 0, st>>>(a);
+      large_kernel<T><<<grid, 512, 0, st>>>(a);
   } else if (l.tile == 128) {
     linear_kernel<T, 2, 2, 4, 4><<<grid, 256, 0, st>>>(a);
   } else {
@@ -623,6 +814,7 @@ int cra_linear_e4m3(const cra_linear* p, const void* x, int64_t ldx, const void*
   a.tiles_m = (int)l.tiles_m, a.tiles_n = l.tiles_n;
   a.wide_x = aligned(x, 16) && ldx * esz % 16 == 0;
   a.wide_y = p->N % 4 == 0 && ldy % 4 == 0 && aligned(y, 4 * esz);
+  a.wide_y8 = p->N % 8 == 0 && ldy % 8 == 0 && aligned(y, 16);
   if (!l.raw) {
     char* ws = static_cast<char*>(workspace);
     if (int e = cra_e4m3_rows(x, ldx, p->M, p->K, p->dtype, ws, ws + l.code_bytes, stream)) return e;
