@@ -18,7 +18,7 @@ from .core import (GPU_SM_MAP, CronRootAttentionV14, CronRootAttentionV14Functio
 from .e4m3 import E4M3Linear, E4M3Weight, linear_e4m3
 from .hybrid import CronRootAttentionHybrid, cron_root_attention_hybrid
 from .module import CronRootAttention, CronRootMultiheadAttention
-from .paged import PagedBatch, PagedKVCache, cron_root_attention_paged
+from .paged import PagedBatch, PagedKVCache, SharedPrefix, cron_root_attention_paged
 from .rotary import RotaryTable, qk_norm_rotary, rotary_embedding
 from . import _native
 
@@ -77,8 +77,8 @@ cron_root_attention = cron_root_attention_v14
 
 # The reference's own list (a star import gives what the reference's gives); what
 # this package adds is reached by name: RotaryTable, rotary_embedding,
-# qk_norm_rotary, PagedKVCache, PagedBatch, cron_root_attention_paged,
-# E4M3Weight, E4M3Linear, linear_e4m3.
+# qk_norm_rotary, PagedKVCache, PagedBatch, SharedPrefix,
+# cron_root_attention_paged, # E4M3Weight, E4M3Linear, linear_e4m3.
 __all__ = [
     "cron_root_attention",
     "cron_root_attention_v14",

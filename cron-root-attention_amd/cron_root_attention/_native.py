@@ -107,6 +107,10 @@ class CraPagedPlan(ctypes.Structure):
                 + [("scale", ctypes.c_float)])
 
 
+class CraPrefix(ctypes.Structure):
+    _fields_ = [("page_table", ctypes.c_void_p), ("length", ctypes.c_void_p), ("pages", ctypes.c_int32)]
+
+
 class CraLinear(ctypes.Structure):
     _fields_ = [("M", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in ("N", "K", "dtype")]
 
@@ -132,6 +136,7 @@ _C = ctypes.POINTER(CraCache)
 _B = ctypes.POINTER(CraBatch)
 _G = ctypes.POINTER(CraPagedPlan)
 _L = ctypes.POINTER(CraLinear)
+_X = ctypes.POINTER(CraPrefix)
 _SIGNATURES = {
     "cra_supported_head_dim": (ctypes.c_int, [ctypes.c_int32]),
     "cra_global_rows": (ctypes.c_int64, [_P]),
@@ -191,6 +196,9 @@ _SIGNATURES = {
     "cra_fwd_paged_workspace_bytes": (ctypes.c_size_t, [_C, _B, _G]),
     "cra_fwd_paged": (ctypes.c_int, [_C, _B, _G, CraTensor, CraTensor, ctypes.c_void_p,
                                      ctypes.c_size_t, ctypes.c_void_p]),
+    "cra_fwd_paged_shared_workspace_bytes": (ctypes.c_size_t, [_C, _B, _G, _X]),
+    "cra_fwd_paged_shared": (ctypes.c_int, [_C, _B, _G, _X, CraTensor, CraTensor, ctypes.c_void_p,
+                                            ctypes.c_size_t, ctypes.c_void_p]),
     "cra_e4m3_rows": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
                                      ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,
                                      ctypes.c_void_p, ctypes.c_void_p]),
@@ -656,10 +664,18 @@ def cache_read(c: CraCache, b: CraBatch, length: int, k, v):
                "cra_cache_read")
 
 
-def forward_paged(c: CraCache, b: CraBatch, p: CraPagedPlan, q, o):
-    """cra_fwd_paged into o."""
+def forward_paged(c: CraCache, b: CraBatch, p: CraPagedPlan, q, o, prefix: Optional[CraPrefix] = None):
+    """cra_fwd_paged (with a prefix: cra_fwd_paged_shared) into o."""
     lib = load_library()
     cp, bp, pp = ctypes.byref(c), ctypes.byref(b), ctypes.byref(p)
+    if prefix is not None:
+        xp = ctypes.byref(prefix)
+        nbytes = lib.cra_fwd_paged_shared_workspace_bytes(cp, bp, pp, xp)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+        with on_device(q):
+            _check(lib.cra_fwd_paged_shared(cp, bp, pp, xp, row_arg(q), row_arg(o), _ptr(ws), nbytes,
+                                            _stream(q)), "cra_fwd_paged_shared")
+        return
     nbytes = lib.cra_fwd_paged_workspace_bytes(cp, bp, pp)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     with on_device(q):

@@ -119,7 +119,7 @@ class CronRootAttention(nn.Module):
             q = self._appended(q, k, v, positions, cache, batch)
             out = cron_root_attention_paged(q, cache, batch.page_table, batch.seq_lens,
                                             batch.cu_seqlens, batch.max_query_len, batch.max_seqlen,
-                                            batch.window, batch.relay)
+                                            batch.window, batch.relay, prefix=batch.prefix)
         elif self.backend_for(x) == "sdpa":
             q, k = self._turned(q, k, positions)
             out = F.scaled_dot_product_attention(q, k, v, is_causal=True,

@@ -312,6 +312,39 @@ def _batch(cache, x, heads, page_table, seq_lens, cu_seqlens, name):
     return batch
 
 
+@dataclasses.dataclass
+class SharedPrefix:
+    """Rows that the sequences of a call have in common: their first ``length`` ones
+    (int32 [1] on the GPU) lie in the pages ``page_table`` (int32 [pages]), which the
+    sequences' own page tables begin with. Where ``length`` is no multiple of the page
+    size, the rows in its last page are the same in each sequence's own copy of it."""
+
+    page_table: torch.Tensor
+    length: torch.Tensor
+
+
+def _prefix(cache, prefix):
+    if prefix is None:
+        return None
+    if not isinstance(prefix, SharedPrefix):
+        raise TypeError("prefix must be a SharedPrefix")
+    for name, t in (("page_table", prefix.page_table), ("length", prefix.length)):
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
+            raise TypeError(f"the prefix's {name} must be an int32 tensor")
+        if t.device != cache.device:
+            raise ValueError(f"the prefix's {name} is on {t.device} but the cache is on {cache.device}")
+        if t.dim() != 1 or not t.is_contiguous():
+            raise ValueError(f"the prefix's {name} must be contiguous and of one dimension")
+    if prefix.length.shape != (1,):
+        raise ValueError(f"the prefix's length must be [1], got {list(prefix.length.shape)}")
+    if prefix.page_table.numel() * cache.page_size > 0x7fff0000:
+        raise ValueError("a prefix of 2^31 - 2^16 rows or more")
+    if prefix.page_table.numel() == 0:
+        return None
+    return _native.CraPrefix(prefix.page_table.data_ptr(), prefix.length.data_ptr(),
+                             prefix.page_table.numel())
+
+
 def _aligned(t: torch.Tensor) -> bool:
     vec = 16 // t.element_size()
     (sb, sh, ss, sd), shape = t.stride(), t.shape
@@ -332,7 +365,8 @@ def cron_root_attention_paged(q: torch.Tensor, cache: PagedKVCache, page_table: 
                               max_query_len: Optional[int] = None,
                               max_seqlen: Optional[int] = None, window: Optional[int] = None,
                               relay: Optional[bool] = None, relay_top_k: int = 2,
-                              out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                              out: Optional[torch.Tensor] = None,
+                              prefix: Optional[SharedPrefix] = None) -> torch.Tensor:
     """Attention of the new tokens of every sequence over the cache, which holds
     their own rows already (:meth:`PagedKVCache.write` comes first). No backward.
 
@@ -354,6 +388,11 @@ def cron_root_attention_paged(q: torch.Tensor, cache: PagedKVCache, page_table: 
         relay_top_k: relay rows a block (1..4).
         out: where the result goes, shaped as q; rows of tokens outside every
             sequence are left as they were.
+        prefix: rows that the sequences begin with together (a window is given then: by
+            the rule each length has blocks of its own). They are read once for all
+            sequences with at most 16 query rows a kv head (new tokens times H_q /
+            heads) whose new tokens lie behind them; the others attend as without. The
+            results are those without a prefix up to rounding.
 
     Returns: like q (laid out as q). Rows of tokens outside every sequence are zeros; so
     is a query that sees no row (more new tokens than the sequence's length). A
@@ -362,17 +401,23 @@ def cron_root_attention_paged(q: torch.Tensor, cache: PagedKVCache, page_table: 
     if torch.is_grad_enabled() and q.requires_grad:
         raise NotImplementedError("cron_root_attention_paged has no backward; call it under "
                                   "torch.no_grad() (training: cron_root_attention)")
+    if prefix is not None and window is None:
+        raise ValueError("a shared prefix needs a window: by the rule each length has blocks of its own")
     op = _native.fast_op("paged_attention")
     if (op is not None and out is None and q.dtype == cache.dtype and window != 0
-            and max_query_len != 0 and max_seqlen != 0):
+            and max_query_len != 0 and max_seqlen != 0
+            and (prefix is None or (type(prefix) is SharedPrefix and isinstance(prefix.page_table, torch.Tensor)
+                                    and isinstance(prefix.length, torch.Tensor)))):
         y = op(q, cache.k, cache.v, cache.k_norm, cache.k_scale, cache.v_scale, page_table, seq_lens,
                cu_seqlens, cache.head_dim, max_query_len or 0, max_seqlen or 0, window or 0,
-               -1 if relay is None else int(bool(relay)), relay_top_k)
+               -1 if relay is None else int(bool(relay)), relay_top_k,
+               None if prefix is None else prefix.page_table, None if prefix is None else prefix.length)
         if y:
             return y[0]
     if _native.has_tangent(q):
         raise NotImplementedError("cron_root_attention_paged has no forward-mode derivatives")
     batch = _batch(cache, q, None, page_table, seq_lens, cu_seqlens, "q")
+    shared = _prefix(cache, prefix)
     Hq, D = q.shape[1], q.shape[3]
     if Hq < 1 or Hq % cache.n_kv_heads:
         raise ValueError(f"H_q={Hq} must be a multiple of the cache's {cache.n_kv_heads} heads")
@@ -400,10 +445,10 @@ def cron_root_attention_paged(q: torch.Tensor, cache: PagedKVCache, page_table: 
         int(out is None), 1.0 / math.sqrt(D))
     qr = _ready(q)
     if D % 8 == 0 and _aligned(o):
-        _native.forward_paged(cache._struct, batch, plan, qr, o)
+        _native.forward_paged(cache._struct, batch, plan, qr, o, shared)
     else:  # through a buffer that the kernels can store to; o's other rows stay
         tmp = _ready(o) if cu_seqlens is not None else torch.empty_like(qr)
-        _native.forward_paged(cache._struct, batch, plan, qr, tmp)
+        _native.forward_paged(cache._struct, batch, plan, qr, tmp, shared)
         o.copy_(tmp[..., :D])
     return o
 
@@ -423,6 +468,7 @@ class PagedBatch:
     max_seqlen: Optional[int] = None
     window: Optional[int] = None
     relay: Optional[bool] = None
+    prefix: Optional[SharedPrefix] = None
 
     def positions(self, tokens: int) -> torch.Tensor:
         """Position of each new token, int32 [N, tokens] or (packed) [1, tokens];

@@ -110,12 +110,21 @@ __host__ __device__ inline int seq_prefix(int i, const SeqPlan& p) {
   return p.rpb * f + (ls != f * p.W ? 1 : 0);
 }
 
+// Global rows among the first P rows of a sequence (P behind its start, window W): those
+// that are read in the prefix alone. A block that P cuts has its first row there; its
+// relay rows depend on what follows.
+__host__ __device__ inline int prefix_slots(int P, int W, int rpb) {
+  const int f = P / W;
+  return rpb * f + (P != f * W ? 1 : 0);
+}
+
 // 32-key tiles of a sequence of n tokens, the last m of them new, that a row of
-// few_kernel meets; key tiles of BN rows that a row tile of the chunk kernels,
+// few_kernel meets (without its first P rows and G0 global rows); key tiles of BN rows that a row tile of the chunk kernels,
 // `span` new tokens wide, meets at most.
-__host__ __device__ inline int few_tile_count(int n, int m, const SeqPlan& p) {
-  const int pos0 = n - m > 0 ? n - m : 0, lo = pos0 - p.W + 1 > 0 ? pos0 - p.W + 1 : 0;
-  return ((n > 0 ? seq_prefix(n - 1, p) : 0) + 31) / 32 + (n - lo + 31) / 32;
+__host__ __device__ inline int few_tile_count(int n, int m, const SeqPlan& p, int P = 0, int G0 = 0) {
+  const int pos0 = n - m > 0 ? n - m : 0, lo = pos0 - p.W + 1 > P ? pos0 - p.W + 1 : P;
+  const int G = n > 0 ? seq_prefix(n - 1, p) : 0;
+  return (G > G0 ? G - G0 + 31 : 0) / 32 + (n - lo + 31) / 32;
 }
 __host__ __device__ inline int chunk_tile_count(int n, int span, int BN, const SeqPlan& p) {
   const int64_t local = (int64_t)p.W + span;

@@ -23,228 +23,11 @@
 #include <type_traits>
 
 #include "cra_paged_dev.hpp"
+#include "cra_paged_tiles.hpp"
 
 namespace cra {
 
 namespace {
-
-// Steps by which operand reads run ahead of their MFMAs: one less for 8-bit stores at
-// D = 128, whose scales and widening need the registers (a spilled one would wait
-// for the next tile's loads).
-template <int D, int STORE>
-constexpr int kAhead = D == 128 && STORE != kSame ? 2 : CRA_FWD_PF;
-
-// Scores of 8-bit keys: the rows' scales (LDS) come in here, exactly as fp32.
-template <int QB>
-__device__ __forceinline__ void scale_scores(f32x4 (&s)[2][QB], const float* ks, int kc, int g) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const f32x4 k = *reinterpret_cast<const f32x4*>(ks + 32 * kc + 16 * h + 4 * g);
-#pragma unroll
-    for (int qb = 0; qb < QB; ++qb) s[h][qb] *= k;
-  }
-}
-
-// One 32-key half: scores (8-bit: times the rows' scales) and exponentials against
-// the running maximum, which is raised where they call for it.
-template <typename T, int STORE, int D, int BN, int QB, bool MASK>
-__device__ __forceinline__ void chunk_softmax(f32x4 (&s)[2][QB], const float* ks, int kc,
-                                              f32x4 (&acc)[D / 16][QB], float (&m_run)[QB],
-                                              float (&l_run)[QB], float c2, int g,
-                                              const TileMask<QB>& mk, const Frag<T>& one,
-                                              Frag<T> (&pf)[QB]) {
-  if constexpr (STORE != kSame) scale_scores<QB>(s, ks, kc, g);
-  float ps[QB];
-  bool high = false;
-#pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
-    half_exp<T, MASK, QB>(s, kc, qb, c2, m_run[qb], g, mk, one, pf[qb], ps[qb]);
-    high |= !(ps[qb] <= kSumMax);
-  }
-  if (__any(high)) {
-#pragma unroll
-    for (int qb = 0; qb < QB; ++qb)
-      if (__any(!(ps[qb] <= kSumMax)))
-        half_rescale<T, D, QB>(s, qb, c2, acc, m_run, l_run, one, pf[qb], ps[qb]);
-  }
-#pragma unroll
-  for (int qb = 0; qb < QB; ++qb) l_run[qb] += ps[qb];
-}
-
-// A tile's halves kc0 .. kc1.
-template <typename T, int STORE, int D, int BN, int QB, bool MASK>
-__device__ __forceinline__ void attend_chunk(const char* tK, const char* tV, const float* ks,
-                                             const LaneOffs<D>& lo, const Frag<T> (&qf)[QB][D / 32],
-                                             f32x4 (&acc)[D / 16][QB], float (&m_run)[QB],
-                                             float (&l_run)[QB], float c2, int g,
-                                             const TileMask<QB>& mk, const Frag<T>& one, int kc0, int kc1) {
-  // (a loop over the halves would hold the accumulators twice, for its copies)
-#pragma unroll
-  for (int kc = 0; kc < BN / 32; ++kc) {
-    if (kc < kc0 || kc > kc1) continue;
-    f32x4 s[2][QB];
-    Frag<T> pf[QB];
-    tile_scores<T, D, BN, QB, kAhead<D, STORE>>(tK, lo, qf, kc, s);
-    chunk_softmax<T, STORE, D, BN, QB, MASK>(s, ks, kc, acc, m_run, l_run, c2, g, mk, one, pf);
-    pv_half<T, D, BN, QB, kAhead<D, STORE>>(tV, kc, lo, pf, acc);
-  }
-}
-
-// Both halves of a tile that every row sees: the second half's scores stand beside
-// the first one's exponentials, the first one's P.V beside the second's.
-template <typename T, int STORE, int D, int BN, int QB>
-__device__ __forceinline__ void attend_whole(const char* tK, const char* tV, const float* ks,
-                                             const LaneOffs<D>& lo, const Frag<T> (&qf)[QB][D / 32],
-                                             f32x4 (&acc)[D / 16][QB], float (&m_run)[QB],
-                                             float (&l_run)[QB], float c2, int g,
-                                             const TileMask<QB>& mk, const Frag<T>& one) {
-  static_assert(BN == 64, "two halves");
-  f32x4 s0[2][QB], s1[2][QB];
-  Frag<T> p0[QB], p1[QB];
-  tile_scores<T, D, BN, QB, kAhead<D, STORE>>(tK, lo, qf, 0, s0);
-  if constexpr (STORE != kSame) scale_scores<QB>(s0, ks, 0, g);
-  float ps[QB];
-  bool high = false;
-#pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
-    half_exp<T, false, QB>(s0, 0, qb, c2, m_run[qb], g, mk, one, p0[qb], ps[qb]);
-    high |= !(ps[qb] <= kSumMax);
-  }
-  tile_scores<T, D, BN, QB, kAhead<D, STORE>>(tK, lo, qf, 1, s1);
-  if (__any(high)) {
-#pragma unroll
-    for (int qb = 0; qb < QB; ++qb)
-      if (__any(!(ps[qb] <= kSumMax)))
-        half_rescale<T, D, QB>(s0, qb, c2, acc, m_run, l_run, one, p0[qb], ps[qb]);
-  }
-#pragma unroll
-  for (int qb = 0; qb < QB; ++qb) l_run[qb] += ps[qb];
-  if constexpr (STORE != kSame) scale_scores<QB>(s1, ks, 1, g);
-  high = false;
-#pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
-    half_exp<T, false, QB>(s1, 1, qb, c2, m_run[qb], g, mk, one, p1[qb], ps[qb]);
-    high |= !(ps[qb] <= kSumMax);
-  }
-  pv_half<T, D, BN, QB, kAhead<D, STORE>>(tV, 0, lo, p0, acc);
-  if (__any(high)) {
-#pragma unroll
-    for (int qb = 0; qb < QB; ++qb)
-      if (__any(!(ps[qb] <= kSumMax)))
-        half_rescale<T, D, QB>(s1, qb, c2, acc, m_run, l_run, one, p1[qb], ps[qb]);
-  }
-#pragma unroll
-  for (int qb = 0; qb < QB; ++qb) l_run[qb] += ps[qb];
-  pv_half<T, D, BN, QB, kAhead<D, STORE>>(tV, 1, lo, p1, acc);
-}
-
-// One query row over the keys of its piece, in fp32, touching only the rows it
-// sees: for rows whose tiles hold elements that are not finite. A lane takes a key
-// of the tile for the scores, D / 64 columns (or one, below 64) for P.V.
-template <typename T, int STORE, int D, int BN>
-__device__ __forceinline__ void careful_row(const PagedArgs& a, const Seq& s, const SeqPlan& p, int b,
-                                            int hk, int r, int pos, int t_first, int ntot, int nglob,
-                                            int gmax, int lo_k, int hi, int nloc, bool bad, int64_t part) {
-  constexpr int kCols = D > 64 ? D / 64 : 1;
-  const int lane = threadIdx.x & 63;
-  const int row_bytes = a.Ds * (STORE == kSame ? 2 : 1);
-  const int32_t* pages = a.c.table + b * a.c.table_stride;
-  const uint32_t* list = a.list + ((int64_t)b * a.c.H_kv + hk) * a.list_cap;
-  const T* q = q_row<T>(a, s, hk, r);
-  const int glen = pos >= 0 ? seq_prefix(pos, p) : 0;
-  auto element = [&](const char* base, uint32_t slot, int col) -> float {
-    const int64_t at = (int64_t)slot * row_bytes;
-    if constexpr (STORE == kSame)
-      return to_f32(reinterpret_cast<const T*>(base + at)[col]);
-    else
-      return code_value<STORE>((uint32_t)(uint8_t)base[at + col], 0);
-  };
-  float m = -kInf, l = 0.f, acc[kCols];
-#pragma unroll
-  for (int c = 0; c < kCols; ++c) acc[c] = 0.f;
-#pragma unroll 1
-  for (int it = t_first; it < ntot; ++it) {
-    const bool loc = it >= nglob;
-    const int ts = loc ? lo_k + (nloc - 1 - (it - nglob)) * BN : it * BN;
-    const bool sees = lane < BN && (loc ? ts + lane <= pos && ts + lane > pos - p.W && ts + lane < hi
-                                        : ts + lane < glen);
-    const uint64_t seen = __ballot(sees);
-    if (!seen) continue;
-    uint32_t slot = 0;
-    if (sees) {
-      if (!loc && p.rpb > 1)
-        slot = list[ts + lane];
-      else
-        slot = seq_row(pages, loc ? ts + lane : (ts + lane) * p.W, a.c.num_pages, a.c.H_kv, a.c.log_page, hk);
-      if (slot == kNoRow) slot = 0;  // the caller's `bad`
-    }
-    float x = 0.f;
-    if (sees) {
-#pragma unroll 1
-      for (int c = 0; c < a.D; c += 8) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x += element(a.c.k, slot, c + i) * to_f32(q[c + i]);
-      }
-    }
-    if constexpr (STORE != kSame) x *= sees ? a.c.k_scale[slot] : 0.f;
-    x = sees ? x * (a.scale * kLog2e) : -kInf;
-    float mx = x;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const float y = __shfl_xor(mx, o);
-      mx = mx > y || mx != mx ? mx : y;  // NaN stays
-    }
-    const float m_new = m != m || mx != mx ? __builtin_nanf("") : fmaxf(m, mx);
-    const float mu = m_new == -kInf ? 0.f : m_new;
-    const float alpha = m == -kInf ? 0.f : __builtin_amdgcn_exp2f(m - mu);
-    float e = sees ? __builtin_amdgcn_exp2f(x - mu) : 0.f, sum = e;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
-    l = l * alpha + sum;
-    if constexpr (STORE != kSame) e *= sees ? a.c.v_scale[slot] : 0.f;
-    m = m_new;
-#pragma unroll
-    for (int c = 0; c < kCols; ++c) acc[c] *= alpha;
-#pragma unroll 1
-    for (int j = 0; j < BN; j += 8) {
-      if (!(seen >> j & 0xff)) continue;
-      float v[8][kCols];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t sl = (uint32_t)__shfl((int)slot, j + i);  // a valid row where it is not seen
-#pragma unroll
-        for (int c = 0; c < kCols; ++c) {
-          const int col = lane * kCols + c;
-          v[i][c] = col < a.D ? element(a.c.v, sl, col) : 0.f;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float ej = __shfl(e, j + i);
-        if (seen >> (j + i) & 1) {
-#pragma unroll
-          for (int c = 0; c < kCols; ++c) acc[c] += ej * v[i][c];
-        }
-      }
-    }
-  }
-  if (bad) l = __builtin_nanf("");
-  if (part >= 0) {
-#pragma unroll
-    for (int c = 0; c < kCols; ++c)
-      if (lane * kCols + c < D) a.part[part * D + lane * kCols + c] = acc[c];
-    if (lane == 0) {
-      a.part_ml[2 * part] = m;
-      a.part_ml[2 * part + 1] = l;
-    }
-  } else {
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    T* o = o_row<T>(a, s, hk, r);
-#pragma unroll
-    for (int c = 0; c < kCols; ++c)
-      if (lane * kCols + c < a.D) o[lane * kCols + c] = from_f32<T>(acc[c] * inv);
-  }
-}
 
 template <int D>
 constexpr int kChunkQB = D > 128 ? 1 : 2;
@@ -500,10 +283,14 @@ void chunk_kernel(PagedArgs a) {
   }
   bad = __syncthreads_or(bad);
   if (__any(odd)) {
+    const KeyTiles keys{pages, list, hk, p.W, p.rpb, nglob, nloc, lo_k};
     for (int r = q0; r < min(q0 + kQW, rows); ++r) {
-      const int64_t at = w.part < 0 ? -1 : w.part + (r - r0);
-      careful_row<T, STORE, D, BN>(a, s, p, b, hk, r, pos_of(r), w.t_first, ntot, nglob, gmax, lo_k, hi,
-                                   nloc, bad, at);
+      const int64_t at = w.part + (r - r0);
+      const int pos = pos_of(r);
+      careful_row<T, STORE, D, BN>(a, keys, q_row<T>(a, s, hk, r), pos >= 0 ? seq_prefix(pos, p) : 0,
+                                   pos - p.W + 1, min(pos, hi - 1), w.t_first, ntot, bad,
+                                   w.part < 0 ? nullptr : a.part + at * D, a.part_ml + 2 * at,
+                                   o_row<T>(a, s, hk, r));
     }
     return;
   }

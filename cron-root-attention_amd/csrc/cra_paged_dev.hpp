@@ -34,6 +34,15 @@ struct PagedArgs {
   int parts;       // pieces of cut sequences (all kv heads) that the workspace holds
   int few_only;    // no chunk_kernel follows: longer sequences are refused (NaN)
   int zero_outside;  // rows of tokens outside every sequence are set to zero
+  // rows that the sequences have in common (SHARED)
+  const int32_t *ptable, *plen;  // their pages, and how many rows
+  int pcap;          // rows that the pages hold
+  uint32_t* plist;   // [H_kv, plist_cap] cache rows of their global rows (relay)
+  int plist_cap;
+  float *ppart, *ppart_ml;  // results of the prefix kernels: [item, BM rows, Dp], and (m, l)
+  int32_t* pinfo;    // [n_seqs] first row of each sequence among theirs, or -1; row tiles, pieces
+  int prefix_grid, prefix_rows;  // workgroups, and rows of one (BM)
+  int prefix_most;   // rows that the workspace holds
 };
 
 // A sequence of the call: length, new tokens, and where they lie in q and o.
@@ -73,6 +82,30 @@ __device__ __forceinline__ Seq wave_seq(const PagedArgs& a, int b) {
 
 __device__ __forceinline__ SeqPlan get_plan(const PagedArgs& a, int n) {
   return seq_plan(n, a.window, a.relay, a.top_k);
+}
+
+// Rows of the shared prefix, and the plan that its global rows follow.
+__device__ __forceinline__ SeqPlan prefix_plan(const PagedArgs& a) {
+  SeqPlan p;
+  const int n = __builtin_amdgcn_readfirstlane(a.plen[0]);
+  p.n = n < 0 ? 0 : n < a.pcap ? n : a.pcap;
+  p.W = a.window;
+  p.rpb = (a.relay < 0 ? p.n > 2048 : a.relay != 0) ? 1 + a.top_k : 1;
+  return p;
+}
+// What a sequence leaves to the prefix kernels: its first P rows and G0 global rows; none
+// (0) with more rows than few_kernel takes, with new tokens among the prefix's, or where
+// its length says otherwise about relay rows than the prefix's does. (A window of the
+// whole length has no global rows.)
+struct Share {
+  int P, G0;
+};
+__device__ __forceinline__ Share share_of(const PagedArgs& a, const SeqPlan& pp, const Seq& s, const SeqPlan& p) {
+  const int64_t rows = (int64_t)s.m * a.grp;
+  if (pp.n < 1 || rows < 1 || rows > a.part_rows || s.n - s.m < pp.n) return Share{0, 0};
+  if (p.W >= s.n) return Share{pp.n, 0};
+  if (pp.rpb != p.rpb) return Share{0, 0};
+  return Share{pp.n, prefix_slots(pp.n, pp.W, pp.rpb)};
 }
 
 // Row r of a kv head's rows is query head r % grp of the kv head, new token r / grp.
@@ -368,6 +401,16 @@ __device__ void join_chunk(const PagedArgs& a, uint32_t items) {
     for (int j = 0; j < 4; ++j) op[j] = from_f32<T>(o[j] * inv);
   }
 }
+
+// Rows and keys of the prefix kernels' tiles.
+struct PrefixTiles {
+  int rows, keys;
+};
+PrefixTiles prefix_tiles(int dtype, int Dp);
+// The shared prefix (a.prefix_grid workgroups), few_kernel over the sequences' own rows,
+// and the joining of both (cra_paged_prefix.hip).
+hipError_t launch_prefix(int dtype, int store, int Dp, const PagedArgs& a, uint32_t combine_grid,
+                         uint32_t few_grid, hipStream_t st);
 
 // chunk_kernel and the joining of its pieces (cra_paged_chunk.hip): grid
 // workgroups, at most join_tiles (sequence, tile, kv head)s of several pieces.

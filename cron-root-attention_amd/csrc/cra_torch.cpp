@@ -53,6 +53,8 @@ struct Api {
   decltype(&cra_cache_append) cache_append = nullptr;
   decltype(&cra_fwd_paged_workspace_bytes) paged_ws = nullptr;
   decltype(&cra_fwd_paged) fwd_paged = nullptr;
+  decltype(&cra_fwd_paged_shared_workspace_bytes) shared_ws = nullptr;
+  decltype(&cra_fwd_paged_shared) fwd_shared = nullptr;
   decltype(&cra_linear_e4m3_workspace_bytes) linear_ws = nullptr;
   decltype(&cra_linear_e4m3) linear_e4m3 = nullptr;
   decltype(&cra_strerror) strerror_ = nullptr;
@@ -93,6 +95,8 @@ void bind(std::string path) {
   resolve(h, path, "cra_cache_append", api.cache_append);
   resolve(h, path, "cra_fwd_paged_workspace_bytes", api.paged_ws);
   resolve(h, path, "cra_fwd_paged", api.fwd_paged);
+  resolve(h, path, "cra_fwd_paged_shared_workspace_bytes", api.shared_ws);
+  resolve(h, path, "cra_fwd_paged_shared", api.fwd_shared);
   resolve(h, path, "cra_linear_e4m3_workspace_bytes", api.linear_ws);
   resolve(h, path, "cra_linear_e4m3", api.linear_e4m3);
   resolve(h, path, "cra_strerror", api.strerror_);
@@ -634,9 +638,18 @@ std::vector<at::Tensor> paged_attention(const at::Tensor& q, const at::Tensor& k
                                         const at::Tensor& table, const at::Tensor& lens,
                                         const OptTensor& cu, int64_t head_dim, int64_t max_query_len,
                                         int64_t max_seqlen, int64_t window, int64_t relay,
-                                        int64_t top_k) {
+                                        int64_t top_k, const OptTensor& prefix_table,
+                                        const OptTensor& prefix_len) {
   cra_cache c;
   cra_batch b;
+  if (prefix_table.has_value() != prefix_len.has_value()) return {};
+  if (prefix_table.has_value() &&
+      (window < 1 || prefix_table->scalar_type() != at::kInt || prefix_len->scalar_type() != at::kInt ||
+       prefix_table->device() != kc.device() || prefix_len->device() != kc.device() || prefix_table->dim() != 1 ||
+       !prefix_table->is_contiguous() || !sizes_fit(*prefix_table) || prefix_table->numel() < 1 ||
+       prefix_len->dim() != 1 || prefix_len->size(0) != 1 ||
+       prefix_table->numel() * kc.size(2) > 0x7fff0000))
+    return {};
   if (!paged_call(q, kc, vc, norm, ks, vs, table, lens, cu, head_dim, c, b) || q.size(1) % kc.size(1) ||
       window < 0 || (relay != 0 && (top_k < 1 || top_k > 4)) || max_query_len < 0 || max_seqlen < 0)
     return {};
@@ -648,8 +661,19 @@ std::vector<at::Tensor> paged_attention(const at::Tensor& q, const at::Tensor& k
                    (int32_t)std::min<int64_t>(held, max_seqlen ? max_seqlen : held), 1,
                    (float)(1.0 / std::sqrt((double)head_dim))};
   at::Tensor o = at::empty_like(q), ws;
-  const size_t n = api().paged_ws(&c, &b, &p);
-  if (n) ws = at::empty({(int64_t)n}, q.options().dtype(at::kByte));
+  auto space = [&](size_t n) {
+    if (n) ws = at::empty({(int64_t)n}, q.options().dtype(at::kByte));
+    return n;
+  };
+  if (prefix_table.has_value()) {
+    const cra_prefix x{prefix_table->data_ptr<int32_t>(), prefix_len->data_ptr<int32_t>(),
+                       (int32_t)prefix_table->numel()};
+    const size_t n = space(api().shared_ws(&c, &b, &p, &x));
+    check(api().fwd_shared(&c, &b, &p, &x, row_arg(q), row_arg(o), ptr_of(ws), n, stream_of(q)),
+          "cra_fwd_paged_shared");
+    return {o};
+  }
+  const size_t n = space(api().paged_ws(&c, &b, &p));
   check(api().fwd_paged(&c, &b, &p, row_arg(q), row_arg(o), ptr_of(ws), n, stream_of(q)), "cra_fwd_paged");
   return {o};
 }
@@ -714,7 +738,8 @@ TORCH_LIBRARY(cra, m) {
   m.def(
       "paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor k_norm, Tensor? k_scale,"
       " Tensor? v_scale, Tensor page_table, Tensor seq_lens, Tensor? cu_seqlens, int head_dim,"
-      " int max_query_len, int max_seqlen, int window, int relay, int top_k) -> Tensor[]");
+      " int max_query_len, int max_seqlen, int window, int relay, int top_k, Tensor? prefix_table,"
+      " Tensor? prefix_len) -> Tensor[]");
   m.def(
       "linear_e4m3(Tensor x, Tensor codes, Tensor exponents, Tensor? bias, int out_features,"
       " int in_features) -> Tensor[]");

@@ -415,6 +415,26 @@ size_t cra_fwd_paged_workspace_bytes(const cra_cache* c, const cra_batch* b, con
 int cra_fwd_paged(const cra_cache* c, const cra_batch* b, const cra_paged_plan* p, cra_tensor q,
                   cra_tensor o, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Rows that the sequences of a call have in common: their first length[0] ones lie in the
+ * pages page_table[0 .. pages - 1] (device memory both; a row beyond them, and length
+ * below 0, counts as no part of it). */
+typedef struct {
+  const int32_t* page_table;
+  const int32_t* length;  /* [1] */
+  int32_t pages;
+} cra_prefix;
+
+/* cra_fwd_paged for sequences that begin with the same rows, which are read once for all
+ * of those with at most 16 query rows a kv head (new tokens x H_q / H_kv) whose new tokens
+ * lie behind them; the sequences' own page tables hold the prefix's pages, too, and
+ * others attend through those. The window is given (p->window >= 1): by the rule each
+ * length has blocks of its own. */
+size_t cra_fwd_paged_shared_workspace_bytes(const cra_cache* c, const cra_batch* b,
+                                            const cra_paged_plan* p, const cra_prefix* x);
+int cra_fwd_paged_shared(const cra_cache* c, const cra_batch* b, const cra_paged_plan* p,
+                         const cra_prefix* x, cra_tensor q, cra_tensor o, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
 /* ---- products in 8-bit floating point --------------------------------------
  * No counterpart in the reference. y = x w^T + bias with x [M, K], w [N, K] as e4m3
  * codes (NaN: 0x7f) and power-of-two scales given as exponent bytes e (2^(e - 127)):
