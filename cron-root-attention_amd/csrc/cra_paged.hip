@@ -72,8 +72,16 @@ template <typename F>
 __device__ __forceinline__ SelWork sel_work(const PagedArgs& a, int steps, F at_once) {
   SelWork k{};
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t bh = div_by(blockIdx.x, a.d_steps);  // workgroups a (sequence, head)
-  const int nw = steps * kSelWaves, w = (int)(blockIdx.x - bh * steps) * kSelWaves + wave;
+  uint32_t bh = div_by(blockIdx.x, a.d_steps);  // workgroups a (sequence, head)
+  const uint32_t own = (uint32_t)a.c.n_seqs * a.c.H_kv;
+  int step = (int)(blockIdx.x - bh * steps);
+  if (bh >= own) {  // the shared prefix has steps of its own
+    const int i = (int)(blockIdx.x - own * steps);
+    steps = (int)(gridDim.x - own * steps) / a.c.H_kv;
+    bh = own + i / steps;
+    step = i % steps;
+  }
+  const int nw = steps * kSelWaves, w = step * kSelWaves + wave;
   k.b = (int)div_by(bh, a.d_hkv);
   k.h = (int)(bh - (uint32_t)k.b * a.c.H_kv);
   int ls, skip = 0;  // blocks of rows below ls, but for the first ones
@@ -321,6 +329,7 @@ struct Launch {
   bool list, wide;        // relay rows are listed; blocks too wide for select_kernel
   int64_t list_cap;
   int sel_steps;          // select workgroups a (sequence, head)
+  int64_t prefix_steps;   // and of a head of the shared prefix
   int part_rows, few_grid;
   bool join;              // a sequence's keys may be cut into pieces
   int64_t items, joins;   // chunk pieces and row tiles of cut sequences, over all kv heads, at most
@@ -404,7 +413,17 @@ Launch plan_launch(const cra_cache* c, const cra_batch* b, const cra_paged_plan*
   // a wave a block while that is at most 4096 workgroups: sixteen a CU hide the
   // loads' latency, more of them cost their launch (the 16 and the 64 sequences of
   // select_kernel's figures with 2048, 4096, 8192: 13.2, 14.5, 19.1 and 12.9, 7.1, 9.6 us)
-  l.sel_steps = (int)std::max<int64_t>(1, std::min<int64_t>((cap + kSelWaves - 1) / kSelWaves, 4096 / bh));
+  auto steps = [](int64_t blocks, int64_t of) {
+    return std::max<int64_t>(1, std::min<int64_t>((blocks + kSelWaves - 1) / kSelWaves, 4096 / of));
+  };
+  l.sel_steps = (int)steps(cap, bh);
+  if (l.plist_cap) {
+    // sequences that share leave the prefix's blocks (all that its pages hold, most
+    // likely) to it
+    const int64_t held_x = (int64_t)x->pages * c->page_size;
+    l.prefix_steps = steps(held_x / p->window, c->H_kv);
+    l.sel_steps = (int)steps(std::max<int64_t>(l.max_len - held_x, 0) / p->window + 1, bh);
+  }
   l.list_bytes = up256(bh * l.list_cap * 4);
   l.part_rows = (int)std::min<int64_t>(kFewRows, most_rows);
   if (l.few) {
@@ -429,7 +448,7 @@ Launch plan_launch(const cra_cache* c, const cra_batch* b, const cra_paged_plan*
     const int64_t items = (rows + t.rows - 1) / t.rows * c->H_kv;  // before their keys are cut
     l.prefix_rows = t.rows;
     l.prefix_most = (int)rows;
-    l.prefix_grid = (int)std::max<int64_t>(256 * (f32 || l.Dp > 128 ? 1 : 2), std::min<int64_t>(items, 1024));
+    l.prefix_grid = (int)std::max<int64_t>(256, std::min<int64_t>(items, 1024));
     const int64_t parts = std::max<int64_t>(items, l.prefix_grid) * t.rows;  // rows of all pieces
     l.ppart_bytes = up256(parts * l.Dp * 4);
     l.pml_bytes = up256(parts * 2 * 4);
@@ -527,7 +546,7 @@ int attend(const cra_cache* c, const cra_batch* b, const cra_paged_plan* p, cons
     return err(CRA_E_WORKSPACE, msg);
   }
   const int64_t bh = (int64_t)b->n_seqs * c->H_kv;
-  const int64_t most = std::max({(bh + c->H_kv) * l.sel_steps, bh * l.part_rows, l.items,
+  const int64_t most = std::max({bh * l.sel_steps + c->H_kv * l.prefix_steps, bh * l.part_rows, l.items,
                                  (int64_t)l.ppart_bytes / (4 * l.Dp) / std::max(1, l.prefix_rows)});
   if (most >= (int64_t)1 << 24) return err(CRA_E_INVALID, "too many sequences or rows for one launch");
   PagedArgs a{};
@@ -567,7 +586,7 @@ int attend(const cra_cache* c, const cra_batch* b, const cra_paged_plan* p, cons
   hipStream_t st = (hipStream_t)stream;
   if (l.list) {
     a.d_steps = fast_div(l.sel_steps);
-    const uint32_t grid = (uint32_t)((bh + (l.plist_cap ? c->H_kv : 0)) * l.sel_steps);
+    const uint32_t grid = (uint32_t)(bh * l.sel_steps + c->H_kv * l.prefix_steps);
     auto kernel = l.wide ? (p->top_k <= 2 ? select_wide_kernel<2> : select_wide_kernel<4>)
                          : select_kernel;
     kernel<<<grid, 64 * kSelWaves, 0, st>>>(a, l.sel_steps);

@@ -23,8 +23,15 @@ namespace cra {
 
 namespace {
 
-constexpr int kPrefixWaves = 4;
+constexpr int kPrefixWaves = 8;
 constexpr int kLeastTiles = 2;  // key tiles of a piece
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+__device__ __forceinline__ int fresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
 
 // A row of a tile: where its q lies (head 0 of the kv head's), its window's start, and how
 // many global rows it sees. Rows behind the last one see nothing.
@@ -55,12 +62,12 @@ struct PrefixWork {
   int rows, tiles, pieces;
 };
 template <int BM, int BN>
-__device__ __forceinline__ PrefixWork prefix_work(const PagedArgs& a, const SeqPlan& pp, const PrefixSeq& first) {
+__device__ __forceinline__ PrefixWork prefix_work(const PagedArgs& a, const SeqPlan& pp) {
   const int lane = threadIdx.x & 63;
   PrefixWork w{};
   const bool tell = blockIdx.x == 0 && threadIdx.x < 64;  // for combine_kernel
   for (int base = 0; base < a.c.n_seqs; base += 64) {
-    const PrefixSeq x = base == 0 ? first : prefix_seq(a, pp, base + lane);
+    const PrefixSeq x = prefix_seq(a, pp, base + lane);
     const int upto = w.rows + (int)wave_upto(x.rows);
     if (tell && base + lane < a.c.n_seqs)
       a.pinfo[base + lane] = x.rows && upto <= a.prefix_most ? upto - x.rows : -1;
@@ -70,7 +77,7 @@ __device__ __forceinline__ PrefixWork prefix_work(const PagedArgs& a, const SeqP
   w.tiles = (w.rows + BM - 1) / BM;
   if (w.tiles > 0) {
     const int keys = (prefix_slots(pp.n, pp.W, pp.rpb) + BN - 1) / BN + (min(pp.n, pp.W) + BN - 1) / BN;
-    w.pieces = max(1, min(a.prefix_grid / (w.tiles * a.c.H_kv), keys / kLeastTiles));
+    w.pieces = uniform(max(1, min(a.prefix_grid / (w.tiles * a.c.H_kv), keys / kLeastTiles)));
   }
   if (tell && lane == 0) {
     a.pinfo[a.c.n_seqs] = w.tiles;
@@ -81,13 +88,13 @@ __device__ __forceinline__ PrefixWork prefix_work(const PagedArgs& a, const SeqP
 
 // Fills a tile's rows (one wave).
 template <int BM>
-__device__ __forceinline__ void prefix_rows(const PagedArgs& a, const SeqPlan& pp, const PrefixSeq& first, int r0,
-                                            int rows, PrefixRow (&info)[BM]) {
+__device__ __forceinline__ void prefix_rows(const PagedArgs& a, const SeqPlan& pp, int r0, int rows,
+                                            PrefixRow (&info)[BM]) {
   const int lane = threadIdx.x & 63;
   for (int i = rows - r0 + lane; i < BM; i += 64) info[i] = PrefixRow{0, pp.n, 0};
   int before = 0;
   for (int base = 0; base < a.c.n_seqs; base += 64) {
-    const PrefixSeq x = base == 0 ? first : prefix_seq(a, pp, base + lane);
+    const PrefixSeq x = prefix_seq(a, pp, base + lane);
     const int upto = before + (int)wave_upto(x.rows);
     int at = upto - x.rows - r0;
     for (int t = 0; t < x.s.m && x.rows; ++t) {
@@ -139,55 +146,81 @@ constexpr int kPrefixBN = D > 128 ? 32 : 64;
 template <int D>
 constexpr int kPrefixBM = 16 * kPrefixQB<D> * kPrefixWaves;
 
-// As chunk_kernel (cra_paged_chunk.hip): four waves of 16 QB rows, K/V tiles gathered
-// straight into LDS, 8-bit codes widened from there.
+// One load of every active lane, 16 or 4 bytes from its own address to LDS, lane after lane.
+template <int BYTES>
+__device__ __forceinline__ void gather_lds(const void* lds, const char* p) {
+  const uint32_t at =
+      __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)lds);
+  if constexpr (BYTES == 16)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(p) : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(at), "v"(p) : "memory", "m0");
+}
+// All but the newest N of the wave's loads have landed, its LDS reads are done, and the
+// other waves are as far.
+template <int N>
+__device__ __forceinline__ void wait_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// Eight waves of 16 QB rows over K/V tiles in four stages of LDS: a tile's rows are on
+// their way while three tiles are computed, the ids of their pages (or list entries) three
+// tiles more. Each wave brings eight rows of a tile (with fewer pieces than waves some
+// bring the same ones) by loads written as instructions: the compiler would wait for all of
+// them before each read of LDS. What bounds it is the softmax beside the MFMAs, as in
+// chunk_kernel; with two stages, four waves and two workgroups a CU it was the loads'
+// latency (64 tokens behind 32768 rows, 32/8 heads D = 128: 97 us).
+constexpr int kStages = 4;
+
 template <typename T, int STORE, int D>
 __global__ __launch_bounds__(64 * kPrefixWaves) __attribute__((amdgpu_waves_per_eu(2)))
 void prefix_kernel(PagedArgs a) {
   constexpr int NW = kPrefixWaves, QB = kPrefixQB<D>, BN = kPrefixBN<D>, kQW = 16 * QB, BM = kPrefixBM<D>;
   using Tile = SwzTile<D, BN>;
   constexpr bool k8 = STORE != kSame;
-  __shared__ __attribute__((aligned(1024))) char stage0[2][Tile::kBytes];
-  __shared__ __attribute__((aligned(1024))) char stage1[2][k8 ? 16 : Tile::kBytes];
-  __shared__ __attribute__((aligned(1024))) char raw[2][k8 ? BN * D : 16];
-  __shared__ __attribute__((aligned(16))) float kscale[2][BN], vscale[2][BN];
-  __shared__ uint32_t slots[2][BN];
+  // a wave's loads: kPer of K and of V, kRows rows each
+  constexpr int kRowBytes = D * (k8 ? 1 : 2), kChunks = kRowBytes / 16, kRows = 64 / kChunks;
+  constexpr int kLoads = BN / kRows, kPer = kLoads > NW ? kLoads / NW : 1, kMine = kPer * kRows;
+  static_assert(kLoads <= NW || kLoads % NW == 0, "loads of a tile");
+  constexpr int kOps = 1 + 2 * kPer + (k8 ? 2 : 0);  // of a tile: ids, rows, scales
+  constexpr int kIds = 8;                            // tiles whose ids are held
+  __shared__ __attribute__((aligned(1024))) char kt[kStages][BN * kRowBytes];
+  __shared__ __attribute__((aligned(1024))) char vt[kStages][BN * kRowBytes];
+  __shared__ __attribute__((aligned(1024))) char wide[2][k8 ? Tile::kBytes : 16];
+  __shared__ __attribute__((aligned(16))) float kscale[kStages][BN], vscale[kStages][BN];
+  __shared__ int32_t ids[kIds][NW][kMine];
   __shared__ PrefixRow info[BM];
 
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) & (NW - 1);
   const SeqPlan pp = prefix_plan(a);
-  const PrefixSeq first_seqs = prefix_seq(a, pp, lane);
-  const PrefixWork work = prefix_work<BM, BN>(a, pp, first_seqs);
+  const PrefixWork work = prefix_work<BM, BN>(a, pp);
   const int items = work.tiles * work.pieces * a.c.H_kv;
   const int row_bytes = a.Ds * (k8 ? 1 : 2);
   const float c2 = a.scale * kLog2e;
   const Frag<T> one = ones_frag<T>();
   LaneOffs<D> lo;
   lo.init(lane);
-  if (D * (k8 ? 1 : 2) > row_bytes) {  // columns that no load fills
-    auto clear = [&](auto& x) {
-      for (int i = tid; i < (int)sizeof(x) / 16; i += 64 * NW)
-        reinterpret_cast<uint4*>(&x[0][0])[i] = make_uint4(0, 0, 0, 0);
-    };
-    if constexpr (k8) {
-      clear(raw);
-    } else {
-      clear(stage0);
-      clear(stage1);
+  if (kRowBytes > row_bytes) {  // columns that no load fills
+    for (int i = tid; i < (int)sizeof(kt) / 16; i += 64 * NW) {
+      reinterpret_cast<uint4*>(&kt[0][0])[i] = make_uint4(0, 0, 0, 0);
+      reinterpret_cast<uint4*>(&vt[0][0])[i] = make_uint4(0, 0, 0, 0);
     }
   }
+  // the wave's rows of a tile: load i, row j of it
+  const int load0 = kLoads < NW ? wave & (kLoads - 1) : wave;
+  auto tile_row = [&](int i, int j) { return (i * NW + load0) * kRows + j; };
   // items of one head stand H_kv apart: with a multiple of 8 heads they meet in one XCD's L2
   for (int item = blockIdx.x; item < items; item += gridDim.x) {
-    const int rest = (int)div_by(item, a.d_hkv), hk = item - rest * a.c.H_kv;
-    const int piece = rest / work.tiles, r0 = (rest - piece * work.tiles) * BM;
+    const int rest = uniform((int)div_by(item, a.d_hkv)), hk = item - rest * a.c.H_kv;
+    const int piece = uniform(rest / work.tiles), r0 = (rest - piece * work.tiles) * BM;
     __syncthreads();  // the rows of the item before are done with
-    if (wave == 0) prefix_rows<BM>(a, pp, first_seqs, r0, work.rows, info);
+    if (wave == 0) prefix_rows<BM>(a, pp, r0, work.rows, info);
     __syncthreads();
     const int rows = min(BM, work.rows - r0);
     const PrefixKeys all = prefix_keys<BM>(info, 0, rows, pp.n);
     const int nglob = (all.gmax + BN - 1) / BN, nloc = (pp.n - all.ls_min + BN - 1) / BN;
-    const int per = (nglob + nloc + work.pieces - 1) / work.pieces;
+    const int per = uniform((nglob + nloc + work.pieces - 1) / work.pieces);
     const int t_first = piece * per, ntot = min(nglob + nloc, t_first + per);
     const KeyTiles keys{a.ptable, a.plist + (int64_t)hk * a.plist_cap, hk, pp.W, pp.rpb, nglob, nloc, all.ls_min};
     bool bad = false;
@@ -195,66 +228,80 @@ void prefix_kernel(PagedArgs a) {
     auto tile_start = [&](int it) {
       return it >= nglob ? all.ls_min + (nloc - 1 - (it - nglob)) * BN : it * BN;
     };
-    auto look_up = [&](int it) -> uint32_t {
-      if (tid >= BN) return 0u;
-      const int ts = tile_start(it), i = it < nglob ? min(ts + tid, all.gmax - 1) : min(ts + tid, pp.n - 1);
-      const uint32_t r = it < nglob && pp.rpb > 1
-                             ? keys.list[i]
-                             : seq_row(keys.pages, it < nglob ? i * pp.W : i, a.c.num_pages, a.c.H_kv, a.c.log_page, hk);
-      bad |= r == kNoRow;
-      return r == kNoRow ? 0u : r;
+    // row of the prefix, or place in its list, of a tile's row (the last one behind the end)
+    auto key_of = [&](int it, int row) {
+      return min(tile_start(it) + row, (it < nglob ? all.gmax : pp.n) - 1);
     };
-    auto keep = [&](int it, uint32_t r) {
-      if (tid < BN) slots[it & 1][tid] = r;
+    auto listed = [&](int it) { return it < nglob && pp.rpb > 1; };
+    // (what follows from the lane is formed anew for each tile: held over the loop it
+    // would leave no registers for the tile's steps)
+    auto fetch_ids = [&](int it) __attribute__((always_inline)) {
+      it = min(it, ntot - 1);
+      const int lane = fresh(threadIdx.x & 63);
+      if (lane < kMine) {
+        const int i = key_of(it, tile_row(lane / kRows, lane % kRows));
+        const int at = listed(it) ? i : (it < nglob ? i * pp.W : i) >> a.c.log_page;
+        gather_lds<4>(ids[it & (kIds - 1)][wave],
+                      reinterpret_cast<const char*>(listed(it) ? reinterpret_cast<const int32_t*>(keys.list) + at
+                                                               : keys.pages + at));
+      }
     };
-    constexpr int kPiecesRow = k8 ? D / 16 : Tile::kCPR;
-    constexpr int kAll = BN * kPiecesRow, kPer = (kAll + 64 * NW - 1) / (64 * NW);
-    auto issue = [&](int it, auto& dst) {
+    auto cache_row_of = [&](int it, int i, int j) -> uint32_t {
+      const int32_t id = ids[it & (kIds - 1)][wave][i * kRows + j];
+      if (listed(it)) return (uint32_t)id;
+      const int key = key_of(it, tile_row(i, j)), row = it < nglob ? key * pp.W : key;
+      if ((uint32_t)id >= (uint32_t)a.c.num_pages) return kNoRow;
+      return cache_row(id, a.c.H_kv, a.c.log_page, hk, row & ((1 << a.c.log_page) - 1));
+    };
+    auto fill = [&](int it, int s) __attribute__((always_inline)) {
+      it = min(it, ntot - 1);
+      const int lane = fresh(threadIdx.x & 63);
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        const int t = i * NW + wave;
-        if (kAll % (64 * NW) != 0 && t * 64 >= kAll) break;
-        const int row = (t * 64 + lane) / kPiecesRow, col = (t * 64 + lane) % kPiecesRow;
-        const int chunk = k8 ? col : col ^ Tile::swz(row);
-        const int64_t at = (int64_t)slots[it & 1][row] * row_bytes + chunk * 16;
+        const int j = lane / kChunks, row = tile_row(i, j);
+        const int chunk = k8 ? lane % kChunks : (lane % kChunks) ^ Tile::swz(row);
+        uint32_t r = cache_row_of(it, i, j);
+        bad |= r == kNoRow;
+        r = r == kNoRow ? 0u : r;
+        const int64_t at = (int64_t)r * row_bytes + chunk * 16;
+        const int dst = (i * NW + load0) * 1024;
         if (chunk * 16 < row_bytes) {
-          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(a.c.k + at),
-                                           CRA_LDS(dst[0] + t * 1024), 16, 0, 0);
-          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(a.c.v + at),
-                                           CRA_LDS(dst[1] + t * 1024), 16, 0, 0);
+          gather_lds<16>(kt[s] + dst, a.c.k + at);
+          gather_lds<16>(vt[s] + dst, a.c.v + at);
+        }
+      }
+      if constexpr (k8) {
+        static_assert(!k8 || kPer == 1, "one load a wave");
+        if (lane < kRows) {
+          uint32_t r = cache_row_of(it, 0, lane);
+          r = r == kNoRow ? 0u : r;
+          gather_lds<4>(kscale[s] + load0 * kRows, reinterpret_cast<const char*>(a.c.k_scale + r));
+          gather_lds<4>(vscale[s] + load0 * kRows, reinterpret_cast<const char*>(a.c.v_scale + r));
         }
       }
     };
-    auto widen = [&](const float (&vs)[BN]) {
+    // codes of stage s into the 16-bit tile
+    auto widen = [&](int s) __attribute__((always_inline)) {
+      const int tid = fresh(threadIdx.x);
+      constexpr int kAll = BN * kChunks, kEach = (kAll + 64 * NW - 1) / (64 * NW);
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int p = i * 64 * NW + tid, row = p / kPiecesRow, col = p % kPiecesRow;
+      for (int i = 0; i < kEach; ++i) {
+        const int p = i * 64 * NW + tid, row = p / kChunks, col = p % kChunks;
         if (kAll % (64 * NW) != 0 && p >= kAll) break;
-        const uint4 k4 = *reinterpret_cast<const uint4*>(raw[0] + p * 16);
-        const uint4 v4 = *reinterpret_cast<const uint4*>(raw[1] + p * 16);
+        const uint4 k4 = *reinterpret_cast<const uint4*>(kt[s] + p * 16);
+        const uint4 v4 = *reinterpret_cast<const uint4*>(vt[s] + p * 16);
         const uint32_t wk[4] = {k4.x, k4.y, k4.z, k4.w}, wv[4] = {v4.x, v4.y, v4.z, v4.w};
-        const float sc = vs[row];
+        const float sc = vscale[s][row];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint2 x = widen4<T, STORE>(wk[2 * h]), y = widen4<T, STORE>(wk[2 * h + 1]);
-          *reinterpret_cast<uint4*>(stage0[0] + Tile::off(row, 2 * col + h)) = make_uint4(x.x, x.y, y.x, y.y);
+          *reinterpret_cast<uint4*>(wide[0] + Tile::off(row, 2 * col + h)) = make_uint4(x.x, x.y, y.x, y.y);
           float f[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) f[j] = code_value<STORE>(wv[2 * h + j / 4], j % 4) * sc;
-          *reinterpret_cast<uint4*>(stage0[1] + Tile::off(row, 2 * col + h)) = pack8<T>(f).w[0];
+          *reinterpret_cast<uint4*>(wide[1] + Tile::off(row, 2 * col + h)) = pack8<T>(f).w[0];
         }
       }
-    };
-    float sk = 0.f, sv = 0.f;  // scales of row `tid` of the tile to come
-    auto load_scales = [&](int it) {
-      if (k8 && tid < BN) {
-        const uint32_t r = slots[it & 1][tid];
-        sk = a.c.k_scale[r];
-        sv = a.c.v_scale[r];
-      }
-    };
-    auto keep_scales = [&](int it) {
-      if (k8 && tid < BN) kscale[it & 1][tid] = sk, vscale[it & 1][tid] = sv;
     };
     const int q0 = wave * kQW;  // the wave's rows of the tile
     const bool active = q0 < rows;
@@ -277,51 +324,30 @@ void prefix_kernel(PagedArgs a) {
 #pragma unroll
       for (int db = 0; db < D / 16; ++db) acc[db][qb] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    uint32_t ahead = 0;
-    if (t_first < ntot) {
-      keep(t_first, look_up(t_first));
-      if (t_first + 1 < ntot) keep(t_first + 1, look_up(t_first + 1));
-      __syncthreads();
-      if constexpr (k8)
-        issue(t_first, raw);
-      else
-        issue(t_first, stage0);
-      load_scales(t_first);
-      keep_scales(t_first);
-    }
-    auto turn = [&](auto second, int it) __attribute__((always_inline)) {
-      constexpr bool kS = decltype(second)::value;
-      wait_vmem();
-      __syncthreads();
-      auto refill = [&](auto& dst) {
-        if (it + 1 >= ntot) return;
-        issue(it + 1, dst);
-        load_scales(it + 1);
-        if (it + 2 < ntot) ahead = look_up(it + 2);
-      };
+    auto turn = [&](int s, int it) __attribute__((always_inline)) {
+      wait_barrier<2 * kOps>();  // the tile has landed, and the one before it has been read
+      fetch_ids(it + 6);
+      fill(it + 3, (s + 3) & 3);
       if constexpr (k8) {
-        widen(vscale[it & 1]);
-        __syncthreads();
-        refill(raw);
-      } else if constexpr (kS) {
-        refill(stage0);
-      } else {
-        refill(stage1);
+        widen(s);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
       }
-      const char *tK = stage0[0], *tV = stage0[1];
-      if constexpr (!k8 && kS) tK = stage1[0], tV = stage1[1];
+      const char *tK = k8 ? wide[0] : kt[s], *tV = k8 ? wide[1] : vt[s];
       const bool loc = it >= nglob;
       const int ts = tile_start(it);
-      if (active && (loc ? ts + BN > mine.ls_min : ts < mine.gmax)) {
-        const bool full = loc ? ts >= mine.ls_max && ts + BN <= pp.n : ts + BN <= mine.g_all;
+      const bool any = active && (loc ? ts + BN > mine.ls_min : ts < mine.gmax);
+      if (uniform(any)) {
+        const bool full = uniform(loc ? ts >= mine.ls_max && ts + BN <= pp.n : ts + BN <= mine.g_all);
         TileMask<QB> mk;
         if (full) {
           if constexpr (BN == 64)
-            attend_whole<T, STORE, D, BN, QB>(tK, tV, kscale[it & 1], lo, qf, acc, m_run, l_run, c2, g, mk, one);
+            attend_whole<T, STORE, D, BN, QB>(tK, tV, kscale[s], lo, qf, acc, m_run, l_run, c2, g, mk, one);
           else
-            attend_chunk<T, STORE, D, BN, QB, false>(tK, tV, kscale[it & 1], lo, qf, acc, m_run, l_run, c2, g, mk,
-                                                     one, 0, 0);
-        } else {
+            attend_chunk<T, STORE, D, BN, QB, false>(tK, tV, kscale[s], lo, qf, acc, m_run, l_run, c2, g, mk, one,
+                                                     0, 0);
+        }
+        // (a branch of its own: with an else the accumulators are held twice)
+        if (uniform(fresh(full ? 0 : 1))) {
           const int vis_lo = loc ? max(0, mine.ls_min - ts) : 0, vis_hi = (loc ? pp.n : mine.gmax) - 1 - ts;
 #pragma unroll
           for (int qb = 0; qb < QB; ++qb) {
@@ -329,20 +355,22 @@ void prefix_kernel(PagedArgs a) {
             mk.hi[qb] = loc ? (r.ls < pp.n ? pp.n - 1 - ts : -1) : r.glen - 1 - ts;
             mk.span[qb] = loc ? (unsigned)max(pp.n - 1 - r.ls, 0) : 0x7fffffffu;
           }
-          attend_chunk<T, STORE, D, BN, QB, true>(tK, tV, kscale[it & 1], lo, qf, acc, m_run, l_run, c2, g, mk, one,
+          attend_chunk<T, STORE, D, BN, QB, true>(tK, tV, kscale[s], lo, qf, acc, m_run, l_run, c2, g, mk, one,
                                                   vis_lo >> 5, min(vis_hi >> 5, BN / 32 - 1));
         }
       }
-      if (it + 1 < ntot) keep_scales(it + 1);
-      if (it + 2 < ntot) keep(it + 2, ahead);
     };
-    if constexpr (k8) {
-      for (int it = t_first; it < ntot; ++it) turn(std::false_type{}, it);
-    } else {
-      for (int it = t_first; it < ntot; it += 2) {
-        turn(std::false_type{}, it);
-        if (it + 1 < ntot) turn(std::true_type{}, it + 1);
+    if (t_first < ntot) {
+#pragma unroll
+      for (int i = 0; i < 3; ++i) fetch_ids(t_first + i);
+      wait_vmem();  // known to the compiler: q's loads too, or it would wait for all in the loop
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {  // in the order of the turns, which count the loads
+        fetch_ids(t_first + 3 + i);
+        fill(t_first + i, i);
       }
+      for (int it = t_first; it < ntot; ++it) turn((it - t_first) & (kStages - 1), it);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // tiles past the last one, too
     }
     bool odd = false;
 #pragma unroll
@@ -386,15 +414,14 @@ __global__ __launch_bounds__(256) void prefix_f32_kernel(PagedArgs a) {
   __shared__ PrefixRow info[BM];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, g = lane >> 4;
   const SeqPlan pp = prefix_plan(a);
-  const PrefixSeq first_seqs = prefix_seq(a, pp, lane);
-  const PrefixWork work = prefix_work<BM, BN>(a, pp, first_seqs);
+  const PrefixWork work = prefix_work<BM, BN>(a, pp);
   const int items = work.tiles * work.pieces * a.c.H_kv;
   const float c2 = a.scale * kLog2e;
   for (int item = blockIdx.x; item < items; item += gridDim.x) {
     const int rest = (int)div_by(item, a.d_hkv), hk = item - rest * a.c.H_kv;
     const int piece = rest / work.tiles, r0 = (rest - piece * work.tiles) * BM;
     __syncthreads();  // the rows of the item before are done with
-    if (wave == 0) prefix_rows<BM>(a, pp, first_seqs, r0, work.rows, info);
+    if (wave == 0) prefix_rows<BM>(a, pp, r0, work.rows, info);
     __syncthreads();
     const int rows = min(BM, work.rows - r0);
     const PrefixKeys all = prefix_keys<BM>(info, 0, rows, pp.n);
