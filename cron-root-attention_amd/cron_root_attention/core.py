@@ -41,6 +41,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _native
+from .e4m3 import E4M3Linear
 
 RELAY_THRESHOLD = 2048          # core.py:2832
 _SUPPORTED_D = (32, 64, 128, 256)
@@ -302,11 +303,11 @@ def _layer_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 
 def _layer_op(proj: nn.Module):
     """The op of a layer whose output projection is ``proj``: _layer_attention
-    where ``proj`` is a plain nn.Linear, which only reads its input. A hook, a
+    where ``proj`` is a plain nn.Linear or E4M3Linear, which only read their input. A hook, a
     subclass or another module may edit it in place, which is for a copy of the
     output to take: the op's contiguous one, copied by the layer's reshape."""
     mod = torch.nn.modules.module
-    plain = (type(proj) is nn.Linear and "forward" not in proj.__dict__
+    plain = (type(proj) in (nn.Linear, E4M3Linear) and "forward" not in proj.__dict__
              and not (proj._forward_pre_hooks or proj._forward_hooks
                       or mod._global_forward_pre_hooks or mod._global_forward_hooks))
     return _layer_attention if plain else cron_root_attention_v14

@@ -132,7 +132,6 @@ class E4M3Weight:
         return (self.codes.float() * s).to(dtype)
 
 
-@torch.compiler.disable
 def linear_e4m3(x: torch.Tensor, weight: E4M3Weight, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x times the weight's transpose (+ bias), both in 8 bits. No backward.
 
@@ -151,24 +150,28 @@ def linear_e4m3(x: torch.Tensor, weight: E4M3Weight, bias: Optional[torch.Tensor
     """
     if not isinstance(weight, E4M3Weight):
         raise TypeError("weight must be an E4M3Weight")
+    return _product(x, weight._codes, weight._exponents, weight.out_features, weight.in_features, bias)
+
+
+@torch.compiler.disable
+def _product(x, codes, exponents, N, K, bias):
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
         raise NotImplementedError("linear_e4m3 has no backward; call it under torch.no_grad()")
     op = _native.fast_op("linear_e4m3")
     if op is not None:
-        y = op(x, weight._codes, weight._exponents, bias, weight.out_features, weight.in_features)
+        y = op(x, codes, exponents, bias, N, K)
         if y:
             return y[0]
     # what the operator does not take (or nobody does: the checks say why)
     if _native.has_tangent(x, bias):
         raise NotImplementedError("linear_e4m3 has no forward-mode derivatives")
-    N, K = weight.out_features, weight.in_features
     if x.dim() < 1 or x.shape[-1] != K:
         raise ValueError(f"x has shape {list(x.shape)}, the weight takes {K} columns")
     if x.dtype not in _DTYPES:
         raise TypeError(f"unsupported dtype {x.dtype}; use float16, bfloat16 or float32")
     _check_gpu("x", x)
-    if x.device != weight.device:
-        raise ValueError(f"x is on {x.device} but the weight is on {weight.device}")
+    if x.device != codes.device:
+        raise ValueError(f"x is on {x.device} but the weight is on {codes.device}")
     if bias is not None:
         if bias.shape != (N,):
             raise ValueError(f"bias must have shape [{N}], got {list(bias.shape)}")
@@ -181,7 +184,7 @@ def linear_e4m3(x: torch.Tensor, weight: E4M3Weight, bias: Optional[torch.Tensor
     if y.numel():
         rows = x.reshape(-1, K)
         rows = rows if rows.stride(1) == 1 or K == 1 else rows.contiguous()
-        _native.linear_e4m3(rows, weight._codes, weight._exponents, bias, y.view(-1, N))
+        _native.linear_e4m3(rows, codes, exponents, bias, y.view(-1, N))
     return y
 
 
@@ -212,7 +215,7 @@ class E4M3Linear(nn.Module):
         return E4M3Weight(self.out_features, self.in_features, self.codes, self.exponents)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        return linear_e4m3(x, self.weight, self.bias)
+        return _product(x, self.codes, self.exponents, self.out_features, self.in_features, self.bias)
 
     def extra_repr(self) -> str:
         return (f"in_features={self.in_features}, out_features={self.out_features}, "

@@ -6,8 +6,9 @@ SDPA below the gfx950 crossover, as ``CronRootAttentionHybrid`` does) and
 ``threshold``; ``rotary`` (a :class:`RotaryTable`) and ``qk_norm`` (a norm of each
 head of q and k, with weights of its own), which stand between the projections
 and the attention (on the GPU: the plain layer's path for CPU tensors has neither);
-and ``cache`` and ``batch`` of forward, which serve new tokens over a
-:class:`PagedKVCache`.  Grouped kv heads go to the kernel natively
+``cache`` and ``batch`` of forward, which serve new tokens over a
+:class:`PagedKVCache`; and ``to_e4m3``, which brings the projections into 8 bits for
+serving.  Grouped kv heads go to the kernel natively
 (``kv_groups``) instead of being expanded with ``repeat_interleave``
 (module.py:111-113); query head h reads kv head h // kv_groups either way, so
 the result is the same.
@@ -21,6 +22,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .core import _layer_op
+from .e4m3 import E4M3Linear
 from .hybrid import dispatch_backend
 from .paged import PagedBatch, PagedKVCache, cron_root_attention_paged
 from .rotary import RotaryTable, qk_norm_rotary, rotary_embedding
@@ -49,6 +51,7 @@ class CronRootAttention(nn.Module):
         self.k_proj = nn.Linear(d_model, self.n_kv_heads * self.head_dim, bias=bias)
         self.v_proj = nn.Linear(d_model, self.n_kv_heads * self.head_dim, bias=bias)
         self.o_proj = nn.Linear(d_model, d_model, bias=bias)
+        self.qkv_proj = None  # the joint projection of to_e4m3
         self.rotary = rotary
         self.norm_eps = norm_eps
         self.q_norm = nn.Parameter(torch.ones(self.head_dim)) if qk_norm else None
@@ -60,6 +63,31 @@ class CronRootAttention(nn.Module):
             nn.init.xavier_uniform_(lin.weight)
             if lin.bias is not None:
                 nn.init.zeros_(lin.bias)
+
+    def to_e4m3(self) -> "CronRootAttention":
+        """Bring the projections into 8 bits (:class:`E4M3Linear`), in place: q_proj,
+        k_proj and v_proj become one product ``qkv_proj``, o_proj another. On the GPU;
+        the layer has no gradients then."""
+        if self.qkv_proj is not None:
+            return self
+        qkv = E4M3Linear.from_linear(self.q_proj, self.k_proj, self.v_proj)
+        o = E4M3Linear.from_linear(self.o_proj)
+        for name in ("q_proj", "k_proj", "v_proj", "o_proj"):
+            delattr(self, name)
+        self.qkv_proj, self.o_proj = qkv, o
+        return self
+
+    def _projected(self, x, kv):
+        """q, k, v as [B, heads, S, head_dim]."""
+        B, S, _ = x.shape
+        if self.qkv_proj is None:
+            return (p(y).view(B, S, h, self.head_dim).transpose(1, 2)
+                    for p, y, h in ((self.q_proj, x, self.n_heads), (self.k_proj, kv, self.n_kv_heads),
+                                    (self.v_proj, kv, self.n_kv_heads)))
+        heads = (self.n_heads, self.n_kv_heads, self.n_kv_heads)
+        y = self.qkv_proj(x).view(B, S, sum(heads), self.head_dim).transpose(1, 2)
+        z = y if kv is x else self.qkv_proj(kv).view(B, S, sum(heads), self.head_dim).transpose(1, 2)
+        return (y.split(heads, 1)[0], *z.split(heads, 1)[1:])
 
     def backend_for(self, x: torch.Tensor) -> str:
         """``"cron_root"`` or ``"sdpa"``: what forward(x) runs.  Without
@@ -112,9 +140,7 @@ class CronRootAttention(nn.Module):
         if positions is not None and self.rotary is None:
             raise ValueError("positions without rotary: the layer has nothing to turn by")
         kv = kv if kv is not None else x
-        q = self.q_proj(x).view(B, S, self.n_heads, self.head_dim).transpose(1, 2)
-        k = self.k_proj(kv).view(B, S, self.n_kv_heads, self.head_dim).transpose(1, 2)
-        v = self.v_proj(kv).view(B, S, self.n_kv_heads, self.head_dim).transpose(1, 2)
+        q, k, v = self._projected(x, kv)
         if cache is not None:
             q = self._appended(q, k, v, positions, cache, batch)
             out = cron_root_attention_paged(q, cache, batch.page_table, batch.seq_lens,
