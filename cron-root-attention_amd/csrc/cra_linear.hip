@@ -137,6 +137,9 @@ struct LinearArgs {
   int64_t M;
   int N, K, Kb, Kp, Ks;  // blocks of a row; columns of codes; exponents of a row
   int tiles_m, tiles_n;
+  int per;               // blocks of a piece of the tiles
+  float* part;           // sums of pieces [piece, M, ldp], or null
+  int64_t ldp;
   int wide_x, wide_y, wide_y8;  // rows of x between 16-byte addresses; four and eight results of y as one store
 };
 
@@ -244,113 +247,9 @@ __device__ __forceinline__ void tile_of(const LinearArgs& a, int& tm, int& tn) {
   tm = __builtin_amdgcn_readfirstlane(first + j - tn * down);
 }
 
-// WM x WN waves of (16 FM) x (16 FN) results over LDS tiles of a block of 128 columns,
-// two stages: the next block's loads run while this one is multiplied.
-template <typename T, int WM, int WN, int FM, int FN>
-__global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)))
-void linear_kernel(LinearArgs a) {
-  constexpr bool kWide = std::is_same<T, float>::value;
-  constexpr int NW = WM * WN, BM = 16 * FM * WM, BN = 16 * FN * WN;
-  static_assert(16 * FN <= kBlock && kBlock % (16 * FN) == 0, "one exponent of w a wave");
-  using TX = CodeTile<BM, NW>;
-  using TW = CodeTile<BN, NW>;
-  __shared__ __attribute__((aligned(1024))) char x0[TX::kBytes], w0[TW::kBytes], x1[TX::kBytes], w1[TW::kBytes];
-  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
-  int tm, tn;
-  tile_of(a, tm, tn);
-  const int64_t m0 = (int64_t)tm * BM;
-  const int n0 = tn * BN;
-  const int mrows = (int)min((int64_t)BM, a.M - m0), nrows = min(BN, a.N - n0);
-  const __amdgpu_buffer_rsrc_t rx = make_rsrc(a.xc + m0 * a.Kp, (uint32_t)mrows * a.Kp);
-  const __amdgpu_buffer_rsrc_t rw = make_rsrc(a.wc + (int64_t)n0 * a.Kp, (uint32_t)nrows * a.Kp);
-  const int ox = TX::lane_off(wave, lane, a.Kp), ow = TW::lane_off(wave, lane, a.Kp);
-  // exponents: of four blocks at once; a lane's rows of x, the wave's block of w
-  const uint32_t* sx[FM];
-#pragma unroll
-  for (int i = 0; i < FM; ++i)
-    sx[i] = reinterpret_cast<const uint32_t*>(a.xs + min(m0 + 16 * (wm * FM + i) + l16, a.M - 1) * a.Ks);
-  const int nb = min((n0 + 16 * FN * wn) / kBlock, (a.N - 1) / kBlock);
-  const uint32_t* sw = reinterpret_cast<const uint32_t*>(a.ws + (int64_t)nb * a.Ks);
-  uint32_t ex[FM], ew;
-  uint32_t ex1[FM], ew1;
-#pragma unroll
-  for (int i = 0; i < FM; ++i) ex1[i] = sx[i][0];
-  ew1 = sw[0];
-
-  f32x4 acc[FN][FM];
-#pragma unroll
-  for (int n = 0; n < FN; ++n)
-#pragma unroll
-    for (int m = 0; m < FM; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-  TX::load(x0, rx, ox, a.Kp, wave);
-  TW::load(w0, rw, ow, a.Kp, wave);
-  auto step = [&](auto second, int kb) __attribute__((always_inline)) {
-    constexpr bool kS = decltype(second)::value;
-    wait_vmem();
-    __syncthreads();
-    if (kb + 1 < a.Kb) {
-      if constexpr (kS) {
-        TX::load(x0, rx, ox + (kb + 1) * kBlock, a.Kp, wave);
-        TW::load(w0, rw, ow + (kb + 1) * kBlock, a.Kp, wave);
-      } else {
-        TX::load(x1, rx, ox + (kb + 1) * kBlock, a.Kp, wave);
-        TW::load(w1, rw, ow + (kb + 1) * kBlock, a.Kp, wave);
-      }
-    }
-    if ((kb & 3) == 0) {
-#pragma unroll
-      for (int i = 0; i < FM; ++i) ex[i] = ex1[i];
-      ew = ew1;
-      const int next = min(kb / 4 + 1, a.Ks / 4 - 1);
-#pragma unroll
-      for (int i = 0; i < FM; ++i) ex1[i] = sx[i][next];
-      ew1 = sw[next];
-    } else {
-#pragma unroll
-      for (int i = 0; i < FM; ++i) ex[i] >>= 8;
-      ew >>= 8;
-    }
-    const char* tx = (kS ? x1 : x0) + wm * FM * 16 * kBlock;
-    const char* tw = (kS ? w1 : w0) + wn * FN * 16 * kBlock;
-    if constexpr (kWide) {
-      Wide xf[FM];
-#pragma unroll
-      for (int m = 0; m < FM; ++m) xf[m] = widen(TX::frag(tx, m, lane), ex[m]);
-#pragma unroll
-      for (int n = 0; n < FN; ++n) {
-        const Wide wf = widen(TW::frag(tw, n, lane), ew);
-#pragma unroll
-        for (int m = 0; m < FM; ++m) acc[n][m] = mma_wide(acc[n][m], wf, xf[m]);
-      }
-    } else {
-      Frag8 xf[FM], wf[2];
-      wf[0] = TW::frag(tw, 0, lane);
-#pragma unroll
-      for (int m = 0; m < FM; ++m) xf[m] = TX::frag(tx, m, lane);
-#pragma unroll
-      for (int n = 0; n < FN; ++n) {
-        if (n + 1 < FN) wf[(n + 1) & 1] = TW::frag(tw, n + 1, lane);
-#pragma unroll
-        for (int m = 0; m < FM; ++m) acc[n][m] = mma8(acc[n][m], wf[n & 1], xf[m], ew, ex[m]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-  };
-  for (int kb = 0; kb < a.Kb; kb += 2) {
-    step(std::false_type{}, kb);
-    if (kb + 1 < a.Kb) step(std::true_type{}, kb + 1);
-  }
-#pragma unroll
-  for (int m = 0; m < FM; ++m)
-#pragma unroll
-    for (int n = 0; n < FN; ++n)
-      store4<T>(a, m0 + 16 * (wm * FM + m) + l16, n0 + 16 * (wn * FN + n) + 4 * g, acc[n][m]);
-}
-
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 // Buffer resource over `bytes` bytes at `base`, in scalar registers.
-__device__ __forceinline__ u32x4 words_of(const void* base, uint32_t bytes) {
+__device__ __forceinline__ u32x4 resource(const void* base, uint32_t bytes) {
   const uint64_t p = reinterpret_cast<uint64_t>(base);
   u32x4 r;
   r[0] = __builtin_amdgcn_readfirstlane((uint32_t)p);
@@ -374,9 +273,124 @@ __device__ __forceinline__ void to_lds(uint32_t lds, u32x4 rsrc, int off, int so
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"
                  :: "s"(lds), "v"(off), "s"(rsrc), "s"(soff) : "memory", "m0");
 }
-// All but the newest eight loads have landed, and the wave's LDS reads are done.
+// All but the newest N loads of the wave have landed, its LDS reads are done, and the other
+// waves are as far.
+template <int N>
 __device__ __forceinline__ void wait_barrier() {
-  asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+typedef const __attribute__((address_space(4))) uint32_t* ConstWords;  // read by scalar loads
+
+// WM x WN waves of (16 FM) x (16 FN) results over LDS tiles of a block of 128 columns, in
+// kStages stages: a block's loads run while the others are multiplied. Bound by the
+// latency of those loads where a workgroup has few blocks, and by the matrix core and
+// LDS reads (a fragment serves two to four MFMAs) where it has many. Few tiles are cut
+// along K (gridDim.y), whose sums join_kernel adds in their order.
+// Measured, bf16 with the rows' own way into 8 bits: 1024 x 4096 x 4096 (tiles of 128) 31.8 us,
+// 512 (of 64) 23.7, 64 (of 64, K in eight pieces) 16; two stages and no pieces 42.5, 28.0, 19.
+template <typename T, int WM, int WN, int FM, int FN, int kStages>
+__global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM * WN / 4)))
+void linear_kernel(LinearArgs a) {
+  constexpr bool kWide = std::is_same<T, float>::value;
+  constexpr int NW = WM * WN, BM = 16 * FM * WM, BN = 16 * FN * WN;
+  static_assert(16 * FN <= kBlock && kBlock % (16 * FN) == 0, "one exponent of w a wave");
+  static_assert(16 * FM <= 64, "a wave's exponents of x are one load");
+  using TX = CodeTile<BM, NW>;
+  using TW = CodeTile<BN, NW>;
+  constexpr int kOps = TX::kPer + TW::kPer + 1;  // loads of a block
+  __shared__ __attribute__((aligned(1024))) char xt[kStages][TX::kBytes], wt[kStages][TW::kBytes];
+  __shared__ uint32_t exps[kStages][NW][16 * FM];
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
+  int tm, tn;
+  tile_of(a, tm, tn);
+  const int64_t m0 = (int64_t)tm * BM;
+  const int n0 = tn * BN;
+  const int mrows = (int)min((int64_t)BM, a.M - m0), nrows = min(BN, a.N - n0);
+  const u32x4 rx = resource(a.xc + m0 * a.Kp, (uint32_t)mrows * a.Kp);
+  const u32x4 rw = resource(a.wc + (int64_t)n0 * a.Kp, (uint32_t)nrows * a.Kp);
+  const u32x4 re = resource(a.xs + m0 * a.Ks, (uint32_t)mrows * a.Ks);
+  const int ox = TX::lane_off(wave, lane, a.Kp), ow = TW::lane_off(wave, lane, a.Kp);
+  const int oe = (wm * 16 * FM + lane) * a.Ks;
+  const int nb = min((n0 + 16 * FN * wn) / kBlock, (a.N - 1) / kBlock);
+  const ConstWords sw = (ConstWords)(a.ws + (int64_t)nb * a.Ks);
+  const int k0 = blockIdx.y * a.per, k1 = min(a.Kb, k0 + a.per);  // blocks of this piece
+  auto fill = [&](int kb, int s) __attribute__((always_inline)) {
+    kb = min(kb, k1 - 1);
+#pragma unroll
+    for (int i = 0; i < TX::kPer; ++i)
+      to_lds<16>(lds_at(xt[s]) + (i * NW + wave) * 1024, rx, ox + i * NW * 8 * a.Kp, kb * kBlock);
+#pragma unroll
+    for (int i = 0; i < TW::kPer; ++i)
+      to_lds<16>(lds_at(wt[s]) + (i * NW + wave) * 1024, rw, ow + i * NW * 8 * a.Kp, kb * kBlock);
+    if (lane < 16 * FM) to_lds<4>(lds_at(exps[s][wave]), re, oe, kb & ~3);
+  };
+  f32x4 acc[FN][FM];
+#pragma unroll
+  for (int n = 0; n < FN; ++n)
+#pragma unroll
+    for (int m = 0; m < FM; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) fill(k0 + i, i);
+  for (int kb = k0; kb < k1; ++kb) {
+    const int s = (kb - k0) & (kStages - 1);
+    wait_barrier<(kStages - 2) * kOps>();  // the block has landed, and the one before it has been read
+    fill(kb + kStages - 1, (s + kStages - 1) & (kStages - 1));
+    const int shift = 8 * (kb & 3);
+    const uint32_t ew = sw[kb >> 2] >> shift;
+    const char *tx = xt[s] + wm * FM * 16 * kBlock, *tw = wt[s] + wn * FN * 16 * kBlock;
+    uint32_t ex[FM];
+#pragma unroll
+    for (int m = 0; m < FM; ++m) ex[m] = exps[s][wave][16 * m + l16] >> shift;
+    if constexpr (kWide) {
+      Wide xf[FM];
+#pragma unroll
+      for (int m = 0; m < FM; ++m) xf[m] = widen(TX::frag(tx, m, lane), ex[m]);
+#pragma unroll
+      for (int n = 0; n < FN; ++n) {
+        const Wide wf = widen(TW::frag(tw, n, lane), ew);
+#pragma unroll
+        for (int m = 0; m < FM; ++m) acc[n][m] = mma_wide(acc[n][m], wf, xf[m]);
+      }
+    } else {
+      Frag8 xf[FM], wf[2];
+      wf[0] = TW::frag(tw, 0, lane);
+#pragma unroll
+      for (int m = 0; m < FM; ++m) xf[m] = TX::frag(tx, m, lane);
+#pragma unroll
+      for (int n = 0; n < FN; ++n) {
+        if (n + 1 < FN) wf[(n + 1) & 1] = TW::frag(tw, n + 1, lane);
+#pragma unroll
+        for (int m = 0; m < FM; ++m) acc[n][m] = mma8(acc[n][m], wf[n & 1], xf[m], ew, ex[m]);
+      }
+    }
+  }
+  wait_vmem();  // loads past the last block, too
+#pragma unroll
+  for (int m = 0; m < FM; ++m)
+#pragma unroll
+    for (int n = 0; n < FN; ++n) {
+      const int64_t row = m0 + 16 * (wm * FM + m) + l16;
+      const int col = n0 + 16 * (wn * FN + n) + 4 * g;
+      if (!a.part)
+        store4<T>(a, row, col, acc[n][m]);
+      else if (row < a.M && col < a.N)  // rows of N up to a multiple of four
+        *reinterpret_cast<f32x4*>(a.part + ((int64_t)blockIdx.y * a.M + row) * a.ldp + col) = acc[n][m];
+    }
+}
+
+// Adds the pieces of a product cut along K: a thread four columns of a row.
+template <typename T>
+__global__ __launch_bounds__(256) void join_kernel(LinearArgs a, int pieces, uint32_t quads, FastDiv d_quads) {
+  const uint32_t i = blockIdx.x * 256u + threadIdx.x;
+  const uint32_t row = div_by(i, d_quads);
+  const int col = (int)(i - row * quads) * 4;
+  if (row >= a.M) return;
+  const float* p = a.part + (int64_t)row * a.ldp + col;
+  f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int k = 0; k < pieces; ++k) s += *reinterpret_cast<const f32x4*>(p + (int64_t)k * a.M * a.ldp);
+  store4<T>(a, row, col, s);
 }
 
 // Large 16-bit products: 256 x 256 results a workgroup, eight waves of 64 x 128, two waves
@@ -409,13 +423,13 @@ void large_kernel(LinearArgs a) {
   const int64_t m0 = (int64_t)tm * BM;
   const int n0 = tn * BN;
   const int mrows = (int)min((int64_t)BM, a.M - m0), nrows = min(BN, a.N - n0);
-  const u32x4 rx = words_of(a.xc + m0 * a.Kp, (uint32_t)mrows * a.Kp);
-  const u32x4 rw = words_of(a.wc + (int64_t)n0 * a.Kp, (uint32_t)nrows * a.Kp);
-  const u32x4 re = words_of(a.xs + m0 * a.Ks, (uint32_t)mrows * a.Ks);
+  const u32x4 rx = resource(a.xc + m0 * a.Kp, (uint32_t)mrows * a.Kp);
+  const u32x4 rw = resource(a.wc + (int64_t)n0 * a.Kp, (uint32_t)nrows * a.Kp);
+  const u32x4 re = resource(a.xs + m0 * a.Ks, (uint32_t)mrows * a.Ks);
   __shared__ uint32_t exps[2][NW][64];
   const int ox = TX::lane_off(wave, lane, a.Kp), ow = TW::lane_off(wave, lane, a.Kp);
   const int nb = min((n0 + 16 * FN * wn) / kBlock, (a.N - 1) / kBlock);
-  const __attribute__((address_space(4))) uint32_t* sw = (const __attribute__((address_space(4))) uint32_t*)(a.ws + (int64_t)nb * a.Ks);
+  const ConstWords sw = (ConstWords)(a.ws + (int64_t)nb * a.Ks);
   uint32_t ex[FM], ew;
   const int oe = (wm * 64 + lane) * a.Ks;
   f32x4 acc[FN][FM];
@@ -443,7 +457,7 @@ void large_kernel(LinearArgs a) {
   fill_w(w10, 0, min(1, last));
   int q = 0;
   Frag8 xf[2][FM];
-  wait_barrier();  // x of the first block (ten loads are newer)
+  wait_barrier<8>();  // x of the first block (ten loads are newer)
 #pragma unroll
   for (int m = 0; m < FM; ++m) xf[0][m] = TX::frag(x0 + wm * FM * 16 * kBlock, m, lane);
   auto step = [&](auto second, int kb) __attribute__((always_inline)) {
@@ -451,7 +465,7 @@ void large_kernel(LinearArgs a) {
     const char* txn = (kS ? x0 : x1) + wm * FM * 16 * kBlock;
     const char* tw0 = (kS ? w10 : w00) + wn * 64 * kBlock;
     const char* tw1 = (kS ? w11 : w01) + wn * 64 * kBlock;
-    wait_barrier();  // the first half of w has landed; x and the other stage's second half have been read
+    wait_barrier<8>();  // the first half of w has landed; x and the other stage's second half have been read
     Frag8 wf[2];
 #pragma unroll
     for (int n = 0; n < 1; ++n) wf[n] = TW::frag(tw0, n, lane);
@@ -476,7 +490,7 @@ void large_kernel(LinearArgs a) {
       for (int m = 0; m < FM; ++m) acc[n][m] = mma8(acc[n][m], wf[n & 1], xf[kS][m], ew, ex[m]);
       __builtin_amdgcn_sched_barrier(0);
     }
-    wait_barrier();  // the second half of w and the next x have landed; the first half has been read
+    wait_barrier<8>();  // the second half of w and the next x have landed; the first half has been read
 #pragma unroll
     for (int n = 0; n < 1; ++n) wf[n] = TW::frag(tw1, n, lane);
     fill_w(kS ? w10 : w00, 0, min(kb + 2, last));
@@ -539,19 +553,21 @@ void large_kernel(LinearArgs a) {
 }
 
 // Few rows of x: bound by the reading of w. A workgroup takes 16 columns of y and all
-// (16 FM) rows, its waves a share of the blocks each, straight from memory into registers,
-// the first ones' loads on their way before x is looked at; they add up through LDS in
-// their order. RAW: x comes as it is, and each wave brings its blocks of the at most
-// kRawRows rows into 8 bits for itself.
-constexpr int kFewWaves = 8, kAheadBlocks = 4, kRawRows = 4, kRawBlocks = 16;
+// rows (kFewRowsMost at most), its waves a share of the blocks each, straight from memory
+// into registers, the first ones' loads on their way before x is looked at; they add up
+// through LDS in their order. RAW: x comes as it is, and each wave brings its blocks of the
+// at most kRawRows rows into 8 bits for itself, kRawPairs blocks of rows at most.
+// Measured, bf16, one row: 6144 x 4096 8.0 us (25 MB of codes: 4.9 by a copy's rate).
+constexpr int kFewWaves = 8, kAheadBlocks = 4, kRawRows = 4, kRawPairs = 32;
+constexpr int kFewRowsMost = 16, kLargeTiles = 128, kMediumTiles = 140;
 
-template <typename T, typename X, int FM, bool RAW>
+template <typename T, bool RAW>
 __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(LinearArgs a) {
   constexpr bool kWide = std::is_same<T, float>::value;
-  constexpr int NW = kFewWaves, R = 16 * FM;
-  constexpr int kRawBytes = RAW ? kRawBlocks * kRawRows * kBlock : 16;
+  constexpr int NW = kFewWaves, R = kFewRowsMost;
+  constexpr int kRawBytes = RAW ? kRawPairs * kBlock : 16;
   __shared__ __attribute__((aligned(16))) char raw[NW][kRawBytes];
-  __shared__ uint8_t raw_e[NW][RAW ? kRawBlocks * kRawRows : 4];
+  __shared__ uint8_t raw_e[NW][RAW ? kRawPairs : 4];
   __shared__ float sums[NW][R][17];
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -576,7 +592,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(LinearArgs a) 
     for (int i = g; i < n; i += 4) {
       const int b = i / M, row = i - b * M, col = (k0 + b) * kBlock + l16 * 8;
       float x[8];
-      load8<X>(static_cast<const X*>(a.x) + row * a.ldx + col, a.K - col, a.wide_x && col + 8 <= a.K, x);
+      load8<T>(static_cast<const T*>(a.x) + row * a.ldx + col, a.K - col, a.wide_x && col + 8 <= a.K, x);
       uint8_t e;
       const uint2 c = codes8(x, lanes_max(largest(x), 4), e);
       *reinterpret_cast<uint2*>(raw[wave] + i * kBlock + l16 * 8) = c;
@@ -584,30 +600,24 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(LinearArgs a) 
     }
     __builtin_amdgcn_wave_barrier();  // the wave's own LDS, in order
   }
-  f32x4 acc[FM];
-#pragma unroll
-  for (int m = 0; m < FM; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int base = k0; base < k1; base += kAheadBlocks) {
 #pragma unroll
     for (int i = 0; i < kAheadBlocks; ++i) {
       const int kb = base + i;
       if (kb >= k1) break;
-      Frag8 xf[FM];
-      uint32_t ex[FM];
-#pragma unroll
-      for (int m = 0; m < FM; ++m) {
-        const int row = 16 * m + l16;
-        if constexpr (RAW) {
-          const int at = (kb - k0) * M + min(row, M - 1);
-          const uint4* p = reinterpret_cast<const uint4*>(raw[wave] + at * kBlock + 16 * g);
-          xf[m] = Frag8{p[0], p[4]};
-          ex[m] = raw_e[wave][at];
-        } else {
-          const int64_t r = min(row, M - 1);
-          const uint4* p = reinterpret_cast<const uint4*>(a.xc + r * a.Kp + (int64_t)kb * kBlock + 16 * g);
-          xf[m] = Frag8{p[0], p[4]};
-          ex[m] = a.xs[r * a.Ks + kb];
-        }
+      Frag8 xf;
+      uint32_t ex;
+      if constexpr (RAW) {
+        const int at = (kb - k0) * M + min(l16, M - 1);
+        const uint4* p = reinterpret_cast<const uint4*>(raw[wave] + at * kBlock + 16 * g);
+        xf = Frag8{p[0], p[4]};
+        ex = raw_e[wave][at];
+      } else {
+        const int64_t row = min(l16, M - 1);
+        const uint4* p = reinterpret_cast<const uint4*>(a.xc + row * a.Kp + (int64_t)kb * kBlock + 16 * g);
+        xf = Frag8{p[0], p[4]};
+        ex = a.xs[row * a.Ks + kb];
       }
       const Frag8 w = wf[i];
       const uint32_t e = ew[i];
@@ -615,20 +625,14 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(LinearArgs a) 
         wf[i] = load_w(kb + kAheadBlocks);
         ew[i] = sw[kb + kAheadBlocks];
       }
-      if constexpr (kWide) {
-        const Wide ww = widen(w, e);
-#pragma unroll
-        for (int m = 0; m < FM; ++m) acc[m] = mma_wide(acc[m], ww, widen(xf[m], ex[m]));
-      } else {
-#pragma unroll
-        for (int m = 0; m < FM; ++m) acc[m] = mma8(acc[m], w, xf[m], e, ex[m]);
-      }
+      if constexpr (kWide)
+        acc = mma_wide(acc, widen(w, e), widen(xf, ex));
+      else
+        acc = mma8(acc, w, xf, e, ex);
     }
   }
 #pragma unroll
-  for (int m = 0; m < FM; ++m)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) sums[wave][16 * m + l16][4 * g + r] = acc[m][r];
+  for (int r = 0; r < 4; ++r) sums[wave][l16][4 * g + r] = acc[r];
   __syncthreads();
   for (int i = tid; i < 4 * R; i += 64 * NW) {
     const int row = i >> 2, c = (i & 3) * 4;
@@ -676,25 +680,38 @@ struct Plan {
   bool few, raw;
   int tile;  // 64, 128, 256
   int64_t tiles_m;
-  int tiles_n;
-  size_t code_bytes, scale_bytes;
+  int tiles_n, pieces;
+  size_t code_bytes, scale_bytes, part_bytes;
+  size_t bytes() const { return code_bytes + scale_bytes + part_bytes; }
 };
 Plan plan_of(const cra_linear* p) {
   Plan l{};
   l.Kb = up(p->K, kBlock);
   l.Kp = l.Kb * kBlock;
   l.Ks = up(l.Kb, 4) * 4;
-  l.few = p->M <= 64;
-  l.raw = p->M <= kRawRows && up(l.Kb, kFewWaves) <= kRawBlocks;
-  l.tile = 256;
+  // where the sides cross (bf16, us): x as it is against brought into 8 bits first, 4 x 4096
+  // x 4096 8.2 and 8.7, 4 x 1024 x 16384 17.5 and 12.7; rows straight from memory against
+  // tiles cut along K, 16 x 4096 x 4096 10.5 and 11.4, 16 x 1024 x 16384 23.2 and 13.2, 16 x
+  // 16384 x 4096 24.8 and 19.1, 32 x 4096 x 4096 13.2 and 12.7
+  l.raw = p->M <= kRawRows && p->M * up(l.Kb, kFewWaves) <= kRawPairs;
+  l.few = l.raw || (p->M <= kFewRowsMost && up(p->N, 16) >= 192 && up(p->N, 16) <= 512);
+  // tiles: 2048 x 4096 x 4096 (128 of 256) 54.4 us, in tiles of 128 55.1; 1024 x 4096 x 4096 (64
+  // and 256) 49.6 and 31.4; 512 x 4096 x 4096 (128 of 128) 26.5, in tiles of 64 24.0
   auto tiles = [&](int t) { return (int64_t)up(p->M, t) * up(p->N, t); };
-  if (tiles(256) < 256) l.tile = 128;
-  if (tiles(128) < 256) l.tile = 64;
+  l.tile = tiles(256) >= kLargeTiles ? 256 : tiles(128) >= kMediumTiles ? 128 : 64;
   l.tiles_m = up(p->M, l.tile);
   l.tiles_n = up(p->N, l.tile);
+  l.pieces = 1;
+  if (!l.few && l.tile < 256) {
+    const int want = (int)std::min<int64_t>(up(l.tile == 128 ? 256 : 512, (int)std::min<int64_t>(tiles(l.tile), 512)),
+                                            std::max(1, l.Kb / 4));
+    l.pieces = up(l.Kb, up(l.Kb, want));
+  }
   if (!l.raw) {
-    l.code_bytes = ((size_t)p->M * l.Kp + 255) / 256 * 256;
-    l.scale_bytes = ((size_t)p->M * l.Ks + 255) / 256 * 256;
+    auto up256 = [](size_t n) { return (n + 255) / 256 * 256; };
+    l.code_bytes = up256((size_t)p->M * l.Kp);
+    l.scale_bytes = up256((size_t)p->M * l.Ks);
+    if (l.pieces > 1) l.part_bytes = up256((size_t)l.pieces * p->M * up(p->N, 4) * 16);
   }
   return l;
 }
@@ -710,25 +727,26 @@ hipError_t run_linear(const LinearArgs& a, const Plan& l, hipStream_t st) {
   if (l.few) {
     const uint32_t grid = (uint32_t)up(a.N, 16);
     if (l.raw)
-      few_rows_kernel<T, T, 1, true><<<grid, 64 * kFewWaves, 0, st>>>(a);
-    else if (a.M <= 16)
-      few_rows_kernel<T, T, 1, false><<<grid, 64 * kFewWaves, 0, st>>>(a);
-    else if (a.M <= 32)
-      few_rows_kernel<T, T, 2, false><<<grid, 64 * kFewWaves, 0, st>>>(a);
+      few_rows_kernel<T, true><<<grid, 64 * kFewWaves, 0, st>>>(a);
     else
-      few_rows_kernel<T, T, 4, false><<<grid, 64 * kFewWaves, 0, st>>>(a);
+      few_rows_kernel<T, false><<<grid, 64 * kFewWaves, 0, st>>>(a);
     return hipGetLastError();
   }
-  const uint32_t grid = (uint32_t)(l.tiles_m * l.tiles_n);
+  const dim3 grid((uint32_t)(l.tiles_m * l.tiles_n), l.pieces);
   if (l.tile == 256) {
     if constexpr (std::is_same<T, float>::value)
-      linear_kernel<T, 4, 2, 4, 8><<<grid, 512, 0, st>>>(a);
+      linear_kernel<T, 4, 2, 4, 8, 2><<<grid, 512, 0, st>>>(a);
     else
       large_kernel<T><<<grid, 512, 0, st>>>(a);
   } else if (l.tile == 128) {
-    linear_kernel<T, 2, 2, 4, 4><<<grid, 256, 0, st>>>(a);
+    linear_kernel<T, 4, 2, 2, 4, 4><<<grid, 512, 0, st>>>(a);
   } else {
-    linear_kernel<T, 2, 2, 2, 2><<<grid, 256, 0, st>>>(a);
+    linear_kernel<T, 2, 2, 2, 2, 4><<<grid, 256, 0, st>>>(a);
+  }
+  if (hipError_t e = hipGetLastError()) return e;
+  if (l.pieces > 1) {
+    const uint32_t quads = (uint32_t)up(a.N, 4);
+    join_kernel<T><<<(uint32_t)up((int64_t)quads * a.M, 256), 256, 0, st>>>(a, l.pieces, quads, fast_div(quads));
   }
   return hipGetLastError();
 }
@@ -785,7 +803,7 @@ int cra_e4m3_weight(const void* w, int64_t ldw, int32_t N, int32_t K, int32_t dt
 size_t cra_linear_e4m3_workspace_bytes(const cra_linear* p) {
   if (check_linear(p)) return 0;
   const Plan l = plan_of(p);
-  return l.code_bytes + l.scale_bytes;
+  return l.bytes();
 }
 
 int cra_linear_e4m3(const cra_linear* p, const void* x, int64_t ldx, const void* w_codes,
@@ -797,7 +815,7 @@ int cra_linear_e4m3(const cra_linear* p, const void* x, int64_t ldx, const void*
   if (!aligned(x, esz) || !aligned(y, esz) || !aligned(bias, esz) || !aligned(w_codes, 16) || !aligned(w_scales, 4))
     return err(CRA_E_LAYOUT, "x, w, bias or y: misaligned pointer");
   const Plan l = plan_of(p);
-  const size_t need = l.code_bytes + l.scale_bytes;
+  const size_t need = l.bytes();
   if (need && (!workspace || !aligned(workspace, 16)))
     return err(CRA_E_INVALID, "workspace: NULL or misaligned pointer");
   if (workspace_bytes < need) return err(CRA_E_WORKSPACE, "workspace too small (cra_linear_e4m3_workspace_bytes)");
@@ -820,6 +838,9 @@ int cra_linear_e4m3(const cra_linear* p, const void* x, int64_t ldx, const void*
     if (int e = cra_e4m3_rows(x, ldx, p->M, p->K, p->dtype, ws, ws + l.code_bytes, stream)) return e;
     a.xc = reinterpret_cast<const uint8_t*>(ws);
     a.xs = reinterpret_cast<const uint8_t*>(ws + l.code_bytes);
+    if (l.pieces > 1) a.part = reinterpret_cast<float*>(ws + l.code_bytes + l.scale_bytes);
+    a.per = up(l.Kb, l.pieces);
+    a.ldp = (int64_t)up(p->N, 4) * 4;
   }
   return hip_err(with_type(p->dtype, [&](auto z) { return run_linear<decltype(z)>(a, l, st); }), "cra_linear_e4m3");
 }
