@@ -138,6 +138,26 @@ def test_heads_and_many_sequences(H, new):
     agree(*make(lens, new, *H, 64, BF16, "same", seed=1), table=table, norm=True)
 
 
+@pytest.mark.parametrize("H,fused", [((6, 2), True), ((6, 2), False), ((5, 1), True)])
+@pytest.mark.parametrize("dtype,D,rot,interleaved", [(BF16, 128, 128, False), (F32, 80, 40, True), (F16, 16, 8, False)])
+def test_many_rows(H, fused, dtype, D, rot, interleaved):
+    new = [2001, 7, 0, 1, 1300, 31, 64, 65]
+    lens = [m + 90 * i for i, m in enumerate(new)]
+    table = cra.RotaryTable(rot, 4096, interleaved=interleaved, device=DEV)
+    args = make(lens, new, *H, D, dtype, "same", seed=D, pad=(3, 70), fused=fused)
+    w = [(1 + 0.3 * torch.randn(D, generator=torch.Generator().manual_seed(i))).to(DEV) for i in (1, 2)]
+    agree(*args, table=table, norm=True, q_weight=w[0], k_weight=w[1])
+
+
+@pytest.mark.parametrize("n", [1, 2, 62, 63, 64, 65, 200])
+def test_numbers_of_sequences(n):
+    new = [(7 * i + 3) % 5 for i in range(n)]
+    new[-1] += n == 2
+    lens = [m + 11 * i % 200 for i, m in enumerate(new)]
+    table = cra.RotaryTable(64, 512, device=DEV)
+    agree(*make(lens, new, 4, 2, 64, F16, "int8", seed=n, pad=(1, 2)), table=table, norm=True)
+
+
 @pytest.mark.parametrize("fused", [True, False])
 def test_layouts_and_single_tokens_without_offsets(fused):
     lens, D = [5, 77, 130], 64
