@@ -197,7 +197,7 @@ __device__ __forceinline__ void select_blocks(const PagedArgs& a, const SelWork&
   }
 }
 
-__global__ __launch_bounds__(64 * kSelWaves) void select_kernel(PagedArgs a, int steps) {
+__global__ __launch_bounds__(64 * kSelWaves) void select_kernel(int steps, PagedArgs a) {
   const SelWork w = sel_work(a, steps, [](int W) { return W <= 121 ? 4 : W <= 249 ? 2 : 1; });
   if (w.first >= w.end) return;
   if (w.p.W <= 121)
@@ -209,7 +209,7 @@ __global__ __launch_bounds__(64 * kSelWaves) void select_kernel(PagedArgs a, int
 }
 
 template <int KEEP>
-__global__ __launch_bounds__(64 * kSelWaves) void select_wide_kernel(PagedArgs a, int steps) {
+__global__ __launch_bounds__(64 * kSelWaves) void select_wide_kernel(int steps, PagedArgs a) {
   const int lane = threadIdx.x & 63;
   const SelWork w = sel_work(a, steps, [](int) { return 1; });
   if (w.first >= w.end) return;
@@ -503,7 +503,7 @@ hipError_t launch_rows(const PagedArgs& a, const Launch& l, int64_t bh, hipStrea
       few_kernel<T, STORE, D, false><<<(uint32_t)l.few_grid, 64 * kFewWaves, 0, st>>>(a);
     if (hipError_t e = hipGetLastError()) return e;
     if (l.join) {
-      combine_kernel<T, false><<<(uint32_t)(bh * l.part_rows), 256, 0, st>>>(a, D);
+      combine_kernel<T, false><<<(uint32_t)(bh * l.part_rows), 256, 0, st>>>(D, a);
       if (hipError_t e = hipGetLastError()) return e;
     }
   }
@@ -512,7 +512,7 @@ hipError_t launch_rows(const PagedArgs& a, const Launch& l, int64_t bh, hipStrea
       f32_kernel<STORE, D, false, false><<<(uint32_t)l.items, 256, 0, st>>>(a);
       if (hipError_t e = hipGetLastError()) return e;
       const uint32_t items = (uint32_t)l.joins * (kF32Rows / join_rows<D>());
-      if (items) f32_join_kernel<D><<<std::min<uint32_t>(items, kJoinGrid), 256, 0, st>>>(a, items);
+      if (items) f32_join_kernel<D><<<std::min<uint32_t>(items, kJoinGrid), 256, 0, st>>>(items, a);
       return hipGetLastError();
     } else {
       return launch_chunk(std::is_same<T, f16>::value ? CRA_F16 : CRA_BF16, STORE, D, a,
@@ -589,7 +589,7 @@ int attend(const cra_cache* c, const cra_batch* b, const cra_paged_plan* p, cons
     const uint32_t grid = (uint32_t)(bh * l.sel_steps + c->H_kv * l.prefix_steps);
     auto kernel = l.wide ? (p->top_k <= 2 ? select_wide_kernel<2> : select_wide_kernel<4>)
                          : select_kernel;
-    kernel<<<grid, 64 * kSelWaves, 0, st>>>(a, l.sel_steps);
+    kernel<<<grid, 64 * kSelWaves, 0, st>>>(l.sel_steps, a);
     if (int e = hip_err(hipGetLastError(), "cra_fwd_paged (relay rows)")) return e;
   }
   return hip_err(with_dim(l.Dp, [&](auto d) {

@@ -323,7 +323,7 @@ void chunk_kernel(PagedArgs a) {
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(256) void join_kernel(PagedArgs a, uint32_t items) {
+__global__ __launch_bounds__(256) void join_kernel(uint32_t items, PagedArgs a) {
   join_chunk<T, 64 * kChunkQB<D>, kChunkBN<D>, D>(a, items);
 }
 
@@ -332,7 +332,7 @@ hipError_t run(const PagedArgs& a, uint32_t grid, uint32_t join_tiles, hipStream
   chunk_kernel<T, STORE, D><<<grid, 64 * kChunkWaves, 0, st>>>(a);
   if (hipError_t e = hipGetLastError()) return e;
   const uint32_t items = join_tiles * (64 * kChunkQB<D> / join_rows<D>());
-  if (items) join_kernel<T, D><<<items < kJoinGrid ? items : kJoinGrid, 256, 0, st>>>(a, items);
+  if (items) join_kernel<T, D><<<items < kJoinGrid ? items : kJoinGrid, 256, 0, st>>>(items, a);
   return hipGetLastError();
 }
 template <typename T, int STORE>

@@ -34,7 +34,8 @@ struct PagedArgs {
   int parts;       // pieces of cut sequences (all kv heads) that the workspace holds
   int few_only;    // no chunk_kernel follows: longer sequences are refused (NaN)
   int zero_outside;  // rows of tokens outside every sequence are set to zero
-  // rows that the sequences have in common (SHARED)
+  // rows that the sequences have in common (SHARED). They stand last, and kernels take their
+  // other arguments before this struct: reading one behind it costs 0.25 us a launch.
   const int32_t *ptable, *plen;  // their pages, and how many rows
   int pcap;          // rows that the pages hold
   uint32_t* plist;   // [H_kv, plist_cap] cache rows of their global rows (relay)

@@ -458,7 +458,7 @@ void few_kernel(PagedArgs a) {
 // Joins the pieces of sequences that have more than one: one workgroup a
 // (sequence, kv head, row), its threads 4 columns each of some of the pieces.
 template <typename T, bool SHARED>
-__global__ __launch_bounds__(256) void combine_kernel(PagedArgs a, int Dp) {
+__global__ __launch_bounds__(256) void combine_kernel(int Dp, PagedArgs a) {
   __shared__ float red[256][4];
   __shared__ float red_l[64];
   const int tid = threadIdx.x;
@@ -755,7 +755,7 @@ __global__ __launch_bounds__(256) void f32_kernel(PagedArgs a) {
 }
 
 template <int D>
-__global__ __launch_bounds__(256) void f32_join_kernel(PagedArgs a, uint32_t items) {
+__global__ __launch_bounds__(256) void f32_join_kernel(uint32_t items, PagedArgs a) {
   join_chunk<float, kF32Rows, kF32Keys, D>(a, items);
 }
 

@@ -539,7 +539,7 @@ hipError_t run(const PagedArgs& a, uint32_t combine_grid, uint32_t few_grid, hip
   else
     few_kernel<T, STORE, D, true><<<few_grid, 64 * kFewWaves, 0, st>>>(a);
   if (hipError_t e = hipGetLastError()) return e;
-  combine_kernel<T, true><<<combine_grid, 256, 0, st>>>(a, D);
+  combine_kernel<T, true><<<combine_grid, 256, 0, st>>>(D, a);
   return hipGetLastError();
 }
 template <typename T, int STORE>
