@@ -696,15 +696,17 @@ Plan plan_of(const cra_linear* p) {
   l.raw = p->M <= kRawRows && p->M * up(l.Kb, kFewWaves) <= kRawPairs;
   l.few = l.raw || (p->M <= kFewRowsMost && up(p->N, 16) >= 192 && up(p->N, 16) <= 512);
   // tiles: 2048 x 4096 x 4096 (128 of 256) 54.4 us, in tiles of 128 55.1; 1024 x 4096 x 4096 (64
-  // and 256) 49.6 and 31.4; 512 x 4096 x 4096 (128 of 128) 26.5, in tiles of 64 24.0
+  // and 256) 49.6 and 31.4; 512 x 4096 x 4096 (128 of 128) 26.5, in tiles of 64 24.0; 600 x
+  // 4096 x 4096 (160 of 128) 29.6 and 34.4
   auto tiles = [&](int t) { return (int64_t)up(p->M, t) * up(p->N, t); };
   l.tile = tiles(256) >= kLargeTiles ? 256 : tiles(128) >= kMediumTiles ? 128 : 64;
   l.tiles_m = up(p->M, l.tile);
   l.tiles_n = up(p->N, l.tile);
   l.pieces = 1;
-  if (!l.few && l.tile < 256) {
-    const int want = (int)std::min<int64_t>(up(l.tile == 128 ? 256 : 512, (int)std::min<int64_t>(tiles(l.tile), 512)),
-                                            std::max(1, l.Kb / 4));
+  // pieces of K: as many as leave all workgroups resident (two a CU). 128 x 2304 x 4096 (72
+  // tiles) in seven 16.8 us, eight 18.3; 300 x 4096 x 4096 (320) in one 22.1, two 26.5
+  if (!l.few && l.tile == 64 && tiles(64) <= 256) {
+    const int want = std::max(1, std::min(512 / (int)tiles(64), l.Kb / 4));
     l.pieces = up(l.Kb, up(l.Kb, want));
   }
   if (!l.raw) {
