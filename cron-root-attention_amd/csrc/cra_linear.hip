@@ -185,12 +185,21 @@ __device__ __forceinline__ f32x4 mma_wide(f32x4 c, const Wide& w, const Wide& x)
 
 // Four results of row m, columns n .. n + 3.
 template <typename T>
-__device__ __forceinline__ void store4(const LinearArgs& a, int64_t m, int n, f32x4 c) {
-  if (m >= a.M || n >= a.N) return;
+__device__ __forceinline__ f32x4 bias4(const LinearArgs& a, int n) {
   const T* bias = static_cast<const T*>(a.bias);
+  f32x4 b = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (bias) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) b[r] = to_f32(bias[min(n + r, a.N - 1)]);
+  }
+  return b;
+}
+template <typename T>
+__device__ __forceinline__ void store4(const LinearArgs& a, int64_t m, int n, f32x4 c, f32x4 b) {
+  if (m >= a.M || n >= a.N) return;
   T e[4];
 #pragma unroll
-  for (int r = 0; r < 4; ++r) e[r] = from_f32<T>(bias ? c[r] + to_f32(bias[min(n + r, a.N - 1)]) : c[r]);
+  for (int r = 0; r < 4; ++r) e[r] = from_f32<T>(c[r] + b[r]);
   T* p = static_cast<T*>(a.y) + m * a.ldy + n;
   if (a.wide_y) {
     if constexpr (sizeof(T) == 2)
@@ -365,6 +374,9 @@ void linear_kernel(LinearArgs a) {
       }
     }
   }
+  f32x4 bias[FN];
+#pragma unroll
+  for (int n = 0; n < FN; ++n) bias[n] = bias4<T>(a, n0 + 16 * (wn * FN + n) + 4 * g);
   wait_vmem();  // loads past the last block, too
 #pragma unroll
   for (int m = 0; m < FM; ++m)
@@ -373,7 +385,7 @@ void linear_kernel(LinearArgs a) {
       const int64_t row = m0 + 16 * (wm * FM + m) + l16;
       const int col = n0 + 16 * (wn * FN + n) + 4 * g;
       if (!a.part)
-        store4<T>(a, row, col, acc[n][m]);
+        store4<T>(a, row, col, acc[n][m], bias[n]);
       else if (row < a.M && col < a.N)  // rows of N up to a multiple of four
         *reinterpret_cast<f32x4*>(a.part + ((int64_t)blockIdx.y * a.M + row) * a.ldp + col) = acc[n][m];
     }
@@ -387,10 +399,11 @@ __global__ __launch_bounds__(256) void join_kernel(LinearArgs a, int pieces, uin
   const int col = (int)(i - row * quads) * 4;
   if (row >= a.M) return;
   const float* p = a.part + (int64_t)row * a.ldp + col;
+  const f32x4 b = bias4<T>(a, col);
   f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int k = 0; k < pieces; ++k) s += *reinterpret_cast<const f32x4*>(p + (int64_t)k * a.M * a.ldp);
-  store4<T>(a, row, col, s);
+  store4<T>(a, row, col, s, b);
 }
 
 // Large 16-bit products: 256 x 256 results a workgroup, eight waves of 64 x 128, two waves
@@ -519,12 +532,7 @@ void large_kernel(LinearArgs a) {
                             : (wave == 6 ? w10 : w11);
 #pragma unroll
     for (int n = 0; n < FN; ++n) {
-      const int col = n0 + 16 * (wn * FN + n) + 4 * g;
-      f32x4 bias = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (a.bias && col < a.N) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) bias[r] = to_f32(static_cast<const T*>(a.bias)[col + r]);
-      }
+      const f32x4 bias = bias4<T>(a, n0 + 16 * (wn * FN + n) + 4 * g);
 #pragma unroll
       for (int m = 0; m < FM; ++m) {
         const int row = 16 * m + l16, chunk = 2 * n + (g >> 1);
@@ -546,10 +554,12 @@ void large_kernel(LinearArgs a) {
     return;
   }
 #pragma unroll
-  for (int m = 0; m < FM; ++m)
+  for (int n = 0; n < FN; ++n) {
+    const int col = n0 + 16 * (wn * FN + n) + 4 * g;
+    const f32x4 bias = bias4<T>(a, col);
 #pragma unroll
-    for (int n = 0; n < FN; ++n)
-      store4<T>(a, m0 + 16 * (wm * FM + m) + l16, n0 + 16 * (wn * FN + n) + 4 * g, acc[n][m]);
+    for (int m = 0; m < FM; ++m) store4<T>(a, m0 + 16 * (wm * FM + m) + l16, col, acc[n][m], bias);
+  }
 }
 
 // Few rows of x: bound by the reading of w. A workgroup takes 16 columns of y and all
@@ -633,6 +643,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(LinearArgs a) 
   }
 #pragma unroll
   for (int r = 0; r < 4; ++r) sums[wave][l16][4 * g + r] = acc[r];
+  const f32x4 bias = bias4<T>(a, n0 + (tid & 3) * 4);
   __syncthreads();
   for (int i = tid; i < 4 * R; i += 64 * NW) {
     const int row = i >> 2, c = (i & 3) * 4;
@@ -641,7 +652,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(LinearArgs a) 
     for (int w = 0; w < NW; ++w)
 #pragma unroll
       for (int r = 0; r < 4; ++r) s[r] += sums[w][row][c + r];
-    store4<T>(a, row, n0 + c, s);
+    store4<T>(a, row, n0 + c, s, bias);
   }
 }
 
