@@ -380,6 +380,9 @@ int check_prefix(const cra_cache* c, const cra_paged_plan* p, const cra_prefix* 
   if (x->pages < 1) return err(CRA_E_INVALID, "prefix: pages must be >= 1");
   if ((int64_t)x->pages * c->page_size > 0x7fff0000) return err(CRA_E_INVALID, "prefix: 2^31 - 2^16 rows or more");
   if (p->window < 1) return err(CRA_E_INVALID, "a shared prefix needs a window (each length has its own by the rule)");
+  const int64_t held = (int64_t)x->pages * c->page_size, rpb = p->relay != 0 ? 1 + p->top_k : 1;
+  if ((held / p->window + 1) * rpb + std::min<int64_t>(p->window, held) >= (int64_t)1 << 30)
+    return err(CRA_E_INVALID, "prefix: 2^30 keys of a query or more");
   return CRA_OK;
 }
 

@@ -124,6 +124,10 @@ def test_shared_prefix_arguments():
                       (N.CraPrefix(PTR + 2, PTR, 2), N.E_LAYOUT), (N.CraPrefix(PTR, PTR, 0), N.E_INVALID),
                       (N.CraPrefix(PTR, PTR, 1 << 27), N.E_INVALID)):
         assert call(bad) == code
+    # keys of a query: global rows of blocks of the window, and the window
+    long = N.CraPrefix(PTR, PTR, (1 << 29) // c.page_size)
+    assert call(long, plan(window=1)) == N.E_INVALID and "2^30" in error()
+    assert call(long, plan(window=1, relay=0), n=0) == N.E_WORKSPACE
     need = lib.cra_fwd_paged_shared_workspace_bytes(*map(ctypes.byref, (c, b, plan(), good)))
     assert need > lib.cra_fwd_paged_workspace_bytes(*map(ctypes.byref, (c, b, plan())))
     assert call(good, n=need - 1) == N.E_WORKSPACE

@@ -219,6 +219,46 @@ def test_captured_and_replayed_on_another_stream(M):
         assert torch.equal(y, want)
 
 
+def test_two_streams_at_once():
+    work = []
+    for i, (M, N, K) in enumerate([(40, 600, 2048), (1, 2000, 4096), (400, 700, 900)]):
+        x, w = make(M, N, K, BF16, seed=i)
+        x, w = x.to(DEV), cra.E4M3Weight.from_dense(w.to(DEV))
+        work.append((x, w, cra.linear_e4m3(x, w), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    results = []
+    for _ in range(10):
+        for x, w, _, stream in work:
+            with torch.cuda.stream(stream):
+                results.append(cra.linear_e4m3(x, w))
+    torch.cuda.synchronize()
+    for i, y in enumerate(results):
+        assert torch.equal(y, work[i % 3][2])
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("M,N,K", [(1000, 1300, 520), (130, 200, 2900), (70, 1030, 1400), (1100, 2050, 300)])
+def test_tiles_of_64_and_128(dtype, M, N, K):
+    x, w = make(M, N, K, dtype, seed=M)
+    b = torch.randn(N, generator=torch.Generator().manual_seed(5)).to(dtype)
+    y = cra.linear_e4m3(x.to(DEV), cra.E4M3Weight.from_dense(w.to(DEV)), b.to(DEV))
+    check(y, quantise(x, 1)[2], quantise(w, 128)[2], b, dtype)
+
+
+@pytest.mark.parametrize("M,N,K", [(600000, 64, 4096), (300000, 8192, 128)])
+def test_rows_behind_2_31_elements(M, N, K):
+    g = torch.Generator(device=DEV).manual_seed(0)
+    x, w = torch.randn(M, K, device=DEV, dtype=BF16, generator=g), torch.randn(N, K, device=DEV, dtype=BF16, generator=g)
+    w = cra.E4M3Weight.from_dense(w)
+    y = cra.linear_e4m3(x, w)
+    for at in (0, M // 2 + 17, M - 40):
+        part = cra.linear_e4m3(x[at:at + 40], w)
+        # sums in another order, cut at 2^-13.3 of sum |p|: a rounding may fall to the other side
+        off = torch.finfo(BF16).eps * part.float().abs() + 2 * 2.0 ** -12 * K
+        assert bool(((y[at:at + 40].float() - part.float()).abs() <= off).all())
+        assert float((y[at:at + 40].float() - part.float()).norm()) <= 2.0 ** -8 * float(part.float().norm())
+
+
 def test_runs_agree_bit_for_bit():
     for M in (1, 50, 500, 3000):
         x, w = make(M, 1500, 1000, BF16, seed=M)

@@ -276,6 +276,96 @@ def test_runs_agree_bit_for_bit():
         assert torch.equal(s.run(q, [1] * 20, window=DENSE), first)
 
 
+def test_two_streams_at_once():
+    work = []
+    for seed, (P, own) in enumerate([(700, [3 + 11 * i for i in range(30)]), (2500, [40 + i for i in range(17)])]):
+        s = Shared(P, own, 2, 64, F16, "same", 16, seed=seed)
+        q = s.q([1] * len(own), 8)
+        work.append((s, q, s.run(q, [1] * len(own), window=DENSE), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    results = []
+    for _ in range(10):
+        for s, q, _, stream in work:
+            with torch.cuda.stream(stream):
+                results.append(s.run(q, [1] * len(s.own), window=DENSE))
+    torch.cuda.synchronize()
+    for i, y in enumerate(results):
+        assert torch.equal(y, work[i % 2][2])
+
+
+def test_two_graphs_of_one_pool():
+    a, b = Shared(300, [5, 90, 33], 2, 64, BF16, "e4m3", 16, seed=1), Shared(2300, [50, 4], 2, 64, BF16, "e4m3", 16, seed=2)
+    stream, graphs, pool = torch.cuda.Stream(), [], None
+    stream.wait_stream(torch.cuda.current_stream())
+    for s in (a, b):
+        q, x, lens = s.q([1] * len(s.own), 4).to(DEV)[:, :, None], s.prefix(), s.ints(s.lens)
+        run = lambda: cra.cron_root_attention_paged(q, s.cache, s.table, lens, window=60, prefix=x)
+        with torch.no_grad(), torch.cuda.stream(stream):
+            want = run().clone()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, pool=pool, stream=stream):
+                y = run()
+            pool = pool or g.pool()
+        graphs.append((g, y, want, q, x, lens))
+    torch.cuda.current_stream().wait_stream(stream)
+    for i in (0, 1, 1, 0, 1, 0):
+        g, y, want = graphs[i][:3]
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+
+
+def test_lengths_that_do_not_fit():
+    """Sequences longer than the bound are NaN, empty and shorter ones than the prefix their own."""
+    s = Shared(200, [0, 30, 300, 7], 2, 64, F16, "same", 16)
+    s.lens = [0, 230, 500, 120]
+    q = s.q([1] * 4, 4)
+    want = cra.cron_root_attention_paged(q.to(DEV)[:, :, None], s.cache, s.table, s.ints(s.lens), window=64, max_seqlen=250)
+    for x in (s.prefix(), s.prefix(150), cra.SharedPrefix(s.prefix().page_table, s.ints([-3])),
+              cra.SharedPrefix(s.table[0, :4].contiguous(), s.ints([1000]))):
+        got = s.run(q, [1] * 4, packed=False, prefix=x, window=64, max_seqlen=250)
+        assert got[2].isnan().all() and want[2].isnan().all()
+        assert bool((got[0] == 0).all())
+        for b in (1, 3):
+            off = (got[b].float() - want[b, :, 0].float()).abs().max()
+            assert float(off) <= 2 * 2.0 ** -11 * float(s.v[0].float().abs().max())  # two roundings of P, V each
+
+
+def test_more_sequences_than_one_look():
+    own = [(i * 37) % 90 for i in range(700)]
+    s = Shared(96, own, 1, 32, BF16, "same", 16)
+    new = [min(1, n) for n in own]
+    q = s.q(new, 2)
+    check(s.run(q, new, window=DENSE, max_query_len=1), *s.expect(q, new, DENSE), BF16)
+
+
+def test_pages_behind_4_gib():
+    """Rows of pages whose bytes and elements lie behind 2^32."""
+    pages, page, H, D = 8800, 1024, 2, 128
+    big = cra.PagedKVCache(pages, H, D, page, BF16, None, device=DEV)
+    small = cra.PagedKVCache(6, H, D, page, BF16, None, device=DEV)
+    assert big.k.numel() > 1 << 31
+    n, new, P = [5000, 4500], [1, 1], 4096
+    high, low = (torch.tensor([[*x, y], [*x, z]], dtype=torch.int32)
+                 for x, y, z in (((8799, 8780, 8500, 8797), 8790, 8401), ((5, 0, 2, 3), 4, 1)))
+    table = cra.RotaryTable(D, 8192, device=DEV)
+    g = torch.Generator().manual_seed(0)
+    results = []
+    for cache, t in ((big, high.to(DEV)), (small, low.to(DEV))):
+        g.manual_seed(0)
+        x = torch.randn(1, sum(n), 6, D, generator=g).to(BF16).to(DEV).transpose(1, 2)
+        x[:, :, 5000:5000 + P] = x[:, :, :P]  # the same prefix
+        with torch.no_grad():
+            cu = Shared.ints([0, 5000, 9500])
+            q = cache.append(x[:, :2], x[:, 2:4], x[:, 4:], t, Shared.ints(n), cu, table=table, norm=True)
+            last = q[:, :, [4999, 9499]].transpose(0, 2).contiguous()
+            results.append([q, *cache.read(t, Shared.ints(n)),
+                            cra.cron_root_attention_paged(last, cache, t, Shared.ints(n), window=DENSE,
+                                                          prefix=cra.SharedPrefix(t[0, :4].contiguous(), Shared.ints([P])))])
+    for y, z in zip(*results):
+        assert torch.equal(y, z)
+
+
 def test_layer_step():
     """A layer that appends and attends behind a prefix gives what it gives without."""
     torch.manual_seed(0)
