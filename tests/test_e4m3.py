@@ -133,7 +133,7 @@ def test_shared_prefix_arguments():
     assert call(good, n=need - 1) == N.E_WORKSPACE
 
 
-CHECKER = r"""
+PROGRAM = r"""
 #include "cra_paged.hpp"
 #include <cstdio>
 using namespace cra;
@@ -165,7 +165,7 @@ int main() {
 @pytest.mark.skipif(not os.path.exists(HIPCC), reason="hipcc not found")
 def test_global_rows_split_at_a_prefix(tmp_path):
     src = tmp_path / "c.cpp"
-    src.write_text(CHECKER)
+    src.write_text(PROGRAM)
     exe = tmp_path / "c"
     subprocess.run([HIPCC, "-x", "hip", "--offload-arch=gfx950", "-O1", "-std=c++17", "-w", f"-I{CSRC}", str(src), "-o", str(exe)],
                    check=True, capture_output=True)
