@@ -181,6 +181,9 @@ void prefix_kernel(PagedArgs a) {
   constexpr int NW = kPrefixWaves, QB = kPrefixQB<D>, BN = kPrefixBN<D>, kQW = 16 * QB, BM = kPrefixBM<D>;
   using Tile = SwzTile<D, BN>;
   constexpr bool k8 = STORE != kSame;
+  // int8 codes are exact in bf16, times their scale they are not: the scale goes with P, one
+  // rounding for both (2.6e-3 of the result's norm -> 2.3e-3; of fp16 it would leave the range)
+  constexpr bool kVS = STORE == kInt8 && std::is_same<T, bf16>::value;
   // a wave's loads: kPer of K and of V, kRows rows each
   constexpr int kRowBytes = D * (k8 ? 1 : 2), kChunks = kRowBytes / 16, kRows = 64 / kChunks;
   constexpr int kLoads = BN / kRows, kPer = kLoads > NW ? kLoads / NW : 1, kMine = kPer * kRows;
@@ -294,7 +297,7 @@ void prefix_kernel(PagedArgs a) {
         const uint4 k4 = *reinterpret_cast<const uint4*>(kt[s] + p * 16);
         const uint4 v4 = *reinterpret_cast<const uint4*>(vt[s] + p * 16);
         const uint32_t wk[4] = {k4.x, k4.y, k4.z, k4.w}, wv[4] = {v4.x, v4.y, v4.z, v4.w};
-        const float sc = vscale[s][row];
+        const float sc = kVS ? 1.f : vscale[s][row];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint2 x = widen4<T, STORE>(wk[2 * h]), y = widen4<T, STORE>(wk[2 * h + 1]);
@@ -344,10 +347,11 @@ void prefix_kernel(PagedArgs a) {
         TileMask<QB> mk;
         if (full) {
           if constexpr (BN == 64)
-            attend_whole<T, STORE, D, BN, QB>(tK, tV, kscale[s], lo, qf, acc, m_run, l_run, c2, g, mk, one);
+            attend_whole<T, STORE, D, BN, QB, kVS>(tK, tV, kscale[s], lo, qf, acc, m_run, l_run, c2, g, mk, one,
+                                                    vscale[s]);
           else
-            attend_chunk<T, STORE, D, BN, QB, false>(tK, tV, kscale[s], lo, qf, acc, m_run, l_run, c2, g, mk, one,
-                                                     0, 0);
+            attend_chunk<T, STORE, D, BN, QB, false, kVS>(tK, tV, kscale[s], lo, qf, acc, m_run, l_run, c2, g, mk,
+                                                          one, 0, 0, vscale[s]);
         }
         // (a branch of its own: with an else the accumulators are held twice)
         if (uniform(fresh(full ? 0 : 1))) {
@@ -358,8 +362,8 @@ void prefix_kernel(PagedArgs a) {
             mk.hi[qb] = loc ? (r.ls < pp.n ? pp.n - 1 - ts : -1) : r.glen - 1 - ts;
             mk.span[qb] = loc ? (unsigned)max(pp.n - 1 - r.ls, 0) : 0x7fffffffu;
           }
-          attend_chunk<T, STORE, D, BN, QB, true>(tK, tV, kscale[s], lo, qf, acc, m_run, l_run, c2, g, mk, one,
-                                                  vis_lo >> 5, min(vis_hi >> 5, BN / 32 - 1));
+          attend_chunk<T, STORE, D, BN, QB, true, kVS>(tK, tV, kscale[s], lo, qf, acc, m_run, l_run, c2, g, mk, one,
+                                                  vis_lo >> 5, min(vis_hi >> 5, BN / 32 - 1), vscale[s]);
         }
       }
     };

@@ -52,13 +52,33 @@ __device__ __forceinline__ void chunk_softmax(f32x4 (&s)[2][QB], const float* ks
   for (int qb = 0; qb < QB; ++qb) l_run[qb] += ps[qb];
 }
 
-// A tile's halves kc0 .. kc1.
-template <typename T, int STORE, int D, int BN, int QB, bool MASK>
+// P of a half times the scales of V's rows, rounded once: V's codes stand unscaled in the
+// tile then.
+template <typename T, int QB>
+__device__ __forceinline__ void scale_p(const f32x4 (&s)[2][QB], const float* vs, int kc, int g, float c2,
+                                        const float (&m_run)[QB], Frag<T> (&pf)[QB]) {
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb) {
+    const float m = m_run[qb] == -kInf ? 0.f : m_run[qb];
+    float pv[8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(vs + 32 * kc + 16 * h + 4 * g);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) pv[4 * h + r] = __builtin_amdgcn_exp2f(fmaf(s[h][qb][r], c2, -m)) * v[r];
+    }
+    pf[qb] = pack8<T>(pv);
+  }
+}
+
+// A tile's halves kc0 .. kc1. VS: V's scales (vs) come in with P.
+template <typename T, int STORE, int D, int BN, int QB, bool MASK, bool VS = false>
 __device__ __forceinline__ void attend_chunk(const char* tK, const char* tV, const float* ks,
                                              const LaneOffs<D>& lo, const Frag<T> (&qf)[QB][D / 32],
                                              f32x4 (&acc)[D / 16][QB], float (&m_run)[QB],
                                              float (&l_run)[QB], float c2, int g,
-                                             const TileMask<QB>& mk, const Frag<T>& one, int kc0, int kc1) {
+                                             const TileMask<QB>& mk, const Frag<T>& one, int kc0, int kc1,
+                                             const float* vs = nullptr) {
   // (a loop over the halves would hold the accumulators twice, for its copies)
 #pragma unroll
   for (int kc = 0; kc < BN / 32; ++kc) {
@@ -67,18 +87,20 @@ __device__ __forceinline__ void attend_chunk(const char* tK, const char* tV, con
     Frag<T> pf[QB];
     tile_scores<T, D, BN, QB, kAhead<D, STORE>>(tK, lo, qf, kc, s);
     chunk_softmax<T, STORE, D, BN, QB, MASK>(s, ks, kc, acc, m_run, l_run, c2, g, mk, one, pf);
+    if constexpr (VS) scale_p<T, QB>(s, vs, kc, g, c2, m_run, pf);
     pv_half<T, D, BN, QB, kAhead<D, STORE>>(tV, kc, lo, pf, acc);
   }
 }
 
 // Both halves of a tile that every row sees: the second half's scores stand beside
 // the first one's exponentials, the first one's P.V beside the second's.
-template <typename T, int STORE, int D, int BN, int QB>
+template <typename T, int STORE, int D, int BN, int QB, bool VS = false>
 __device__ __forceinline__ void attend_whole(const char* tK, const char* tV, const float* ks,
                                              const LaneOffs<D>& lo, const Frag<T> (&qf)[QB][D / 32],
                                              f32x4 (&acc)[D / 16][QB], float (&m_run)[QB],
                                              float (&l_run)[QB], float c2, int g,
-                                             const TileMask<QB>& mk, const Frag<T>& one) {
+                                             const TileMask<QB>& mk, const Frag<T>& one,
+                                             const float* vs = nullptr) {
   static_assert(BN == 64, "two halves");
   f32x4 s0[2][QB], s1[2][QB];
   Frag<T> p0[QB], p1[QB];
@@ -107,6 +129,7 @@ __device__ __forceinline__ void attend_whole(const char* tK, const char* tV, con
     half_exp<T, false, QB>(s1, 1, qb, c2, m_run[qb], g, mk, one, p1[qb], ps[qb]);
     high |= !(ps[qb] <= kSumMax);
   }
+  if constexpr (VS) scale_p<T, QB>(s0, vs, 0, g, c2, m_run, p0);
   pv_half<T, D, BN, QB, kAhead<D, STORE>>(tV, 0, lo, p0, acc);
   if (__any(high)) {
 #pragma unroll
@@ -116,6 +139,7 @@ __device__ __forceinline__ void attend_whole(const char* tK, const char* tV, con
   }
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) l_run[qb] += ps[qb];
+  if constexpr (VS) scale_p<T, QB>(s1, vs, 1, g, c2, m_run, p1);
   pv_half<T, D, BN, QB, kAhead<D, STORE>>(tV, 1, lo, p1, acc);
 }
 
