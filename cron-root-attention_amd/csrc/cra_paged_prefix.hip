@@ -181,9 +181,7 @@ void prefix_kernel(PagedArgs a) {
   constexpr int NW = kPrefixWaves, QB = kPrefixQB<D>, BN = kPrefixBN<D>, kQW = 16 * QB, BM = kPrefixBM<D>;
   using Tile = SwzTile<D, BN>;
   constexpr bool k8 = STORE != kSame;
-  // int8 codes are exact in bf16, times their scale they are not: the scale goes with P, one
-  // rounding for both (2.6e-3 of the result's norm -> 2.3e-3; of fp16 it would leave the range)
-  constexpr bool kVS = STORE == kInt8 && std::is_same<T, bf16>::value;
+  constexpr bool kVS = STORE == kInt8;  // scale_p(): 2.6e-3 of a bf16 result's norm -> 2.4e-3
   // a wave's loads: kPer of K and of V, kRows rows each
   constexpr int kRowBytes = D * (k8 ? 1 : 2), kChunks = kRowBytes / 16, kRows = 64 / kChunks;
   constexpr int kLoads = BN / kRows, kPer = kLoads > NW ? kLoads / NW : 1, kMine = kPer * kRows;
@@ -297,7 +295,7 @@ void prefix_kernel(PagedArgs a) {
         const uint4 k4 = *reinterpret_cast<const uint4*>(kt[s] + p * 16);
         const uint4 v4 = *reinterpret_cast<const uint4*>(vt[s] + p * 16);
         const uint32_t wk[4] = {k4.x, k4.y, k4.z, k4.w}, wv[4] = {v4.x, v4.y, v4.z, v4.w};
-        const float sc = kVS ? 1.f : vscale[s][row];
+        const float sc = kVS ? scale_of_codes<T>(vscale[s][row]) : vscale[s][row];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint2 x = widen4<T, STORE>(wk[2 * h]), y = widen4<T, STORE>(wk[2 * h + 1]);

@@ -52,8 +52,17 @@ __device__ __forceinline__ void chunk_softmax(f32x4 (&s)[2][QB], const float* ks
   for (int qb = 0; qb < QB; ++qb) l_run[qb] += ps[qb];
 }
 
-// P of a half times the scales of V's rows, rounded once: V's codes stand unscaled in the
-// tile then.
+// int8 codes are exact in 16 bits, times their scale they are not, so the scale of V's rows
+// goes with P, one rounding for both: all of it (bf16), or (fp16, whose range P would leave)
+// its significand, the codes standing in the tile times its power of two.
+template <typename T>
+__device__ __forceinline__ float scale_of_codes(float s) {
+  return std::is_same<T, bf16>::value ? 1.f : __uint_as_float(__float_as_uint(s) & 0x7f800000u);
+}
+template <typename T>
+__device__ __forceinline__ float scale_of_p(float s) {
+  return std::is_same<T, bf16>::value ? s : __uint_as_float((__float_as_uint(s) & 0x7fffffu) | 0x3f800000u);
+}
 template <typename T, int QB>
 __device__ __forceinline__ void scale_p(const f32x4 (&s)[2][QB], const float* vs, int kc, int g, float c2,
                                         const float (&m_run)[QB], Frag<T> (&pf)[QB]) {
@@ -65,7 +74,7 @@ __device__ __forceinline__ void scale_p(const f32x4 (&s)[2][QB], const float* vs
     for (int h = 0; h < 2; ++h) {
       const f32x4 v = *reinterpret_cast<const f32x4*>(vs + 32 * kc + 16 * h + 4 * g);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) pv[4 * h + r] = __builtin_amdgcn_exp2f(fmaf(s[h][qb][r], c2, -m)) * v[r];
+      for (int r = 0; r < 4; ++r) pv[4 * h + r] = __builtin_amdgcn_exp2f(fmaf(s[h][qb][r], c2, -m)) * scale_of_p<T>(v[r]);
     }
     pf[qb] = pack8<T>(pv);
   }
