@@ -21,6 +21,7 @@
 // token each of 64 sequences, 32 heads and 8 9.
 #include <stdio.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "cra_cache_dev.hpp"
@@ -151,7 +152,7 @@ __device__ __forceinline__ void append_rows(const AppendArgs& a, uint32_t block,
   }
 
   // rows of v: as they are stored, up to two a thread (a stored row takes at most
-  // twice the lanes of a turned one)
+  // twice the lanes of a turned one: cra_cache_append sees to it)
   const int wlane = threadIdx.x & ((1 << a.log_w) - 1), wrow = threadIdx.x >> a.log_w;
   const int wrows = kThreads >> a.log_w;
   const bool have = wlane * 8 < g.D;
@@ -340,9 +341,14 @@ int cra_cache_append(const cra_cache* c, const cra_batch* b, const cra_turn* p, 
   }
   const cra_tensor* ts[3] = {&q, &k, &yq};
   const void* ws[2] = {p->norm ? wq : nullptr, p->norm ? wk : nullptr};
-  const TurnShape sh = turn_shape(p, ts, 3, ws);
+  TurnShape sh = turn_shape(p, ts, 3, ws);
   if (sh.V < 2) return err(CRA_E_UNSUPPORTED, "weights or turned halves between 4-byte steps are not built");
   AppendArgs a{};
+  a.Ds = c->D;
+  while ((8 << a.log_w) < c->D) ++a.log_w;
+  // a workgroup stores two rows a thread (append_rows): heads far narrower than the cache's
+  // rows take more lanes than they have units for
+  sh.log_l = std::max(sh.log_l, a.log_w - 1);
   fill_args(a.g, p, sh);
   a.heads = p->H_q % kHeads == 0 && (int64_t)p->B * p->S * p->H_q >= kManyRows ? kHeads : 1;
   a.xsh = q.sh, a.ysh = yq.sh;
@@ -356,8 +362,6 @@ int cra_cache_append(const cra_cache* c, const cra_batch* b, const cra_turn* p, 
   a.c = paged_view(c, b);
   a.v = v.ptr, a.vsb = v.sb, a.vsh = v.sh, a.vss = v.ss;
   a.k_norm = c->k_norm, a.k_scale = c->k_scale, a.v_scale = c->v_scale;
-  a.Ds = c->D;
-  while ((8 << a.log_w) < c->D) ++a.log_w;
   if (((int64_t)a.g.t[0].blocks + a.g.t[1].blocks) * kThreads >= (int64_t)1 << 32)
     return err(CRA_E_INVALID, "too many rows for one launch");
   const hipStream_t st = (hipStream_t)stream;

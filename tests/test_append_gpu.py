@@ -300,3 +300,37 @@ def test_refusals():
     with ad.dual_level(), torch.no_grad():
         no(NotImplementedError, ad.make_dual(q, q), k, v, pages, n, cu, table=table)
     assert math.isfinite(float(cache.k.float().sum()))
+
+
+@pytest.mark.parametrize("dtype,store", [(F16, "same"), (BF16, "e4m3"), (F32, "int8"), (F32, "same")])
+@pytest.mark.parametrize("D,width,rot", [(64, 256, 0), (64, 128, 64), (32, 128, 32), (16, 64, 16), (8, 256, 0), (40, 256, 8),
+                                         (24, 32, 24)])
+def test_heads_narrower_than_the_rows_of_the_cache(dtype, store, D, width, rot):
+    """Through the C ABI, which takes any head up to the cache's row: every token's row is stored,
+    as the write stores the turned rows."""
+    from cron_root_attention import _native as N
+    lib, B, H, S, page = N.load_library(), 3, 2, 150, 16
+    g = torch.Generator().manual_seed(D + width)
+    k, v = (torch.randn(B, H, S, D, generator=g).to(dtype).to(DEV) for _ in "kv")
+    wk = (1 + 0.3 * torch.randn(D, generator=g)).to(dtype).to(DEV)
+    table = cra.RotaryTable(rot, 256, device=DEV) if rot else None
+    pages = torch.randperm(40, generator=g)[:30].view(B, 10).to(torch.int32).to(DEV)
+    lens = ints([150, 153, 160])
+    batch = N.CraBatch(pages.data_ptr(), 10, lens.data_ptr(), None, B, 10, 0, S)
+
+    def cache():
+        own = [torch.full((40, H, page, n), 3.0, device=DEV).to(t or dtype)
+               for n, t in ((width, STORES[store]),) * 2 + ((1, F32),) * 3]
+        scales = [t.data_ptr() if store != "same" else None for t in own[3:]]
+        return own, N.CraCache(*(t.data_ptr() for t in own[:3]), *scales, 40, H, page, width, N.dtype_code(dtype),
+                               list(STORES).index(store))
+    turn = N.CraTurn(B, H, H, S, D, rot, 0, 1, N.dtype_code(dtype), N.dtype_code(dtype), 0, 1e-6,
+                     table.table.data_ptr() if rot else None, 256 if rot else 0, None, 0, 0)
+    (a, ca), (b, cb), y = cache(), cache(), torch.empty_like(k)
+    stream = torch.cuda.current_stream().cuda_stream
+    ref = [N.ctypes.byref(x) for x in (ca, batch, turn, cb)]
+    w = wk.data_ptr()
+    assert lib.cra_cache_append(ref[0], ref[1], ref[2], N.row_arg(k), N.row_arg(k), N.row_arg(v), w, w, N.row_arg(y), stream) == 0
+    assert lib.cra_cache_write(ref[3], ref[1], N.row_arg(y), N.row_arg(v), D, stream) == 0
+    for s, t in zip(a, b):
+        assert same_bits(s, t)
