@@ -622,6 +622,8 @@ std::vector<at::Tensor> cache_append(const at::Tensor& q, const at::Tensor& k, c
   if (pos.defined() && !positions_fit(pos, q)) return {};
   if (!weights_fit(wq, wk, q) || (normed && !(eps >= 0)) || (!normed && (wq.defined() || wk.defined())))
     return {};
+  for (const at::Tensor& w : {wq, wk})
+    if (w.defined() && w._fw_grad(0).defined()) return {};
   c10::DeviceGuard guard(q.device());
   at::Tensor y = at::empty_like(q);
   if (!paged_rows(y)) return {};

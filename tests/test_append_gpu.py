@@ -334,3 +334,13 @@ def test_heads_narrower_than_the_rows_of_the_cache(dtype, store, D, width, rot):
     assert lib.cra_cache_write(ref[3], ref[1], N.row_arg(y), N.row_arg(v), D, stream) == 0
     for s, t in zip(a, b):
         assert same_bits(s, t)
+
+
+def test_tangents_of_the_norm_weights_are_refused():
+    import torch.autograd.forward_ad as ad
+    table = cra.RotaryTable(64, 64, device=DEV)
+    cache, q, k, v, pages, n, cu = make([4, 5], [1, 2], 4, 2, 64, BF16, "same")
+    w = torch.ones(64, device=DEV)
+    for name in ("q_weight", "k_weight"):
+        with ad.dual_level(), torch.no_grad(), pytest.raises(NotImplementedError):
+            cache.append(q, k, v, pages, n, cu, table=table, norm=True, **{name: ad.make_dual(w, w)})
