@@ -14,8 +14,8 @@
 // Sums: the 8-bit MFMA cuts the products it adds at about 2^-16 of the largest (measured:
 // 1.4e-5 of the result's norm for random operands, whatever K; its accumulator is fp32).
 // That is below the rounding of 16-bit results (fp16: 2e-4). fp32 results take the codes
-// widened to bf16 with their scales (exact) through the bf16 MFMA instead, at half its
-// rate or less: 3e-7.
+// widened to bf16 with their scales (exact: w_shift) through the bf16 MFMA instead, at half
+// its rate or less: 3e-7.
 #include <stdio.h>
 
 #include <algorithm>
@@ -161,7 +161,7 @@ __device__ __forceinline__ f32x4 mma8(f32x4 c, const Frag8& w, const Frag8& x, u
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, (int)sw, 0, (int)sx);
 }
 
-// The codes as bf16 numbers, scale included.
+// The codes as bf16 numbers, times 2^(e - 127).
 struct Wide {
   Frag<bf16> f[4];
 };
@@ -181,6 +181,20 @@ __device__ __forceinline__ f32x4 mma_wide(f32x4 c, const Wide& w, const Wide& x)
 #pragma unroll
   for (int i = 0; i < 4; ++i) c = mma(c, w.f[i], x.f[i]);
   return c;
+}
+
+// Codes reach down to 2^-9 and scales to 2^-126, bf16 to 2^-133, so one operand's scale goes
+// into it four times as large and the other's a quarter (the product is the same): w's where
+// its own is small (up to 2^-123; what x loses then is below 2^-200 in the product), else x's -
+// unless a row of the wave stands too high for that (a scale from 2^118), and elements
+// below 2^-133 beside it round to multiples of that. The power of two that w takes:
+__device__ __forceinline__ int w_shift(uint32_t ew, bool high) {
+  return (ew & 0xffu) <= 4u ? 2 : __any(high) ? 0 : -2;
+}
+__device__ __forceinline__ bool high_row(uint32_t ex) { return (ex & 0xffu) > 244u; }
+__device__ __forceinline__ Wide widen_w(const Frag8& c, uint32_t ew, int shift) { return widen(c, (ew & 0xffu) + shift); }
+__device__ __forceinline__ Wide widen_x(const Frag8& c, uint32_t ex, int shift) {
+  return widen(c, max((int)(ex & 0xffu) - shift, 0));
 }
 
 // Four results of row m, columns n .. n + 3.
@@ -352,12 +366,16 @@ void linear_kernel(LinearArgs a) {
 #pragma unroll
     for (int m = 0; m < FM; ++m) ex[m] = exps[s][wave][16 * m + l16] >> shift;
     if constexpr (kWide) {
+      bool high = false;
+#pragma unroll
+      for (int m = 0; m < FM; ++m) high |= high_row(ex[m]);
+      const int shift = w_shift(ew, high);
       Wide xf[FM];
 #pragma unroll
-      for (int m = 0; m < FM; ++m) xf[m] = widen(TX::frag(tx, m, lane), ex[m]);
+      for (int m = 0; m < FM; ++m) xf[m] = widen_x(TX::frag(tx, m, lane), ex[m], shift);
 #pragma unroll
       for (int n = 0; n < FN; ++n) {
-        const Wide wf = widen(TW::frag(tw, n, lane), ew);
+        const Wide wf = widen_w(TW::frag(tw, n, lane), ew, shift);
 #pragma unroll
         for (int m = 0; m < FM; ++m) acc[n][m] = mma_wide(acc[n][m], wf, xf[m]);
       }
@@ -635,10 +653,12 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(LinearArgs a) 
         wf[i] = load_w(kb + kAheadBlocks);
         ew[i] = sw[kb + kAheadBlocks];
       }
-      if constexpr (kWide)
-        acc = mma_wide(acc, widen(w, e), widen(xf, ex));
-      else
+      if constexpr (kWide) {
+        const int shift = w_shift(__builtin_amdgcn_readfirstlane(e), high_row(ex));
+        acc = mma_wide(acc, widen_w(w, e, shift), widen_x(xf, ex, shift));
+      } else {
         acc = mma8(acc, w, xf, e, ex);
+      }
     }
   }
 #pragma unroll

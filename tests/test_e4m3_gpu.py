@@ -295,3 +295,35 @@ def test_refusals():
         cra.E4M3Weight.from_dense(w)
     with pytest.raises(ValueError):
         cra.E4M3Weight.from_dense(w.to(DEV)[:, :0])
+
+
+@pytest.mark.parametrize("power", [-126, -125, -120, -117, -116, -100])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("M,N", [(2, 130), (9, 3200), (70, 130), (1000, 2400), (4100, 4097)])
+def test_every_code_counts_at_the_smallest_scales(dtype, power, M, N):
+    """Weights, and rows, of one element each that is a code times a scale near the smallest: the product with a
+    power of two is exact."""
+    K = 256
+    codes = torch.arange(1, 127, dtype=torch.uint8).view(torch.float8_e4m3fn)  # 2^-9 .. 448
+    values = codes.float().double()
+    at = torch.arange(N) % 126
+    w = torch.zeros(N, K, dtype=torch.uint8)
+    w[torch.arange(N), torch.arange(N) % K] = torch.arange(1, 127, dtype=torch.uint8)[at]
+    scales = torch.full((-(-N // 128), 2), 2.0 ** power)
+    weight = cra.E4M3Weight.from_tensors(w.view(torch.float8_e4m3fn).to(DEV), scales.to(DEV))
+    big = 2.0 ** 100
+    y = cra.linear_e4m3(torch.full((M, K), big, dtype=dtype, device=DEV), weight)
+    assert torch.equal(y.double().cpu(), (values[at] * 2.0 ** power * big).expand(M, N))
+    if dtype == F32:  # (in bf16 the smallest elements of x are not numbers of their own)
+        row = torch.arange(M) % 126
+        x = torch.zeros(M, K, dtype=torch.float64)
+        x[torch.arange(M), torch.arange(M) % K] = values[row] * 2.0 ** power
+        x[torch.arange(M), (torch.arange(M) % K) // 128 * 128 + 127] = 448 * 2.0 ** power  # the block's scale
+        x[torch.arange(M) % 128 == 127] = 0
+        weight = cra.E4M3Weight.from_tensors(torch.zeros(N, K, dtype=torch.float8_e4m3fn, device=DEV),
+                                             torch.full((-(-N // 128), 2), big, device=DEV))
+        weight._codes[:, :] = 0x38  # ones
+        weight._codes[:, 127::128] = 0
+        y = cra.linear_e4m3(x.float().to(DEV), weight)
+        want = torch.where(torch.arange(M) % 128 == 127, 0.0, values[row] * 2.0 ** power * big)
+        assert torch.equal(y.double().cpu(), want[:, None].expand(M, N))
