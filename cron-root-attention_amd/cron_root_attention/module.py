@@ -58,6 +58,11 @@ class CronRootAttention(nn.Module):
         self.k_norm = nn.Parameter(torch.ones(self.head_dim)) if qk_norm else None
         self._reset_parameters()
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if "qkv_proj" not in self._modules:  # a layer pickled before there was one
+            self.__dict__.setdefault("qkv_proj", None)
+
     def _reset_parameters(self):
         for lin in (self.q_proj, self.k_proj, self.v_proj, self.o_proj):
             nn.init.xavier_uniform_(lin.weight)

@@ -189,3 +189,15 @@ def test_python_refusals_without_a_gpu():
         cra.linear_e4m3(w, w)
     with pytest.raises(RuntimeError):
         cra.CronRootAttention(64, 2).to_e4m3()
+
+
+def test_a_layer_pickled_before_it_could_hold_a_joint_projection():
+    torch.manual_seed(0)
+    layer = cra.CronRootAttention(64, 2).eval()
+    state = {k: v for k, v in layer.__dict__.items() if k != "qkv_proj"}
+    other = cra.CronRootAttention.__new__(cra.CronRootAttention)
+    other.__setstate__(state)
+    x = torch.randn(1, 9, 64)
+    with torch.no_grad():
+        assert torch.equal(other(x), layer(x))
+    assert "qkv_proj" not in other.state_dict()
