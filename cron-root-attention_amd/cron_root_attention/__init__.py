@@ -78,7 +78,7 @@ cron_root_attention = cron_root_attention_v14
 # The reference's own list (a star import gives what the reference's gives); what
 # this package adds is reached by name: RotaryTable, rotary_embedding,
 # qk_norm_rotary, PagedKVCache, PagedBatch, SharedPrefix,
-# cron_root_attention_paged, # E4M3Weight, E4M3Linear, linear_e4m3.
+# cron_root_attention_paged, E4M3Weight, E4M3Linear, linear_e4m3.
 __all__ = [
     "cron_root_attention",
     "cron_root_attention_v14",

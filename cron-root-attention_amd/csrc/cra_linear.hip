@@ -241,13 +241,6 @@ struct CodeTile {
     const int row = wave * 8 + (lane >> 3);
     return row * Kp + (((lane & 7) ^ (row >> 1 & 7)) << 4);
   }
-  // rows behind the resource's last one load as zeros
-  __device__ __forceinline__ static void load(char* lds, __amdgpu_buffer_rsrc_t rsrc, int off, int Kp, int wave) {
-    const int w = __builtin_amdgcn_readfirstlane(wave) & (NW - 1);
-#pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, CRA_LDS(lds + (i * NW + w) * 1024), 16, off + i * NW * 8 * Kp, 0, 0, 0);
-  }
   // 32 codes of row 16 blk + lane % 16: chunks g and g + 4
   __device__ __forceinline__ static Frag8 frag(const char* lds, int blk, int lane) {
     const int row = lane & 15, g = lane >> 4;
