@@ -138,8 +138,9 @@ def linear_e4m3(x: torch.Tensor, weight: E4M3Weight, bias: Optional[torch.Tensor
     Each row of x is brought into e4m3 with a power-of-two scale for each 128 columns
     (the smallest with which the largest element fits); products are summed in fp32
     and rounded once.  16-bit results take the 8-bit matrix core, whose sums are off by
-    about 1.4e-5 of the result's norm; fp32 ones the 16-bit one.  A block of x that
-    holds an infinity or NaN makes its row's results NaN.
+    about 1.4e-5 of the result's norm (of the terms' where these cancel); fp32 ones the
+    16-bit one, whose sums are fp32's.  A block of x that holds an infinity or NaN makes
+    its row's results NaN.
 
     Args:
         x: [..., in_features] float16, bfloat16 or float32 on the GPU, any strides

@@ -391,8 +391,10 @@ def cron_root_attention_paged(q: torch.Tensor, cache: PagedKVCache, page_table: 
         prefix: rows that the sequences begin with together (a window is given then: by
             the rule each length has blocks of its own). They are read once for all
             sequences with at most 16 query rows a kv head (new tokens times H_q /
-            heads) whose new tokens lie behind them; the others attend as without. The
-            results are those without a prefix up to rounding.
+            heads) whose new tokens lie behind them; the others (longer chunks, wider
+            groups) attend as without. The results are those without a prefix up to
+            rounding. Worth it from about 2^16 rows that are so read once (sequences
+            times the prefix's rows): below, the call is up to 17 us faster without.
 
     Returns: like q (laid out as q). Rows of tokens outside every sequence are zeros; so
     is a query that sees no row (more new tokens than the sequence's length). A

@@ -303,7 +303,7 @@ typedef const __attribute__((address_space(4))) uint32_t* ConstWords;  // read b
 // LDS reads (a fragment serves two to four MFMAs) where it has many. Few tiles are cut
 // along K (gridDim.y), whose sums join_kernel adds in their order.
 // Measured, bf16 with the rows' own way into 8 bits: 1024 x 4096 x 4096 (tiles of 128) 31.8 us,
-// 512 (of 64) 23.7, 64 (of 64, K in eight pieces) 16; two stages and no pieces 42.5, 28.0, 19.
+// 512 (of 64) 23.7, 64 (of 64, K in eight pieces) 16; 16384 x 6144 x 4096 fp32 (of 256) 700-735; two stages and no pieces 42.5, 28.0, 19.
 template <typename T, int WM, int WN, int FM, int FN, int kStages>
 __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM * WN / 4)))
 void linear_kernel(LinearArgs a) {
@@ -431,8 +431,8 @@ __global__ __launch_bounds__(256) void join_kernel(LinearArgs a, int pieces, uin
 // loads. The loads are written as instructions: the compiler would wait for all of
 // them before each read of LDS.
 //
-// Measured, 8192 x 8192 x 8192 bf16: 384 us, 2.86 PFLOP/s; 16384 x 6144 x 4096: 297 us, 2.78
-// (library products of one scale: 2.66 and 2.98).
+// Measured, 8192 x 8192 x 8192 bf16: 384 us, 2.86 PFLOP/s; 16384 x 6144 x 4096: 297-350 us by
+// box, 2.4-2.8 (library products of one scale: 2.66 and 2.98).
 template <typename T>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2)))
 void large_kernel(LinearArgs a) {
@@ -714,7 +714,8 @@ Plan plan_of(const cra_linear* p) {
   l.Kp = l.Kb * kBlock;
   l.Ks = up(l.Kb, 4) * 4;
   // where the sides cross (bf16, us): x as it is against brought into 8 bits first, 4 x 4096
-  // x 4096 8.2 and 8.7, 4 x 1024 x 16384 17.5 and 12.7; rows straight from memory against
+  // x 4096 8.2 and 8.7, 4 x 1024 x 16384 17.5 and 12.7 (one and two rows, which stay: 1 x 128 x
+  // 4096 5.0 and 8.0, 1 x 1024 x 16384 11.3 and 11.0, 2 x 1024 x 16384 13.2 and 11.6); rows straight from memory against
   // tiles cut along K, 16 x 4096 x 4096 10.5 and 11.4, 16 x 1024 x 16384 23.2 and 13.2, 16 x
   // 16384 x 4096 24.8 and 19.1, 32 x 4096 x 4096 13.2 and 12.7
   l.raw = p->M <= kRawRows && p->M * up(l.Kb, kFewWaves) <= kRawPairs;
